@@ -23,6 +23,9 @@ HV_EPI_I8, HV_EPI_I32, HV_EPI_GELU, HV_EPI_RESIDUAL = 0, 1, 2, 3
 HV_A_ROWS, HV_A_GATHER, HV_A_UNSIGNED = 0, 1, 4
 HV_SELECTOR_NOALLOC_MAX_BATCH = 1024
 HV_FWD_PIPELINED = 1
+HV_T_F32, HV_T_F16, HV_T_BF16, HV_T_I32 = 0, 1, 2, 3
+HV_Q_E4M3, HV_Q_I8 = 0, 1
+HV_LOG_PROBS_MAX_TOP = 64
 ABI_VERSION = 5
 PROF_CLASSES = ("patch", "layernorm", "gemm_qkv", "attention", "gemm_proj", "gemm_ffn1",
                 "gemm_ffn2", "selector", "head", "other", "ffn")
@@ -106,6 +109,27 @@ class BlockCkpt(C.Structure):
                                    "ffn_out", "score", "prob")]
 
 
+class RmsNormDesc(C.Structure):
+    _fields_ = [(n, _vp) for n in ("x", "residual", "weight", "residual_out", "q", "exps", "scale",
+                                   "rows_dev")] + [
+        (n, C.c_int64) for n in ("x_ld", "residual_ld", "residual_out_ld", "q_ld", "exps_ld")] + [
+        (n, _i32) for n in ("rows", "width", "type", "format", "block")] + [("eps", C.c_float)]
+
+
+class GemmF8Desc(C.Structure):
+    _fields_ = [(n, _vp) for n in ("a", "a_exps", "w_packed", "w_exps", "row_scale", "bias", "c",
+                                   "m_dev")] + [
+        (n, C.c_int64) for n in ("lda", "a_exps_ld", "ldc")] + [
+        (n, _i32) for n in ("m", "n", "k", "type")]
+
+
+class LogProbsDesc(C.Structure):
+    _fields_ = [(n, _vp) for n in ("logits", "tokens", "logp", "entropy", "top_logp", "top_index",
+                                   "rows_dev")] + [
+        (n, C.c_int64) for n in ("logits_ld", "tokens_ld")] + [
+        (n, _i32) for n in ("rows", "width", "type", "n_tokens", "top")] + [("scale", C.c_float)]
+
+
 _LIB = None
 
 
@@ -167,6 +191,13 @@ def _declare(L):
     L.hv_schedule_packed_bytes.argtypes = [C.POINTER(Schedule)]
     L.hv_schedule_bind.argtypes = [C.POINTER(Schedule), _vp, C.c_size_t, _vp, C.c_size_t,
                                    C.POINTER(ModelDev), _vp]
+    L.hv_rms_norm_q8.argtypes = [C.POINTER(RmsNormDesc), _vp]
+    L.hv_gemm_f8_workspace_bytes.restype = C.c_size_t
+    L.hv_gemm_f8_workspace_bytes.argtypes = [C.c_int, C.c_int, C.c_int]
+    L.hv_gemm_f8.argtypes = [C.POINTER(GemmF8Desc), _vp, C.c_size_t, _vp]
+    L.hv_log_probs_workspace_bytes.restype = C.c_size_t
+    L.hv_log_probs_workspace_bytes.argtypes = [C.c_int, C.c_int, C.c_int]
+    L.hv_log_probs.argtypes = [C.POINTER(LogProbsDesc), _vp, C.c_size_t, _vp]
     L.hv_profile_enable.argtypes = [C.c_int]
     L.hv_profile_read.argtypes = [_vp, _vp, C.c_int]
 
@@ -196,4 +227,5 @@ def exported_symbols():
             "hv_model_workspace_bytes", "hv_model_forward", "hv_model_forward_f32",
             "hv_model_forward_ex", "hv_model_forward_f32_ex",
             "hv_quantize_images", "hv_schedule_compile", "hv_schedule_packed_bytes",
-            "hv_schedule_bind")
+            "hv_schedule_bind", "hv_rms_norm_q8", "hv_gemm_f8_workspace_bytes", "hv_gemm_f8",
+            "hv_log_probs_workspace_bytes", "hv_log_probs")

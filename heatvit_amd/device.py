@@ -170,3 +170,65 @@ class DeviceModel:
         s.head_w_exp = params.head_w_scale_exp
         self.struct = s
         self.device = self.holder.device
+
+
+F8_BLOCK = 128  # k and n that share an exponent
+
+
+def quantise_f8_weight(w):
+    """A float matrix W[K][N] as e4m3 values and the exponents
+    [ceil(K/128)][ceil(N/128)] (int8) of its 128 x 128 blocks: the smallest
+    power of two that holds the block's largest value, at least 2^-127."""
+    k, n = w.shape
+    kb, nb = -(-k // F8_BLOCK), -(-n // F8_BLOCK)
+    w = w.float()
+    amax = torch.nn.functional.pad(w.abs(), (0, nb * F8_BLOCK - n, 0, kb * F8_BLOCK - k))
+    amax = amax.view(kb, F8_BLOCK, nb, F8_BLOCK).amax((1, 3))
+    m, e = torch.frexp(amax)  # 448 = 0.875 * 2^9
+    e = torch.where(amax > 0, (e - 9 + (m > 0.875)).clamp(min=-127), -127)
+    up = torch.exp2(-e.double()).float()
+    up = up.repeat_interleave(F8_BLOCK, 0)[:k].repeat_interleave(F8_BLOCK, 1)[:, :n]
+    return (w * up).to(torch.float8_e4m3fn), e.to(torch.int8)
+
+
+def pack_f8x64(w):
+    """Pack an e4m3 matrix W[K][N] into the f8x64 layout of
+    include/heatvit_hip.h: [N64/64][K128/128][4 j][2 h][64 lanes][16 bytes],
+    element (k, n) at tile (n // 64, k // 128), j = n % 16 // 4,
+    h = k % 128 // 64, lane 4 * (n % 64 // 16) + n % 4 + 16 * (k % 64 // 16),
+    byte k % 16, zero-padded."""
+    k, n = w.shape
+    kb, ng = -(-k // F8_BLOCK), -(-n // 64)
+    p = torch.zeros((kb * F8_BLOCK, ng * 64), dtype=torch.uint8, device=w.device)
+    p[:k, :n] = w.view(torch.uint8)
+    # k = (block, h, lane / 16, byte), n = (group, lane / 4 % 4, j, lane % 4)
+    p = p.view(kb, 2, 4, 16, ng, 4, 4, 4).permute(4, 0, 6, 1, 2, 5, 7, 3)
+    return p.reshape(-1)
+
+
+class DeviceF8Weight:
+    """A weight W[K][N] of heatvit_amd.lm.gemm_f8, laid out once: a float
+    matrix, quantised here in 128 x 128 blocks, or float8_e4m3fn values with
+    their int8 exponents [ceil(K/128)][ceil(N/128)].  Either order of storage
+    is taken (a checkpoint's [N][K] as `w.t()`)."""
+
+    def __init__(self, w, exps=None, device=None):
+        if w.dim() != 2 or not w.numel():
+            raise ValueError("a weight is a matrix [K][N]")
+        if device is None:
+            device = w.device if w.is_cuda else "cuda"
+        k, n = w.shape
+        if k % 16:
+            raise ValueError(f"the inner size {k} is not a multiple of 16")
+        if exps is None:
+            if w.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+                raise TypeError("a weight without exponents is float32, float16 or bfloat16")
+            w, exps = quantise_f8_weight(w.to(device))
+        elif w.dtype != torch.float8_e4m3fn or exps.dtype != torch.int8:
+            raise TypeError("a quantised weight is float8_e4m3fn with int8 exponents")
+        elif tuple(exps.shape) != (-(-k // F8_BLOCK), -(-n // F8_BLOCK)):
+            raise ValueError(f"exponents of a {k} x {n} weight are [ceil(K/128)][ceil(N/128)]")
+        self.inner, self.width = k, n
+        self.packed = pack_f8x64(w.to(device))
+        self.exps = exps.to(device).contiguous()
+        self.device = self.packed.device

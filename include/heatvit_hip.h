@@ -394,6 +394,119 @@ int hv_model_forward_f32_ex(const hv_model_dev *p, const float *images, int batc
                             size_t workspace_bytes, int options, hv_stream_t stream);
 
 /* ------------------------------------------------------------------ */
+/* Operators of language models (no counterpart in the reference): the   */
+/* path norm -> product -> answer of rows of floating-point activations. */
+/* Scales are powers of two, held as int8 exponents in [-127, 127]; a    */
+/* block is 128 columns (the last one of a row may be shorter).          */
+/* ------------------------------------------------------------------ */
+
+/* Element types of activations, outputs and logits. */
+#define HV_T_F32 0
+#define HV_T_F16 1
+#define HV_T_BF16 2
+#define HV_T_I32 3 /* logits only */
+
+/* 8-bit output formats. */
+#define HV_Q_E4M3 0 /* OCP e4m3 (largest 448, NaN, no infinities) */
+#define HV_Q_I8 1   /* int8 in [-127, 127]                        */
+
+#define HV_NORM_MAX_WIDTH (1 << 20)
+
+/* Root-mean-square norm of rows with the residual's addition, in 8 bits:
+ *   h = x + residual, summed in 32 bits and rounded once to the type (h = x
+ *       without a residual), written to residual_out
+ *   scale[r] = 1 / sqrt(mean of h^2 over the row + eps)
+ *   p = weight * h in 32 bits
+ *   exps[r][b] = smallest e >= -127 with |p| <= L * 2^e over block b, L = 448
+ *       (HV_Q_E4M3) or 127 (HV_Q_I8); block 128, or 0: one for the row
+ *   q[r][c] = p * 2^-e, rounded to nearest, ties to even
+ * so q * 2^exps * scale stands for the normalised row.  q and exps depend on
+ * p alone, bit for bit.  An infinity or NaN in p gives NaN in e4m3, and in
+ * int8 the end of the range or 0; the row's scale is then 0 or NaN.  The
+ * squares are summed in 32 bits: |h| has to stay under 2^60.
+ * residual_out is NULL exactly when residual is; it may be residual or x
+ * itself (same stride), q, exps and scale overlap nothing else.  rows_dev
+ * (optional, device): the live row count; rows behind it are left as they
+ * were.  Strides are in elements.  Pointers are aligned to their elements;
+ * 16-byte aligned rows of a width that 8 divides take wide loads. */
+typedef struct {
+  const void *x, *residual, *weight; /* [rows][x_ld], [rows][residual_ld], [width] of `type` */
+  void *residual_out;
+  void *q;       /* [rows][q_ld] bytes               */
+  int8_t *exps;  /* [rows][exps_ld], a block's each  */
+  float *scale;  /* [rows]                           */
+  const int32_t *rows_dev;
+  int64_t x_ld, residual_ld, residual_out_ld, q_ld, exps_ld;
+  int32_t rows, width, type, format, block;
+  float eps;
+} hv_rms_norm_desc;
+
+int hv_rms_norm_q8(const hv_rms_norm_desc *d, hv_stream_t stream);
+
+/* Matrix product of e4m3 rows and weights with an exponent for each block:
+ *   c[m][n] = row_scale[m] * sum over blocks b of 2^(a_exps[m][b] + w_exps[b][n/128])
+ *             * sum over k in b of a[m][k] w[k][n], + bias[n]
+ * rounded once to `type`.  A float32 output is summed in 32 bits from exact
+ * products; for a 16-bit output the 8-bit matrix cores cut a product's bits
+ * that lie below 2^-13 of the largest product beside it (about 1.5e-5 of the
+ * result's norm) and sum in 32 bits from there.  w_exps is
+ * [ceil(k/128)][ceil(n/128)].  Packed weights ("f8x64"): w[K][N] padded with
+ * zeros to K128 = ceil(K/128)*128 by N64 = ceil(N/64)*64 and stored as
+ * [N64/64][K128/128][4][2][64][16] bytes: element (k, n) lies at tile
+ * (n/64, k/128), part j = (n%16)/4, half h = (k%128)/64, lane
+ * 4*((n%64)/16) + n%4 + 16*((k%64)/16), byte k%16, so each of the four parts
+ * is the first operand of one 16x16x128 MFMA, and result lane l holds
+ * channels 16*(l/16) .. +15 of a row in parts of four.
+ * k and lda are multiples of 16, a and w_packed 16-byte aligned.  row_scale
+ * [m] and bias [n] are optional.  m_dev (optional, device): the live row
+ * count; rows behind it are left as they were. */
+#define HV_GEMM_F8_MAX_DIM (1 << 22)  /* k and n */
+#define HV_GEMM_F8_MAX_ROWS (1 << 24) /* m       */
+
+typedef struct {
+  const void *a;        /* [m][lda] e4m3            */
+  const int8_t *a_exps; /* [m][a_exps_ld]           */
+  const void *w_packed;
+  const int8_t *w_exps;
+  const float *row_scale, *bias;
+  void *c;              /* [m][ldc] of `type`       */
+  const int32_t *m_dev;
+  int64_t lda, a_exps_ld, ldc;
+  int32_t m, n, k, type;
+} hv_gemm_f8_desc;
+
+size_t hv_gemm_f8_workspace_bytes(int m, int n, int k);
+int hv_gemm_f8(const hv_gemm_f8_desc *d, void *workspace, size_t workspace_bytes,
+               hv_stream_t stream);
+
+/* Log probabilities of given tokens under softmax(scale * logits), the
+ * entropy, and the `top` most probable tokens in order (equal logits by the
+ * lower index), from rows of logits of `type` (HV_T_I32: whole numbers, as
+ * hv_model_forward's logits with scale 2^-14).  A token below 0 asks for
+ * nothing and gets 0, one past the width NaN.  Logits of -inf have
+ * probability 0; a row of nothing else gets log probabilities of -inf and
+ * entropy 0.  A NaN or +inf makes the row's log probabilities and entropy
+ * NaN; a NaN counts as the largest logit.  rows_dev as above. */
+#define HV_LOG_PROBS_MAX_TOP 64
+
+typedef struct {
+  const void *logits;    /* [rows][logits_ld]           */
+  const int32_t *tokens; /* [rows][tokens_ld] or NULL   */
+  float *logp;           /* [rows][n_tokens]            */
+  float *entropy;        /* [rows]                      */
+  float *top_logp;       /* [rows][top]                 */
+  int32_t *top_index;    /* [rows][top]                 */
+  const int32_t *rows_dev;
+  int64_t logits_ld, tokens_ld;
+  int32_t rows, width, type, n_tokens, top;
+  float scale;
+} hv_log_probs_desc;
+
+size_t hv_log_probs_workspace_bytes(int rows, int width, int top);
+int hv_log_probs(const hv_log_probs_desc *d, void *workspace, size_t workspace_bytes,
+                 hv_stream_t stream);
+
+/* ------------------------------------------------------------------ */
 /* Kernel-class timing with HIP events (for benchmarks).  While enabled, */
 /* every kernel the forwards launch carries a start/stop event pair      */
 /* recorded by its own dispatch; hv_profile_read() waits for them and    */
