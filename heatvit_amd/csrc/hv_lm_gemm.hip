@@ -33,21 +33,21 @@ struct GemmF8Args {
   int64_t lda, a_exps_ld, ldc;
   int m, n, k;
   int kb, nb;  // blocks of 128 along k and n
-  bool vec;    // four outputs of a row may be stored at once
+  int vec;     // outputs stored at once: 2: 16 bytes, 1: four, 0: one
 };
 
 static constexpr int kTileBytes = 64 * 128;  // 64 channels by 128 k, packed
 
 // Operands of one block of 128 and their product: W fragment (16 channels) by
-// activation fragment (16 rows), added to acc with the factor 2^(we + ae).
+// activation fragment (16 rows), added to acc with the factor 2^(we + ae - 254) of the scale bytes
+// in the low bits of we and ae.
 struct Fast {
   typedef v8i frag;
   static __device__ __forceinline__ frag of(v4i lo, v4i hi) {
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   }
   static __device__ __forceinline__ v4f mma(const frag &w, const frag &a, v4f acc, int we, int ae) {
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, acc, 0, 0, 0, we + 127, 0,
-                                                            ae + 127);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, acc, 0, 0, 0, we, 0, ae);
   }
 };
 struct Exact {
@@ -69,34 +69,50 @@ struct Exact {
   }
   static __device__ __forceinline__ v4f mma(const frag &w, const frag &a, v4f acc, int we, int ae) {
     v4f t = {};
+    const int e = (we & 255) + (ae & 255) - 254;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.v[i], a.v[i], t, 0, 0, 0);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] += ldexpf(t[i], we + ae);
+    for (int i = 0; i < 4; ++i) acc[i] += ldexpf(t[i], e);
     return acc;
   }
 };
 
-// Four channels n .. n + 3 of row m.
-template <typename T>
-__device__ __forceinline__ void store4(const GemmF8Args &g, int m, int n, v4f v, float scale) {
+// CNT (a multiple of 4) adjacent channels n .. of row m.
+template <typename T, int CNT>
+__device__ __forceinline__ void store_run(const GemmF8Args &g, int m, int n, float *v, float scale) {
   T *p = (T *)g.c + m * g.ldc + n;
-  v *= scale;
-  if (g.bias) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (n + i < g.n) v[i] += g.bias[n + i];
+  for (int i = 0; i < CNT; ++i) {
+    v[i] *= scale;
+    if (g.bias && n + i < g.n) v[i] += g.bias[n + i];
   }
-  if (g.vec && n + 4 <= g.n) {
-    typedef T v4 __attribute__((ext_vector_type(4)));
-    v4 t;
+  constexpr int kWide = 16 / sizeof(T);
+  if (CNT % kWide == 0 && g.vec == 2 && n + CNT <= g.n) {
+    typedef T vt __attribute__((ext_vector_type(kWide)));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) t[i] = (T)v[i];
-    *reinterpret_cast<v4 *>(p) = t;
+    for (int i = 0; i < CNT; i += kWide) {
+      vt t;
+#pragma unroll
+      for (int j = 0; j < kWide; ++j) t[j] = (T)v[i + j];
+      *reinterpret_cast<vt *>(p + i) = t;
+    }
+  } else if (g.vec) {
+    typedef T v4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int i = 0; i < CNT; i += 4) {
+      if (n + i + 4 <= g.n) {
+        *reinterpret_cast<v4 *>(p + i) = v4{(T)v[i], (T)v[i + 1], (T)v[i + 2], (T)v[i + 3]};
+      } else {
+#pragma unroll
+        for (int j = i; j < i + 4; ++j)
+          if (n + j < g.n) p[j] = (T)v[j];
+      }
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < CNT; ++i)
       if (n + i < g.n) p[i] = (T)v[i];
   }
 }
@@ -131,7 +147,7 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_f8_direct(GemmF8Args g) {
       const v4i hi = *reinterpret_cast<const v4i *>(w + (size_t)b * kTileBytes + j * 2048 + 1024);
       wf[j] = Mma::of(lo, hi);
     }
-    const int we = g.w_exps[(size_t)b * g.nb + blockIdx.x / 2];
+    const int we = g.w_exps[(size_t)b * g.nb + blockIdx.x / 2] + 127;
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
       // past the end of k: zeros
@@ -140,7 +156,7 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_f8_direct(GemmF8Args g) {
       if (k < g.k) lo = *reinterpret_cast<const v4i *>(a[i] + b * 128);
       if (k + 64 < g.k) hi = *reinterpret_cast<const v4i *>(a[i] + b * 128 + 64);
       const typename Mma::frag af = Mma::of(lo, hi);
-      const int e = ae[i][b];
+      const int e = ae[i][b] + 127;
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[i][j] = Mma::mma(wf[j], af, acc[i][j], we, e);
     }
@@ -157,12 +173,181 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_f8_direct(GemmF8Args g) {
     for (int k = 1; k < NW; ++k) v += part[k][f][lane];
     const int m = m0 + 16 * (f / 4) + col;
     const int n = blockIdx.x * 64 + 16 * grp + 4 * (f % 4);
-    if (m < rows) store4<T>(g, m, n, v, g.row_scale ? g.row_scale[m] : 1.f);
+    float r[4] = {v[0], v[1], v[2], v[3]};
+    if (m < rows) store_run<T, 4>(g, m, n, r, g.row_scale ? g.row_scale[m] : 1.f);
   }
+}
+
+// 16 bytes a lane straight to LDS, the wavefront's 64 lanes one after another
+// from `to` on: from base + offset of a buffer of `size` bytes (zeros for an
+// offset behind it), or from a lane's address.
+__device__ __forceinline__ void buffer_to_lds(const uint8_t *base, int size, int offset,
+                                              uint8_t *to) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(
+      __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, size, 0x00020000),
+      (__attribute__((address_space(3))) void *)to, 16, offset, 0, 0, 0);
+}
+__device__ __forceinline__ void global_to_lds(const uint8_t *from, uint8_t *to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
+                                   (__attribute__((address_space(3))) void *)to, 16, 0, 0);
+}
+
+// Blocks of k whose exponents a workgroup keeps in LDS at a time.
+static constexpr int kExpSteps = 32;
+
+template <int BM, int BN>
+struct TileLds {
+  uint8_t a[BM * 128];
+  uint8_t b[BN * 128];
+};
+
+// BM x BN outputs a workgroup, WM x WN wavefronts. A block of 128 of k at a
+// time goes from memory into one of two LDS stages (16 bytes a lane, straight
+// to LDS) while the other one is multiplied.
+//   rows: 128 bytes each, their 16-byte chunks at chunk ^ (row & 7), so that
+//         16 rows' reads of one chunk spread over the banks
+//   weights: as they are packed, in the order the lanes take them
+// The exponents of kExpSteps blocks wait in LDS too: a load of theirs in the
+// loop would have to wait for the stage's loads in front of it.
+template <typename T, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void k_gemm_f8_tile(GemmF8Args g) {
+  typedef typename std::conditional<std::is_same<T, float>::value, Exact, Fast>::type Mma;
+  constexpr int kWaves = WM * WN, TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
+  constexpr int NB = (BN + 127) / 128;  // 128-column blocks of the tile
+  static_assert(TN <= 64 && 64 % TN == 0 && FM % 2 == 0, "a wavefront's columns share an exponent");
+  __shared__ TileLds<BM, BN> stage0, stage1;
+  __shared__ uint8_t a_exp[kExpSteps][WM][16][FM];
+  __shared__ uint8_t w_exp[kExpSteps][NB];
+
+  const int rows = g.m_dev ? min(g.m, *g.m_dev) : g.m;
+  // Tiles in bands of kBand along m; the eight XCDs, which take workgroups in
+  // turn, each get a contiguous range, whose operands meet in their L2.
+  constexpr int kBand = 4;
+  const int tn = (g.n + BN - 1) / BN, tm = (g.m + BM - 1) / BM, total = tm * tn;
+  int id = blockIdx.x;
+  if (total >= 16) {
+    const int per = total / 8, rem = total % 8, x = id % 8;
+    id = x * per + min(x, rem) + id / 8;
+  }
+  const int band = id / (kBand * tn), in = id - band * (kBand * tn);
+  const int high = min(kBand, tm - band * kBand);
+  const int m0 = (band * kBand + in % high) * BM, n0 = in / high * BN;
+  if (m0 >= rows) return;
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN, col = lane & 15, grp = lane >> 4;
+
+  // Loads: wavefront `wave` takes 8 rows (1 KiB) of every kWaves x 8.
+  constexpr int LA = BM / 8 / kWaves, LB = BN / 8 / kWaves;
+  static_assert(LA * 8 * kWaves == BM && LB * 8 * kWaves == BN, "whole loads");
+  const int last = rows - 1 - m0;  // of the tile's rows, those past it repeat it
+  const uint8_t *a_base = g.a + (int64_t)m0 * g.lda;
+  const int a_size = (int)(min(last, BM - 1) * g.lda + g.k);
+  const int chunk = (lane & 7) ^ ((lane >> 3) & 7);
+  int a_off[LA];
+#pragma unroll
+  for (int i = 0; i < LA; ++i)
+    a_off[i] = min((i * kWaves + wave) * 8 + (lane >> 3), last) * (int)g.lda + chunk * 16;
+  const uint8_t *w_at[LB];
+#pragma unroll
+  for (int i = 0; i < LB; ++i) {
+    const int kib = i * kWaves + wave;  // of the stage's BN / 8
+    const int group = min(n0 / 64 + kib / 8, (g.n - 1) / 64);
+    w_at[i] = g.w + (size_t)group * g.kb * kTileBytes + kib % 8 * 1024 + lane * 16;
+  }
+  auto load = [&](TileLds<BM, BN> &s, int b) {
+    // behind the last of k the buffer load gives zeros
+    const bool past = b * 128 + chunk * 16 >= g.k;
+#pragma unroll
+    for (int i = 0; i < LA; ++i)
+      buffer_to_lds(a_base, a_size, past ? 0x7FFFFFF0 : a_off[i] + b * 128,
+                    s.a + (i * kWaves + wave) * 1024);
+#pragma unroll
+    for (int i = 0; i < LB; ++i)
+      global_to_lds(w_at[i] + (size_t)b * kTileBytes, s.b + (i * kWaves + wave) * 1024);
+  };
+
+  v4f acc[FM][FN] = {};
+  auto multiply = [&](const TileLds<BM, BN> &s, int e) {
+    typename Mma::frag wf[FN];
+    const uint8_t *wb = s.b + wn * TN / 64 * 8192 + wn * TN % 64 / 16 * 2048 + lane * 16;
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+      wf[j] = Mma::of(*reinterpret_cast<const v4i *>(wb + j * 2048),
+                      *reinterpret_cast<const v4i *>(wb + j * 2048 + 1024));
+    const int we = w_exp[e][wn * TN / 128];
+    int ae[(FM + 3) / 4] = {};
+    __builtin_memcpy(ae, a_exp[e][wm][col], FM);
+    const uint8_t *ab = s.a + (wm * TM + col) * 128;
+    const int c0 = (grp ^ (col & 7)) * 16;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      const typename Mma::frag af = Mma::of(*reinterpret_cast<const v4i *>(ab + i * 2048 + c0),
+                                            *reinterpret_cast<const v4i *>(ab + i * 2048 + (c0 ^ 64)));
+      const int x = (unsigned)ae[i / 4] >> (8 * (i % 4));
+#pragma unroll
+      for (int j = 0; j < FN; ++j) acc[i][j] = Mma::mma(wf[j], af, acc[i][j], we, x);
+    }
+  };
+  auto load_exps = [&](int b0) {
+    const int steps = min(kExpSteps, g.kb - b0);
+    for (int i = tid; i < BM * kExpSteps; i += 64 * kWaves) {
+      const int r = i / kExpSteps, b = i % kExpSteps;
+      if (b < steps)
+        a_exp[b][r / TM][r % 16][r % TM / 16] =
+            (uint8_t)(g.a_exps[(int64_t)(m0 + min(r, last)) * g.a_exps_ld + b0 + b] + 127);
+    }
+    for (int i = tid; i < kExpSteps * NB; i += 64 * kWaves) {
+      const int b = i / NB, n = min(n0 / 128 + i % NB, g.nb - 1);
+      if (b < steps) w_exp[b][i % NB] = (uint8_t)(g.w_exps[(size_t)(b0 + b) * g.nb + n] + 127);
+    }
+  };
+
+  load(stage0, 0);
+  load_exps(0);
+  __syncthreads();
+  for (int b = 0; b < g.kb; b += 2) {
+    if (b && b % kExpSteps == 0) {
+      load_exps(b);
+      __syncthreads();
+    }
+    if (b + 1 < g.kb) load(stage1, b + 1);
+    multiply(stage0, b % kExpSteps);
+    __syncthreads();
+    if (b + 1 >= g.kb) break;
+    if (b + 2 < g.kb) load(stage0, b + 2);
+    multiply(stage1, (b + 1) % kExpSteps);
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    const int m = m0 + wm * TM + 16 * i + col;
+    const int n = n0 + wn * TN / 64 * 64 + 16 * grp + wn * TN % 64 / 4;
+    float v[4 * FN];
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[4 * j + k] = acc[i][j][k];
+    if (m < rows && n < g.n)
+      store_run<T, 4 * FN>(g, m, n, v, g.row_scale ? g.row_scale[m] : 1.f);
+  }
+}
+
+template <typename T, int BM, int BN, int WM, int WN>
+static void tile_launch(const GemmF8Args &g, hipStream_t s) {
+  const int tiles = ((g.n + BN - 1) / BN) * ((g.m + BM - 1) / BM);
+  hv_launch(k_gemm_f8_tile<T, BM, BN, WM, WN>, dim3(tiles), dim3(64 * WM * WN), 0, s, g);
 }
 
 template <typename T>
 static void gemm_f8_launch(const GemmF8Args &g, hipStream_t s) {
+  const char *e = getenv("HV_CFG");
+  const int cfg = e ? atoi(e) : 0;
+  if (cfg == 1) return tile_launch<T, 256, 256, 2, 4>(g, s);
+  if (cfg == 2) return tile_launch<T, 128, 128, 2, 2>(g, s);
+  if (cfg == 3) return tile_launch<T, 64, 64, 2, 2>(g, s);
+  if (cfg == 4) return tile_launch<T, 128, 256, 2, 4>(g, s);
   hv_launch(k_gemm_f8_direct<T, 4, 4>, dim3((g.n + 63) / 64, (g.m + 63) / 64), dim3(256), 0, s, g);
 }
 
@@ -207,7 +392,8 @@ int hv_gemm_f8(const hv_gemm_f8_desc *d, void *workspace, size_t workspace_bytes
   g.row_scale = d->row_scale; g.bias = d->bias; g.c = d->c; g.m_dev = d->m_dev;
   g.lda = d->lda; g.a_exps_ld = d->a_exps_ld; g.ldc = d->ldc;
   g.m = d->m; g.n = d->n; g.k = d->k;
-  g.vec = d->ldc % 4 == 0 && !((uintptr_t)d->c & (4 * size - 1));
+  const uintptr_t c_at = (uintptr_t)d->c | (uintptr_t)(d->ldc * size);
+  g.vec = !(c_at & 15) ? 2 : !(c_at & (4 * size - 1));
   const hipStream_t s = (hipStream_t)stream;
   if (d->type == HV_T_F32) gemm_f8_launch<float>(g, s);
   else if (d->type == HV_T_F16) gemm_f8_launch<f16>(g, s);
