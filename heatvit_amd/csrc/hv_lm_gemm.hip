@@ -43,9 +43,7 @@ static constexpr int kTileBytes = 64 * 128;  // 64 channels by 128 k, packed
 // in the low bits of we and ae.
 struct Fast {
   typedef v8i frag;
-  static __device__ __forceinline__ frag of(v4i lo, v4i hi) {
-    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-  }
+  static __device__ __forceinline__ frag of(v8i raw) { return raw; }
   static __device__ __forceinline__ v4f mma(const frag &w, const frag &a, v4f acc, int we, int ae) {
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, acc, 0, 0, 0, we, 0, ae);
   }
@@ -54,11 +52,11 @@ struct Exact {
   struct frag {
     v8bf v[4];
   };
-  static __device__ __forceinline__ frag of(v4i lo, v4i hi) {
+  static __device__ __forceinline__ frag of(v8i raw) {
     frag f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int x = i < 2 ? lo[2 * i] : hi[2 * i - 4], y = i < 2 ? lo[2 * i + 1] : hi[2 * i - 3];
+      const int x = raw[2 * i], y = raw[2 * i + 1];
       const v2bf a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.f, false);
       const v2bf b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.f, true);
       const v2bf c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y, 1.f, false);
@@ -78,6 +76,10 @@ struct Exact {
     return acc;
   }
 };
+
+__device__ __forceinline__ v8i join(v4i lo, v4i hi) {
+  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
 
 // CNT (a multiple of 4) adjacent channels n .. of row m.
 template <typename T, int CNT>
@@ -145,7 +147,7 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_f8_direct(GemmF8Args g) {
     for (int j = 0; j < 4; ++j) {
       const v4i lo = *reinterpret_cast<const v4i *>(w + (size_t)b * kTileBytes + j * 2048);
       const v4i hi = *reinterpret_cast<const v4i *>(w + (size_t)b * kTileBytes + j * 2048 + 1024);
-      wf[j] = Mma::of(lo, hi);
+      wf[j] = Mma::of(join(lo, hi));
     }
     const int we = g.w_exps[(size_t)b * g.nb + blockIdx.x / 2] + 127;
 #pragma unroll
@@ -155,7 +157,7 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_f8_direct(GemmF8Args g) {
       const int k = b * 128 + 16 * grp;
       if (k < g.k) lo = *reinterpret_cast<const v4i *>(a[i] + b * 128);
       if (k + 64 < g.k) hi = *reinterpret_cast<const v4i *>(a[i] + b * 128 + 64);
-      const typename Mma::frag af = Mma::of(lo, hi);
+      const typename Mma::frag af = Mma::of(join(lo, hi));
       const int e = ae[i][b] + 127;
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[i][j] = Mma::mma(wf[j], af, acc[i][j], we, e);
@@ -193,7 +195,7 @@ __device__ __forceinline__ void global_to_lds(const uint8_t *from, uint8_t *to) 
 }
 
 // Blocks of k whose exponents a workgroup keeps in LDS at a time.
-static constexpr int kExpSteps = 32;
+static constexpr int kExpSteps = 64;
 
 template <int BM, int BN>
 struct TileLds {
@@ -201,12 +203,36 @@ struct TileLds {
   uint8_t b[BN * 128];
 };
 
+// The workgroup's tile. Tiles lie in bands of kBand along m; the eight XCDs,
+// which take workgroups in turn, each get a contiguous range of them, whose
+// operands meet in their L2.
+template <int BM, int BN>
+__device__ __forceinline__ void tile_of(const GemmF8Args &g, int &m0, int &n0) {
+  constexpr int kBand = 4;
+  const int tn = (g.n + BN - 1) / BN, tm = (g.m + BM - 1) / BM, total = tm * tn;
+  int id = blockIdx.x;
+  const int per = total / 8, rem = total % 8, x = id % 8;
+  id = x * per + min(x, rem) + id / 8;
+  const int band = id / (kBand * tn), in = id - band * (kBand * tn);
+  const int high = min(kBand, tm - band * kBand);
+  m0 = (band * kBand + in % high) * BM;
+  n0 = in / high * BN;
+}
+
 // BM x BN outputs a workgroup, WM x WN wavefronts. A block of 128 of k at a
 // time goes from memory into one of two LDS stages (16 bytes a lane, straight
-// to LDS) while the other one is multiplied.
-//   rows: 128 bytes each, their 16-byte chunks at chunk ^ (row & 7), so that
-//         16 rows' reads of one chunk spread over the banks
+// to LDS):
+//   rows: 128 bytes each, their 16-byte chunks at chunk ^ (row / 2 & 7), so
+//         that 16 rows' reads of one chunk take each of the 64 banks once
 //   weights: as they are packed, in the order the lanes take them
+// A wavefront multiplies its FM row fragments one after another and reads them
+// two ahead. When it has read the last one it waits for its loads of the next
+// block, and a barrier tells it that everybody's are there and that nobody
+// reads this stage any more: the last two fragments' products then run beside
+// the reads of the next block's first fragments, and the stage is filled again
+// with the block after that. Loads are spread over four fragments' products,
+// because a wavefront that issues them all at once stands still until the
+// memory pipeline has taken them.
 // The exponents of kExpSteps blocks wait in LDS too: a load of theirs in the
 // loop would have to wait for the stage's loads in front of it.
 template <typename T, int BM, int BN, int WM, int WN>
@@ -214,26 +240,15 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm_f8_tile(GemmF8Args g) {
   typedef typename std::conditional<std::is_same<T, float>::value, Exact, Fast>::type Mma;
   constexpr int kWaves = WM * WN, TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
   constexpr int NB = (BN + 127) / 128;  // 128-column blocks of the tile
-  static_assert(TN <= 64 && 64 % TN == 0 && FM % 2 == 0, "a wavefront's columns share an exponent");
+  static_assert(TN <= 64 && 64 % TN == 0 && FM % 4 == 0, "a wavefront's columns share an exponent");
   __shared__ TileLds<BM, BN> stage0, stage1;
   __shared__ uint8_t a_exp[kExpSteps][WM][16][FM];
   __shared__ uint8_t w_exp[kExpSteps][NB];
 
   const int rows = g.m_dev ? min(g.m, *g.m_dev) : g.m;
-  // Tiles in bands of kBand along m; the eight XCDs, which take workgroups in
-  // turn, each get a contiguous range, whose operands meet in their L2.
-  constexpr int kBand = 4;
-  const int tn = (g.n + BN - 1) / BN, tm = (g.m + BM - 1) / BM, total = tm * tn;
-  int id = blockIdx.x;
-  if (total >= 16) {
-    const int per = total / 8, rem = total % 8, x = id % 8;
-    id = x * per + min(x, rem) + id / 8;
-  }
-  const int band = id / (kBand * tn), in = id - band * (kBand * tn);
-  const int high = min(kBand, tm - band * kBand);
-  const int m0 = (band * kBand + in % high) * BM, n0 = in / high * BN;
+  int m0, n0;
+  tile_of<BM, BN>(g, m0, n0);
   if (m0 >= rows) return;
-
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN, col = lane & 15, grp = lane >> 4;
 
@@ -243,82 +258,156 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm_f8_tile(GemmF8Args g) {
   const int last = rows - 1 - m0;  // of the tile's rows, those past it repeat it
   const uint8_t *a_base = g.a + (int64_t)m0 * g.lda;
   const int a_size = (int)(min(last, BM - 1) * g.lda + g.k);
-  const int chunk = (lane & 7) ^ ((lane >> 3) & 7);
+  static_assert(kWaves % 2 == 0, "a wavefront's units of 8 rows lie alike in 16");
+  const int chunk = (lane & 7) ^ (wave % 2 * 4 + (lane >> 4));
   int a_off[LA];
 #pragma unroll
   for (int i = 0; i < LA; ++i)
     a_off[i] = min((i * kWaves + wave) * 8 + (lane >> 3), last) * (int)g.lda + chunk * 16;
-  const uint8_t *w_at[LB];
-#pragma unroll
-  for (int i = 0; i < LB; ++i) {
-    const int kib = i * kWaves + wave;  // of the stage's BN / 8
-    const int group = min(n0 / 64 + kib / 8, (g.n - 1) / 64);
-    w_at[i] = g.w + (size_t)group * g.kb * kTileBytes + kib % 8 * 1024 + lane * 16;
-  }
-  auto load = [&](TileLds<BM, BN> &s, int b) {
+  // A quarter of block b's loads; past the last block it loads that again.
+  auto load = [&](TileLds<BM, BN> &s, int b, int quarter) {
+    b = min(b, g.kb - 1);
     // behind the last of k the buffer load gives zeros
     const bool past = b * 128 + chunk * 16 >= g.k;
 #pragma unroll
-    for (int i = 0; i < LA; ++i)
-      buffer_to_lds(a_base, a_size, past ? 0x7FFFFFF0 : a_off[i] + b * 128,
-                    s.a + (i * kWaves + wave) * 1024);
-#pragma unroll
-    for (int i = 0; i < LB; ++i)
-      global_to_lds(w_at[i] + (size_t)b * kTileBytes, s.b + (i * kWaves + wave) * 1024);
+    for (int i = 0; i < LA + LB; ++i) {
+      if (i * 4 / (LA + LB) != quarter) continue;
+      if (i < LA) {
+        buffer_to_lds(a_base, a_size, past ? 0x7FFFFFF0 : a_off[i] + b * 128,
+                      s.a + (i * kWaves + wave) * 1024);
+      } else {
+        const int kib = (i - LA) * kWaves + wave;  // of the stage's BN / 8
+        const int group = min(n0 / 64 + kib / 8, (g.n - 1) / 64);
+        buffer_to_lds(g.w + ((size_t)group * g.kb + b) * kTileBytes + kib % 8 * 1024, 1024,
+                      lane * 16, s.b + kib * 1024);
+      }
+    }
   };
 
   v4f acc[FM][FN] = {};
-  auto multiply = [&](const TileLds<BM, BN> &s, int e) {
-    typename Mma::frag wf[FN];
-    const uint8_t *wb = s.b + wn * TN / 64 * 8192 + wn * TN % 64 / 16 * 2048 + lane * 16;
+  v8i wf[2][FN], af[4];
+  int we[2], ae[2][(FM + 3) / 4] = {};
+  const int c0 = (grp ^ (col >> 1)) * 16;
+  auto read_a = [&](const TileLds<BM, BN> &s, int i) {
+    const uint8_t *p = s.a + (wm * TM + i * 16 + col) * 128;
+    af[i % 4] = join(*reinterpret_cast<const v4i *>(p + c0),
+                     *reinterpret_cast<const v4i *>(p + (c0 ^ 64)));
+  };
+  auto read_w = [&](const TileLds<BM, BN> &s, int p) {
+    const uint8_t *at = s.b + wn * TN / 64 * 8192 + wn * TN % 64 / 16 * 2048 + lane * 16;
 #pragma unroll
     for (int j = 0; j < FN; ++j)
-      wf[j] = Mma::of(*reinterpret_cast<const v4i *>(wb + j * 2048),
-                      *reinterpret_cast<const v4i *>(wb + j * 2048 + 1024));
-    const int we = w_exp[e][wn * TN / 128];
-    int ae[(FM + 3) / 4] = {};
-    __builtin_memcpy(ae, a_exp[e][wm][col], FM);
-    const uint8_t *ab = s.a + (wm * TM + col) * 128;
-    const int c0 = (grp ^ (col & 7)) * 16;
+      wf[p][j] = join(*reinterpret_cast<const v4i *>(at + j * 2048),
+                      *reinterpret_cast<const v4i *>(at + j * 2048 + 1024));
+  };
+  auto read_exps = [&](int b, int p) {
+    we[p] = w_exp[b % kExpSteps][wn * TN / 128];
+    __builtin_memcpy(ae[p], a_exp[b % kExpSteps][wm][col], FM);
+  };
+  // Exponents of blocks b0 .. b0 + kExpSteps - 1 as scale bytes: 16 blocks of
+  // a row at a time, at once unless that would end behind the last row's.
+  const int8_t *exp_end = g.a_exps + (int64_t)(rows - 1) * g.a_exps_ld + g.kb;
+  auto load_exps = [&](int b0, auto at_once) {
+    constexpr int kParts = kExpSteps / 16, kEach = BM * kParts / (64 * kWaves);
+    constexpr int kOnce = decltype(at_once)::value ? kEach : 1;
+    static_assert(kEach * 64 * kWaves == BM * kParts, "whole loads");
+#pragma unroll 1
+    for (int j0 = 0; j0 < kEach; j0 += kOnce) {
+      v4i v[kOnce];
+#pragma unroll
+      for (int j = 0; j < kOnce; ++j) {
+        const int i = (j0 + j) * 64 * kWaves + tid, b = b0 + i % kParts * 16;
+        const int8_t *from = g.a_exps + (int64_t)(m0 + min(i / kParts, last)) * g.a_exps_ld + b;
+        if (b + 16 <= g.kb || from + 16 <= exp_end) {
+          __builtin_memcpy(&v[j], from, 16);
+        } else {
+          v[j] = v4i{};
+#pragma unroll
+          for (int k = 0; k < 16; ++k)
+            if (b + k < g.kb) v[j][k / 4] |= (uint8_t)from[k] << (8 * (k % 4));
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kOnce; ++j) {
+        const int i = (j0 + j) * 64 * kWaves + tid, r = i / kParts, b = i % kParts * 16;
+#pragma unroll
+        for (int k = 0; k < 16; ++k)  // e + 127 = (e ^ 128) - 1, e >= -127
+          a_exp[b + k][r / TM][r % 16][r % TM / 16] =
+              (uint8_t)(((v[j][k / 4] ^ 0x80808080) - 0x01010101) >> (8 * (k % 4)));
+      }
+    }
+#pragma unroll 1
+    for (int i = tid; i < kExpSteps * NB; i += 64 * kWaves) {
+      const int b = min(b0 + i / NB, g.kb - 1), n = min(n0 / 128 + i % NB, g.nb - 1);
+      w_exp[i / NB][i % NB] = (uint8_t)(g.w_exps[(size_t)b * g.nb + n] + 127);
+    }
+  };
+  // This wavefront's reads and loads are done; then everybody's.
+  auto meet = [&]() {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0x0070);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // Block b from stage s, its fragments of W and its first two of the rows
+  // already read (into half p); the other stage takes block b + 1.
+  auto step = [&](int b, TileLds<BM, BN> &s, TileLds<BM, BN> &other, int p) {
+    typename Mma::frag w[FN];
+#pragma unroll
+    for (int j = 0; j < FN; ++j) w[j] = Mma::of(wf[p][j]);
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
-      const typename Mma::frag af = Mma::of(*reinterpret_cast<const v4i *>(ab + i * 2048 + c0),
-                                            *reinterpret_cast<const v4i *>(ab + i * 2048 + (c0 ^ 64)));
-      const int x = (unsigned)ae[i / 4] >> (8 * (i % 4));
+      if (i + 2 < FM) read_a(s, i + 2);
+      if (i < 2) load(other, b + 1, 2 + i);
+      if (i == FM - 2) {
+        meet();
+        read_a(other, 0);
+        read_w(other, 1 - p);
+      }
+      if (i == FM - 1) {
+        read_a(other, 1);
+        read_exps(b + 1, 1 - p);
+      }
+      if (i >= FM - 2) load(s, b + 2, i - (FM - 2));
+      __builtin_amdgcn_sched_barrier(0);
+      const typename Mma::frag a = Mma::of(af[i % 4]);
+      const int x = (unsigned)ae[p][i / 4] >> (8 * (i % 4));
 #pragma unroll
-      for (int j = 0; j < FN; ++j) acc[i][j] = Mma::mma(wf[j], af, acc[i][j], we, x);
+      for (int j = 0; j < FN; ++j) acc[i][j] = Mma::mma(w[j], a, acc[i][j], we[p], x);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
-  auto load_exps = [&](int b0) {
-    const int steps = min(kExpSteps, g.kb - b0);
-    for (int i = tid; i < BM * kExpSteps; i += 64 * kWaves) {
-      const int r = i / kExpSteps, b = i % kExpSteps;
-      if (b < steps)
-        a_exp[b][r / TM][r % 16][r % TM / 16] =
-            (uint8_t)(g.a_exps[(int64_t)(m0 + min(r, last)) * g.a_exps_ld + b0 + b] + 127);
-    }
-    for (int i = tid; i < kExpSteps * NB; i += 64 * kWaves) {
-      const int b = i / NB, n = min(n0 / 128 + i % NB, g.nb - 1);
-      if (b < steps) w_exp[b][i % NB] = (uint8_t)(g.w_exps[(size_t)(b0 + b) * g.nb + n] + 127);
-    }
+  auto next_exps = [&](int b) {
+    if (b == 0 || b % kExpSteps) return;
+    __syncthreads();
+    load_exps(b, std::false_type());  // few registers are free here
+    __syncthreads();
+    read_exps(b, 0);
   };
 
-  load(stage0, 0);
-  load_exps(0);
-  __syncthreads();
-  for (int b = 0; b < g.kb; b += 2) {
-    if (b && b % kExpSteps == 0) {
-      load_exps(b);
-      __syncthreads();
-    }
-    if (b + 1 < g.kb) load(stage1, b + 1);
-    multiply(stage0, b % kExpSteps);
-    __syncthreads();
-    if (b + 1 >= g.kb) break;
-    if (b + 2 < g.kb) load(stage0, b + 2);
-    multiply(stage1, (b + 1) % kExpSteps);
-    __syncthreads();
+#pragma unroll
+  for (int q = 0; q < 4; ++q) load(stage0, 0, q);
+  load_exps(0, std::true_type());
+  meet();
+  load(stage1, 1, 0);
+  load(stage1, 1, 1);
+  read_w(stage0, 0);
+  read_a(stage0, 0);
+  read_a(stage0, 1);
+  read_exps(0, 0);
+  int b = 0;
+  for (; b + 1 < g.kb; b += 2) {
+    next_exps(b);
+    step(b, stage0, stage1, 0);
+    step(b + 1, stage1, stage0, 1);
   }
+  if (b < g.kb) {
+    next_exps(b);
+    step(b, stage0, stage1, 0);
+  }
+  __builtin_amdgcn_s_waitcnt(0x0070);  // the loads behind the last block
 
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
@@ -342,12 +431,12 @@ static void tile_launch(const GemmF8Args &g, hipStream_t s) {
 
 template <typename T>
 static void gemm_f8_launch(const GemmF8Args &g, hipStream_t s) {
-  const char *e = getenv("HV_CFG");
-  const int cfg = e ? atoi(e) : 0;
-  if (cfg == 1) return tile_launch<T, 256, 256, 2, 4>(g, s);
-  if (cfg == 2) return tile_launch<T, 128, 128, 2, 2>(g, s);
-  if (cfg == 3) return tile_launch<T, 64, 64, 2, 2>(g, s);
-  if (cfg == 4) return tile_launch<T, 128, 256, 2, 4>(g, s);
+  // A tile's offsets into the rows are 32-bit.
+  const bool near = g.lda < (int64_t)1 << 22;
+  const int64_t tiles = (int64_t)((g.m + 255) / 256) * ((g.n + 255) / 256);
+  if (near && g.m >= 192 && tiles >= 192 && !std::is_same<T, float>::value)
+    return tile_launch<T, 256, 256, 2, 4>(g, s);
+  if (near && g.m >= 96) return tile_launch<T, 128, 128, 2, 2>(g, s);
   hv_launch(k_gemm_f8_direct<T, 4, 4>, dim3((g.n + 63) / 64, (g.m + 63) / 64), dim3(256), 0, s, g);
 }
 
