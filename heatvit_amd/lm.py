@@ -47,44 +47,57 @@ class LogProbs(NamedTuple):
 
 
 def _matrix(name, t, dtypes):
+    """(rows, columns, row stride) of a matrix with adjacent columns."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch tensor")
     if t.dtype not in dtypes:
         raise TypeError(f"{name} has type {t.dtype}")
     if t.dim() != 2:
         raise ValueError(f"{name} must be [rows][columns]")
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    rows, columns = t.shape
+    ld, step = t.stride()
+    if step != 1 and columns > 1:
         raise ValueError(f"{name} must have adjacent columns")
-    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+    if rows <= 1:
+        ld = columns
+    elif ld < columns:
         raise ValueError(f"the rows of {name} overlap")
-    return t
+    return rows, columns, ld
 
 
-def _given(name, t, shape, dtype, strided=False):
-    """A result or vector that the caller passes."""
+def _given(name, t, shape, dtype):
+    """A contiguous vector or result that the caller passes."""
     if not isinstance(t, torch.Tensor) or t.dtype != dtype:
         raise TypeError(f"{name} must be a tensor of {dtype}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} must have the shape {list(shape)}")
-    if strided:
-        _matrix(name, t, (dtype,))
-    elif not t.is_contiguous():
+    if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
-    return t
 
 
-def _ld(t):
-    """Row stride of a matrix; one that has a single row may have any."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+def _given_matrix(name, t, shape, dtype):
+    """Row stride of a matrix that the caller passes."""
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype:
+        raise TypeError(f"{name} must be a tensor of {dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must have the shape {list(shape)}")
+    return _matrix(name, t, (dtype,))[2]
 
 
-def _on(device, **tensors):
-    """All tensors on the one GPU `device`."""
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, not on {device}")
-    if device.type != "cuda":
-        raise ValueError("the inputs must be on a GPU")
+def _call(entry, what, index, tensors, *args):
+    """The library call on the current stream of GPU `index`, where all of the
+    tensors are.  (The stream's handle comes from the getter behind
+    torch.cuda.current_stream(), which takes 2.4 us to wrap it.)"""
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"{what}: tensors on cuda:{index} and on {t.device}")
+    if torch.cuda.current_device() == index:
+        rc = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        raise _lib.error(rc, what)
 
 
 def _live(live_rows):
@@ -99,22 +112,16 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _call(entry, what, device, *args):
-    """The library call, on the device's current stream."""
-    if torch.cuda.current_device() == device.index:
-        rc = entry(*args, torch.cuda.current_stream().cuda_stream)
-    else:
-        with torch.cuda.device(device):
-            rc = entry(*args, torch.cuda.current_stream().cuda_stream)
-    _lib.check(rc, what)
-
-
-def _workspace(workspace, size, device):
+def _workspace(workspace, size, like):
+    """(tensor, pointer, bytes)"""
     if workspace is None:
-        return torch.empty(size, dtype=torch.uint8, device=device) if size else None
-    if workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.numel() < size:
+        if not size:
+            return None, None, 0
+        workspace = like.new_empty(size, dtype=torch.uint8)
+    elif workspace.dtype != torch.uint8 or not workspace.is_contiguous() or \
+            workspace.numel() < size:
         raise ValueError(f"workspace must be {size} contiguous bytes (uint8)")
-    return workspace
+    return workspace, workspace.data_ptr(), workspace.numel()
 
 
 def rms_norm_q8(x, weight, *, residual=None, eps=1e-6, fmt="e4m3", block=F8_BLOCK,
@@ -127,44 +134,45 @@ def rms_norm_q8(x, weight, *, residual=None, eps=1e-6, fmt="e4m3", block=F8_BLOC
     bfloat16); fmt "e4m3" or "int8"; block 128 columns, or 0 for one exponent
     a row.  `out`: the Q8Rows to write; its residual may be `residual` or `x`
     itself.  Returns Q8Rows(q, exps, scale, residual)."""
-    _matrix("x", x, _TYPES)
+    rows, width, x_ld = _matrix("x", x, _TYPES)
     if fmt not in _FORMATS:
         raise ValueError("fmt must be 'e4m3' or 'int8'")
-    if block not in (0, F8_BLOCK):
+    if block != 0 and block != F8_BLOCK:
         raise ValueError("block must be 128, or 0 for one exponent a row")
-    rows, width = x.shape
     if not width:
         raise ValueError("x has no columns")
     form, q_type = _FORMATS[fmt]
     blocks = -(-width // F8_BLOCK) if block else 1
-    _given("weight", weight, (width,), x.dtype)
+    dtype = x.dtype
+    _given("weight", weight, (width,), dtype)
+    residual_ld = kept_ld = 0
     if residual is not None:
-        _matrix("residual", residual, (x.dtype,))
-        if residual.shape != x.shape:
-            raise ValueError("residual must have the shape of x")
+        residual_ld = _given_matrix("residual", residual, x.shape, dtype)
     if out is None:
-        out = Q8Rows(torch.empty((rows, width), dtype=q_type, device=x.device),
-                     torch.empty((rows, blocks), dtype=torch.int8, device=x.device),
-                     torch.empty(rows, dtype=torch.float32, device=x.device),
-                     None if residual is None else
-                     torch.empty((rows, width), dtype=x.dtype, device=x.device))
-    else:
-        _given("out.q", out.q, (rows, width), q_type, strided=True)
-        _given("out.exps", out.exps, (rows, blocks), torch.int8, strided=True)
-        _given("out.scale", out.scale, (rows,), torch.float32)
-        if (residual is None) != (out.residual is None):
-            raise ValueError("out.residual goes with residual")
+        q = torch.empty_like(x, dtype=q_type, memory_format=torch.contiguous_format)
+        exps = x.new_empty((rows, blocks), dtype=torch.int8)
+        scale = x.new_empty(rows, dtype=torch.float32)
+        kept, q_ld, exps_ld, kept_ld = None, width, blocks, width
         if residual is not None:
-            _given("out.residual", out.residual, (rows, width), x.dtype, strided=True)
-    q, exps, scale, kept = out
-    _on(x.device, weight=weight, residual=residual, q=q, exps=exps, scale=scale, kept=kept,
-        live_rows=live_rows)
+            kept = torch.empty_like(x, memory_format=torch.contiguous_format)
+        out = Q8Rows(q, exps, scale, kept)
+    else:
+        q, exps, scale, kept = out
+        q_ld = _given_matrix("out.q", q, x.shape, q_type)
+        exps_ld = _given_matrix("out.exps", exps, (rows, blocks), torch.int8)
+        _given("out.scale", scale, (rows,), torch.float32)
+        if (residual is None) != (kept is None):
+            raise ValueError("out.residual goes with residual")
+        if kept is not None:
+            kept_ld = _given_matrix("out.residual", kept, x.shape, dtype)
     d = _lib.RmsNormDesc(
         x.data_ptr(), _ptr(residual), weight.data_ptr(), _ptr(kept), q.data_ptr(),
-        exps.data_ptr(), scale.data_ptr(), _live(live_rows), _ld(x),
-        0 if residual is None else _ld(residual), 0 if kept is None else _ld(kept), _ld(q),
-        _ld(exps), rows, width, _TYPES[x.dtype], form, block, eps)
-    _call(_lib.lib().hv_rms_norm_q8, "rms_norm_q8", x.device, d)
+        exps.data_ptr(), scale.data_ptr(), _live(live_rows), x_ld, residual_ld, kept_ld, q_ld,
+        exps_ld, rows, width, _TYPES[dtype], form, block, eps)
+    if not x.is_cuda:
+        raise ValueError("the inputs must be on a GPU")
+    _call(_lib.lib().hv_rms_norm_q8, "rms_norm_q8", x.get_device(),
+          (weight, residual, q, exps, scale, kept, live_rows), d)
     return out
 
 
@@ -181,33 +189,32 @@ def gemm_f8(a, a_exps, w, *, row_scale=None, bias=None, out_dtype=torch.bfloat16
     Returns [M][N] (`out` if given)."""
     if not isinstance(w, DeviceF8Weight):
         raise TypeError("w must be a DeviceF8Weight")
-    _matrix("a", a, (torch.float8_e4m3fn,))
-    _matrix("a_exps", a_exps, (torch.int8,))
-    rows, inner = a.shape
+    rows, inner, lda = _matrix("a", a, (torch.float8_e4m3fn,))
+    width = w.width
     if inner != w.inner:
         raise ValueError(f"K mismatch: a has {inner}, w has {w.inner}")
-    if tuple(a_exps.shape) != (rows, -(-inner // F8_BLOCK)):
-        raise ValueError("a_exps must be [M][ceil(K/128)]")
+    exps_ld = _given_matrix("a_exps", a_exps, (rows, -(-inner // F8_BLOCK)), torch.int8)
     if out_dtype not in _TYPES:
         raise TypeError(f"out_dtype {out_dtype} is not float32, float16 or bfloat16")
     if row_scale is not None:
         _given("row_scale", row_scale, (rows,), torch.float32)
     if bias is not None:
-        _given("bias", bias, (w.width,), torch.float32)
+        _given("bias", bias, (width,), torch.float32)
     if out is None:
-        out = torch.empty((rows, w.width), dtype=out_dtype, device=a.device)
+        out, ldc = a.new_empty((rows, width), dtype=out_dtype), width
     else:
-        _given("out", out, (rows, w.width), out_dtype, strided=True)
-    _on(a.device, a_exps=a_exps, w=w, row_scale=row_scale, bias=bias, out=out,
-        live_rows=live_rows, workspace=workspace)
+        ldc = _given_matrix("out", out, (rows, width), out_dtype)
+    if not a.is_cuda:
+        raise ValueError("the inputs must be on a GPU")
     L = _lib.lib()
-    workspace = _workspace(workspace, L.hv_gemm_f8_workspace_bytes(rows, w.width, inner), a.device)
+    workspace, ws_at, ws_size = _workspace(
+        workspace, L.hv_gemm_f8_workspace_bytes(rows, width, inner), a)
     d = _lib.GemmF8Desc(
         a.data_ptr(), a_exps.data_ptr(), w.packed.data_ptr(), w.exps.data_ptr(), _ptr(row_scale),
-        _ptr(bias), out.data_ptr(), _live(live_rows), _ld(a) if rows > 1 else -(-inner // 16) * 16,
-        _ld(a_exps), _ld(out), rows, w.width, inner, _TYPES[out_dtype])
-    _call(L.hv_gemm_f8, "gemm_f8", a.device, d, _ptr(workspace),
-          0 if workspace is None else workspace.numel())
+        _ptr(bias), out.data_ptr(), _live(live_rows), lda, exps_ld, ldc, rows, width, inner,
+        _TYPES[out_dtype])
+    _call(L.hv_gemm_f8, "gemm_f8", a.get_device(),
+          (a_exps, w.packed, row_scale, bias, out, live_rows, workspace), d, ws_at, ws_size)
     return out
 
 
@@ -222,14 +229,12 @@ def log_probs(logits, tokens=None, *, scale_exp=0, temperature=1.0, top=0, live_
     logits by the lower index.  Logits of -inf have probability 0; a NaN or
     +inf makes its row's log probabilities and entropy NaN.
     Returns LogProbs(logp, entropy, top_logp, top_index) (`out` if given)."""
-    _matrix("logits", logits, _LOGIT_TYPES)
-    rows, width = logits.shape
+    rows, width, ld = _matrix("logits", logits, _LOGIT_TYPES)
     if not width:
         raise ValueError("logits has no columns")
-    top = int(top)
     if not 0 <= top <= min(_lib.HV_LOG_PROBS_MAX_TOP, width):
         raise ValueError(f"top {top} outside [0, {_lib.HV_LOG_PROBS_MAX_TOP}] or over the width")
-    if not (temperature > 0 and math.isfinite(temperature)):
+    if not 0 < temperature < math.inf:
         raise ValueError("temperature must be positive and finite")
     scale = math.ldexp(1.0, scale_exp) / temperature
     count = 0
@@ -239,32 +244,36 @@ def log_probs(logits, tokens=None, *, scale_exp=0, temperature=1.0, top=0, live_
         if tokens.dim() not in (1, 2) or tokens.shape[0] != rows or not tokens.is_contiguous():
             raise ValueError("tokens must be contiguous, [R] or [R][G]")
         count = 1 if tokens.dim() == 1 else tokens.shape[1]
-    f32 = dict(dtype=torch.float32, device=logits.device)
     if out is None:
-        out = LogProbs(None if tokens is None else torch.empty(tokens.shape, **f32),
-                       torch.empty(rows, **f32),
-                       torch.empty((rows, top), **f32) if top else None,
-                       torch.empty((rows, top), dtype=torch.int32, device=logits.device)
-                       if top else None)
+        logp = top_logp = top_index = None
+        f32 = torch.float32
+        if tokens is not None:
+            logp = torch.empty_like(tokens, dtype=f32, memory_format=torch.contiguous_format)
+        entropy = logits.new_empty(rows, dtype=f32)
+        if top:
+            top_logp = logits.new_empty((rows, top), dtype=f32)
+            top_index = logits.new_empty((rows, top), dtype=torch.int32)
+        out = LogProbs(logp, entropy, top_logp, top_index)
     else:
-        if (tokens is None) != (out.logp is None) or bool(top) != (out.top_logp is not None) or \
-                bool(top) != (out.top_index is not None):
+        logp, entropy, top_logp, top_index = out
+        if (tokens is None) != (logp is None) or bool(top) != (top_logp is not None) or \
+                bool(top) != (top_index is not None):
             raise ValueError("out.logp goes with tokens, out.top_logp and out.top_index with top")
         if tokens is not None:
-            _given("out.logp", out.logp, tuple(tokens.shape), torch.float32)
-        _given("out.entropy", out.entropy, (rows,), torch.float32)
+            _given("out.logp", logp, tokens.shape, torch.float32)
+        _given("out.entropy", entropy, (rows,), torch.float32)
         if top:
-            _given("out.top_logp", out.top_logp, (rows, top), torch.float32)
-            _given("out.top_index", out.top_index, (rows, top), torch.int32)
-    _on(logits.device, tokens=tokens, logp=out.logp, entropy=out.entropy, top_logp=out.top_logp,
-        top_index=out.top_index, live_rows=live_rows, workspace=workspace)
+            _given("out.top_logp", top_logp, (rows, top), torch.float32)
+            _given("out.top_index", top_index, (rows, top), torch.int32)
+    if not logits.is_cuda:
+        raise ValueError("the inputs must be on a GPU")
     L = _lib.lib()
-    workspace = _workspace(workspace, L.hv_log_probs_workspace_bytes(rows, width, top),
-                           logits.device)
+    workspace, ws_at, ws_size = _workspace(
+        workspace, L.hv_log_probs_workspace_bytes(rows, width, top), logits)
     d = _lib.LogProbsDesc(
-        logits.data_ptr(), _ptr(tokens), _ptr(out.logp), out.entropy.data_ptr(),
-        _ptr(out.top_logp), _ptr(out.top_index), _live(live_rows), _ld(logits), count, rows,
-        width, _LOGIT_TYPES[logits.dtype], count, top, scale)
-    _call(L.hv_log_probs, "log_probs", logits.device, d, _ptr(workspace),
-          0 if workspace is None else workspace.numel())
+        logits.data_ptr(), _ptr(tokens), _ptr(logp), entropy.data_ptr(), _ptr(top_logp),
+        _ptr(top_index), _live(live_rows), ld, count, rows, width, _LOGIT_TYPES[logits.dtype],
+        count, top, scale)
+    _call(L.hv_log_probs, "log_probs", logits.get_device(),
+          (tokens, logp, entropy, top_logp, top_index, live_rows, workspace), d, ws_at, ws_size)
     return out
