@@ -33,7 +33,6 @@ struct GemmF8Args {
   int64_t lda, a_exps_ld, ldc;
   int m, n, k;
   int kb, nb;  // blocks of 128 along k and n
-  int vec;     // outputs stored at once: 2: 16 bytes, 1: four, 0: one
 };
 
 static constexpr int kTileBytes = 64 * 128;  // 64 channels by 128 k, packed
@@ -81,102 +80,135 @@ __device__ __forceinline__ v8i join(v4i lo, v4i hi) {
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// CNT (a multiple of 4) adjacent channels n .. of row m.
-template <typename T, int CNT>
-__device__ __forceinline__ void store_run(const GemmF8Args &g, int m, int n, float *v, float scale) {
+// RUN adjacent channels of row m from n on. A row may start at any element:
+// wide stores need no more alignment than that.
+template <typename T, int RUN>
+__device__ __forceinline__ void store_run(const GemmF8Args &g, int m, int n, const float *v) {
   T *p = (T *)g.c + m * g.ldc + n;
+  if (n + RUN <= g.n) {
+    typedef T vt __attribute__((ext_vector_type(RUN)));
+    vt t;
 #pragma unroll
-  for (int i = 0; i < CNT; ++i) {
-    v[i] *= scale;
-    if (g.bias && n + i < g.n) v[i] += g.bias[n + i];
-  }
-  constexpr int kWide = 16 / sizeof(T);
-  if (CNT % kWide == 0 && g.vec == 2 && n + CNT <= g.n) {
-    typedef T vt __attribute__((ext_vector_type(kWide)));
-#pragma unroll
-    for (int i = 0; i < CNT; i += kWide) {
-      vt t;
-#pragma unroll
-      for (int j = 0; j < kWide; ++j) t[j] = (T)v[i + j];
-      *reinterpret_cast<vt *>(p + i) = t;
-    }
-  } else if (g.vec) {
-    typedef T v4 __attribute__((ext_vector_type(4)));
-#pragma unroll
-    for (int i = 0; i < CNT; i += 4) {
-      if (n + i + 4 <= g.n) {
-        *reinterpret_cast<v4 *>(p + i) = v4{(T)v[i], (T)v[i + 1], (T)v[i + 2], (T)v[i + 3]};
-      } else {
-#pragma unroll
-        for (int j = i; j < i + 4; ++j)
-          if (n + j < g.n) p[j] = (T)v[j];
-      }
-    }
+    for (int i = 0; i < RUN; ++i) t[i] = (T)v[i];
+    __builtin_memcpy(p, &t, sizeof t);
   } else {
 #pragma unroll
-    for (int i = 0; i < CNT; ++i)
+    for (int i = 0; i < RUN; ++i)
       if (n + i < g.n) p[i] = (T)v[i];
   }
 }
 
-// One wavefront's part of FM x 16 rows by 64 channels; the NW wavefronts of a
-// workgroup take every NW-th block of k and add up through LDS. Fragments come
-// straight from memory: the packed weights are in the order the lanes take
-// them.
-template <typename T, int FM, int NW>
-__global__ __launch_bounds__(64 * NW) void k_gemm_f8_direct(GemmF8Args g) {
+// Channel of a group of 64 at which lane group grp's four of part j start: with
+// parts 2 J and 2 J + 1 a lane has eight adjacent channels.
+__device__ __forceinline__ int channel_of(int j, int grp) {
+  return j / 2 * 32 + grp * 8 + j % 2 * 4;
+}
+
+// One lane's outputs of FM x FN fragments: rows m0 + 16 i, parts j0 .. of the
+// group of 64 at n0.
+template <typename T, int FM, int FN>
+__device__ __forceinline__ void store_tile(const GemmF8Args &g, int rows, int m0, int n0, int j0,
+                                           int grp, const v4f (&acc)[FM][FN]) {
+  constexpr int RUN = FN >= 2 ? 8 : 4;
+  float bias[FN][4] = {}, scale[FM];
+  if (g.bias) {
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        bias[j][k] = g.bias[min(n0 + channel_of(j0 + j, grp) + k, g.n - 1)];
+  }
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+    scale[i] = g.row_scale ? g.row_scale[min(m0 + 16 * i, rows - 1)] : 1.f;
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    const int m = m0 + 16 * i;
+    if (m >= rows) continue;
+#pragma unroll
+    for (int j = 0; j < FN; j += RUN / 4) {
+      float v[RUN];
+#pragma unroll
+      for (int k = 0; k < RUN; ++k)
+        v[k] = __builtin_fmaf(acc[i][j + k / 4][k % 4], scale[i], bias[j + k / 4][k % 4]);
+      store_run<T, RUN>(g, m, n0 + channel_of(j0 + j, grp), v);
+    }
+  }
+}
+
+// Few rows: a workgroup takes FM x 16 rows by J parts of 16 channels of a
+// group of 64, its NW wavefronts every NW-th block of k each, and adds their
+// sums up through LDS in a fixed order. Fragments come straight from memory:
+// the packed weights are in the order the lanes take them, each read once.
+template <typename T, int FM, int J, int NW>
+__global__ __launch_bounds__(64 * NW) void k_gemm_f8_rows(GemmF8Args g) {
   typedef typename std::conditional<std::is_same<T, float>::value, Exact, Fast>::type Mma;
   const int rows = g.m_dev ? min(g.m, *g.m_dev) : g.m;
   const int m0 = blockIdx.y * (16 * FM);
   if (m0 >= rows) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, grp = lane >> 4;
-  const uint8_t *w = g.w + (size_t)blockIdx.x * g.kb * kTileBytes + lane * 16;
+  const int group = blockIdx.x / (4 / J), j0 = blockIdx.x % (4 / J) * J;
+  const uint8_t *w = g.w + (size_t)group * g.kb * kTileBytes + j0 * 2048 + lane * 16;
   const uint8_t *a[FM];
   const int8_t *ae[FM];
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
     const int64_t m = min(m0 + 16 * i + col, rows - 1);  // rows past the end repeat the last
-    a[i] = g.a + m * g.lda + 16 * grp;
+    a[i] = g.a + m * g.lda;
     ae[i] = g.a_exps + m * g.a_exps_ld;
   }
-  v4f acc[FM][4] = {};
-  for (int b = wave; b < g.kb; b += NW) {
-    typename Mma::frag wf[4];
+  // The loads of U blocks are on their way before the first is waited for.
+  constexpr int U = FM * J >= 8 ? 1 : FM * J >= 4 ? 2 : 4;
+  v4f acc[FM][J] = {};
+  for (int b0 = wave; b0 < g.kb; b0 += U * NW) {
+    v8i wf[U][J], af[U][FM];
+    int we[U], e[U][FM];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const v4i lo = *reinterpret_cast<const v4i *>(w + (size_t)b * kTileBytes + j * 2048);
-      const v4i hi = *reinterpret_cast<const v4i *>(w + (size_t)b * kTileBytes + j * 2048 + 1024);
-      wf[j] = Mma::of(join(lo, hi));
-    }
-    const int we = g.w_exps[(size_t)b * g.nb + blockIdx.x / 2] + 127;
+    for (int u = 0; u < U; ++u) {
+      const int b = min(b0 + u * NW, g.kb - 1);
 #pragma unroll
-    for (int i = 0; i < FM; ++i) {
-      // past the end of k: zeros
-      v4i lo = {}, hi = {};
+      for (int j = 0; j < J; ++j)
+        wf[u][j] = join(
+            *reinterpret_cast<const v4i *>(w + (size_t)b * kTileBytes + j * 2048),
+            *reinterpret_cast<const v4i *>(w + (size_t)b * kTileBytes + j * 2048 + 1024));
+      we[u] = g.w_exps[(size_t)b * g.nb + group / 2] + 127;
       const int k = b * 128 + 16 * grp;
-      if (k < g.k) lo = *reinterpret_cast<const v4i *>(a[i] + b * 128);
-      if (k + 64 < g.k) hi = *reinterpret_cast<const v4i *>(a[i] + b * 128 + 64);
-      const typename Mma::frag af = Mma::of(join(lo, hi));
-      const int e = ae[i][b] + 127;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = Mma::mma(wf[j], af, acc[i][j], we, e);
+      for (int i = 0; i < FM; ++i) {
+        // zeros past the end of k, and for a block past the last
+        const bool lo = b0 + u * NW < g.kb && k < g.k, hi = b0 + u * NW < g.kb && k + 64 < g.k;
+        v4i x = *reinterpret_cast<const v4i *>(a[i] + (lo ? k : 0));
+        v4i y = *reinterpret_cast<const v4i *>(a[i] + (hi ? k + 64 : 0));
+        af[u][i] = join(lo ? x : v4i{}, hi ? y : v4i{});
+        e[u][i] = ae[i][b] + 127;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      typename Mma::frag wo[J];
+#pragma unroll
+      for (int j = 0; j < J; ++j) wo[j] = Mma::of(wf[u][j]);
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        const typename Mma::frag ao = Mma::of(af[u][i]);
+#pragma unroll
+        for (int j = 0; j < J; ++j) acc[i][j] = Mma::mma(wo[j], ao, acc[i][j], we[u], e[u][i]);
+      }
     }
   }
-  __shared__ v4f part[NW][FM * 4][64];
+  __shared__ v4f part[NW][FM * J][64];
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) part[wave][i * 4 + j][lane] = acc[i][j];
+    for (int j = 0; j < J; ++j) part[wave][i * J + j][lane] = acc[i][j];
   __syncthreads();
-  for (int f = wave; f < FM * 4; f += NW) {
+  for (int f = wave; f < FM * J; f += NW) {
     v4f v = part[0][f][lane];
 #pragma unroll
     for (int k = 1; k < NW; ++k) v += part[k][f][lane];
-    const int m = m0 + 16 * (f / 4) + col;
-    const int n = blockIdx.x * 64 + 16 * grp + 4 * (f % 4);
-    float r[4] = {v[0], v[1], v[2], v[3]};
-    if (m < rows) store_run<T, 4>(g, m, n, r, g.row_scale ? g.row_scale[m] : 1.f);
+    const v4f one[1][1] = {{v}};
+    store_tile<T>(g, rows, m0 + 16 * (f / J) + col, group * 64, j0 + f % J, grp, one);
   }
 }
 
@@ -409,18 +441,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm_f8_tile(GemmF8Args g) {
   }
   __builtin_amdgcn_s_waitcnt(0x0070);  // the loads behind the last block
 
-#pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    const int m = m0 + wm * TM + 16 * i + col;
-    const int n = n0 + wn * TN / 64 * 64 + 16 * grp + wn * TN % 64 / 4;
-    float v[4 * FN];
-#pragma unroll
-    for (int j = 0; j < FN; ++j)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[4 * j + k] = acc[i][j][k];
-    if (m < rows && n < g.n)
-      store_run<T, 4 * FN>(g, m, n, v, g.row_scale ? g.row_scale[m] : 1.f);
-  }
+  store_tile<T>(g, rows, m0 + wm * TM + col, n0 + wn * TN / 64 * 64, wn * TN % 64 / 16, grp, acc);
 }
 
 template <typename T, int BM, int BN, int WM, int WN>
@@ -429,15 +450,47 @@ static void tile_launch(const GemmF8Args &g, hipStream_t s) {
   hv_launch(k_gemm_f8_tile<T, BM, BN, WM, WN>, dim3(tiles), dim3(64 * WM * WN), 0, s, g);
 }
 
+template <typename T, int FM, int J, int NW>
+static void rows_launch(const GemmF8Args &g, hipStream_t s) {
+  const dim3 grid((g.n + 63) / 64 * (4 / J), (g.m + 16 * FM - 1) / (16 * FM));
+  hv_launch(k_gemm_f8_rows<T, FM, J, NW>, grid, dim3(64 * NW), 0, s, g);
+}
+
 template <typename T>
 static void gemm_f8_launch(const GemmF8Args &g, hipStream_t s) {
+#ifdef HV_DEV
+  const char *e = getenv("HV_CFG");
+  switch (e ? atoi(e) : 0) {
+    case 1: return tile_launch<T, 256, 256, 2, 4>(g, s);
+    case 2: return tile_launch<T, 128, 128, 2, 2>(g, s);
+    case 3: return tile_launch<T, 64, 64, 1, 4>(g, s);
+    case 4: return tile_launch<T, 128, 256, 2, 4>(g, s);
+    case 5: return tile_launch<T, 64, 128, 1, 4>(g, s);
+    case 6: return tile_launch<T, 64, 256, 1, 4>(g, s);
+    case 7: return tile_launch<T, 256, 128, 4, 2>(g, s);
+    case 11: return rows_launch<T, 1, 1, 16>(g, s);
+    case 12: return rows_launch<T, 1, 1, 8>(g, s);
+    case 13: return rows_launch<T, 1, 2, 8>(g, s);
+    case 14: return rows_launch<T, 1, 4, 8>(g, s);
+    case 21: return rows_launch<T, 2, 1, 16>(g, s);
+    case 22: return rows_launch<T, 2, 1, 8>(g, s);
+    case 23: return rows_launch<T, 2, 2, 8>(g, s);
+    case 24: return rows_launch<T, 2, 4, 8>(g, s);
+    case 41: return rows_launch<T, 4, 1, 16>(g, s);
+    case 42: return rows_launch<T, 4, 1, 8>(g, s);
+    case 43: return rows_launch<T, 4, 2, 8>(g, s);
+    case 44: return rows_launch<T, 4, 4, 4>(g, s);
+    case 45: return rows_launch<T, 4, 2, 4>(g, s);
+    case 46: return rows_launch<T, 4, 1, 4>(g, s);
+  }
+#endif
   // A tile's offsets into the rows are 32-bit.
   const bool near = g.lda < (int64_t)1 << 22;
   const int64_t tiles = (int64_t)((g.m + 255) / 256) * ((g.n + 255) / 256);
   if (near && g.m >= 192 && tiles >= 192 && !std::is_same<T, float>::value)
     return tile_launch<T, 256, 256, 2, 4>(g, s);
   if (near && g.m >= 96) return tile_launch<T, 128, 128, 2, 2>(g, s);
-  hv_launch(k_gemm_f8_direct<T, 4, 4>, dim3((g.n + 63) / 64, (g.m + 63) / 64), dim3(256), 0, s, g);
+  rows_launch<T, 4, 4, 4>(g, s);
 }
 
 }  // namespace hv
@@ -481,8 +534,6 @@ int hv_gemm_f8(const hv_gemm_f8_desc *d, void *workspace, size_t workspace_bytes
   g.row_scale = d->row_scale; g.bias = d->bias; g.c = d->c; g.m_dev = d->m_dev;
   g.lda = d->lda; g.a_exps_ld = d->a_exps_ld; g.ldc = d->ldc;
   g.m = d->m; g.n = d->n; g.k = d->k;
-  const uintptr_t c_at = (uintptr_t)d->c | (uintptr_t)(d->ldc * size);
-  g.vec = !(c_at & 15) ? 2 : !(c_at & (4 * size - 1));
   const hipStream_t s = (hipStream_t)stream;
   if (d->type == HV_T_F32) gemm_f8_launch<float>(g, s);
   else if (d->type == HV_T_F16) gemm_f8_launch<f16>(g, s);

@@ -194,15 +194,15 @@ def quantise_f8_weight(w):
 def pack_f8x64(w):
     """Pack an e4m3 matrix W[K][N] into the f8x64 layout of
     include/heatvit_hip.h: [N64/64][K128/128][4 j][2 h][64 lanes][16 bytes],
-    element (k, n) at tile (n // 64, k // 128), j = n % 16 // 4,
-    h = k % 128 // 64, lane 4 * (n % 64 // 16) + n % 4 + 16 * (k % 64 // 16),
+    element (k, n) at tile (n // 64, k // 128), j = n % 64 // 32 * 2 + n % 8 // 4,
+    h = k % 128 // 64, lane 4 * (n % 32 // 8) + n % 4 + 16 * (k % 64 // 16),
     byte k % 16, zero-padded."""
     k, n = w.shape
     kb, ng = -(-k // F8_BLOCK), -(-n // 64)
     p = torch.zeros((kb * F8_BLOCK, ng * 64), dtype=torch.uint8, device=w.device)
     p[:k, :n] = w.view(torch.uint8)
-    # k = (block, h, lane / 16, byte), n = (group, lane / 4 % 4, j, lane % 4)
-    p = p.view(kb, 2, 4, 16, ng, 4, 4, 4).permute(4, 0, 6, 1, 2, 5, 7, 3)
+    # k = (block, h, lane / 16, byte), n = (group, j / 2, lane / 4 % 4, j % 2, lane % 4)
+    p = p.view(kb, 2, 4, 16, ng, 2, 4, 2, 4).permute(4, 0, 5, 7, 1, 2, 6, 8, 3)
     return p.reshape(-1)
 
 

@@ -453,10 +453,10 @@ int hv_rms_norm_q8(const hv_rms_norm_desc *d, hv_stream_t stream);
  * [ceil(k/128)][ceil(n/128)].  Packed weights ("f8x64"): w[K][N] padded with
  * zeros to K128 = ceil(K/128)*128 by N64 = ceil(N/64)*64 and stored as
  * [N64/64][K128/128][4][2][64][16] bytes: element (k, n) lies at tile
- * (n/64, k/128), part j = (n%16)/4, half h = (k%128)/64, lane
- * 4*((n%64)/16) + n%4 + 16*((k%64)/16), byte k%16, so each of the four parts
- * is the first operand of one 16x16x128 MFMA, and result lane l holds
- * channels 16*(l/16) .. +15 of a row in parts of four.
+ * (n/64, k/128), part j = 2*((n%64)/32) + (n%8)/4, half h = (k%128)/64, lane
+ * 4*((n%32)/8) + n%4 + 16*((k%64)/16), byte k%16, so each of the four parts is
+ * the first operand of one 16x16x128 MFMA, and result lane l holds channels
+ * 8*(l/16) .. +7 and 32 + 8*(l/16) .. +7 of a row.
  * k and lda are multiples of 16, a and w_packed 16-byte aligned.  row_scale
  * [m] and bias [n] are optional.  m_dev (optional, device): the live row
  * count; rows behind it are left as they were. */

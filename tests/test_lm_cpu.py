@@ -29,8 +29,9 @@ def test_f8x64_layout(size):
     want = np.zeros(ng * kb * 8192, np.uint8)
     for kk in range(k):
         for nn in range(n):
-            lane = 4 * (nn % 64 // 16) + nn % 4 + 16 * (kk % 64 // 16)
-            at = ((nn // 64) * kb + kk // 128) * 8192 + (nn % 16 // 4) * 2048 + \
+            lane = 4 * (nn % 32 // 8) + nn % 4 + 16 * (kk % 64 // 16)
+            part = nn % 64 // 32 * 2 + nn % 8 // 4
+            at = ((nn // 64) * kb + kk // 128) * 8192 + part * 2048 + \
                 (kk % 128 // 64) * 1024 + lane * 16 + kk % 16
             want[at] = raw[kk, nn]
     assert np.array_equal(pack_f8x64(w).numpy(), want)
