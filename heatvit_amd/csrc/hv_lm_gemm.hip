@@ -158,15 +158,16 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_f8_rows(GemmF8Args g) {
     a[i] = g.a + m * g.lda;
     ae[i] = g.a_exps + m * g.a_exps_ld;
   }
-  // The loads of U blocks are on their way before the first is waited for.
-  constexpr int U = FM * J >= 8 ? 1 : FM * J >= 4 ? 2 : 4;
   v4f acc[FM][J] = {};
-  for (int b0 = wave; b0 < g.kb; b0 += U * NW) {
+  // Blocks b0, b0 + NW, ..: the loads of all U are on their way before the
+  // first is waited for.
+  auto blocks = [&](int b0, auto n_blocks) {
+    constexpr int U = decltype(n_blocks)::value;
     v8i wf[U][J], af[U][FM];
     int we[U], e[U][FM];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int b = min(b0 + u * NW, g.kb - 1);
+      const int b = b0 + u * NW;
 #pragma unroll
       for (int j = 0; j < J; ++j)
         wf[u][j] = join(
@@ -174,12 +175,11 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_f8_rows(GemmF8Args g) {
             *reinterpret_cast<const v4i *>(w + (size_t)b * kTileBytes + j * 2048 + 1024));
       we[u] = g.w_exps[(size_t)b * g.nb + group / 2] + 127;
       const int k = b * 128 + 16 * grp;
+      const bool lo = k < g.k, hi = k + 64 < g.k;  // zeros past the end of k
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
-        // zeros past the end of k, and for a block past the last
-        const bool lo = b0 + u * NW < g.kb && k < g.k, hi = b0 + u * NW < g.kb && k + 64 < g.k;
-        v4i x = *reinterpret_cast<const v4i *>(a[i] + (lo ? k : 0));
-        v4i y = *reinterpret_cast<const v4i *>(a[i] + (hi ? k + 64 : 0));
+        const v4i x = *reinterpret_cast<const v4i *>(a[i] + (lo ? k : 0));
+        const v4i y = *reinterpret_cast<const v4i *>(a[i] + (hi ? k + 64 : 0));
         af[u][i] = join(lo ? x : v4i{}, hi ? y : v4i{});
         e[u][i] = ae[i][b] + 127;
       }
@@ -196,7 +196,11 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_f8_rows(GemmF8Args g) {
         for (int j = 0; j < J; ++j) acc[i][j] = Mma::mma(wo[j], ao, acc[i][j], we[u], e[u][i]);
       }
     }
-  }
+  };
+  constexpr int U = FM * J >= 4 ? 2 : 4;
+  int b = wave;
+  for (; b + (U - 1) * NW < g.kb; b += U * NW) blocks(b, std::integral_constant<int, U>());
+  for (; b < g.kb; b += NW) blocks(b, std::integral_constant<int, 1>());
   __shared__ v4f part[NW][FM * J][64];
 #pragma unroll
   for (int i = 0; i < FM; ++i)
@@ -213,17 +217,14 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_f8_rows(GemmF8Args g) {
 }
 
 // 16 bytes a lane straight to LDS, the wavefront's 64 lanes one after another
-// from `to` on: from base + offset of a buffer of `size` bytes (zeros for an
-// offset behind it), or from a lane's address.
+// from `to` on, from base + offset + uniform of a buffer of `size` bytes (zeros
+// for an offset behind it).  base, size and uniform are the same in all lanes.
 __device__ __forceinline__ void buffer_to_lds(const uint8_t *base, int size, int offset,
-                                              uint8_t *to) {
+                                              int uniform, uint8_t *to) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(
       __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, size, 0x00020000),
-      (__attribute__((address_space(3))) void *)to, 16, offset, 0, 0, 0);
-}
-__device__ __forceinline__ void global_to_lds(const uint8_t *from, uint8_t *to) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
-                                   (__attribute__((address_space(3))) void *)to, 16, 0, 0);
+      (__attribute__((address_space(3))) void *)to, 16, offset,
+      __builtin_amdgcn_readfirstlane(uniform), 0, 0);
 }
 
 // Blocks of k whose exponents a workgroup keeps in LDS at a time.
@@ -251,8 +252,11 @@ __device__ __forceinline__ void tile_of(const GemmF8Args &g, int &m0, int &n0) {
   n0 = in / high * BN;
 }
 
+// s_waitcnt: all LDS reads done, and all but the last VM loads.
+constexpr int wait_loads(int vm) { return 0x70 | (vm & 15) | (vm >> 4) << 14; }
+
 // BM x BN outputs a workgroup, WM x WN wavefronts. A block of 128 of k at a
-// time goes from memory into one of two LDS stages (16 bytes a lane, straight
+// time goes from memory into one of S LDS stages (16 bytes a lane, straight
 // to LDS):
 //   rows: 128 bytes each, their 16-byte chunks at chunk ^ (row / 2 & 7), so
 //         that 16 rows' reads of one chunk take each of the 64 banks once
@@ -262,18 +266,24 @@ __device__ __forceinline__ void tile_of(const GemmF8Args &g, int &m0, int &n0) {
 // block, and a barrier tells it that everybody's are there and that nobody
 // reads this stage any more: the last two fragments' products then run beside
 // the reads of the next block's first fragments, and the stage is filled again
-// with the block after that. Loads are spread over four fragments' products,
+// with block b + S. Loads are spread over four fragments' products,
 // because a wavefront that issues them all at once stands still until the
 // memory pipeline has taken them.
 // The exponents of kExpSteps blocks wait in LDS too: a load of theirs in the
 // loop would have to wait for the stage's loads in front of it.
-template <typename T, int BM, int BN, int WM, int WN>
+template <typename T, int BM, int BN, int WM, int WN, int S>
 __global__ __launch_bounds__(64 * WM * WN) void k_gemm_f8_tile(GemmF8Args g) {
   typedef typename std::conditional<std::is_same<T, float>::value, Exact, Fast>::type Mma;
   constexpr int kWaves = WM * WN, TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
   constexpr int NB = (BN + 127) / 128;  // 128-column blocks of the tile
   static_assert(TN <= 64 && 64 % TN == 0 && FM % 4 == 0, "a wavefront's columns share an exponent");
+  // Each stage a variable of its own: the compiler then sees that a read of one
+  // need not wait for loads into another.
+  static_assert(S == 2 || S == 4, "stages");
   __shared__ TileLds<BM, BN> stage0, stage1;
+  __shared__ TileLds<S == 4 ? BM : 1, S == 4 ? BN : 1> stage2_, stage3_;
+  auto &stage2 = reinterpret_cast<TileLds<BM, BN> &>(stage2_);
+  auto &stage3 = reinterpret_cast<TileLds<BM, BN> &>(stage3_);
   __shared__ uint8_t a_exp[kExpSteps][WM][16][FM];
   __shared__ uint8_t w_exp[kExpSteps][NB];
 
@@ -296,23 +306,31 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm_f8_tile(GemmF8Args g) {
 #pragma unroll
   for (int i = 0; i < LA; ++i)
     a_off[i] = min((i * kWaves + wave) * 8 + (lane >> 3), last) * (int)g.lda + chunk * 16;
+  // The tile's groups of weights, and how far each of this wavefront's loads is
+  // in them; groups past the last repeat it.
+  const int groups = min(BN / 64, (g.n - 1) / 64 - n0 / 64 + 1);
+  const uint8_t *w_base = g.w + (size_t)(n0 / 64) * g.kb * kTileBytes;
+  int w_off[LB];
+#pragma unroll
+  for (int i = 0; i < LB; ++i) {
+    const int kib = i * kWaves + wave;  // of the stage's BN / 8
+    w_off[i] = min(kib / 8, groups - 1) * g.kb * kTileBytes + kib % 8 * 1024;
+  }
+  const int tail = (g.k - 1) % 128 / 16;  // the last block's last chunk of 16
   // A quarter of block b's loads; past the last block it loads that again.
   auto load = [&](TileLds<BM, BN> &s, int b, int quarter) {
-    b = min(b, g.kb - 1);
+    b = __builtin_amdgcn_readfirstlane(min(b, g.kb - 1));
     // behind the last of k the buffer load gives zeros
-    const bool past = b * 128 + chunk * 16 >= g.k;
+    const bool past = b == g.kb - 1 && chunk > tail;
 #pragma unroll
     for (int i = 0; i < LA + LB; ++i) {
       if (i * 4 / (LA + LB) != quarter) continue;
-      if (i < LA) {
-        buffer_to_lds(a_base, a_size, past ? 0x7FFFFFF0 : a_off[i] + b * 128,
+      if (i < LA)
+        buffer_to_lds(a_base, a_size, past ? 0x7FFFFFF0 : a_off[i], b * 128,
                       s.a + (i * kWaves + wave) * 1024);
-      } else {
-        const int kib = (i - LA) * kWaves + wave;  // of the stage's BN / 8
-        const int group = min(n0 / 64 + kib / 8, (g.n - 1) / 64);
-        buffer_to_lds(g.w + ((size_t)group * g.kb + b) * kTileBytes + kib % 8 * 1024, 1024,
-                      lane * 16, s.b + kib * 1024);
-      }
+      else
+        buffer_to_lds(w_base, groups * g.kb * kTileBytes, lane * 16, w_off[i - LA] + b * kTileBytes,
+                      s.b + ((i - LA) * kWaves + wave) * 1024);
     }
   };
 
@@ -350,8 +368,13 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm_f8_tile(GemmF8Args g) {
       for (int j = 0; j < kOnce; ++j) {
         const int i = (j0 + j) * 64 * kWaves + tid, b = b0 + i % kParts * 16;
         const int8_t *from = g.a_exps + (int64_t)(m0 + min(i / kParts, last)) * g.a_exps_ld + b;
-        if (b + 16 <= g.kb || from + 16 <= exp_end) {
-          __builtin_memcpy(&v[j], from, 16);
+        const int over = (int)max((int64_t)0, from + 16 - exp_end);  // 0 .. 15, or all of it
+        if (exp_end - g.a_exps >= 16) {
+          // the last 16 instead, moved down
+          unsigned __int128 t;
+          __builtin_memcpy(&t, over < 16 ? from - over : exp_end - 16, 16);
+          t = over < 16 ? t >> (8 * over) : 0;
+          __builtin_memcpy(&v[j], &t, 16);
         } else {
           v[j] = v4i{};
 #pragma unroll
@@ -374,35 +397,38 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm_f8_tile(GemmF8Args g) {
       w_exp[i / NB][i % NB] = (uint8_t)(g.w_exps[(size_t)b * g.nb + n] + 127);
     }
   };
-  // This wavefront's reads and loads are done; then everybody's.
+  // This wavefront's reads are done and its loads of the next block; then
+  // everybody's.
   auto meet = [&]() {
     __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_waitcnt(0x0070);
+    __builtin_amdgcn_s_waitcnt(wait_loads((S - 2) * (LA + LB)));
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
   // Block b from stage s, its fragments of W and its first two of the rows
-  // already read (into half p); the other stage takes block b + 1.
-  auto step = [&](int b, TileLds<BM, BN> &s, TileLds<BM, BN> &other, int p) {
+  // already read (into half p). The stage before takes the rest of block
+  // b + S - 1, this one the first half of block b + S.
+  auto step = [&](int b, TileLds<BM, BN> &before, TileLds<BM, BN> &s, TileLds<BM, BN> &after,
+                  int p) {
     typename Mma::frag w[FN];
 #pragma unroll
     for (int j = 0; j < FN; ++j) w[j] = Mma::of(wf[p][j]);
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
       if (i + 2 < FM) read_a(s, i + 2);
-      if (i < 2) load(other, b + 1, 2 + i);
+      if (i < 2) load(before, b + S - 1, 2 + i);
       if (i == FM - 2) {
         meet();
-        read_a(other, 0);
-        read_w(other, 1 - p);
+        read_a(after, 0);
+        read_w(after, 1 - p);
       }
       if (i == FM - 1) {
-        read_a(other, 1);
+        read_a(after, 1);
         read_exps(b + 1, 1 - p);
       }
-      if (i >= FM - 2) load(s, b + 2, i - (FM - 2));
+      if (i >= FM - 2) load(s, b + S, i - (FM - 2));
       __builtin_amdgcn_sched_barrier(0);
       const typename Mma::frag a = Mma::of(af[i % 4]);
       const int x = (unsigned)ae[p][i / 4] >> (8 * (i % 4));
@@ -419,35 +445,58 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm_f8_tile(GemmF8Args g) {
     read_exps(b, 0);
   };
 
+  load_exps(0, std::true_type());
+  // Blocks 0 .. S - 2 and the first half of S - 1, which goes on in step 0.
 #pragma unroll
   for (int q = 0; q < 4; ++q) load(stage0, 0, q);
-  load_exps(0, std::true_type());
+  if (S == 4) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) load(stage1, 1, q);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) load(stage2, 2, q);
+  }
   meet();
-  load(stage1, 1, 0);
-  load(stage1, 1, 1);
+  load(S == 4 ? stage3 : stage1, S - 1, 0);
+  load(S == 4 ? stage3 : stage1, S - 1, 1);
   read_w(stage0, 0);
   read_a(stage0, 0);
   read_a(stage0, 1);
   read_exps(0, 0);
   int b = 0;
-  for (; b + 1 < g.kb; b += 2) {
-    next_exps(b);
-    step(b, stage0, stage1, 0);
-    step(b + 1, stage1, stage0, 1);
-  }
-  if (b < g.kb) {
-    next_exps(b);
-    step(b, stage0, stage1, 0);
+  if (S == 4) {
+    for (; b + 3 < g.kb; b += 4) {
+      next_exps(b);
+      step(b, stage3, stage0, stage1, 0);
+      step(b + 1, stage0, stage1, stage2, 1);
+      step(b + 2, stage1, stage2, stage3, 0);
+      step(b + 3, stage2, stage3, stage0, 1);
+    }
+    if (b < g.kb) {
+      next_exps(b);
+      step(b, stage3, stage0, stage1, 0);
+    }
+    if (b + 1 < g.kb) step(b + 1, stage0, stage1, stage2, 1);
+    if (b + 2 < g.kb) step(b + 2, stage1, stage2, stage3, 0);
+  } else {
+    for (; b + 1 < g.kb; b += 2) {
+      next_exps(b);
+      step(b, stage1, stage0, stage1, 0);
+      step(b + 1, stage0, stage1, stage0, 1);
+    }
+    if (b < g.kb) {
+      next_exps(b);
+      step(b, stage1, stage0, stage1, 0);
+    }
   }
   __builtin_amdgcn_s_waitcnt(0x0070);  // the loads behind the last block
 
   store_tile<T>(g, rows, m0 + wm * TM + col, n0 + wn * TN / 64 * 64, wn * TN % 64 / 16, grp, acc);
 }
 
-template <typename T, int BM, int BN, int WM, int WN>
+template <typename T, int BM, int BN, int WM, int WN, int S>
 static void tile_launch(const GemmF8Args &g, hipStream_t s) {
   const int tiles = ((g.n + BN - 1) / BN) * ((g.m + BM - 1) / BM);
-  hv_launch(k_gemm_f8_tile<T, BM, BN, WM, WN>, dim3(tiles), dim3(64 * WM * WN), 0, s, g);
+  hv_launch(k_gemm_f8_tile<T, BM, BN, WM, WN, S>, dim3(tiles), dim3(64 * WM * WN), 0, s, g);
 }
 
 template <typename T, int FM, int J, int NW>
@@ -461,13 +510,13 @@ static void gemm_f8_launch(const GemmF8Args &g, hipStream_t s) {
 #ifdef HV_DEV
   const char *e = getenv("HV_CFG");
   switch (e ? atoi(e) : 0) {
-    case 1: return tile_launch<T, 256, 256, 2, 4>(g, s);
-    case 2: return tile_launch<T, 128, 128, 2, 2>(g, s);
-    case 3: return tile_launch<T, 64, 64, 1, 4>(g, s);
-    case 4: return tile_launch<T, 128, 256, 2, 4>(g, s);
-    case 5: return tile_launch<T, 64, 128, 1, 4>(g, s);
-    case 6: return tile_launch<T, 64, 256, 1, 4>(g, s);
-    case 7: return tile_launch<T, 256, 128, 4, 2>(g, s);
+    case 1: return tile_launch<T, 256, 256, 2, 4, 2>(g, s);
+    case 2: return tile_launch<T, 128, 128, 2, 2, 2>(g, s);
+    case 3: return tile_launch<T, 64, 64, 1, 4, 2>(g, s);
+    case 5: return tile_launch<T, 64, 128, 1, 4, 2>(g, s);
+    case 32: return tile_launch<T, 128, 128, 2, 2, 4>(g, s);
+    case 33: return tile_launch<T, 64, 64, 1, 4, 4>(g, s);
+    case 35: return tile_launch<T, 64, 128, 1, 4, 4>(g, s);
     case 11: return rows_launch<T, 1, 1, 16>(g, s);
     case 12: return rows_launch<T, 1, 1, 8>(g, s);
     case 13: return rows_launch<T, 1, 2, 8>(g, s);
@@ -484,13 +533,45 @@ static void gemm_f8_launch(const GemmF8Args &g, hipStream_t s) {
     case 46: return rows_launch<T, 4, 1, 4>(g, s);
   }
 #endif
-  // A tile's offsets into the rows are 32-bit.
-  const bool near = g.lda < (int64_t)1 << 22;
-  const int64_t tiles = (int64_t)((g.m + 255) / 256) * ((g.n + 255) / 256);
-  if (near && g.m >= 192 && tiles >= 192 && !std::is_same<T, float>::value)
-    return tile_launch<T, 256, 256, 2, 4>(g, s);
-  if (near && g.m >= 96) return tile_launch<T, 128, 128, 2, 2>(g, s);
-  rows_launch<T, 4, 4, 4>(g, s);
+  // Up to 16 rows (us at k = 4096): the weights' bytes bound them, and parts of
+  // 16 channels keep every CU busy up to 8192 channels; wider weights take two
+  // parts a workgroup (1 row by 4096 channels 4.8, two parts 4.9; by 14336
+  // 12.1, 10.4; by 131072 97.7, 88.1). Up to 32 rows while that leaves few
+  // workgroups (24 by 4096 7.3, tiles 9.3; by 14336 25.4, tiles 12.7).
+  const int parts = (g.n + 63) / 64 * 4;
+  const bool near = g.lda < (int64_t)1 << 22;  // a tile's offsets into the rows are 32-bit
+  if (g.m <= 16 || !near) {
+    if (parts <= 512) return rows_launch<T, 1, 1, 8>(g, s);
+    return rows_launch<T, 1, 2, 8>(g, s);
+  }
+  if (g.m <= 32 && parts <= 256) return rows_launch<T, 2, 1, 8>(g, s);
+  // Tiles by what a block of k costs (measured at k = 4096, us a round of
+  // tiles): small ones, several to a CU, where there are few, large ones, which
+  // read less for each product, where they fill the card.
+  //   16-bit: 64 x 64 10 with one to a CU, 16 with two; 128 x 128 21 with one
+  //   (four stages), 36 with two (two stages); 256 x 256 45
+  //   float32: 64 x 64 21 and 28; 128 x 128 46 and 66
+  // 1024 x 4096 outputs: 30.0, 21.4, 26.3, 43.9 us; 2048 x 4096: 56.8, 41.8,
+  // 35.8, 45.3; 4096 x 4096: 115, 83, 74, 56.
+  constexpr bool kF32 = std::is_same<T, float>::value;
+  auto tiles = [&](int size) {
+    return (int64_t)((g.m + size - 1) / size) * ((g.n + size - 1) / size);
+  };
+  auto cost = [&](int64_t t, int one, int two) {  // two to a CU: 512 a round
+    return t <= 256 ? one : (t + 511) / 512 * two;
+  };
+  const int64_t c64 = cost(tiles(64), kF32 ? 21 : 10, kF32 ? 28 : 16);
+  if (kF32) {
+    if (c64 <= cost(tiles(128), 46, 66)) return tile_launch<T, 64, 64, 1, 4, 4>(g, s);
+    return tile_launch<T, 128, 128, 2, 2, 2>(g, s);
+  } else {
+    const int64_t c128 = (tiles(128) + 511) / 512 * 36, c128deep = (tiles(128) + 255) / 256 * 21;
+    const int64_t c256 = (tiles(256) + 255) / 256 * 45;
+    if (c64 <= c128 && c64 <= c128deep && c64 <= c256) return tile_launch<T, 64, 64, 1, 4, 4>(g, s);
+    if (c128deep <= c128 && c128deep <= c256) return tile_launch<T, 128, 128, 2, 2, 4>(g, s);
+    if (c128 <= c256) return tile_launch<T, 128, 128, 2, 2, 2>(g, s);
+    return tile_launch<T, 256, 256, 2, 4, 2>(g, s);
+  }
 }
 
 }  // namespace hv
