@@ -118,125 +118,100 @@ struct Sums {
 
 static constexpr int kAnswerWaves = 4;
 static constexpr int kMaxParts = 64;
-static constexpr int kKeep = 192;  // candidates a wavefront holds
+static constexpr int kThreads = 64 * kAnswerWaves;
+static constexpr int kSlots = 8;       // maxima that a thread keeps of its logits
+static constexpr int kKeep = 1024;     // candidates for the alternatives
+
+template <typename V>
+struct Lowest {
+  static __device__ __forceinline__ V value() { return Logit<V>::lowest(); }
+};
+template <>
+struct Lowest<u64> {  // of keys
+  static __device__ __forceinline__ u64 value() { return 0; }
+};
 
 // The smallest power of two that is at least n.
 __device__ __forceinline__ int pow2_from(int n) {
   return n <= 1 ? 1 : 1 << (32 - __builtin_clz(n - 1));
 }
 
-// A lower bound on the `top`-th largest of all keys, from a key of each lane,
-// its own largest: lanes fall into at least `top` classes (lane mod classes),
-// whose largest keys are that many different keys, the least of which bounds.
-// 0 where a class has none.
-__device__ __forceinline__ u64 bound_of_lanes(u64 key, int classes) {
-  for (int o = 32; o; o >>= 1) {
-    const u64 other = __shfl_xor(key, o);
-    if (o >= classes) key = other > key ? other : key;
-    else key = other < key ? other : key;
-  }
-  return key;
-}
-
-__device__ __forceinline__ void wave_lds_fence() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
-typedef __attribute__((address_space(3))) u64 lds_u64;
-
-// Cuts a wavefront's list of count <= kKeep keys down to its `top` largest, in
-// order: a key's place is the number of larger ones. Returns the last one's
-// key, 0 if there are fewer.
-static __device__ __noinline__ u64 cut_list(lds_u64 *list, int count, int top) {
-  const int lane = threadIdx.x & 63;
-  wave_lds_fence();
-  u64 mine[kKeep / 64];
-  int place[kKeep / 64] = {};
+// The `top` largest of m different keys, in order: a key's place is the number
+// of larger ones.
+__device__ __forceinline__ void rank_keys(const u64 *keys, int m, int top, u64 *out) {
+  for (int i = threadIdx.x; i < m; i += kThreads) {
+    const u64 mine = keys[i];
+    int place = 0, j = 0;
+    for (; j + 8 <= m; j += 8) {
+      u64 other[8];
 #pragma unroll
-  for (int i = 0; i < kKeep / 64; ++i) mine[i] = i * 64 + lane < count ? list[i * 64 + lane] : 0;
-  for (int j = 0; j < count; ++j) {
-    const u64 other = list[j];
+      for (int k = 0; k < 8; ++k) other[k] = keys[j + k];
 #pragma unroll
-    for (int i = 0; i < kKeep / 64; ++i) place[i] += other > mine[i];
-  }
-  wave_lds_fence();
-#pragma unroll
-  for (int i = 0; i < kKeep / 64; ++i)
-    if (mine[i] && place[i] < top) list[place[i]] = mine[i];
-  wave_lds_fence();
-  return count >= top ? list[top - 1] : 0;
-}
-
-// A wavefront's candidates for the `top` largest keys: all its keys that are
-// not under a bound, which rises whenever kKeep is nearly full and the list is
-// cut down to `top`.
-template <typename V>
-struct Candidates {
-  lds_u64 *list;  // kKeep
-  int count, top;
-  u64 bound;  // no key under it is wanted
-  V value;    // its value
-
-  __device__ __forceinline__ void set_bound(u64 b) {
-    bound = b;
-    key_value(b, value);
-  }
-  // Each lane's key where `there`, all lanes together.
-  __device__ __forceinline__ void push(u64 key, bool there) {
-    const bool in = there && key >= bound;
-    const u64 who = __ballot(in);
-    if (!who) return;
-    if (in) list[count + __builtin_amdgcn_mbcnt_hi((unsigned)(who >> 32),
-                                                   __builtin_amdgcn_mbcnt_lo((unsigned)who, 0))] = key;
-    count += __popcll(who);
-    if (count > kKeep - 64) {
-      const u64 b = cut_list(list, count, top);
-      if (b) set_bound(b);
-      count = min(count, top);
+      for (int k = 0; k < 8; ++k) place += other[k] > mine;
     }
-  }
-};
-
-// The `top` largest of n different keys, in order, into `out`, by a whole
-// workgroup: a bound as above over its threads' largest, then the places of
-// those that are not under it. `left` holds n keys.
-__device__ void largest_keys(const u64 *keys, int n, int top, u64 *left, u64 *out) {
-  __shared__ u64 wave_bound[kAnswerWaves];
-  __shared__ int n_left;
-  const int tid = threadIdx.x;
-  u64 best = 0;
-  for (int i = tid; i < n; i += 64 * kAnswerWaves) best = keys[i] > best ? keys[i] : best;
-  const int classes = max(1, pow2_from(top) / kAnswerWaves);
-  best = bound_of_lanes(best, classes);
-  if ((tid & 63) == 0) wave_bound[tid >> 6] = best;
-  if (tid == 0) n_left = 0;
-  __syncthreads();
-  for (int w = 0; w < kAnswerWaves; ++w) best = wave_bound[w] < best ? wave_bound[w] : best;
-  best = best ? best : 1;  // 0 is no key
-  for (int i = tid; i < n; i += 64 * kAnswerWaves)
-    if (keys[i] >= best) left[atomicAdd(&n_left, 1)] = keys[i];
-  __syncthreads();
-  const int m = n_left;
-  for (int i = tid; i < m; i += 64 * kAnswerWaves) {
-    const u64 mine = left[i];
-    int place = 0;
-    for (int j = 0; j < m; ++j) place += left[j] > mine;
+    for (; j < m; ++j) place += keys[j] > mine;
     if (place < top) out[place] = mine;
   }
-  __syncthreads();
 }
 
-// The same by `top` passes over the row, for a row with a NaN or +inf in it.
+// A lower bound on the `top`-th largest of a workgroup's values, from each
+// thread's largest. For a small `top` the threads fall into at least that many
+// classes (thread mod classes): their largest values are different logits', and
+// the least of them bounds, loosely (about top log(top) logits reach it). For a
+// large one it is the `top`-th largest of the threads' values itself, which
+// takes a comparison of each with each.
+static constexpr int kClassTop = 8;
+template <typename V>
+__device__ V bound_of(V best, int top) {
+  __shared__ V of_thread[kThreads];
+  const int tid = threadIdx.x, lane = tid & 63;
+  if (top > kClassTop) {
+    of_thread[tid] = best;
+    __syncthreads();
+    int reach = 0;  // threads that reach this one's value
+#pragma unroll 16
+    for (int i = 0; i < kThreads; ++i) reach += of_thread[i] >= best;
+    V least = reach >= top ? best : Lowest<V>::value();
+    for (int o = 32; o; o >>= 1) {
+      const V other = __shfl_xor(least, o);
+      least = other > least ? other : least;
+    }
+    __syncthreads();
+    if (lane == 0) of_thread[tid >> 6] = least;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kAnswerWaves; ++w) least = of_thread[w] > least ? of_thread[w] : least;
+    return least;
+  }
+  const int classes = pow2_from(top);
+  for (int o = 32; o >= classes; o >>= 1) {
+    const V other = __shfl_xor(best, o);
+    best = other > best ? other : best;
+  }
+  of_thread[tid] = best;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kAnswerWaves; ++w) {
+    const V other = of_thread[w * 64 + lane];
+    best = other > best ? other : best;
+  }
+  for (int o = classes / 2; o; o >>= 1) {
+    const V other = __shfl_xor(best, o);
+    best = other < best ? other : best;
+  }
+  return best;
+}
+
+// The `top` largest keys of logits [lo, hi) by as many passes over them, for a
+// row with a NaN or +inf in it, or with more equal logits than kKeep.
 template <typename T>
-__device__ void largest_keys_slow(const T *x, int width, int top, u64 *out) {
+__device__ void largest_keys_slow(const T *x, int lo, int hi, int top, u64 *out) {
   typedef typename Logit<T>::type V;
   __shared__ u64 wave_key[kAnswerWaves];
   u64 last = ~0ull;
   for (int k = 0; k < top; ++k) {
     u64 best = 0;
-    for (int c = threadIdx.x; c < width; c += 64 * kAnswerWaves) {
+    for (int c = lo + threadIdx.x; c < hi; c += kThreads) {
       const u64 key = key_of((V)x[c], c);
       if (key < last && key > best) best = key;
     }
@@ -256,7 +231,7 @@ __device__ void largest_keys_slow(const T *x, int width, int top, u64 *out) {
 // What a row gives, from its sums and its largest keys (LDS).
 template <typename T>
 __device__ void write_answer(const AnswerArgs &a, int64_t row, const T *x, const Sums<T> &s,
-                             const u64 *best, bool slow_done) {
+                             const u64 *best) {
   typedef Logit<T> L;
   typedef typename L::type V;
   constexpr float kLn2 = 0.69314718056f;
@@ -267,22 +242,25 @@ __device__ void write_answer(const AnswerArgs &a, int64_t row, const T *x, const
   auto logp = [&](V v) {
     return none ? -__builtin_inff() : L::below(v, s.max) * a.scale - log_sum;
   };
-  for (int i = tid; i < a.n_tokens; i += 64 * kAnswerWaves) {
+  for (int i = tid; i < a.n_tokens; i += kThreads) {
     const int t = a.tokens[row * a.tokens_ld + i];
     a.logp[row * a.n_tokens + i] =
         t < 0 ? 0.f : t >= a.width ? __builtin_nanf("") : logp((V)x[t]);
   }
-  for (int i = tid; i < a.top; i += 64 * kAnswerWaves) {
-    const int t = (int)~(unsigned)best[i];
-    a.top_index[row * a.top + i] = t;
-    a.top_logp[row * a.top + i] = logp((V)x[t]);
+  for (int i = tid; i < a.top; i += kThreads) {
+    V v;
+    key_value(best[i], v);
+    a.top_index[row * a.top + i] = (int)~(unsigned)best[i];
+    a.top_logp[row * a.top + i] = logp(v);
   }
 }
 
-// One workgroup a row or a part of one, in one pass: each lane keeps a running
-// maximum with its sums, each wavefront the candidates for the alternatives.
+// One workgroup a row or a part of one, in one pass: each thread keeps a running
+// maximum with its sums, and for the alternatives the maxima of up to kSlots
+// stretches of its logits. These give a bound that the `top` largest logits are
+// not under, and only the few stretches that reach it are read again.
 template <typename T, bool TOP>
-__global__ __launch_bounds__(64 * kAnswerWaves) void k_log_probs(AnswerArgs a) {
+__global__ __launch_bounds__(kThreads) void k_log_probs(AnswerArgs a) {
   typedef Logit<T> L;
   typedef typename L::type V;
   constexpr int E = 16 / sizeof(T), U = 4;  // logits a load, loads in a turn
@@ -294,12 +272,13 @@ __global__ __launch_bounds__(64 * kAnswerWaves) void k_log_probs(AnswerArgs a) {
   const T *x = (const T *)a.logits + row * a.logits_ld;
   const float c = a.scale * 1.44269504089f;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  __shared__ u64 list[TOP ? kAnswerWaves * kKeep : 1];
-  __shared__ u64 left[TOP ? kAnswerWaves * kKeep : 1];
+  __shared__ V slots[TOP ? kSlots * kThreads : 1];
+  __shared__ u64 keys[TOP ? kKeep : 1];
   __shared__ u64 best[TOP ? HV_LOG_PROBS_MAX_TOP : 1];
+  __shared__ uint16_t hits[TOP ? kSlots * kThreads : 1];
+  __shared__ int n_keys, n_hits;
   __shared__ V wave_max[kAnswerWaves];
   __shared__ float wave_sum[2][kAnswerWaves];
-  __shared__ int n_list;
 
   // [lo, hi): whole loads of 16 bytes from `first` on, n of them, and up to
   // E - 1 logits on either side.
@@ -307,63 +286,30 @@ __global__ __launch_bounds__(64 * kAnswerWaves) void k_log_probs(AnswerArgs a) {
   const int first = min(hi, lo + (int)((16 - ((uintptr_t)(x + lo) & 15)) % 16 / sizeof(T)));
   const int n = (hi - first) / E;
   const vt *xv = reinterpret_cast<const vt *>(x + first);
+  constexpr int kTurn = kThreads * U;  // a turn's loads
+  const int turns = (n + kTurn - 1) / kTurn, each = (turns + kSlots - 1) / kSlots;  // turns a slot
+  auto number = [&](int at, int u) { return at + u * kThreads + tid; };
 
   Sums<T> s;
-  Candidates<V> cand;
-  if (TOP) {
-    cand.list = (lds_u64 *)(list + wave * kKeep);
-    cand.count = 0;
-    cand.top = a.top;
-    cand.set_bound(0);
-  }
-  bool begun = false;  // a bound from this wavefront's first turn
-  constexpr int kTurn = 64 * kAnswerWaves * U;  // a turn's loads, the workgroup's
-  const int mine_at = wave * 64 + lane;
-  auto number = [&](int at, int u) { return at + u * 64 * kAnswerWaves + mine_at; };
+  V high = L::lowest(), highest = L::lowest();  // this slot's, and all
   auto turn = [&](const vt (&v)[U], int at, auto whole) {
     // whole: all of the turn's loads are there
     constexpr bool kWhole = decltype(whole)::value;
-    V high[U], m = s.max;
+    V m = L::lowest();
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const bool there = kWhole || number(at, u) < n;
-      high[u] = L::lowest();
+      V h = L::lowest();
 #pragma unroll
-      for (int i = 0; i < E; ++i) high[u] = L::larger(high[u], (V)v[u][i]);
-      if (!there) high[u] = L::lowest();
-      m = L::larger(m, high[u]);
+      for (int i = 0; i < E; ++i) h = L::larger(h, (V)v[u][i]);
+      m = kWhole || number(at, u) < n ? L::larger(m, h) : m;
     }
-    s.raise(m, c);
+    high = L::larger(high, m);
+    s.raise(L::larger(s.max, m), c);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const bool there = kWhole || number(at, u) < n;
 #pragma unroll
       for (int i = 0; i < E; ++i) s.add((V)v[u][i], c, there);
-    }
-    if (!TOP) return;
-    if (!begun) {
-      begun = true;
-      u64 mine = 0;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const bool there = kWhole || number(at, u) < n;
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-          const u64 key = key_of((V)v[u][i], first + number(at, u) * E + i);
-          if (there && key > mine) mine = key;
-        }
-      }
-      cand.set_bound(bound_of_lanes(mine, pow2_from(a.top)));
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool there = kWhole || number(at, u) < n;
-      if (!__ballot(there && high[u] >= cand.value)) continue;
-#pragma unroll
-      for (int i = 0; i < E; ++i) {
-        if (!__ballot(there && (V)v[u][i] >= cand.value)) continue;
-        cand.push(key_of((V)v[u][i], first + number(at, u) * E + i), there);
-      }
     }
   };
   auto fetch = [&](vt (&v)[U], int at) {
@@ -374,23 +320,30 @@ __global__ __launch_bounds__(64 * kAnswerWaves) void k_log_probs(AnswerArgs a) {
     // the next turn's loads are on their way while one is added up
     vt now[U], next[U];
     fetch(now, 0);
+    int slot = 0, left = each;
     for (int at = 0; at < n; at += kTurn) {
       fetch(next, at + kTurn);
       if (at + kTurn <= n) turn(now, at, std::true_type());
       else turn(now, at, std::false_type());
+      if (TOP && (--left == 0 || at + kTurn >= n)) {
+        slots[slot++ * kThreads + tid] = high;
+        highest = L::larger(highest, high);
+        high = L::lowest();
+        left = each;
+      }
 #pragma unroll
       for (int u = 0; u < U; ++u) now[u] = next[u];
     }
   }
+  // the logits on either side of the loads, at most one a lane
+  const int tail = first + n * E, before = first - lo;
+  const int edge = lane < before ? lo + lane : tail + lane - before;
+  const bool has_edge = wave == 0 && edge < hi;
+  const V at_edge = has_edge ? (V)x[edge] : L::lowest();
   if (wave == 0) {
-    // the logits on either side of the loads, at most one a lane
-    const int tail = first + n * E, before = first - lo;
-    const int at = lane < before ? lo + lane : tail + lane - before;
-    const bool there = at < hi;
-    const V v = there ? (V)x[at] : L::lowest();
-    s.raise(L::larger(s.max, v), c);
-    s.add(v, c, there);
-    if (TOP) cand.push(key_of(v, at), there);
+    s.raise(L::larger(s.max, at_edge), c);
+    s.add(at_edge, c, has_edge);
+    highest = L::larger(highest, at_edge);
   }
 
   s.join_lanes(c);
@@ -399,40 +352,54 @@ __global__ __launch_bounds__(64 * kAnswerWaves) void k_log_probs(AnswerArgs a) {
     wave_sum[0][wave] = s.sum;
     wave_sum[1][wave] = s.weighted;
   }
-  if (TOP && tid == 0) n_list = 0;
-  __syncthreads();
-  for (int w = 1; w < kAnswerWaves; ++w) {
+  if (TOP && tid == 0) n_keys = n_hits = 0;
+  V bound = L::lowest();
+  if (TOP) bound = bound_of<V>(highest, a.top);  // with a barrier
+  else __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kAnswerWaves; ++w) {
     Sums<T> t;
     t.max = wave_max[w];
     t.sum = wave_sum[0][w];
     t.weighted = wave_sum[1][w];
-    Sums<T> mine;
-    mine.max = wave_max[0];
-    mine.sum = wave_sum[0][0];
-    mine.weighted = wave_sum[1][0];
-    if (w == 1) s = mine;
-    s.join(t, c);
+    if (w == 0) s = t;
+    else s.join(t, c);
   }
-  const bool odd = s.sum != s.sum;
   if (TOP) {
-    // the wavefronts' lists one behind the other
-    int total = 0;
-    if (!odd || a.parts > 1) {
-      int at = 0;
-      if (lane == 0) at = atomicAdd(&n_list, cand.count);
-      at = __shfl(at, 0);
-      for (int i = lane; i < cand.count; i += 64) left[at + i] = cand.list[i];
-      __syncthreads();
-      total = n_list;
-      if (tid < a.top) best[tid] = 0;
-      __syncthreads();
-      largest_keys(left, total, a.top, list, best);
-    } else {
-      __syncthreads();
-      largest_keys_slow<T>(x, a.width, a.top, best);
+    auto keep = [&](V v, int at) {
+      const int to = atomicAdd(&n_keys, 1);
+      if (to < kKeep) keys[to] = key_of(v, at);
+    };
+    for (int slot = 0; slot * each < turns; ++slot)
+      if (slots[slot * kThreads + tid] >= bound)
+        hits[atomicAdd(&n_hits, 1)] = (uint16_t)(slot * kThreads + tid);
+    __syncthreads();
+    // a load of a stretch that reaches the bound for each thread
+    const int loads = U * each, all = n_hits * loads;
+    for (int i = tid; i < all; i += kThreads) {
+      const int hit = hits[i / loads], of = i % loads;
+      const int at = (hit / kThreads * each + of / U) * kTurn + of % U * kThreads + hit % kThreads;
+      if (at >= n) continue;
+      const vt v = xv[at];
+#pragma unroll
+      for (int k = 0; k < E; ++k)
+        if ((V)v[k] >= bound) keep((V)v[k], first + at * E + k);
     }
+    if (has_edge && at_edge >= bound) keep(at_edge, edge);
+    // Fewer than `top` finite logits: -inf ones follow, by their index. The
+    // first 2 top logits hold enough of them.
+    if (bound <= L::lowest() && tid < 2 * a.top && lo + tid < hi) {
+      const V v = (V)x[lo + tid];
+      if (v < L::lowest()) keep(v, lo + tid);
+    }
+    if (tid < a.top) best[tid] = 0;
+    __syncthreads();
+    const int m = n_keys;
+    if (m > kKeep || s.sum != s.sum) largest_keys_slow<T>(x, lo, hi, min(a.top, hi - lo), best);
+    else rank_keys(keys, m, a.top, best);
+    __syncthreads();
   }
-  if (a.parts == 1) return write_answer<T>(a, row, x, s, best, odd);
+  if (a.parts == 1) return write_answer<T>(a, row, x, s, best);
   const int64_t p = row * a.parts + part;
   if (tid == 0) a.part[p] = {__builtin_bit_cast(int, s.max), s.sum, s.weighted};
   if (TOP && tid < a.top) a.keys[p * a.top + tid] = best[tid];
@@ -440,15 +407,17 @@ __global__ __launch_bounds__(64 * kAnswerWaves) void k_log_probs(AnswerArgs a) {
 
 // Joins the parts of a row.
 template <typename T, bool TOP>
-__global__ __launch_bounds__(64 * kAnswerWaves) void k_log_probs_join(AnswerArgs a) {
+__global__ __launch_bounds__(kThreads) void k_log_probs_join(AnswerArgs a) {
   typedef typename Logit<T>::type V;
   const int rows = a.rows_dev ? min(a.rows, *a.rows_dev) : a.rows;
   const int64_t row = blockIdx.x;
   if (row >= rows) return;
   const T *x = (const T *)a.logits + row * a.logits_ld;
-  __shared__ u64 left[TOP ? kMaxParts * HV_LOG_PROBS_MAX_TOP : 1];
+  __shared__ u64 keys[TOP ? kMaxParts * HV_LOG_PROBS_MAX_TOP : 1];
   __shared__ u64 best[TOP ? HV_LOG_PROBS_MAX_TOP : 1];
-  const int lane = threadIdx.x & 63;
+  __shared__ int n_keys;
+  const int tid = threadIdx.x, lane = tid & 63, n = a.parts * a.top;
+  const u64 *from = a.keys + row * n;
   Sums<T> s;
   if (lane < a.parts) {
     const AnswerPart p = a.part[row * a.parts + lane];
@@ -456,12 +425,24 @@ __global__ __launch_bounds__(64 * kAnswerWaves) void k_log_probs_join(AnswerArgs
     s.sum = p.sum;
     s.weighted = p.weighted;
   }
+  u64 high = 0;
+  if (TOP) {
+    if (tid == 0) n_keys = 0;
+    for (int i = tid; i < n; i += kThreads) high = from[i] > high ? from[i] : high;
+  }
   s.join_lanes(a.scale * 1.44269504089f);
   if (TOP) {
-    if (s.sum != s.sum) largest_keys_slow<T>(x, a.width, a.top, best);
-    else largest_keys(a.keys + row * a.parts * a.top, a.parts * a.top, a.top, left, best);
+    // keys of 0 stand where a part had fewer than `top`
+    u64 bound = bound_of<u64>(high, a.top);
+    bound = bound ? bound : 1;
+    for (int i = tid; i < n; i += kThreads)
+      if (from[i] >= bound) keys[atomicAdd(&n_keys, 1)] = from[i];
+    __syncthreads();
+    if (s.sum != s.sum) largest_keys_slow<T>(x, 0, a.width, a.top, best);
+    else rank_keys(keys, n_keys, a.top, best);
+    __syncthreads();
   }
-  write_answer<T>(a, row, x, s, best, false);
+  write_answer<T>(a, row, x, s, best);
 }
 
 // Parts of a row. A row is read by one workgroup where there are rows enough
@@ -480,9 +461,9 @@ static int answer_parts(int rows, int width, int *part_width) {
 template <typename T, bool TOP>
 static void answer_launch(const AnswerArgs &a, hipStream_t s) {
   hv_launch(k_log_probs<T, TOP>, dim3((unsigned)((int64_t)a.rows * a.parts)),
-            dim3(64 * kAnswerWaves), 0, s, a);
+            dim3(kThreads), 0, s, a);
   if (a.parts > 1)
-    hv_launch(k_log_probs_join<T, TOP>, dim3(a.rows), dim3(64 * kAnswerWaves), 0, s, a);
+    hv_launch(k_log_probs_join<T, TOP>, dim3(a.rows), dim3(kThreads), 0, s, a);
 }
 template <typename T>
 static void answer_launch(const AnswerArgs &a, hipStream_t s) {
