@@ -122,15 +122,6 @@ static constexpr int kThreads = 64 * kAnswerWaves;
 static constexpr int kSlots = 8;       // maxima that a thread keeps of its logits
 static constexpr int kKeep = 1024;     // candidates for the alternatives
 
-template <typename V>
-struct Lowest {
-  static __device__ __forceinline__ V value() { return Logit<V>::lowest(); }
-};
-template <>
-struct Lowest<u64> {  // of keys
-  static __device__ __forceinline__ u64 value() { return 0; }
-};
-
 // The smallest power of two that is at least n.
 __device__ __forceinline__ int pow2_from(int n) {
   return n <= 1 ? 1 : 1 << (32 - __builtin_clz(n - 1));
@@ -171,7 +162,7 @@ __device__ V bound_of(V best, int top) {
     int reach = 0;  // threads that reach this one's value
 #pragma unroll 16
     for (int i = 0; i < kThreads; ++i) reach += of_thread[i] >= best;
-    V least = reach >= top ? best : Lowest<V>::value();
+    V least = reach >= top ? best : Logit<V>::lowest();
     for (int o = 32; o; o >>= 1) {
       const V other = __shfl_xor(least, o);
       least = other > least ? other : least;
@@ -228,10 +219,23 @@ __device__ void largest_keys_slow(const T *x, int lo, int hi, int top, u64 *out)
   }
 }
 
+// The logit of the thread's first given token, asked for before it is needed.
+template <typename T>
+struct Given {
+  int token = -1;
+  typename Logit<T>::type logit = 0;
+  __device__ __forceinline__ Given(const AnswerArgs &a, int64_t row, const T *x) {
+    if ((int)threadIdx.x < a.n_tokens) {
+      token = a.tokens[row * a.tokens_ld + threadIdx.x];
+      if (token >= 0 && token < a.width) logit = (typename Logit<T>::type)x[token];
+    }
+  }
+};
+
 // What a row gives, from its sums and its largest keys (LDS).
 template <typename T>
 __device__ void write_answer(const AnswerArgs &a, int64_t row, const T *x, const Sums<T> &s,
-                             const u64 *best) {
+                             const u64 *best, const Given<T> &given) {
   typedef Logit<T> L;
   typedef typename L::type V;
   constexpr float kLn2 = 0.69314718056f;
@@ -243,9 +247,9 @@ __device__ void write_answer(const AnswerArgs &a, int64_t row, const T *x, const
     return none ? -__builtin_inff() : L::below(v, s.max) * a.scale - log_sum;
   };
   for (int i = tid; i < a.n_tokens; i += kThreads) {
-    const int t = a.tokens[row * a.tokens_ld + i];
-    a.logp[row * a.n_tokens + i] =
-        t < 0 ? 0.f : t >= a.width ? __builtin_nanf("") : logp((V)x[t]);
+    const int t = i == tid ? given.token : a.tokens[row * a.tokens_ld + i];
+    const V v = i == tid ? given.logit : t >= 0 && t < a.width ? (V)x[t] : V(0);
+    a.logp[row * a.n_tokens + i] = t < 0 ? 0.f : t >= a.width ? __builtin_nanf("") : logp(v);
   }
   for (int i = tid; i < a.top; i += kThreads) {
     V v;
@@ -280,6 +284,7 @@ __global__ __launch_bounds__(kThreads) void k_log_probs(AnswerArgs a) {
   __shared__ V wave_max[kAnswerWaves];
   __shared__ float wave_sum[2][kAnswerWaves];
 
+  const Given<T> given(a.parts == 1 ? a : AnswerArgs{}, row, x);
   // [lo, hi): whole loads of 16 bytes from `first` on, n of them, and up to
   // E - 1 logits on either side.
   const int lo = part * a.part_width, hi = min(a.width, lo + a.part_width);
@@ -399,7 +404,7 @@ __global__ __launch_bounds__(kThreads) void k_log_probs(AnswerArgs a) {
     else rank_keys(keys, m, a.top, best);
     __syncthreads();
   }
-  if (a.parts == 1) return write_answer<T>(a, row, x, s, best);
+  if (a.parts == 1) return write_answer<T>(a, row, x, s, best, given);
   const int64_t p = row * a.parts + part;
   if (tid == 0) a.part[p] = {__builtin_bit_cast(int, s.max), s.sum, s.weighted};
   if (TOP && tid < a.top) a.keys[p * a.top + tid] = best[tid];
@@ -418,6 +423,7 @@ __global__ __launch_bounds__(kThreads) void k_log_probs_join(AnswerArgs a) {
   __shared__ int n_keys;
   const int tid = threadIdx.x, lane = tid & 63, n = a.parts * a.top;
   const u64 *from = a.keys + row * n;
+  const Given<T> given(a, row, x);
   Sums<T> s;
   if (lane < a.parts) {
     const AnswerPart p = a.part[row * a.parts + lane];
@@ -425,16 +431,29 @@ __global__ __launch_bounds__(kThreads) void k_log_probs_join(AnswerArgs a) {
     s.sum = p.sum;
     s.weighted = p.weighted;
   }
-  u64 high = 0;
+  u64 bound = 1;  // keys of 0 stand where a part had fewer than `top`
   if (TOP) {
     if (tid == 0) n_keys = 0;
-    for (int i = tid; i < n; i += kThreads) high = from[i] > high ? from[i] : high;
+    // Each part's keys are in order. `each` of a part's keys are not under its
+    // each-th, so the need-th largest of these bounds need * each >= top keys.
+    const int each = (a.top + a.parts - 1) / a.parts, need = (a.top + each - 1) / each;
+    const u64 mine = lane < a.parts ? from[lane * a.top + each - 1] : 0;
+    int reach = 0;
+    for (int i = 0; i < a.parts; ++i) {
+      const unsigned low = __builtin_amdgcn_readlane((int)mine, i);
+      const unsigned high = __builtin_amdgcn_readlane((int)(mine >> 32), i);
+      reach += ((u64)high << 32 | low) >= mine;
+    }
+    u64 least = reach >= need ? mine : 0;
+    for (int o = 32; o; o >>= 1) {
+      const u64 other = __shfl_xor(least, o);
+      least = other > least ? other : least;
+    }
+    bound = least ? least : 1;
   }
   s.join_lanes(a.scale * 1.44269504089f);
   if (TOP) {
-    // keys of 0 stand where a part had fewer than `top`
-    u64 bound = bound_of<u64>(high, a.top);
-    bound = bound ? bound : 1;
+    __syncthreads();
     for (int i = tid; i < n; i += kThreads)
       if (from[i] >= bound) keys[atomicAdd(&n_keys, 1)] = from[i];
     __syncthreads();
@@ -442,13 +461,13 @@ __global__ __launch_bounds__(kThreads) void k_log_probs_join(AnswerArgs a) {
     else rank_keys(keys, n_keys, a.top, best);
     __syncthreads();
   }
-  write_answer<T>(a, row, x, s, best);
+  write_answer<T>(a, row, x, s, best, given);
 }
 
 // Parts of a row. A row is read by one workgroup where there are rows enough
 // to keep the card busy; fewer rows are cut until kAnswerGroups workgroups
 // are at work, in parts of at least kMinPart logits.
-static constexpr int kAnswerGroups = 512, kMinPart = 4096;
+static constexpr int kAnswerGroups = 512, kMinPart = 8192;
 static int answer_parts(int rows, int width, int *part_width) {
   int parts = (int)((kAnswerGroups + (int64_t)rows - 1) / (rows > 0 ? rows : 1));
   parts = parts < width / kMinPart ? parts : width / kMinPart;
