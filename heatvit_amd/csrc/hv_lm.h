@@ -14,23 +14,32 @@ typedef __bf16 bf16;
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 
-// Eight elements at p as 32-bit floats: with VEC one or two 16-byte loads
-// (p 16-byte aligned, all eight there), else the first n, the rest zero.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T *p, int n, float *v) {
-  if (VEC) {
-    typedef T vt __attribute__((ext_vector_type(16 / sizeof(T))));
+// Eight adjacent elements: in 16-byte accesses at any element's alignment
+// where all eight are there, else the first n (the rest zero).
+template <typename T>
+struct Eight {
+  typedef T v8 __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ v8 load(const T *p, int n) {
+    v8 t = {};
+    if (n == 8) {
+      __builtin_memcpy(&t, p, sizeof t);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; i += 16 / sizeof(T)) {
-      const vt t = *reinterpret_cast<const vt *>(p + i);
-#pragma unroll
-      for (int j = 0; j < (int)(16 / sizeof(T)); ++j) v[i + j] = (float)t[j];
+      for (int i = 0; i < 8; ++i)
+        if (i < n) t[i] = p[i];
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? (float)p[i] : 0.f;
+    return t;
   }
-}
+  static __device__ __forceinline__ void store(T *p, int n, v8 t) {
+    if (n == 8) {
+      __builtin_memcpy(p, &t, sizeof t);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < n) p[i] = t[i];
+    }
+  }
+};
 
 // The value of another lane of the same 16 (n lanes on, cyclically).
 template <int N>

@@ -507,32 +507,6 @@ static void rows_launch(const GemmF8Args &g, hipStream_t s) {
 
 template <typename T>
 static void gemm_f8_launch(const GemmF8Args &g, hipStream_t s) {
-#ifdef HV_DEV
-  const char *e = getenv("HV_CFG");
-  switch (e ? atoi(e) : 0) {
-    case 1: return tile_launch<T, 256, 256, 2, 4, 2>(g, s);
-    case 2: return tile_launch<T, 128, 128, 2, 2, 2>(g, s);
-    case 3: return tile_launch<T, 64, 64, 1, 4, 2>(g, s);
-    case 5: return tile_launch<T, 64, 128, 1, 4, 2>(g, s);
-    case 32: return tile_launch<T, 128, 128, 2, 2, 4>(g, s);
-    case 33: return tile_launch<T, 64, 64, 1, 4, 4>(g, s);
-    case 35: return tile_launch<T, 64, 128, 1, 4, 4>(g, s);
-    case 11: return rows_launch<T, 1, 1, 16>(g, s);
-    case 12: return rows_launch<T, 1, 1, 8>(g, s);
-    case 13: return rows_launch<T, 1, 2, 8>(g, s);
-    case 14: return rows_launch<T, 1, 4, 8>(g, s);
-    case 21: return rows_launch<T, 2, 1, 16>(g, s);
-    case 22: return rows_launch<T, 2, 1, 8>(g, s);
-    case 23: return rows_launch<T, 2, 2, 8>(g, s);
-    case 24: return rows_launch<T, 2, 4, 8>(g, s);
-    case 41: return rows_launch<T, 4, 1, 16>(g, s);
-    case 42: return rows_launch<T, 4, 1, 8>(g, s);
-    case 43: return rows_launch<T, 4, 2, 8>(g, s);
-    case 44: return rows_launch<T, 4, 4, 4>(g, s);
-    case 45: return rows_launch<T, 4, 2, 4>(g, s);
-    case 46: return rows_launch<T, 4, 1, 4>(g, s);
-  }
-#endif
   // Up to 16 rows (us at k = 4096): the weights' bytes bound them, and parts of
   // 16 channels keep every CU busy up to 8192 channels; wider weights take two
   // parts a workgroup (1 row by 4096 channels 4.8, two parts 4.9; by 14336

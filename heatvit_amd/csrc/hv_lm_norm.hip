@@ -57,69 +57,53 @@ __device__ __forceinline__ int quant4(const float *p, float inv) {
   return r;
 }
 
-template <bool VEC>
-__device__ __forceinline__ void store_q8(uint8_t *q, int n, int lo, int hi) {
-  if (VEC) {
-    *reinterpret_cast<v2i *>(q) = v2i{lo, hi};
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < n) q[i] = (uint8_t)((i < 4 ? lo : hi) >> (8 * (i & 3)));
-  }
+template <int FMT>
+__device__ __forceinline__ void store_q8(uint8_t *q, int n, const float *p, float inv) {
+  const v2i t = {quant4<FMT>(p, inv), quant4<FMT>(p + 4, inv)};
+  Eight<uint8_t>::v8 b;
+  __builtin_memcpy(&b, &t, sizeof b);
+  Eight<uint8_t>::store(q, n, b);
 }
 
-// One workgroup a row; each thread takes eight columns at a time, so a block
-// of 128 is 16 adjacent lanes.
-template <typename T, int FMT, bool VEC, bool ROW>
-__global__ __launch_bounds__(256) void k_rms_norm_q8(NormArgs a) {
+// LANES threads a row (16: sixteen rows a workgroup, 64: four, else one); each
+// takes eight columns at a time, so a block of 128 is 16 adjacent lanes.
+template <typename T, int FMT, bool ROW, int LANES>
+__global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void k_rms_norm_q8(NormArgs a) {
+  constexpr int kRows = LANES < 256 ? 256 / LANES : 1, kWaves = LANES / 64;
   const int rows = a.rows_dev ? min(a.rows, *a.rows_dev) : a.rows;
-  const int row = blockIdx.x;
-  if (row >= rows) return;
+  const int tid = threadIdx.x % LANES;
+  // Of a wavefront with several rows, lanes past the last row repeat it and
+  // write nothing: its other lanes need them active.
+  const int64_t mine = (int64_t)blockIdx.x * kRows + threadIdx.x / LANES;
+  if (LANES >= 64 ? mine >= rows : (int64_t)blockIdx.x * kRows >= rows) return;
+  const bool live = mine < rows;
+  const int64_t row = live ? mine : rows - 1;
   const T *x = (const T *)a.x + row * a.x_ld;
   const T *res = a.residual ? (const T *)a.residual + row * a.residual_ld : nullptr;
   T *out = a.residual ? (T *)a.residual_out + row * a.residual_out_ld : nullptr;
   const T *w = (const T *)a.weight;
+  typedef typename Eight<T>::v8 v8;
   uint8_t *q = a.q + row * a.q_ld;
   int8_t *exps = a.exps + row * a.exps_ld;
-  const int tid = threadIdx.x;
-  __shared__ float part[2][4];
-
   float sum = 0.f, amax = 0.f;
-  for (int c = 0; c < a.width; c += 2048) {
+  for (int c = 0; c < a.width; c += LANES * 8) {
     const int c0 = c + tid * 8;
     const int n = min(8, a.width - c0);
     float h[8] = {}, p[8] = {};
     if (n > 0) {
-      load8<T, VEC>(x + c0, n, h);
+      v8 t = Eight<T>::load(x + c0, n);
+      const v8 g = Eight<T>::load(w + c0, n);
       if (res) {
-        float r[8];
-        load8<T, VEC>(res + c0, n, r);
-        typedef T v8 __attribute__((ext_vector_type(8)));
-        v8 t;
+        const v8 r = Eight<T>::load(res + c0, n);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          t[i] = (T)(h[i] + r[i]);
-          h[i] = (float)t[i];
-        }
-        if (VEC) {
-          typedef T vt __attribute__((ext_vector_type(16 / sizeof(T))));
-#pragma unroll
-          for (int i = 0; i < 8; i += 16 / sizeof(T)) {
-            vt s;
-#pragma unroll
-            for (int j = 0; j < (int)(16 / sizeof(T)); ++j) s[j] = t[i + j];
-            *reinterpret_cast<vt *>(out + c0 + i) = s;
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (i < n) out[c0 + i] = t[i];
-        }
+        for (int i = 0; i < 8; ++i) t[i] = (T)((float)t[i] + (float)r[i]);
+        if (live) Eight<T>::store(out + c0, n, t);
       }
-      float g[8];
-      load8<T, VEC>(w + c0, n, g);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) p[i] = h[i] * g[i];
+      for (int i = 0; i < 8; ++i) {
+        h[i] = (float)t[i];
+        p[i] = h[i] * (float)g[i];
+      }
     }
     float m = 0.f;
 #pragma unroll
@@ -132,58 +116,80 @@ __global__ __launch_bounds__(256) void k_rms_norm_q8(NormArgs a) {
     } else {
       const int e = block_exp<FMT>(max16(m));
       const float inv = __builtin_bit_cast(float, (127 - e) << 23);
-      if (n > 0) {
-        store_q8<VEC>(q + c0, n, quant4<FMT>(p, inv), quant4<FMT>(p + 4, inv));
+      if (n > 0 && live) {
+        store_q8<FMT>(q + c0, n, p, inv);
         if ((tid & 15) == 0) exps[c0 / kNormBlock] = (int8_t)e;
       }
     }
   }
 
-  sum = sum64(sum);
-  if (ROW) amax = max64(amax);
-  if ((tid & 63) == 0) {
-    part[0][tid >> 6] = sum;
-    part[1][tid >> 6] = amax;
+  if (LANES == 16) {
+    sum = sum16(sum);
+    if (ROW) amax = max16(amax);
+  } else {
+    sum = sum64(sum);
+    if (ROW) amax = max64(amax);
   }
-  __syncthreads();
-  if (tid == 0) {
-    sum = (part[0][0] + part[0][1]) + (part[0][2] + part[0][3]);
-    a.scale[row] = 1.f / sqrtf(sum / (float)a.width + a.eps);
+  if (LANES > 64) {
+    __shared__ float part[2][kWaves > 0 ? kWaves : 1];
+    if ((tid & 63) == 0) {
+      part[0][tid >> 6] = sum;
+      part[1][tid >> 6] = amax;
+    }
+    __syncthreads();
+    sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      sum += part[0][w];
+      amax = fmaxf(amax, part[1][w]);
+    }
   }
+  if (!live) return;
+  if (tid == 0) a.scale[row] = 1.f / sqrtf(sum / (float)a.width + a.eps);
   if (!ROW) return;
-  amax = fmaxf(fmaxf(part[1][0], part[1][1]), fmaxf(part[1][2], part[1][3]));
   const int e = block_exp<FMT>(amax);
   const float inv = __builtin_bit_cast(float, (127 - e) << 23);
   if (tid == 0) exps[0] = (int8_t)e;
   // Every thread reads again what it read or wrote itself.
   const T *kept = out ? out : x;
-  for (int c0 = tid * 8; c0 < a.width; c0 += 2048) {
+  for (int c0 = tid * 8; c0 < a.width; c0 += LANES * 8) {
     const int n = min(8, a.width - c0);
-    float h[8], g[8];
-    load8<T, VEC>(kept + c0, n, h);
-    load8<T, VEC>(w + c0, n, g);
+    const v8 t = Eight<T>::load(kept + c0, n), g = Eight<T>::load(w + c0, n);
+    float p[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] *= g[i];
-    store_q8<VEC>(q + c0, n, quant4<FMT>(h, inv), quant4<FMT>(h + 4, inv));
+    for (int i = 0; i < 8; ++i) p[i] = (float)t[i] * (float)g[i];
+    store_q8<FMT>(q + c0, n, p, inv);
   }
 }
 
-template <typename T, int FMT, bool VEC>
+template <typename T, int FMT, int LANES>
 static void norm_launch(const NormArgs &a, bool row, hipStream_t s) {
-  const dim3 grid(a.rows), block(256);
-  if (row) hv_launch(k_rms_norm_q8<T, FMT, VEC, true>, grid, block, 0, s, a);
-  else hv_launch(k_rms_norm_q8<T, FMT, VEC, false>, grid, block, 0, s, a);
+  constexpr int kRows = LANES < 256 ? 256 / LANES : 1;
+  const dim3 grid((unsigned)(((int64_t)a.rows + kRows - 1) / kRows));
+  const dim3 block(LANES < 256 ? 256 : LANES);
+  if (row) hv_launch(k_rms_norm_q8<T, FMT, true, LANES>, grid, block, 0, s, a);
+  else hv_launch(k_rms_norm_q8<T, FMT, false, LANES>, grid, block, 0, s, a);
+}
+
+// Threads a row (us by 16, 64, 256 and 1024): many short rows want few, since
+// a workgroup of idle threads costs as much as one at work (65536 x 64 bf16
+// 9.1, 22.4, 55, 190; 50432 x 192 13.5, 18.5, 44, 150; 16384 x 768 17.7, 17.0,
+// 19.5, 53; 8192 x 2048 32.2, 26.5, 25.0, 41), long rows and few rows many,
+// whose loads are then on their way at once (16384 x 8192 228, 185, 174, 164;
+// 32 x 8192 50, 14.1, 5.2, 3.6; 512 x 4096 32.7, 9.6, 5.0, 4.9).
+template <typename T, int FMT>
+static void norm_launch(const NormArgs &a, bool row, hipStream_t s) {
+  const bool few = a.rows <= 512;
+  if (a.width <= (few ? 128 : 512)) return norm_launch<T, FMT, 16>(a, row, s);
+  if (a.width <= (few ? 512 : 1024)) return norm_launch<T, FMT, 64>(a, row, s);
+  if (a.width <= (few ? 2048 : 8191)) return norm_launch<T, FMT, 256>(a, row, s);
+  norm_launch<T, FMT, 1024>(a, row, s);
 }
 
 template <typename T>
-static void norm_launch(const NormArgs &a, int format, bool vec, bool row, hipStream_t s) {
-  if (format == HV_Q_E4M3) {
-    if (vec) norm_launch<T, HV_Q_E4M3, true>(a, row, s);
-    else norm_launch<T, HV_Q_E4M3, false>(a, row, s);
-  } else {
-    if (vec) norm_launch<T, HV_Q_I8, true>(a, row, s);
-    else norm_launch<T, HV_Q_I8, false>(a, row, s);
-  }
+static void norm_launch(const NormArgs &a, int format, bool row, hipStream_t s) {
+  if (format == HV_Q_E4M3) norm_launch<T, HV_Q_E4M3>(a, row, s);
+  else norm_launch<T, HV_Q_I8>(a, row, s);
 }
 
 }  // namespace hv
@@ -222,15 +228,9 @@ extern "C" int hv_rms_norm_q8(const hv_rms_norm_desc *d, hv_stream_t stream) {
   a.x_ld = d->x_ld; a.residual_ld = d->residual_ld; a.residual_out_ld = d->residual_out_ld;
   a.q_ld = d->q_ld; a.exps_ld = d->exps_ld;
   a.rows = d->rows; a.width = d->width; a.eps = d->eps;
-  // 16-byte loads and 8-byte stores where every row and chunk of eight allows it.
-  uintptr_t at = (uintptr_t)d->x | (uintptr_t)d->residual | (uintptr_t)d->residual_out |
-                 (uintptr_t)d->weight | (uintptr_t)(d->x_ld * size);
-  if (d->residual) at |= (uintptr_t)(d->residual_ld * size) | (uintptr_t)(d->residual_out_ld * size);
-  const bool vec = d->width % 8 == 0 && !(at & 15) &&
-                   !(((uintptr_t)d->q | (uintptr_t)d->q_ld) & 7);
   const hipStream_t s = (hipStream_t)stream;
-  if (d->type == HV_T_F32) norm_launch<float>(a, d->format, vec, d->block == 0, s);
-  else if (d->type == HV_T_F16) norm_launch<f16>(a, d->format, vec, d->block == 0, s);
-  else norm_launch<bf16>(a, d->format, vec, d->block == 0, s);
+  if (d->type == HV_T_F32) norm_launch<float>(a, d->format, d->block == 0, s);
+  else if (d->type == HV_T_F16) norm_launch<f16>(a, d->format, d->block == 0, s);
+  else norm_launch<bf16>(a, d->format, d->block == 0, s);
   return check_hip(hipGetLastError(), "k_rms_norm_q8 launch");
 }

@@ -16,7 +16,7 @@ from dataclasses import dataclass
 import numpy as np
 import torch
 
-from . import _lib
+from . import _lib, lm
 from .device import DeviceModel
 from .image import float_images
 from .params import HeatViTParams, coerce
@@ -24,6 +24,7 @@ from .params import HeatViTParams, coerce
 LOGIT_SCALE_EXP = -14
 WARN_HEAD_DEN_ZERO, WARN_PACKAGE_DEN_ZERO, WARN_LN_NEGATIVE_VARIANCE = 1, 2, 4
 IMAGE_BYTES = 224 * 224 * 3
+CLASSES = 1000
 CKPT_NAMES = (["patch"] + [f"selector_{i:02d}" for i in range(1, 4)] +
               [f"block_{i:02d}" for i in range(1, 13)] + ["final_ln"])
 
@@ -45,6 +46,15 @@ class BatchResult:
     selector_state: np.ndarray  # [n_selectors][B][5]: count, package, kept, pruned, warnings
     warnings: np.ndarray = None  # [B] engine warning bits of each image's forward
     checkpoints: list = None   # per image dict when requested
+
+
+@dataclass(frozen=True)
+class BatchScores:
+    """What the logits say of each image, under softmax(logits * 2^output_scale_exp)."""
+    logp: np.ndarray           # float32, the shape of the labels (None without)
+    entropy: np.ndarray        # [B] float32
+    top_logp: np.ndarray       # [B][top] float32
+    top_index: np.ndarray      # [B][top] int32: the best classes, equal logits by the lower one
 
 
 class Engine:
@@ -195,6 +205,39 @@ class HeatViTModel:
         (p2_sim.forward_image's front end, tools/p2/p2_sim.py:536-543)."""
         return self._run(float_images(images), params, checkpoints)
 
+    @staticmethod
+    def _state(state, params):
+        """The selectors' states on the host; raises for a rejected image."""
+        state = state.cpu().numpy()[:len(params.selectors)]
+        if (state[:, :, 0] < 0).any():
+            e = ValueError("selector input invalid for some image (too few tokens)")
+            e.error_class = _lib.HV_ERR_TOKEN_COUNT
+            raise e
+        return state
+
+    def score_batch(self, images, params, labels=None, top=5):
+        """Log probabilities of the given classes, entropy and the `top` best
+        classes of every image, computed on the device from the forward's int32
+        logits (lm.log_probs).  images: int8 as for infer_batch, or float CHW
+        as for infer_float_batch; labels (optional): class numbers [B] or
+        [B][G]; top <= 64."""
+        floats = images.is_floating_point() if isinstance(images, torch.Tensor) else \
+            np.asarray(images).dtype.kind == "f"
+        dev = float_images(images) if floats else torch.from_numpy(_images(images)).cuda()
+        if labels is not None:
+            labels = np.asarray(labels)
+            if labels.dtype.kind not in "iu":
+                raise TypeError("labels must hold integers")
+            if labels.ndim not in (1, 2) or len(labels) != dev.shape[0]:
+                raise ValueError("labels must be [B] or [B][G]")
+            if labels.size and (labels.min() < 0 or labels.max() >= CLASSES):
+                raise ValueError(f"labels outside [0, {CLASSES})")
+            labels = torch.from_numpy(np.ascontiguousarray(labels, np.int32)).cuda()
+        logits, _, state, _ = self._engine(params, dev.shape[0]).forward(dev)
+        r = lm.log_probs(logits, labels, scale_exp=LOGIT_SCALE_EXP, top=top)
+        self._state(state, params)
+        return BatchScores(*[None if t is None else t.cpu().numpy() for t in r])
+
     def _run(self, dev, params, checkpoints):
         b = dev.shape[0]
         eng = self._engine(params, b)
@@ -203,12 +246,7 @@ class HeatViTModel:
             ck = torch.zeros((b, 17, 197, 192), dtype=torch.int8, device="cuda")
             ck_rows = torch.zeros((b, 17), dtype=torch.int32, device="cuda")
         logits, counts, state, warnings = eng.forward(dev, ck, ck_rows)
-        n_sel = len(params.selectors)
-        state = state.cpu().numpy()[:n_sel]
-        if (state[:, :, 0] < 0).any():
-            e = ValueError("selector input invalid for some image (too few tokens)")
-            e.error_class = _lib.HV_ERR_TOKEN_COUNT
-            raise e
+        state = self._state(state, params)
         cks = None
         if checkpoints:
             ck, ck_rows = ck.cpu().numpy(), ck_rows.cpu().numpy()

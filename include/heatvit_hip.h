@@ -427,8 +427,7 @@ int hv_model_forward_f32_ex(const hv_model_dev *p, const float *images, int batc
  * residual_out is NULL exactly when residual is; it may be residual or x
  * itself (same stride), q, exps and scale overlap nothing else.  rows_dev
  * (optional, device): the live row count; rows behind it are left as they
- * were.  Strides are in elements.  Pointers are aligned to their elements;
- * 16-byte aligned rows of a width that 8 divides take wide loads. */
+ * were.  Strides are in elements, pointers aligned to their elements. */
 typedef struct {
   const void *x, *residual, *weight; /* [rows][x_ld], [rows][residual_ld], [width] of `type` */
   void *residual_out;

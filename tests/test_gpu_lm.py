@@ -184,7 +184,9 @@ def _exps(shape, seed, low, high):
 GEMM_SIZES = ((1, 1, 16), (1, 64, 128), (3, 17, 48), (16, 64, 192), (17, 65, 144), (5, 130, 512),
               (33, 200, 1040), (64, 256, 256), (65, 127, 384), (100, 129, 128), (128, 128, 2048),
               (129, 300, 640), (200, 1000, 192), (256, 256, 256), (257, 513, 400), (300, 70, 1152),
-              (520, 260, 272), (1, 1000, 4096), (40, 4100, 512), (70, 1030, 1664), (1030, 300, 528))
+              (520, 260, 272), (1, 1000, 4096), (40, 4100, 512), (70, 1030, 1664), (1030, 300, 528),
+              (24, 1030, 1040), (32, 4200, 256), (8, 9000, 128), (2100, 1030, 384), (4000, 4100, 144),
+              (4100, 4000, 272), (600, 600, 256), (1500, 2100, 128))
 
 
 @pytest.mark.parametrize("size", GEMM_SIZES, ids=str)
@@ -233,6 +235,29 @@ def test_gemm_values(kind, size):
         # the rounding of an output smaller than the type's normal numbers
         tiny = torch.finfo(TYPES[kind]).tiny * torch.finfo(TYPES[kind]).eps
         assert (off <= bound + (np.abs(y) + bound) * ref.HALF[TYPES[kind]] + tiny).all()
+
+
+@pytest.mark.parametrize("size", ((5, 64, 16400), (70, 200, 8208), (1100, 1030, 8336),
+                                  (4100, 4100, 8464), (70, 64, 20000), (600, 260, 16640)), ids=str)
+def test_gemm_long_inner(size):
+    """Inner sizes past the exponents that a tile holds at once (64 blocks),
+    and at every number of blocks modulo the stages."""
+    from heatvit_amd import lm
+    from heatvit_amd.device import DeviceF8Weight
+    m, n, k = size
+    for cut in (0, 128, 256, 384):
+        kk = k - cut
+        kb, nb = -(-kk // 128), -(-n // 128)
+        a, w = _whole((m, kk), 1, 1), _whole((kk, n), 2, 1)
+        # |sum| <= k < 2^24 units of 2^-4
+        ae, we = _exps((m, kb), 3, -2, 0), _exps((kb, nb), 4, -2, 0)
+        dw = DeviceF8Weight(w, we)
+        s = torch.from_numpy(ref.spread(ae.numpy(), 128, kk)).float().cuda()
+        t = torch.from_numpy(np.repeat(ref.spread(we.numpy(), 128, n), 128, 0)[:kk]).float().cuda()
+        want = (a.float().cuda() * s) @ (w.float().cuda() * t)  # exact: whole multiples of 2^-4
+        for dtype in (torch.bfloat16, torch.float32):
+            got = lm.gemm_f8(a.cuda(), ae.cuda(), dw, out_dtype=dtype)
+            assert torch.equal(got, want.to(dtype)), (cut, dtype)
 
 
 def test_gemm_every_exponent():
@@ -300,6 +325,22 @@ def test_gemm_strides_live_rows_and_nothing_outside():
                 assert torch.equal(c[:rows, pad:pad + n].cpu(), want[:rows]), (m, live, pad)
                 assert (c[rows:] == 55).all()
                 assert (c[:, :pad] == 55).all() and (c[:, pad + n:] == 55).all()
+
+
+def test_gemm_rows_far_apart():
+    """Rows 2^22 and more bytes apart, where a tile's 32-bit offsets end."""
+    from heatvit_amd import lm
+    from heatvit_amd.device import DeviceF8Weight
+    m, n, k = 70, 130, 400
+    a, w = _whole((m, k), 1), _whole((k, n), 2)
+    ae, we = _exps((m, 4), 3, -2, 0), _exps((4, 2), 4, -3, 0)
+    want, _ = ref.gemm_f8(a, ae.numpy(), w, we.numpy(), None, None)
+    for ld in (1 << 22, (1 << 22) - 16):
+        far = torch.zeros((m, ld), dtype=torch.uint8, device="cuda")
+        far[:, :k] = a.view(torch.uint8).cuda()
+        got = lm.gemm_f8(far.view(torch.float8_e4m3fn)[:, :k], ae.cuda(), DeviceF8Weight(w, we),
+                         out_dtype=torch.float32)
+        assert np.array_equal(got.cpu().double().numpy(), want)
 
 
 def test_weight_quantised_here():
@@ -478,6 +519,37 @@ def test_norm_product_answer(rows):
     off = np.abs(logits.cpu().double().numpy() - y)
     assert (off <= bound + (np.abs(y) + bound) * 2.0 ** -8).all()
     _check_answer(answer, logits.cpu().double().numpy(), tokens.numpy(), 1.0, 5)
+
+
+def test_model_scores():
+    """The classifier's answers: HeatViTModel.score_batch on the logits that
+    infer_batch gives, for int8 and for float images."""
+    from heatvit_amd import synth
+    from heatvit_amd.model import HeatViTModel
+    images, params = synth.pruned_workload(5)
+    model = HeatViTModel()
+    logits = model.infer_batch(images, params).logits
+    labels = np.random.default_rng(4).integers(0, 1000, (5, 3))
+    labels[:, 0] = logits.argmax(1)
+    want = ref.log_probs(logits.astype(np.float64), labels, 2.0 ** -14, 5)
+    floats = np.asarray(images, np.float32).reshape(5, 224, 224, 3).transpose(0, 3, 1, 2) * \
+        np.float32(2.0 ** params.patch.image_scale_exp)
+    for x in (images, np.ascontiguousarray(floats)):
+        got = model.score_batch(x, params, labels)
+        for name in ("logp", "entropy", "top_logp"):
+            off = np.abs(getattr(got, name).astype(np.float64) - want[name])
+            assert (off <= want[name + "_bound"]).all(), name
+        assert np.array_equal(got.top_index, want["top_index"])
+        assert np.array_equal(got.top_index[:, 0], labels[:, 0])
+    one = model.score_batch(images, params, labels[:, 1], top=0)
+    assert np.array_equal(one.logp, got.logp[:, 1]) and one.top_index is None
+    assert model.score_batch(images, params, top=1).logp is None
+    for bad, error in ((labels[:4], ValueError), (labels + 1000, ValueError), (-labels - 1, ValueError),
+                       (labels.astype(float), TypeError)):
+        with pytest.raises(error):
+            model.score_batch(images, params, bad)
+    with pytest.raises(ValueError):
+        model.score_batch(images, params, top=65)
 
 
 def test_step_in_a_graph_and_on_streams():
