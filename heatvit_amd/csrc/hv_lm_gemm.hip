@@ -105,32 +105,28 @@ __device__ __forceinline__ int channel_of(int j, int grp) {
 }
 
 // One lane's outputs of FM x FN fragments: rows m0 + 16 i, parts j0 .. of the
-// group of 64 at n0.
-template <typename T, int FM, int FN>
+// group of 64 at n0. scale(i) and bias(n): a row's factor, a channel's addend.
+template <typename T, int FM, int FN, typename Scale, typename Bias>
 __device__ __forceinline__ void store_tile(const GemmF8Args &g, int rows, int m0, int n0, int j0,
-                                           int grp, const v4f (&acc)[FM][FN]) {
+                                           int grp, const v4f (&acc)[FM][FN], Scale scale,
+                                           Bias bias) {
   constexpr int RUN = FN >= 2 ? 8 : 4;
-  float bias[FN][4] = {}, scale[FM];
-  if (g.bias) {
+  float add[FN][4];
 #pragma unroll
-    for (int j = 0; j < FN; ++j)
+  for (int j = 0; j < FN; ++j)
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        bias[j][k] = g.bias[min(n0 + channel_of(j0 + j, grp) + k, g.n - 1)];
-  }
-#pragma unroll
-  for (int i = 0; i < FM; ++i)
-    scale[i] = g.row_scale ? g.row_scale[min(m0 + 16 * i, rows - 1)] : 1.f;
+    for (int k = 0; k < 4; ++k) add[j][k] = bias(n0 + channel_of(j0 + j, grp) + k);
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
     const int m = m0 + 16 * i;
     if (m >= rows) continue;
+    const float f = scale(i);
 #pragma unroll
     for (int j = 0; j < FN; j += RUN / 4) {
       float v[RUN];
 #pragma unroll
       for (int k = 0; k < RUN; ++k)
-        v[k] = __builtin_fmaf(acc[i][j + k / 4][k % 4], scale[i], bias[j + k / 4][k % 4]);
+        v[k] = __builtin_fmaf(acc[i][j + k / 4][k % 4], f, add[j + k / 4][k % 4]);
       store_run<T, RUN>(g, m, n0 + channel_of(j0 + j, grp), v);
     }
   }
@@ -212,7 +208,11 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_f8_rows(GemmF8Args g) {
 #pragma unroll
     for (int k = 1; k < NW; ++k) v += part[k][f][lane];
     const v4f one[1][1] = {{v}};
-    store_tile<T>(g, rows, m0 + 16 * (f / J) + col, group * 64, j0 + f % J, grp, one);
+    const int m = m0 + 16 * (f / J) + col;
+    store_tile<T>(
+        g, rows, m, group * 64, j0 + f % J, grp, one,
+        [&](int) { return g.row_scale ? g.row_scale[m] : 1.f; },
+        [&](int n) { return g.bias ? g.bias[min(n, g.n - 1)] : 0.f; });
   }
 }
 
@@ -286,6 +286,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm_f8_tile(GemmF8Args g) {
   auto &stage3 = reinterpret_cast<TileLds<BM, BN> &>(stage3_);
   __shared__ uint8_t a_exp[kExpSteps][WM][16][FM];
   __shared__ uint8_t w_exp[kExpSteps][NB];
+  __shared__ float row_scale[BM], bias[BN];
 
   const int rows = g.m_dev ? min(g.m, *g.m_dev) : g.m;
   int m0, n0;
@@ -445,8 +446,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm_f8_tile(GemmF8Args g) {
     read_exps(b, 0);
   };
 
-  load_exps(0, std::true_type());
   // Blocks 0 .. S - 2 and the first half of S - 1, which goes on in step 0.
+  // Everything that the tile needs later is asked for beside them.
 #pragma unroll
   for (int q = 0; q < 4; ++q) load(stage0, 0, q);
   if (S == 4) {
@@ -455,6 +456,13 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm_f8_tile(GemmF8Args g) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) load(stage2, 2, q);
   }
+#pragma unroll
+  for (int i = tid; i < BM; i += 64 * kWaves)
+    row_scale[i] = g.row_scale ? g.row_scale[m0 + min(i, last)] : 1.f;
+#pragma unroll
+  for (int i = tid; i < BN; i += 64 * kWaves)
+    bias[i] = g.bias ? g.bias[min(n0 + i, g.n - 1)] : 0.f;
+  load_exps(0, std::true_type());
   meet();
   load(S == 4 ? stage3 : stage1, S - 1, 0);
   load(S == 4 ? stage3 : stage1, S - 1, 1);
@@ -490,7 +498,9 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm_f8_tile(GemmF8Args g) {
   }
   __builtin_amdgcn_s_waitcnt(0x0070);  // the loads behind the last block
 
-  store_tile<T>(g, rows, m0 + wm * TM + col, n0 + wn * TN / 64 * 64, wn * TN % 64 / 16, grp, acc);
+  store_tile<T>(
+      g, rows, m0 + wm * TM + col, n0 + wn * TN / 64 * 64, wn * TN % 64 / 16, grp, acc,
+      [&](int i) { return row_scale[wm * TM + 16 * i + col]; }, [&](int n) { return bias[n - n0]; });
 }
 
 template <typename T, int BM, int BN, int WM, int WN, int S>
