@@ -192,9 +192,7 @@ def _declare(L):
     L.hv_schedule_bind.argtypes = [C.POINTER(Schedule), _vp, C.c_size_t, _vp, C.c_size_t,
                                    C.POINTER(ModelDev), _vp]
     L.hv_rms_norm_q8.argtypes = [C.POINTER(RmsNormDesc), _vp]
-    L.hv_gemm_f8_workspace_bytes.restype = C.c_size_t
-    L.hv_gemm_f8_workspace_bytes.argtypes = [C.c_int, C.c_int, C.c_int]
-    L.hv_gemm_f8.argtypes = [C.POINTER(GemmF8Desc), _vp, C.c_size_t, _vp]
+    L.hv_gemm_f8.argtypes = [C.POINTER(GemmF8Desc), _vp]
     L.hv_log_probs_workspace_bytes.restype = C.c_size_t
     L.hv_log_probs_workspace_bytes.argtypes = [C.c_int, C.c_int, C.c_int]
     L.hv_log_probs.argtypes = [C.POINTER(LogProbsDesc), _vp, C.c_size_t, _vp]
@@ -227,5 +225,5 @@ def exported_symbols():
             "hv_model_workspace_bytes", "hv_model_forward", "hv_model_forward_f32",
             "hv_model_forward_ex", "hv_model_forward_f32_ex",
             "hv_quantize_images", "hv_schedule_compile", "hv_schedule_packed_bytes",
-            "hv_schedule_bind", "hv_rms_norm_q8", "hv_gemm_f8_workspace_bytes", "hv_gemm_f8",
+            "hv_schedule_bind", "hv_rms_norm_q8", "hv_gemm_f8",
             "hv_log_probs_workspace_bytes", "hv_log_probs")

@@ -199,12 +199,12 @@ template <typename T>
 __device__ void largest_keys_slow(const T *x, int lo, int hi, int top, u64 *out) {
   typedef typename Logit<T>::type V;
   __shared__ u64 wave_key[kAnswerWaves];
-  u64 last = ~0ull;
+  u64 last = 0;
   for (int k = 0; k < top; ++k) {
     u64 best = 0;
     for (int c = lo + threadIdx.x; c < hi; c += kThreads) {
       const u64 key = key_of((V)x[c], c);
-      if (key < last && key > best) best = key;
+      if ((k == 0 || key < last) && key > best) best = key;
     }
     for (int o = 32; o; o >>= 1) {
       const u64 other = __shfl_xor(best, o);

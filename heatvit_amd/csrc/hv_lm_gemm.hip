@@ -564,14 +564,7 @@ using namespace hv;
 
 extern "C" {
 
-size_t hv_gemm_f8_workspace_bytes(int m, int n, int k) {
-  (void)m; (void)n; (void)k;
-  return 0;
-}
-
-int hv_gemm_f8(const hv_gemm_f8_desc *d, void *workspace, size_t workspace_bytes,
-               hv_stream_t stream) {
-  (void)workspace; (void)workspace_bytes;
+int hv_gemm_f8(const hv_gemm_f8_desc *d, hv_stream_t stream) {
   clear_error();
   if (!d) return fail(HV_EVALUE, HV_ERR_ADDRESS, "gemm_f8: null descriptor");
   if (d->type != HV_T_F32 && d->type != HV_T_F16 && d->type != HV_T_BF16)

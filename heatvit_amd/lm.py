@@ -10,7 +10,8 @@ answer of rows of floating-point activations.
 
 Inputs and results are torch tensors on one GPU; every call only enqueues its
 kernels on that GPU's current stream and may be captured into a HIP graph
-(with `out=` and `workspace=`, or with the capture's own allocations).
+(with `out=` and `workspace=`, or with the capture's own allocations; a
+workspace serves one call at a time).
 `live_rows`, an int32 tensor of one value on the device, gives the rows that
 count; rows behind it are left as they were.  Results that the caller does
 not pass in `out` are new tensors.  There is no gradient: the inputs are taken
@@ -177,7 +178,7 @@ def rms_norm_q8(x, weight, *, residual=None, eps=1e-6, fmt="e4m3", block=F8_BLOC
 
 
 def gemm_f8(a, a_exps, w, *, row_scale=None, bias=None, out_dtype=torch.bfloat16, live_rows=None,
-            out=None, workspace=None):
+            out=None):
     """row_scale[m] * sum_k a[m][k] 2^a_exps[m][k/128] W[k][n] 2^w_exps[k/128][n/128]
     + bias[n], rounded once to out_dtype.  A float32 output is summed in
     float32 from exact products; a 16-bit one on the 8-bit matrix cores, which
@@ -206,15 +207,12 @@ def gemm_f8(a, a_exps, w, *, row_scale=None, bias=None, out_dtype=torch.bfloat16
         ldc = _given_matrix("out", out, (rows, width), out_dtype)
     if not a.is_cuda:
         raise ValueError("the inputs must be on a GPU")
-    L = _lib.lib()
-    workspace, ws_at, ws_size = _workspace(
-        workspace, L.hv_gemm_f8_workspace_bytes(rows, width, inner), a)
     d = _lib.GemmF8Desc(
         a.data_ptr(), a_exps.data_ptr(), w.packed.data_ptr(), w.exps.data_ptr(), _ptr(row_scale),
         _ptr(bias), out.data_ptr(), _live(live_rows), lda, exps_ld, ldc, rows, width, inner,
         _TYPES[out_dtype])
-    _call(L.hv_gemm_f8, "gemm_f8", a.get_device(),
-          (a_exps, w.packed, row_scale, bias, out, live_rows, workspace), d, ws_at, ws_size)
+    _call(_lib.lib().hv_gemm_f8, "gemm_f8", a.get_device(),
+          (a_exps, w.packed, row_scale, bias, out, live_rows), d)
     return out
 
 

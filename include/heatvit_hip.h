@@ -474,9 +474,7 @@ typedef struct {
   int32_t m, n, k, type;
 } hv_gemm_f8_desc;
 
-size_t hv_gemm_f8_workspace_bytes(int m, int n, int k);
-int hv_gemm_f8(const hv_gemm_f8_desc *d, void *workspace, size_t workspace_bytes,
-               hv_stream_t stream);
+int hv_gemm_f8(const hv_gemm_f8_desc *d, hv_stream_t stream);
 
 /* Log probabilities of given tokens under softmax(scale * logits), the
  * entropy, and the `top` most probable tokens in order (equal logits by the
@@ -485,7 +483,9 @@ int hv_gemm_f8(const hv_gemm_f8_desc *d, void *workspace, size_t workspace_bytes
  * nothing and gets 0, one past the width NaN.  Logits of -inf have
  * probability 0; a row of nothing else gets log probabilities of -inf and
  * entropy 0.  A NaN or +inf makes the row's log probabilities and entropy
- * NaN; a NaN counts as the largest logit.  rows_dev as above. */
+ * NaN; a NaN counts as the largest logit.  scale lies in (0, 1e30].  rows_dev
+ * as above.  The workspace (8-byte aligned) holds what the parts of a row
+ * leave, for the call alone; calls that overlap need one each. */
 #define HV_LOG_PROBS_MAX_TOP 64
 
 typedef struct {

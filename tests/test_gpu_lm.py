@@ -420,6 +420,48 @@ def test_answer_orders(kind, width):
         _check_answer(got, x.double().numpy(), None, 2.0 ** e, top)
 
 
+@pytest.mark.parametrize("kind", ("bf16", "f32", "i32"))
+def test_answer_more_equal_logits_than_candidates(kind):
+    """Rows that are flat, or flat but for a few logits, past what the
+    alternatives are picked from, the largest values of the type among them."""
+    from heatvit_amd import lm
+    width = 20000
+    x = torch.zeros(6, width)
+    x[1, 19990:] = 1.0
+    x[2, ::2] = -3.0
+    x[4] = torch.arange(width) % 2
+    x = x.to(torch.int32) if kind == "i32" else x.to(TYPES[kind])
+    x[3] = 2 ** 31 - 1 if kind == "i32" else torch.finfo(TYPES[kind]).max
+    x[5] = -2 ** 31 if kind == "i32" else torch.finfo(TYPES[kind]).min
+    for rows in (slice(0, 6), slice(3, 4), slice(4, 6)):
+        part = x[rows]
+        got = lm.log_probs(part.cuda(), scale_exp=-2, top=17)
+        _check_answer(got, part.double().numpy(), None, 0.25, 17)
+    big = x.repeat(100, 1)  # a row to each workgroup
+    got = lm.log_probs(big.cuda(), scale_exp=-2, top=3)
+    _check_answer(got, big.double().numpy(), None, 0.25, 3)
+
+
+@pytest.mark.parametrize("rows", (1, 600))
+def test_answer_nan_and_few_left_in_wide_rows(rows):
+    """NaN at either end of a wide row (in parts, and a row to a workgroup),
+    and rows whose mask leaves fewer logits than alternatives."""
+    from heatvit_amd import lm
+    width = 20011
+    for at in (0, 9000, width - 1):
+        x = torch.randn(rows, width, generator=_gen(at))
+        x[-1, at] = float("nan")
+        got = lm.log_probs(x.cuda(), top=4)
+        assert got.entropy[-1].isnan() and got.top_logp[-1].isnan().all()
+        want = x[-1].clone()
+        want[at] = float("inf")
+        assert got.top_index[-1].tolist() == torch.sort(want, descending=True, stable=True)[1][:4].tolist()
+    x = torch.full((rows, width), -float("inf"))
+    x[:, 7], x[:, 12345] = 1.0, 2.0
+    got = lm.log_probs(x.cuda(), torch.full((rows,), 7, dtype=torch.int32).cuda(), top=20)
+    _check_answer(got, x.double().numpy(), np.full((rows, 1), 7), 1.0, 20)
+
+
 def test_answer_int32_range():
     """int32 logits over their whole range: differences past 2^31."""
     from heatvit_amd import lm

@@ -200,9 +200,9 @@ def test_gemm_c_refusals(library):
         v = dict(a=PTR, a_exps=PTR, w_packed=PTR, w_exps=PTR, c=PTR, lda=256, a_exps_ld=2, ldc=64,
                  m=4, n=64, k=256, type=_lib.HV_T_BF16)
         v.update(k)
-        return L.hv_gemm_f8(_lib.GemmF8Desc(**v), None, 0, None)
+        return L.hv_gemm_f8(_lib.GemmF8Desc(**v), None)
 
-    _refused(L, L.hv_gemm_f8(None, None, 0, None), _lib.HV_ERR_ADDRESS)
+    _refused(L, L.hv_gemm_f8(None, None), _lib.HV_ERR_ADDRESS)
     for k in (dict(type=3), dict(type=-1)):
         _refused(L, call(**k), _lib.HV_ERR_OPCODE)
     for k in (dict(m=-1), dict(n=0), dict(k=0), dict(k=250), dict(n=(1 << 22) + 1),
