@@ -545,7 +545,7 @@ static void gemm_f8_launch(const GemmF8Args &g, hipStream_t s) {
     return t <= 256 ? one : (t + 511) / 512 * two;
   };
   const int64_t c64 = cost(tiles(64), kF32 ? 21 : 10, kF32 ? 28 : 16);
-  if (kF32) {
+  if constexpr (kF32) {
     if (c64 <= cost(tiles(128), 46, 66)) return tile_launch<T, 64, 64, 1, 4, 4>(g, s);
     return tile_launch<T, 128, 128, 2, 2, 2>(g, s);
   } else {
