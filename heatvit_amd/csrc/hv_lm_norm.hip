@@ -176,13 +176,14 @@ static void norm_launch(const NormArgs &a, bool row, hipStream_t s) {
 // 9.1, 22.4, 55, 190; 50432 x 192 13.5, 18.5, 44, 150; 16384 x 768 17.7, 17.0,
 // 19.5, 53; 8192 x 2048 32.2, 26.5, 25.0, 41), long rows and few rows many,
 // whose loads are then on their way at once (16384 x 8192 228, 185, 174, 164;
-// 32 x 8192 50, 14.1, 5.2, 3.6; 512 x 4096 32.7, 9.6, 5.0, 4.9).
+// 32 x 8192 50, 14.1, 5.2, 3.6; 512 x 4096 32.7, 9.6, 5.0, 4.9). A launch has
+// less than 2^32 threads.
 template <typename T, int FMT>
 static void norm_launch(const NormArgs &a, bool row, hipStream_t s) {
   const bool few = a.rows <= 512;
   if (a.width <= (few ? 128 : 512)) return norm_launch<T, FMT, 16>(a, row, s);
   if (a.width <= (few ? 512 : 1024)) return norm_launch<T, FMT, 64>(a, row, s);
-  if (a.width <= (few ? 2048 : 8191)) return norm_launch<T, FMT, 256>(a, row, s);
+  if (a.width <= (few ? 2048 : 8191) || a.rows >= 1 << 22) return norm_launch<T, FMT, 256>(a, row, s);
   norm_launch<T, FMT, 1024>(a, row, s);
 }
 
@@ -206,7 +207,8 @@ extern "C" int hv_rms_norm_q8(const hv_rms_norm_desc *d, hv_stream_t stream) {
   if (d->block != 0 && d->block != kNormBlock)
     return fail(HV_EVALUE, HV_ERR_DIMENSION, "rms_norm: block %d is neither 128 nor 0 (the row)",
                 d->block);
-  if (d->rows < 0 || d->width < 1 || d->width > HV_NORM_MAX_WIDTH)
+  if (d->rows < 0 || d->rows > HV_LM_MAX_ROWS || d->width < 1 ||
+      d->width > HV_NORM_MAX_WIDTH)
     return fail(HV_EVALUE, HV_ERR_DIMENSION, "rms_norm: %d rows of %d columns", d->rows, d->width);
   if (!(d->eps >= 0.f) || d->eps > 3e38f)
     return fail(HV_EVALUE, HV_ERR_DIMENSION, "rms_norm: eps must be finite and not negative");

@@ -410,6 +410,7 @@ int hv_model_forward_f32_ex(const hv_model_dev *p, const float *images, int batc
 #define HV_Q_E4M3 0 /* OCP e4m3 (largest 448, NaN, no infinities) */
 #define HV_Q_I8 1   /* int8 in [-127, 127]                        */
 
+#define HV_LM_MAX_ROWS ((1 << 24) - 1) /* norm and log probabilities: a launch's threads */
 #define HV_NORM_MAX_WIDTH (1 << 20)
 
 /* Root-mean-square norm of rows with the residual's addition, in 8 bits:

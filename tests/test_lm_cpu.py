@@ -181,7 +181,8 @@ def test_norm_c_refusals(library):
     _refused(L, L.hv_rms_norm_q8(None, None), _lib.HV_ERR_ADDRESS)
     for k in (dict(type=3), dict(type=-1), dict(format=2)):
         _refused(L, L.hv_rms_norm_q8(desc(**k), None), _lib.HV_ERR_OPCODE)
-    for k in (dict(block=64), dict(rows=-1), dict(width=0), dict(width=(1 << 20) + 1),
+    for k in (dict(block=64), dict(rows=-1), dict(rows=1 << 24), dict(width=0),
+              dict(width=(1 << 20) + 1),
               dict(eps=-1.0), dict(eps=float("nan")), dict(eps=float("inf")), dict(x_ld=255),
               dict(q_ld=8), dict(exps_ld=1), dict(residual=PTR, residual_out=PTR, residual_ld=8,
                                                   residual_out_ld=256)):
@@ -229,8 +230,8 @@ def test_answer_c_refusals(library):
     _refused(L, L.hv_log_probs(None, None, 0, None), _lib.HV_ERR_ADDRESS)
     for k in (dict(type=4), dict(type=-1)):
         _refused(L, call(**k), _lib.HV_ERR_OPCODE)
-    for k in (dict(rows=-1), dict(width=0), dict(n_tokens=-1), dict(logits_ld=99),
-              dict(tokens_ld=1), dict(top=-1), dict(top=65), dict(top=101), dict(scale=0.0),
+    for k in (dict(rows=-1), dict(rows=1 << 24), dict(width=0), dict(n_tokens=-1),
+              dict(logits_ld=99), dict(tokens_ld=1), dict(top=-1), dict(top=65), dict(top=101), dict(scale=0.0),
               dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf"))):
         _refused(L, call(**k), _lib.HV_ERR_DIMENSION)
     for k in (dict(logits=None), dict(entropy=None), dict(tokens=None), dict(logp=None),
