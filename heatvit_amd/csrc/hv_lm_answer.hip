@@ -7,6 +7,12 @@
 // The order of the alternatives is that of the logits themselves, equal ones
 // by the lower index: a 64-bit key holds the value's ordered bits above the
 // complemented index, and no two keys are equal.
+//
+// The logits' bytes bound it: 2048 rows of 131072 bf16 logits with five
+// alternatives take 109 us, which is the rate of a large copy (4.9 TB/s); passes
+// for the maximum, the sums and each alternative apart took 1984. One row of
+// 131072 with 20 takes 9.6 and 4.4 us in its two kernels, 256 rows of 1000 int32
+// logits with five 6.8.
 #include <type_traits>
 
 #include "hv_lm.h"
@@ -149,8 +155,8 @@ __device__ __forceinline__ void rank_keys(const u64 *keys, int m, int top, u64 *
 // thread's largest. For a small `top` the threads fall into at least that many
 // classes (thread mod classes): their largest values are different logits', and
 // the least of them bounds, loosely (about top log(top) logits reach it). For a
-// large one it is the `top`-th largest of the threads' values itself, which
-// takes a comparison of each with each.
+// large one, where that would be many, it is the `top`-th largest of the
+// threads' values itself, which takes a comparison of each with each.
 static constexpr int kClassTop = 8;
 template <typename V>
 __device__ V bound_of(V best, int top) {
@@ -194,7 +200,9 @@ __device__ V bound_of(V best, int top) {
 }
 
 // The `top` largest keys of logits [lo, hi) by as many passes over them, for a
-// row with a NaN or +inf in it, or with more equal logits than kKeep.
+// row with a NaN or +inf in it, or with more than kKeep logits that reach the
+// bound, which takes equal ones (2048 rows of 131072 equal logits: 0.68 ms for
+// the largest, 2.3 for five, 8.3 for 20).
 template <typename T>
 __device__ void largest_keys_slow(const T *x, int lo, int hi, int top, u64 *out) {
   typedef typename Logit<T>::type V;
@@ -262,7 +270,9 @@ __device__ void write_answer(const AnswerArgs &a, int64_t row, const T *x, const
 // One workgroup a row or a part of one, in one pass: each thread keeps a running
 // maximum with its sums, and for the alternatives the maxima of up to kSlots
 // stretches of its logits. These give a bound that the `top` largest logits are
-// not under, and only the few stretches that reach it are read again.
+// not under, and only the few stretches that reach it are read again (2048 x
+// 131072: 109 us with five, 97 without; a list of candidates kept up with a
+// rising bound in the pass itself took 145).
 template <typename T, bool TOP>
 __global__ __launch_bounds__(kThreads) void k_log_probs(AnswerArgs a) {
   typedef Logit<T> L;
@@ -466,7 +476,8 @@ __global__ __launch_bounds__(kThreads) void k_log_probs_join(AnswerArgs a) {
 
 // Parts of a row. A row is read by one workgroup where there are rows enough
 // to keep the card busy; fewer rows are cut until kAnswerGroups workgroups
-// are at work, in parts of at least kMinPart logits.
+// are at work, in parts of at least kMinPart logits (of 4096 and of 8192: 1 row
+// of 131072 with 20 alternatives 14.6, 13.5 us; 16 rows 15.8, 14.0).
 static constexpr int kAnswerGroups = 512, kMinPart = 8192;
 static int answer_parts(int rows, int width, int *part_width) {
   int parts = (int)((kAnswerGroups + (int64_t)rows - 1) / (rows > 0 ? rows : 1));

@@ -276,6 +276,39 @@ def test_gemm_every_exponent():
         assert np.array_equal(got[fine], want[fine]), e
 
 
+@pytest.mark.parametrize("size", ((255, 32000), (16, 8300)), ids=str)
+def test_gemm_far_exponents_beside_near_ones(size):
+    """The same where a float32 output's conversion applies the factors, with
+    rows of factors inside and outside what it takes beside each other, and a
+    far smaller block behind another (264 additions of 2^-23 each)."""
+    from heatvit_amd import lm
+    from heatvit_amd.device import DeviceF8Weight
+    m, n = size
+    a, w = _whole((m, 256), 1), _whole((256, n), 2)
+    ae = torch.arange(-127, 128).to(torch.int8)[torch.arange(m) * (255 // m)][:, None]
+    w64 = w.double().cuda()
+    for e in (-127, -60, 0, 60, 120):
+        for second in (None, -127):
+            exps = ae.repeat(1, 2)
+            if second is not None:
+                exps[:, 1] = second
+            dw = DeviceF8Weight(w, torch.full((2, -(-n // 128)), e, dtype=torch.int8))
+            got = lm.gemm_f8(a.cuda(), exps.cuda(), dw, out_dtype=torch.float32)
+            factor = torch.exp2(exps.double().cuda() + e)
+            x = a.double().cuda()
+            want = (x[:, :128] * factor[:, :1]) @ w64[:128]
+            total = ae[:, 0].int() + e
+            fine = (total >= -126) & (total <= 113)
+            want += (x[:, 128:] * factor[:, -1:]) @ w64[128:]
+            if second is None:  # whole multiples, below 2^12, of one unit: exact
+                assert torch.equal(got[fine.cuda()], want[fine.cuda()].float()), e
+                continue
+            size = (x[:, :128].abs() * factor[:, :1]) @ w64[:128].abs() + \
+                (x[:, 128:].abs() * factor[:, -1:]) @ w64[128:].abs()
+            off = (got.double() - want).abs()
+            assert (off <= size * 264 * 2.0 ** -23 + 2.0 ** -126)[fine.cuda()].all(), e
+
+
 def test_gemm_nan_stays_in_its_row():
     """NaN in a row of `a`, at the last of k and in what follows the rows in
     memory, reaches that row alone."""
