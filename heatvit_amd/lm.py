@@ -82,6 +82,8 @@ def _given_matrix(name, t, shape, dtype):
         raise TypeError(f"{name} must be a tensor of {dtype}")
     if t.shape != shape:
         raise ValueError(f"{name} must have the shape {list(shape)}")
+    if t.is_contiguous():  # the strides need not be looked at
+        return shape[1]
     return _matrix(name, t, (dtype,))[2]
 
 
