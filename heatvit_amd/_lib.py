@@ -8,6 +8,7 @@ code of the failure (HV_ERR_*, heatvit_pkg.sv:109-118).
 """
 
 import ctypes as C
+import struct
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libheatvit_hip.so"
@@ -130,6 +131,14 @@ class LogProbsDesc(C.Structure):
         (n, _i32) for n in ("rows", "width", "type", "n_tokens", "top")] + [("scale", C.c_float)]
 
 
+def packer(desc):
+    """pack(*values): a descriptor's bytes, which an entry point takes as its
+    address (0.6 us a call where making the structure takes 1.4)."""
+    s = struct.Struct("".join(t._type_ for _, t in desc._fields_))  # native sizes and alignment
+    assert s.size == C.sizeof(desc)
+    return s.pack
+
+
 _LIB = None
 
 
@@ -191,11 +200,11 @@ def _declare(L):
     L.hv_schedule_packed_bytes.argtypes = [C.POINTER(Schedule)]
     L.hv_schedule_bind.argtypes = [C.POINTER(Schedule), _vp, C.c_size_t, _vp, C.c_size_t,
                                    C.POINTER(ModelDev), _vp]
-    L.hv_rms_norm_q8.argtypes = [C.POINTER(RmsNormDesc), _vp]
-    L.hv_gemm_f8.argtypes = [C.POINTER(GemmF8Desc), _vp]
+    L.hv_rms_norm_q8.argtypes = [_vp, _vp]
+    L.hv_gemm_f8.argtypes = [_vp, _vp]
     L.hv_log_probs_workspace_bytes.restype = C.c_size_t
     L.hv_log_probs_workspace_bytes.argtypes = [C.c_int, C.c_int, C.c_int]
-    L.hv_log_probs.argtypes = [C.POINTER(LogProbsDesc), _vp, C.c_size_t, _vp]
+    L.hv_log_probs.argtypes = [_vp, _vp, C.c_size_t, _vp]
     L.hv_profile_enable.argtypes = [C.c_int]
     L.hv_profile_read.argtypes = [_vp, _vp, C.c_int]
 

@@ -19,6 +19,7 @@ as they are, and the outputs require none.
 """
 
 import math
+import struct
 from typing import NamedTuple, Optional
 
 import torch
@@ -29,6 +30,8 @@ from .device import F8_BLOCK, DeviceF8Weight
 _TYPES = {torch.float32: _lib.HV_T_F32, torch.float16: _lib.HV_T_F16,
           torch.bfloat16: _lib.HV_T_BF16}
 _LOGIT_TYPES = {**_TYPES, torch.int32: _lib.HV_T_I32}
+_NORM, _GEMM, _ANSWER = (_lib.packer(d) for d in (_lib.RmsNormDesc, _lib.GemmF8Desc,
+                                                  _lib.LogProbsDesc))
 _FORMATS = {"e4m3": (_lib.HV_Q_E4M3, torch.float8_e4m3fn), "int8": (_lib.HV_Q_I8, torch.int8)}
 
 
@@ -87,32 +90,37 @@ def _given_matrix(name, t, shape, dtype):
     return _matrix(name, t, (dtype,))[2]
 
 
-def _call(entry, what, index, tensors, *args):
-    """The library call on the current stream of GPU `index`, where all of the
-    tensors are.  (The stream's handle comes from the getter behind
-    torch.cuda.current_stream(), which takes 2.4 us to wrap it.)"""
+def _call(entry, what, index, tensors, pack, values, *args):
+    """The library call, with the values as its descriptor, on the current
+    stream of GPU `index`, where all of the tensors are.  (The stream's handle
+    comes from the getter behind torch.cuda.current_stream(), which takes 2.4
+    us to wrap it.)"""
     for t in tensors:
         if t is not None and t.get_device() != index:
             raise ValueError(f"{what}: tensors on cuda:{index} and on {t.device}")
+    try:
+        d = pack(*values)
+    except (struct.error, OverflowError) as e:
+        raise ValueError(f"{what}: a size or number is out of range ({e})") from None
     if torch.cuda.current_device() == index:
-        rc = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+        rc = entry(d, *args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
-            rc = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+            rc = entry(d, *args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         raise _lib.error(rc, what)
 
 
 def _live(live_rows):
     if live_rows is None:
-        return None
+        return 0
     if live_rows.dtype != torch.int32 or live_rows.numel() != 1:
         raise ValueError("live_rows must be an int32 tensor of one value")
     return live_rows.data_ptr()
 
 
 def _ptr(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
 def _workspace(workspace, size, like):
@@ -168,14 +176,14 @@ def rms_norm_q8(x, weight, *, residual=None, eps=1e-6, fmt="e4m3", block=F8_BLOC
             raise ValueError("out.residual goes with residual")
         if kept is not None:
             kept_ld = _given_matrix("out.residual", kept, x.shape, dtype)
-    d = _lib.RmsNormDesc(
+    values = (
         x.data_ptr(), _ptr(residual), weight.data_ptr(), _ptr(kept), q.data_ptr(),
         exps.data_ptr(), scale.data_ptr(), _live(live_rows), x_ld, residual_ld, kept_ld, q_ld,
         exps_ld, rows, width, _TYPES[dtype], form, block, eps)
     if not x.is_cuda:
         raise ValueError("the inputs must be on a GPU")
     _call(_lib.lib().hv_rms_norm_q8, "rms_norm_q8", x.get_device(),
-          (weight, residual, q, exps, scale, kept, live_rows), d)
+          (weight, residual, q, exps, scale, kept, live_rows), _NORM, values)
     return out
 
 
@@ -209,12 +217,12 @@ def gemm_f8(a, a_exps, w, *, row_scale=None, bias=None, out_dtype=torch.bfloat16
         ldc = _given_matrix("out", out, (rows, width), out_dtype)
     if not a.is_cuda:
         raise ValueError("the inputs must be on a GPU")
-    d = _lib.GemmF8Desc(
+    values = (
         a.data_ptr(), a_exps.data_ptr(), w.packed.data_ptr(), w.exps.data_ptr(), _ptr(row_scale),
         _ptr(bias), out.data_ptr(), _live(live_rows), lda, exps_ld, ldc, rows, width, inner,
         _TYPES[out_dtype])
     _call(_lib.lib().hv_gemm_f8, "gemm_f8", a.get_device(),
-          (a_exps, w.packed, row_scale, bias, out, live_rows), d)
+          (a_exps, w.packed, row_scale, bias, out, live_rows), _GEMM, values)
     return out
 
 
@@ -270,10 +278,11 @@ def log_probs(logits, tokens=None, *, scale_exp=0, temperature=1.0, top=0, live_
     L = _lib.lib()
     workspace, ws_at, ws_size = _workspace(
         workspace, L.hv_log_probs_workspace_bytes(rows, width, top), logits)
-    d = _lib.LogProbsDesc(
+    values = (
         logits.data_ptr(), _ptr(tokens), _ptr(logp), entropy.data_ptr(), _ptr(top_logp),
         _ptr(top_index), _live(live_rows), ld, count, rows, width, _LOGIT_TYPES[logits.dtype],
         count, top, scale)
     _call(L.hv_log_probs, "log_probs", logits.get_device(),
-          (tokens, logp, entropy, top_logp, top_index, live_rows, workspace), d, ws_at, ws_size)
+          (tokens, logp, entropy, top_logp, top_index, live_rows, workspace), _ANSWER,
+          values, ws_at, ws_size)
     return out

@@ -676,3 +676,12 @@ def test_step_in_a_graph_and_on_streams():
         for out in many:
             for a, b in zip(out, want):
                 assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def test_numbers_that_no_descriptor_holds():
+    from heatvit_amd import lm
+    x = torch.zeros(2, 64).cuda()
+    for call in (lambda: lm.rms_norm_q8(x, x[0], eps=1e300), lambda: lm.rms_norm_q8(x, x[0], eps=-1.0),
+                 lambda: lm.log_probs(x, temperature=1e-300), lambda: lm.log_probs(x, scale_exp=200)):
+        with pytest.raises(ValueError):
+            call()

@@ -3,6 +3,7 @@ weight quantiser, and every refusal, of the Python entry points (before any
 GPU is touched) and of the C entry points (before any launch)."""
 
 import ctypes as C
+import struct
 from pathlib import Path
 
 import numpy as np
@@ -166,6 +167,18 @@ def _refused(L, rc, cls):
     assert L.hv_last_error()
 
 
+@pytest.mark.parametrize("desc", (_lib.RmsNormDesc, _lib.GemmF8Desc, _lib.LogProbsDesc))
+def test_packed_descriptors(desc):
+    """The packed bytes are the structure's, and a value too wide is an error."""
+    values = [0.5 if t is C.c_float else 3 + i for i, (_, t) in enumerate(desc._fields_)]
+    pack = _lib.packer(desc)
+    assert pack(*values) == bytes(desc(*values))
+    at = [t for _, t in desc._fields_].index(C.c_int32)
+    values[at] = 1 << 31
+    with pytest.raises(struct.error):
+        pack(*values)
+
+
 PTR = 4096  # never read: every call is refused, or has no rows
 
 
@@ -176,7 +189,7 @@ def test_norm_c_refusals(library):
         v = dict(x=PTR, weight=PTR, q=PTR, exps=PTR, scale=PTR, x_ld=256, q_ld=256, exps_ld=2,
                  rows=4, width=256, type=_lib.HV_T_BF16, format=_lib.HV_Q_E4M3, block=128, eps=1e-6)
         v.update(k)
-        return _lib.RmsNormDesc(**v)
+        return C.byref(_lib.RmsNormDesc(**v))
 
     _refused(L, L.hv_rms_norm_q8(None, None), _lib.HV_ERR_ADDRESS)
     for k in (dict(type=3), dict(type=-1), dict(format=2)):
@@ -201,7 +214,7 @@ def test_gemm_c_refusals(library):
         v = dict(a=PTR, a_exps=PTR, w_packed=PTR, w_exps=PTR, c=PTR, lda=256, a_exps_ld=2, ldc=64,
                  m=4, n=64, k=256, type=_lib.HV_T_BF16)
         v.update(k)
-        return L.hv_gemm_f8(_lib.GemmF8Desc(**v), None)
+        return L.hv_gemm_f8(C.byref(_lib.GemmF8Desc(**v)), None)
 
     _refused(L, L.hv_gemm_f8(None, None), _lib.HV_ERR_ADDRESS)
     for k in (dict(type=3), dict(type=-1)):
@@ -225,7 +238,7 @@ def test_answer_c_refusals(library):
                  logits_ld=100, tokens_ld=2, rows=4, width=100, type=_lib.HV_T_F32, n_tokens=2,
                  top=5, scale=1.0)
         v.update(k)
-        return L.hv_log_probs(_lib.LogProbsDesc(**v), None, 0, None)
+        return L.hv_log_probs(C.byref(_lib.LogProbsDesc(**v)), None, 0, None)
 
     _refused(L, L.hv_log_probs(None, None, 0, None), _lib.HV_ERR_ADDRESS)
     for k in (dict(type=4), dict(type=-1)):
