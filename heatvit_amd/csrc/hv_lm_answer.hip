@@ -521,8 +521,9 @@ int hv_log_probs(const hv_log_probs_desc *d, void *workspace, size_t workspace_b
   if (!d) return fail(HV_EVALUE, HV_ERR_ADDRESS, "log_probs: null descriptor");
   if (d->type < HV_T_F32 || d->type > HV_T_I32)
     return fail(HV_EVALUE, HV_ERR_OPCODE, "log_probs: bad element type %d", d->type);
-  if (d->rows < 0 || d->rows > HV_LM_MAX_ROWS || d->width < 1 || d->n_tokens < 0 ||
-      d->logits_ld < d->width || (d->n_tokens && d->tokens_ld < d->n_tokens))
+  if (d->rows < 0 || d->rows > HV_LM_MAX_ROWS || d->width < 1 ||
+      d->width > HV_LOG_PROBS_MAX_WIDTH || d->n_tokens < 0 ||
+      d->n_tokens > HV_LOG_PROBS_MAX_WIDTH || d->logits_ld < d->width || (d->n_tokens && d->tokens_ld < d->n_tokens))
     return fail(HV_EVALUE, HV_ERR_DIMENSION, "log_probs: %d rows of %d logits, %d tokens each",
                 d->rows, d->width, d->n_tokens);
   if (d->top < 0 || d->top > HV_LOG_PROBS_MAX_TOP || d->top > d->width)

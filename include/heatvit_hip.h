@@ -488,6 +488,7 @@ int hv_gemm_f8(const hv_gemm_f8_desc *d, hv_stream_t stream);
  * as above.  The workspace (8-byte aligned) holds what the parts of a row
  * leave, for the call alone; calls that overlap need one each. */
 #define HV_LOG_PROBS_MAX_TOP 64
+#define HV_LOG_PROBS_MAX_WIDTH (1 << 30) /* and of tokens asked for in a row */
 
 typedef struct {
   const void *logits;    /* [rows][logits_ld]           */

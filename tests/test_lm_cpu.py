@@ -244,6 +244,8 @@ def test_answer_c_refusals(library):
     for k in (dict(type=4), dict(type=-1)):
         _refused(L, call(**k), _lib.HV_ERR_OPCODE)
     for k in (dict(rows=-1), dict(rows=1 << 24), dict(width=0), dict(n_tokens=-1),
+              dict(width=(1 << 30) + 1, logits_ld=1 << 31),
+              dict(n_tokens=(1 << 30) + 1, tokens_ld=1 << 31),
               dict(logits_ld=99), dict(tokens_ld=1), dict(top=-1), dict(top=65), dict(top=101), dict(scale=0.0),
               dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf"))):
         _refused(L, call(**k), _lib.HV_ERR_DIMENSION)
