@@ -260,7 +260,7 @@ def log_probs(logits, tokens=None, *, scale_exp=0, temperature=1.0, top=0, live_
         entropy = logits.new_empty(rows, dtype=f32)
         if top:
             top_logp = logits.new_empty((rows, top), dtype=f32)
-            top_index = logits.new_empty((rows, top), dtype=torch.int32)
+            top_index = torch.empty_like(top_logp, dtype=torch.int32)
         out = LogProbs(logp, entropy, top_logp, top_index)
     else:
         logp, entropy, top_logp, top_index = out
