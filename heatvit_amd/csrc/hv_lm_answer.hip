@@ -77,6 +77,22 @@ struct Logit<int> {
   }
 };
 
+// The largest of the wavefront's, all lanes active.
+template <typename T>
+__device__ __forceinline__ typename Logit<T>::type wave_max(typename Logit<T>::type v) {
+  typedef Logit<T> L;
+  typedef typename L::type V;
+  v = L::larger(v, ror16<8>(v));
+  v = L::larger(v, ror16<4>(v));
+  v = L::larger(v, ror16<2>(v));
+  v = L::larger(v, ror16<1>(v));
+  const int bits = __builtin_bit_cast(int, v);
+  auto of = [&](int lane) {
+    return __builtin_bit_cast(V, __builtin_amdgcn_readlane(bits, lane));
+  };
+  return L::larger(L::larger(of(0), of(16)), L::larger(of(32), of(48)));
+}
+
 // Sum of 2^d and of 2^d d over logits, d = c (x - max), c = scale log2(e),
 // and the maximum they are relative to.
 template <typename T>
@@ -102,23 +118,11 @@ struct Sums {
     sum += e;
     weighted = __builtin_fmaf(e, fmaxf(d, -200.f), weighted);
   }
-  __device__ __forceinline__ void join(const Sums &o, float c) {
-    const typename L::type m = L::larger(max, o.max);
-    Sums t = o;
-    t.raise(m, c);
-    raise(m, c);
-    sum += t.sum;
-    weighted += t.weighted;
-  }
+  // The wavefront's, in every lane.
   __device__ __forceinline__ void join_lanes(float c) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) {
-      Sums t;
-      t.max = __shfl_xor(max, o);
-      t.sum = __shfl_xor(sum, o);
-      t.weighted = __shfl_xor(weighted, o);
-      join(t, c);
-    }
+    raise(wave_max<T>(max), c);
+    sum = sum64(sum);
+    weighted = sum64(weighted);
   }
 };
 
@@ -127,11 +131,6 @@ static constexpr int kMaxParts = 64;
 static constexpr int kThreads = 64 * kAnswerWaves;
 static constexpr int kSlots = 8;       // maxima that a thread keeps of its logits
 static constexpr int kKeep = 1024;     // candidates for the alternatives
-
-// The smallest power of two that is at least n.
-__device__ __forceinline__ int pow2_from(int n) {
-  return n <= 1 ? 1 : 1 << (32 - __builtin_clz(n - 1));
-}
 
 // The `top` largest of m different keys, in order: a key's place is the number
 // of larger ones.
@@ -152,51 +151,38 @@ __device__ __forceinline__ void rank_keys(const u64 *keys, int m, int top, u64 *
 }
 
 // A lower bound on the `top`-th largest of a workgroup's values, from each
-// thread's largest. For a small `top` the threads fall into at least that many
-// classes (thread mod classes): their largest values are different logits', and
-// the least of them bounds, loosely (about top log(top) logits reach it). For a
-// large one, where that would be many, it is the `top`-th largest of the
-// threads' values itself, which takes a comparison of each with each.
-static constexpr int kClassTop = 8;
-template <typename V>
-__device__ V bound_of(V best, int top) {
+// thread's largest: the `top`-th largest of 64 groups' maxima (threads of one
+// lane), which takes 64 comparisons and, while `top` is well below 64, lets few
+// more logits through; of all threads' for a larger one.
+static constexpr int kGroupsTop = 32;
+template <typename T>
+__device__ typename Logit<T>::type bound_of(typename Logit<T>::type best, int top) {
+  typedef Logit<T> L;
+  typedef typename L::type V;
   __shared__ V of_thread[kThreads];
   const int tid = threadIdx.x, lane = tid & 63;
-  if (top > kClassTop) {
-    of_thread[tid] = best;
-    __syncthreads();
-    int reach = 0;  // threads that reach this one's value
-#pragma unroll 16
-    for (int i = 0; i < kThreads; ++i) reach += of_thread[i] >= best;
-    V least = reach >= top ? best : Logit<V>::lowest();
-    for (int o = 32; o; o >>= 1) {
-      const V other = __shfl_xor(least, o);
-      least = other > least ? other : least;
-    }
-    __syncthreads();
-    if (lane == 0) of_thread[tid >> 6] = least;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kAnswerWaves; ++w) least = of_thread[w] > least ? of_thread[w] : least;
-    return least;
-  }
-  const int classes = pow2_from(top);
-  for (int o = 32; o >= classes; o >>= 1) {
-    const V other = __shfl_xor(best, o);
-    best = other > best ? other : best;
-  }
   of_thread[tid] = best;
   __syncthreads();
+  int reach = 0;  // maxima that reach this one
+  if (top <= kGroupsTop) {
 #pragma unroll
-  for (int w = 0; w < kAnswerWaves; ++w) {
-    const V other = of_thread[w * 64 + lane];
-    best = other > best ? other : best;
+    for (int w = 0; w < kAnswerWaves; ++w) best = L::larger(best, of_thread[w * 64 + lane]);
+    if (top == 1) return wave_max<T>(best);
+    const int bits = __builtin_bit_cast(int, best);
+#pragma unroll 16
+    for (int i = 0; i < 64; ++i)
+      reach += __builtin_bit_cast(V, __builtin_amdgcn_readlane(bits, i)) >= best;
+    return wave_max<T>(reach >= top ? best : L::lowest());
   }
-  for (int o = classes / 2; o; o >>= 1) {
-    const V other = __shfl_xor(best, o);
-    best = other < best ? other : best;
-  }
-  return best;
+#pragma unroll 16
+  for (int i = 0; i < kThreads; ++i) reach += of_thread[i] >= best;
+  V least = wave_max<T>(reach >= top ? best : L::lowest());
+  __syncthreads();
+  if (lane == 0) of_thread[tid >> 6] = least;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kAnswerWaves; ++w) least = L::larger(least, of_thread[w]);
+  return least;
 }
 
 // The `top` largest keys of logits [lo, hi) by as many passes over them, for a
@@ -291,7 +277,7 @@ __global__ __launch_bounds__(kThreads) void k_log_probs(AnswerArgs a) {
   __shared__ u64 best[TOP ? HV_LOG_PROBS_MAX_TOP : 1];
   __shared__ uint16_t hits[TOP ? kSlots * kThreads : 1];
   __shared__ int n_keys, n_hits;
-  __shared__ V wave_max[kAnswerWaves];
+  __shared__ V of_wave[kAnswerWaves];
   __shared__ float wave_sum[2][kAnswerWaves];
 
   const Given<T> given(a.parts == 1 ? a : AnswerArgs{}, row, x);
@@ -363,22 +349,28 @@ __global__ __launch_bounds__(kThreads) void k_log_probs(AnswerArgs a) {
 
   s.join_lanes(c);
   if (lane == 0) {
-    wave_max[wave] = s.max;
+    of_wave[wave] = s.max;
     wave_sum[0][wave] = s.sum;
     wave_sum[1][wave] = s.weighted;
   }
   if (TOP && tid == 0) n_keys = n_hits = 0;
   V bound = L::lowest();
-  if (TOP) bound = bound_of<V>(highest, a.top);  // with a barrier
+  if (TOP) bound = bound_of<T>(highest, a.top);  // with a barrier
   else __syncthreads();
+  V m = of_wave[0];
+#pragma unroll
+  for (int w = 1; w < kAnswerWaves; ++w) m = L::larger(m, of_wave[w]);
+  s = Sums<T>();
+  s.max = m;
 #pragma unroll
   for (int w = 0; w < kAnswerWaves; ++w) {
     Sums<T> t;
-    t.max = wave_max[w];
+    t.max = of_wave[w];
     t.sum = wave_sum[0][w];
     t.weighted = wave_sum[1][w];
-    if (w == 0) s = t;
-    else s.join(t, c);
+    t.raise(m, c);
+    s.sum += t.sum;
+    s.weighted += t.weighted;
   }
   if (TOP) {
     auto keep = [&](V v, int at) {
