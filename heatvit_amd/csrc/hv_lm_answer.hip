@@ -153,7 +153,10 @@ __device__ __forceinline__ void rank_keys(const u64 *keys, int m, int top, u64 *
 // A lower bound on the `top`-th largest of a workgroup's values, from each
 // thread's largest: the `top`-th largest of 64 groups' maxima (threads of one
 // lane), which takes 64 comparisons and, while `top` is well below 64, lets few
-// more logits through; of all threads' for a larger one.
+// more logits through; of all threads' for a larger one (64 groups and all
+// threads: 1 row of 131072 with 9 alternatives 9.7, 11.4 us, with 32 11.4, 13.3,
+// with 50 14.7, 14.6, with 64 40.2, 16.1; 2048 rows with 32 113.9, 114.1, with 50
+// 125.0, 117.8).
 static constexpr int kGroupsTop = 32;
 template <typename T>
 __device__ typename Logit<T>::type bound_of(typename Logit<T>::type best, int top) {
