@@ -546,15 +546,26 @@ static void gemm_f8_launch(const GemmF8Args &g, hipStream_t s) {
   // Up to 16 rows (us at k = 4096): the weights' bytes bound them, and parts of
   // 16 channels keep every CU busy up to 8192 channels; wider weights take two
   // parts a workgroup (1 row by 4096 channels 4.8, two parts 4.9; by 14336
-  // 12.1, 10.4; by 131072 97.7, 88.1). Up to 32 rows while that leaves few
-  // workgroups (24 by 4096 7.3, tiles 9.3; by 14336 25.4, tiles 12.7).
+  // 12.1, 10.4; by 131072 97.7, 88.1).
   const int parts = (g.n + 63) / 64 * 4;
   const bool near = g.lda < (int64_t)1 << 22;  // a tile's offsets into the rows are 32-bit
   if (g.m <= 16 || !near) {
     if (parts <= 512) return rows_launch<T, 1, 1, 8>(g, s);
     return rows_launch<T, 1, 2, 8>(g, s);
   }
-  if (g.m <= 32 && parts <= 256) return rows_launch<T, 2, 1, 8>(g, s);
+  // More rows, few channels: 16 or 32 rows (float32 outputs, whose tiles' products
+  // take longer, 64 too) by 16 channels while that is at most a workgroup a CU,
+  // since its wavefronts share the blocks of k (us at k = 4096 by 16 rows, 32 and
+  // 64, and tiles; bf16: 64 rows by 1000 channels 5.5, 8.0, 13.2, 8.7; by 2048 8.6,
+  // 8.2, 13.5, 9.1; by 4096 15.3, 14.3, 13.9, 9.7; float32: 5.7, 8.4, 13.7, 19.4;
+  // 9.2, 9.0, 14.2, 19.7; 17.0, 16.3, 15.0, 19.8; 100 by 4096 25.1, 24.9, 23.9,
+  // 20.0).
+  constexpr bool kF32 = std::is_same<T, float>::value;
+  auto lone = [&](int rows) { return (int64_t)parts * ((g.m + rows - 1) / rows) <= 256; };
+  if (lone(16)) return rows_launch<T, 1, 1, 8>(g, s);
+  if (lone(32)) return rows_launch<T, 2, 1, 8>(g, s);
+  if constexpr (kF32)
+    if (lone(64)) return rows_launch<T, 4, 1, 8>(g, s);
   // Tiles by what a block of k costs (measured at k = 4096, us a round of
   // tiles): small ones, several to a CU, where there are few, large ones, which
   // read less for each product, where they fill the card.
@@ -563,7 +574,6 @@ static void gemm_f8_launch(const GemmF8Args &g, hipStream_t s) {
   //   float32: 64 x 64 21 and 28; 128 x 128 46 and 66
   // 1024 x 4096 outputs: 30.0, 21.4, 26.3, 43.9 us; 2048 x 4096: 56.8, 41.8,
   // 35.8, 45.3; 4096 x 4096: 115, 83, 74, 56.
-  constexpr bool kF32 = std::is_same<T, float>::value;
   auto tiles = [&](int size) {
     return (int64_t)((g.m + size - 1) / size) * ((g.n + size - 1) / size);
   };
