@@ -175,6 +175,10 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_f8_rows(GemmF8Args g) {
   const uint8_t *w = g.w + (size_t)group * g.kb * kTileBytes + j0 * 2048 + lane * 16;
   const uint8_t *a[FM];
   const int8_t *ae[FM];
+  // Odd rows load the upper halves of their lines beside even rows' lower ones:
+  // rows lie whole lines apart as a rule, and one load of the same halves of 16
+  // lines takes longer (16 rows by 256 channels, k = 8192: 8.2 us, so 6.7).
+  const int odd = col & 1;
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
     const int64_t m = min(m0 + 16 * i + col, rows - 1);  // rows past the end repeat the last
@@ -186,7 +190,8 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_f8_rows(GemmF8Args g) {
   // first is waited for.
   auto blocks = [&](int b0, auto n_blocks) {
     constexpr int U = decltype(n_blocks)::value;
-    v8i wf[U][J], af[U][FM];
+    v8i wf[U][J];
+    v4i first[U][FM], second[U][FM];
     int we[U], e[U][FM];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -197,23 +202,28 @@ __global__ __launch_bounds__(64 * NW) void k_gemm_f8_rows(GemmF8Args g) {
             *reinterpret_cast<const v4i *>(w + (size_t)b * kTileBytes + j * 2048),
             *reinterpret_cast<const v4i *>(w + (size_t)b * kTileBytes + j * 2048 + 1024));
       we[u] = g.w_exps[(size_t)b * g.nb + group / 2] + 127;
-      const int k = b * 128 + 16 * grp;
-      const bool lo = k < g.k, hi = k + 64 < g.k;  // zeros past the end of k
+      const int k1 = b * 128 + 16 * grp + 64 * odd, k2 = k1 ^ 64;
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
-        const v4i x = *reinterpret_cast<const v4i *>(a[i] + (lo ? k : 0));
-        const v4i y = *reinterpret_cast<const v4i *>(a[i] + (hi ? k + 64 : 0));
-        af[u][i] = join(lo ? x : v4i{}, hi ? y : v4i{});
+        first[u][i] = *reinterpret_cast<const v4i *>(a[i] + (k1 < g.k ? k1 : 0));
+        second[u][i] = *reinterpret_cast<const v4i *>(a[i] + (k2 < g.k ? k2 : 0));
         e[u][i] = ae[i][b] + 127;
       }
     }
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       typename Mma::frag wo[J];
 #pragma unroll
       for (int j = 0; j < J; ++j) wo[j] = Mma::of(wf[u][j]);
+      const int k = (b0 + u * NW) * 128 + 16 * grp;
 #pragma unroll
-      for (int i = 0; i < FM; ++i) Mma::add(wo, af[u][i], acc[i], we[u], e[u][i]);
+      for (int i = 0; i < FM; ++i) {
+        v4i x = odd ? second[u][i] : first[u][i], y = odd ? first[u][i] : second[u][i];
+        if (k >= g.k) x = v4i{};  // zeros past the end of k
+        if (k + 64 >= g.k) y = v4i{};
+        Mma::add(wo, join(x, y), acc[i], we[u], e[u][i]);
+      }
     }
   };
   constexpr int U = FM * J >= 4 ? 2 : 4;
@@ -556,10 +566,10 @@ static void gemm_f8_launch(const GemmF8Args &g, hipStream_t s) {
   // More rows, few channels: 16 or 32 rows (float32 outputs, whose tiles' products
   // take longer, 64 too) by 16 channels while that is at most a workgroup a CU,
   // since its wavefronts share the blocks of k (us at k = 4096 by 16 rows, 32 and
-  // 64, and tiles; bf16: 64 rows by 1000 channels 5.5, 8.0, 13.2, 8.7; by 2048 8.6,
-  // 8.2, 13.5, 9.1; by 4096 15.3, 14.3, 13.9, 9.7; float32: 5.7, 8.4, 13.7, 19.4;
-  // 9.2, 9.0, 14.2, 19.7; 17.0, 16.3, 15.0, 19.8; 100 by 4096 25.1, 24.9, 23.9,
-  // 20.0).
+  // 64, and tiles; bf16: 64 rows by 1000 channels 4.8, 6.7, 10.5, 8.7; by 2048 7.4,
+  // 7.0, 11.0, 9.1; by 4096 13.2, 12.6, 11.4, 9.6; float32: 5.0, 7.2, 11.1, 19.3;
+  // 7.7, 7.7, 11.8, 19.7; 13.9, 14.0, 12.4, 19.9; 100 by 4096 20.8, 23.8, 20.0,
+  // 20.1).
   constexpr bool kF32 = std::is_same<T, float>::value;
   auto lone = [&](int rows) { return (int64_t)parts * ((g.m + rows - 1) / rows) <= 256; };
   if (lone(16)) return rows_launch<T, 1, 1, 8>(g, s);
