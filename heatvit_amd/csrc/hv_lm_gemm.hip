@@ -554,13 +554,14 @@ static void rows_launch(const GemmF8Args &g, hipStream_t s) {
 template <typename T>
 static void gemm_f8_launch(const GemmF8Args &g, hipStream_t s) {
   // Up to 16 rows (us at k = 4096): the weights' bytes bound them, and parts of
-  // 16 channels keep every CU busy up to 8192 channels; wider weights take two
-  // parts a workgroup (1 row by 4096 channels 4.8, two parts 4.9; by 14336
-  // 12.1, 10.4; by 131072 97.7, 88.1).
+  // 16 channels leave a CU a workgroup up to 4096 channels; wider weights take two
+  // parts a workgroup (1 row by 2048 channels 3.6, two parts 3.8; by 4096 5.2, 5.0;
+  // by 8192 9.0, 7.2; by 131072 104, 91; 16 rows to float32 by 2048 5.1, 5.6; by
+  // 8192 9.9, 8.5).
   const int parts = (g.n + 63) / 64 * 4;
   const bool near = g.lda < (int64_t)1 << 22;  // a tile's offsets into the rows are 32-bit
   if (g.m <= 16 || !near) {
-    if (parts <= 512) return rows_launch<T, 1, 1, 8>(g, s);
+    if (parts <= 256) return rows_launch<T, 1, 1, 8>(g, s);
     return rows_launch<T, 1, 2, 8>(g, s);
   }
   // More rows, few channels: 16 or 32 rows (float32 outputs, whose tiles' products
