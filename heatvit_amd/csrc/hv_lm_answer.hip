@@ -9,10 +9,10 @@
 // complemented index, and no two keys are equal.
 //
 // The logits' bytes bound it: 2048 rows of 131072 bf16 logits with five
-// alternatives take 109 us, which is the rate of a large copy (4.9 TB/s); passes
+// alternatives take 106 us, which is the rate of a large copy (4.9 TB/s); passes
 // for the maximum, the sums and each alternative apart took 1984. One row of
-// 131072 with 20 takes 9.6 and 4.4 us in its two kernels, 256 rows of 1000 int32
-// logits with five 6.7.
+// 131072 with 20 takes 7.4 and 4.7 us in its two kernels, 256 rows of 1000 int32
+// logits with five 6.4.
 #include <type_traits>
 
 #include "hv_lm.h"
@@ -260,7 +260,7 @@ __device__ void write_answer(const AnswerArgs &a, int64_t row, const T *x, const
 // maximum with its sums, and for the alternatives the maxima of up to kSlots
 // stretches of its logits. These give a bound that the `top` largest logits are
 // not under, and only the few stretches that reach it are read again (2048 x
-// 131072: 109 us with five, 97 without; a list of candidates kept up with a
+// 131072: 106 us with five, 96 without; a list of candidates kept up with a
 // rising bound in the pass itself took 145).
 template <typename T, bool TOP>
 __global__ __launch_bounds__(kThreads) void k_log_probs(AnswerArgs a) {

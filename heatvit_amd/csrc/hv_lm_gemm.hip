@@ -160,9 +160,9 @@ __device__ __forceinline__ void store_tile(const GemmF8Args &g, int rows, int m0
 // group of 64, its NW wavefronts every NW-th block of k each, and adds their
 // sums up through LDS in a fixed order. Fragments come straight from memory:
 // the packed weights are in the order the lanes take them, each read once.
-// One row by 4096 x 4096 takes 4.4 us beside a warm L2 and 6 from HBM (16.8 MB,
-// 3.4 us at a copy's rate): a wavefront has four blocks, all asked for at once,
-// so what is left over the bytes is one load's latency and the launch.
+// One row by 4096 x 4096 takes 5.2 us (16.8 MB, 3.4 us at a copy's rate): a
+// wavefront has four blocks, all asked for at once, so what is left over the
+// bytes is one load's latency and the launch.
 template <typename T, int FM, int J, int NW>
 __global__ __launch_bounds__(64 * NW) void k_gemm_f8_rows(GemmF8Args g) {
   typedef typename std::conditional<std::is_same<T, float>::value, Exact, Fast>::type Mma;
