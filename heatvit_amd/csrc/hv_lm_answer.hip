@@ -546,7 +546,8 @@ int hv_log_probs(const hv_log_probs_desc *d, void *workspace, size_t workspace_b
   if (a.parts > 1) {
     if (!workspace || ((uintptr_t)workspace & 7) ||
         workspace_bytes < hv_log_probs_workspace_bytes(a.rows, a.width, a.top))
-      return fail(HV_EVALUE, HV_ERR_ADDRESS, "log_probs: workspace too small or not 8-byte aligned");
+      return fail(HV_EVALUE, HV_ERR_ADDRESS,
+                  "log_probs: workspace too small or not 8-byte aligned");
     a.keys = (unsigned long long *)workspace;
     a.part = (AnswerPart *)(a.keys + (size_t)a.rows * a.parts * a.top);
   }

@@ -536,7 +536,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm_f8_tile(GemmF8Args g) {
 
   store_tile<T>(
       g, rows, m0 + wm * TM + col, n0 + wn * TN / 64 * 64, wn * TN % 64 / 16, grp, acc,
-      [&](int i) { return row_scale[wm * TM + 16 * i + col]; }, [&](int n) { return bias[n - n0]; });
+      [&](int i) { return row_scale[wm * TM + 16 * i + col]; },
+      [&](int n) { return bias[n - n0]; });
 }
 
 template <typename T, int BM, int BN, int WM, int WN, int S>

@@ -188,7 +188,8 @@ static void norm_launch(const NormArgs &a, bool row, hipStream_t s) {
   const bool few = a.rows <= 512;
   if (a.width <= (few ? 128 : 512)) return norm_launch<T, FMT, 16>(a, row, s);
   if (a.width <= (few ? 512 : 1024)) return norm_launch<T, FMT, 64>(a, row, s);
-  if (a.width <= (few ? 2048 : 8191) || a.rows >= 1 << 22) return norm_launch<T, FMT, 256>(a, row, s);
+  if (a.width <= (few ? 2048 : 8191) || a.rows >= 1 << 22)
+    return norm_launch<T, FMT, 256>(a, row, s);
   norm_launch<T, FMT, 1024>(a, row, s);
 }
 
