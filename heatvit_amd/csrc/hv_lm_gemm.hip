@@ -39,7 +39,8 @@ static constexpr int kTileBytes = 64 * 128;  // 64 channels by 128 k, packed
 
 // Products of one block of 128: FN fragments of W (16 channels each) by one of
 // the rows (16), added to acc with the factor 2^(we + ae - 254) of the scale
-// bytes in the low bits of we and ae; we is the same for the wavefront.
+// bytes in the low bits of we and ae, or NaN where one of them is 255 (an
+// exponent of -128); we is the same for the wavefront.
 struct Fast {
   typedef v8i frag;
   static __device__ __forceinline__ frag of(v8i raw) { return raw; }
@@ -53,6 +54,7 @@ struct Fast {
   }
 };
 struct Exact {
+  static constexpr int kNoFactor = 1 << 10;  // outside what the conversion applies
   struct frag {
     v8bf v[4];
   };
@@ -78,7 +80,9 @@ struct Exact {
   template <int FN>
   static __device__ __forceinline__ void add(const frag (&w)[FN], v8i raw, v4f (&acc)[FN], int we,
                                              int ae) {
-    const int e = (we & 255) + (ae & 255) - 254, in = FN > 1 ? min(max(e, -100), 100) : 0;
+    const int w8 = we & 255, a8 = ae & 255;
+    const int e = max(w8, a8) == 255 ? kNoFactor : w8 + a8 - 254;
+    const int in = FN > 1 ? min(max(e, -100), 100) : 0;
     const frag a = of(raw, __builtin_bit_cast(float, (in + 127) << 23));
     if (FN > 1 && __builtin_amdgcn_ballot_w64(in != e) == 0) {
 #pragma unroll
@@ -87,9 +91,10 @@ struct Exact {
         for (int j = 0; j < FN; ++j)
           acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[j].v[i], a.v[i], acc[j], 0, 0, 0);
     } else {
+      const float from = e == kNoFactor ? __builtin_nanf("") : 0.f;
 #pragma unroll
       for (int j = 0; j < FN; ++j) {
-        v4f t = {};
+        v4f t = {from, from, from, from};
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[j].v[i], a.v[i], t, 0, 0, 0);
@@ -426,9 +431,12 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm_f8_tile(GemmF8Args g) {
       for (int j = 0; j < kOnce; ++j) {
         const int i = (j0 + j) * 64 * kWaves + tid, r = i / kParts, b = i % kParts * 16;
 #pragma unroll
-        for (int k = 0; k < 16; ++k)  // e + 127 = (e ^ 128) - 1, e >= -127
+        for (int k = 0; k < 16; ++k) {
+          // e + 127 of four bytes at once, without a carry from one to the next
+          const unsigned x = v[j][k / 4];
           a_exp[b + k][r / TM][r % 16][r % TM / 16] =
-              (uint8_t)(((v[j][k / 4] ^ 0x80808080) - 0x01010101) >> (8 * (k % 4)));
+              (uint8_t)((((x & 0x7F7F7F7F) + 0x7F7F7F7F) ^ (x & 0x80808080)) >> (8 * (k % 4)));
+        }
       }
     }
 #pragma unroll 1

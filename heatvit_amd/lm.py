@@ -195,7 +195,7 @@ def gemm_f8(a, a_exps, w, *, row_scale=None, bias=None, out_dtype=torch.bfloat16
     cut a product's bits below 2^-13 of the largest one beside it.
 
     a [M][K] float8_e4m3fn and a_exps [M][ceil(K/128)] int8 (rms_norm_q8
-    writes both, and row_scale); w a DeviceF8Weight [K][N]; row_scale [M] and
+    writes both, and row_scale) in [-127, 127] (-128 makes the row NaN); w a DeviceF8Weight [K][N]; row_scale [M] and
     bias [N] float32.  The rows of `a` start at multiples of 16 bytes.
     Returns [M][N] (`out` if given)."""
     if not isinstance(w, DeviceF8Weight):

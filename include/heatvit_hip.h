@@ -396,7 +396,8 @@ int hv_model_forward_f32_ex(const hv_model_dev *p, const float *images, int batc
 /* ------------------------------------------------------------------ */
 /* Operators of language models (no counterpart in the reference): the   */
 /* path norm -> product -> answer of rows of floating-point activations. */
-/* Scales are powers of two, held as int8 exponents in [-127, 127]; a    */
+/* Scales are powers of two, held as int8 exponents in [-127, 127] (a    */
+/* product takes -128 as no number: what its block reaches is NaN); a    */
 /* block is 128 columns (the last one of a row may be shorter).          */
 /* ------------------------------------------------------------------ */
 

@@ -1,0 +1,76 @@
+"""Edges of the language-model operators (heatvit_amd.lm): exponents, weights,
+squares and differences at the ends of their ranges."""
+
+import numpy as np
+import pytest
+import torch
+
+import lm_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _whole(shape, seed, high=3):
+    """Small whole numbers as e4m3: every partial sum is exact in 32 bits."""
+    return torch.randint(-high, high + 1, shape, generator=_gen(seed)).float().to(
+        torch.float8_e4m3fn)
+
+
+def _exps(shape, seed, low, high):
+    return torch.randint(low, high + 1, shape, generator=_gen(seed)).to(torch.int8)
+
+
+# ------------------------------------------------------------------ gemm_f8
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("size", ((5, 64, 400), (40, 4200, 400), (600, 600, 400), (600, 600, 8576)),
+                         ids=str)
+def test_gemm_exponent_minus_128(size, kind):
+    """An exponent of -128 is no number: its row is NaN, over a block of
+    zeros too, and every other row and the row's other blocks keep theirs."""
+    from heatvit_amd import lm
+    from heatvit_amd.device import DeviceF8Weight
+    m, n, k = size
+    kb, nb = -(-k // 128), -(-n // 128)
+    a, w = _whole((m, k), 1, 1), _whole((k, n), 2, 1)
+    ae, we = _exps((m, kb), 3, -2, 0), _exps((kb, nb), 4, -2, 0)
+    dw = DeviceF8Weight(w, we)
+    s = torch.from_numpy(ref.spread(ae.numpy(), 128, k)).float().cuda()
+    t = torch.from_numpy(np.repeat(ref.spread(we.numpy(), 128, n), 128, 0)[:k]).float().cuda()
+    # exact: whole multiples of 2^-4, at most k of them
+    want = ((a.float().cuda() * s) @ (w.float().cuda() * t)).to(TYPES[kind])
+    bad = torch.zeros(m, dtype=torch.bool)
+    for row, block in ((0, 0), (1, kb - 1), (3, 1), (m - 1, kb // 2)):
+        ae[row, block] = -128
+        bad[row] = True
+    a[3, 128:256] = 0
+    bad = bad.cuda()
+    got = lm.gemm_f8(a.cuda(), ae.cuda(), dw, out_dtype=TYPES[kind])
+    assert got[bad].isnan().all()
+    assert torch.equal(got[~bad], want[~bad])
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("size", ((5, 300, 400), (40, 4200, 400), (600, 600, 400)), ids=str)
+def test_gemm_weight_exponent_minus_128(size, kind):
+    """The same in a weight that was changed behind the constructor's check:
+    the block's 128 channels are NaN, the others keep their values."""
+    from heatvit_amd import lm
+    from heatvit_amd.device import DeviceF8Weight
+    m, n, k = size
+    kb, nb = -(-k // 128), -(-n // 128)
+    a, w = _whole((m, k), 1), _whole((k, n), 2)
+    ae, we = _exps((m, kb), 3, -2, 0), _exps((kb, nb), 4, -3, 0)
+    want, _ = ref.gemm_f8(a, ae.numpy(), w, we.numpy(), None, None)
+    dw = DeviceF8Weight(w, we)
+    dw.exps[2, 1] = -128
+    got = lm.gemm_f8(a.cuda(), ae.cuda(), dw, out_dtype=TYPES[kind]).cpu()
+    assert got[:, 128:256].isnan().all()
+    want = torch.from_numpy(want).to(TYPES[kind])
+    assert torch.equal(got[:, :128], want[:, :128]) and torch.equal(got[:, 256:], want[:, 256:])
