@@ -178,11 +178,13 @@ F8_BLOCK = 128  # k and n that share an exponent
 def quantise_f8_weight(w):
     """A float matrix W[K][N] as e4m3 values and the exponents
     [ceil(K/128)][ceil(N/128)] (int8) of its 128 x 128 blocks: the smallest
-    power of two that holds the block's largest value, at least 2^-127."""
+    power of two that holds the block's largest finite value, at least 2^-127.
+    NaN and infinities become NaN (e4m3 has no infinities)."""
     k, n = w.shape
     kb, nb = -(-k // F8_BLOCK), -(-n // F8_BLOCK)
     w = w.float()
-    amax = torch.nn.functional.pad(w.abs(), (0, nb * F8_BLOCK - n, 0, kb * F8_BLOCK - k))
+    amax = torch.where(w.isfinite(), w.abs(), 0.0)
+    amax = torch.nn.functional.pad(amax, (0, nb * F8_BLOCK - n, 0, kb * F8_BLOCK - k))
     amax = amax.view(kb, F8_BLOCK, nb, F8_BLOCK).amax((1, 3))
     m, e = torch.frexp(amax)  # 448 = 0.875 * 2^9
     e = torch.where(amax > 0, (e - 9 + (m > 0.875)).clamp(min=-127), -127)

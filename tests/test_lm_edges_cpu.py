@@ -1,9 +1,11 @@
 """Edges of the language-model operators that need no GPU."""
 
+import math
+
 import pytest
 import torch
 
-from heatvit_amd.device import DeviceF8Weight
+from heatvit_amd.device import DeviceF8Weight, quantise_f8_weight
 
 
 def test_weight_exponent_minus_128_is_refused():
@@ -13,3 +15,22 @@ def test_weight_exponent_minus_128_is_refused():
     e[1, 0] = -128
     with pytest.raises(ValueError):
         DeviceF8Weight(f8, e, device="cpu")
+
+
+@pytest.mark.parametrize("value", (math.inf, -math.inf, math.nan))
+def test_weight_not_finite_stays_alone(value):
+    """A NaN or an infinity in a weight is NaN where it stands; the rest of
+    its block has the values and the exponent that it has without it."""
+    w = torch.randn(300, 140, generator=torch.Generator().manual_seed(3)) * 700
+    w[5, 7], w[200, 139], w[299, 0] = 0, 0, 0
+    want, e_want = quantise_f8_weight(w)
+    for k, n in ((5, 7), (200, 139), (299, 0)):
+        w[k, n] = value
+    w[128:256, 128:] = torch.where(torch.arange(12) == 11, value, 0.0)  # nothing else in a block
+    want.view(torch.uint8)[128:256, 128:] = 0
+    e_want[1, 1] = -127
+    q, e = quantise_f8_weight(w)
+    assert torch.equal(e, e_want)
+    finite = w.isfinite()
+    assert q.float()[~finite].isnan().all()
+    assert torch.equal(q.view(torch.uint8)[finite], want.view(torch.uint8)[finite])
