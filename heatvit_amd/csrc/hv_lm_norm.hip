@@ -13,6 +13,8 @@
 // 5120 f16 with one exponent a row (147 MB, the row read again from the L2)
 // 33 us, 5.8 and 4.4 TB/s. One row of 4096 takes 2.5 us, 1003 x 1000 f32 3.8:
 // a load's latency, the reduction and the stores.
+#include <type_traits>
+
 #include "hv_lm.h"
 
 namespace hv {
@@ -68,6 +70,23 @@ __device__ __forceinline__ void store_q8(uint8_t *q, int n, const float *p, floa
   Eight<uint8_t>::v8 b;
   __builtin_memcpy(&b, &t, sizeof b);
   Eight<uint8_t>::store(q, n, b);
+}
+
+// Sum over a row's LANES threads, in every one of them; all of the row's
+// threads have to be here.
+template <int LANES>
+__device__ __forceinline__ double row_sum(double v, int tid) {
+#pragma unroll
+  for (int o = 1; o < (LANES < 64 ? LANES : 64); o *= 2) v += __shfl_xor(v, o);
+  if (LANES > 64) {
+    __shared__ double part[LANES / 64 > 0 ? LANES / 64 : 1];
+    if ((tid & 63) == 0) part[tid >> 6] = v;
+    __syncthreads();
+    v = 0.;
+#pragma unroll
+    for (int w = 0; w < LANES / 64; ++w) v += part[w];
+  }
+  return v;
 }
 
 // LANES threads a row (16: sixteen rows a workgroup, 64: four, else one); each
@@ -149,14 +168,27 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void k_rms_norm_q8(NormA
       amax = fmaxf(amax, part[1][w]);
     }
   }
-  if (!live) return;
-  if (tid == 0) a.scale[row] = 1.f / sqrtf(sum / (float)a.width + a.eps);
-  if (!ROW) return;
+  // Every thread reads again what it read or wrote itself.
+  const T *kept = out ? out : x;
+  const float mean = sum / (float)a.width + a.eps;
+  // Squares above float32's numbers, or below its normal ones where eps does
+  // not hide that, are summed again in 64 bits. (A float16's never are.)
+  if (!std::is_same<T, f16>::value && (mean < 0x1p-100f || mean == __builtin_inff())) {
+    double again = 0.;
+    for (int c0 = tid * 8; c0 < a.width; c0 += LANES * 8) {
+      const v8 t = Eight<T>::load(kept + c0, min(8, a.width - c0));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) again += (double)(float)t[i] * (double)(float)t[i];
+    }
+    again = row_sum<LANES>(again, tid);
+    if (live && tid == 0) a.scale[row] = (float)(1. / sqrt(again / a.width + (double)a.eps));
+  } else if (live && tid == 0) {
+    a.scale[row] = 1.f / sqrtf(mean);
+  }
+  if (!ROW || !live) return;
   const int e = block_exp<FMT>(amax);
   const float inv = __builtin_bit_cast(float, (127 - e) << 23);
   if (tid == 0) exps[0] = (int8_t)e;
-  // Every thread reads again what it read or wrote itself.
-  const T *kept = out ? out : x;
   for (int c0 = tid * 8; c0 < a.width; c0 += LANES * 8) {
     const int n = min(8, a.width - c0);
     const v8 t = Eight<T>::load(kept + c0, n), g = Eight<T>::load(w + c0, n);

@@ -425,7 +425,7 @@ int hv_model_forward_f32_ex(const hv_model_dev *p, const float *images, int batc
  * so q * 2^exps * scale stands for the normalised row.  q and exps depend on
  * p alone, bit for bit.  An infinity or NaN in p gives NaN in e4m3, and in
  * int8 the end of the range or 0; the row's scale is then 0 or NaN.  The
- * squares are summed in 32 bits: |h| has to stay under 2^60.
+ * squares are summed in 32 bits, or in 64 where they leave float32's numbers.
  * residual_out is NULL exactly when residual is; it may be residual or x
  * itself (same stride), q, exps and scale overlap nothing else.  rows_dev
  * (optional, device): the live row count; rows behind it are left as they

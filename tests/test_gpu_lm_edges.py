@@ -74,3 +74,48 @@ def test_gemm_weight_exponent_minus_128(size, kind):
     assert got[:, 128:256].isnan().all()
     want = torch.from_numpy(want).to(TYPES[kind])
     assert torch.equal(got[:, :128], want[:, :128]) and torch.equal(got[:, 256:], want[:, 256:])
+
+
+# ------------------------------------------------------------------ rms_norm_q8
+
+@pytest.mark.parametrize("residual", (False, True))
+@pytest.mark.parametrize("kind", ("bf16", "f32"))
+@pytest.mark.parametrize("size", ((20, 100), (5, 100), (5, 300), (3, 1500), (600, 700), (2, 4096)),
+                         ids=str)
+def test_norm_squares_outside_float32(size, kind, residual):
+    """Rows whose squares, or their sum, lie above or below float32's numbers:
+    the factor is that of the formula all the same."""
+    from heatvit_amd import lm
+    rows, width = size
+    dtype = TYPES[kind]
+    row = torch.arange(rows)
+    # the rows' sizes go through 2^-140 .. 2^126, some rows' values all alike
+    size_of = -140 + (row * 37 + width) % 267
+    x = torch.randn(rows, width, generator=_gen(width)).clamp(-1.9, 1.9)
+    x[row % 4 == 1] = 1.0
+    x = torch.ldexp(x.double(), size_of[:, None]).to(dtype)
+    x[rows - 1] = 0
+    if rows > 4:
+        x[2, width // 2] = float("inf")
+        x[3, 1] = float("nan")
+    w = torch.ones(width, dtype=dtype)
+    # without a residual's own values the sum is x itself
+    r = torch.zeros(rows, width, dtype=dtype).cuda() if residual else None
+    for eps in (0.0, 1e-36, 1e-6):
+        for fmt, block in (("e4m3", 128), ("int8", 0)):
+            got = lm.rms_norm_q8(x.cuda(), w.cuda(), residual=r, eps=eps, fmt=fmt, block=block)
+            with np.errstate(all="ignore"):
+                eps32 = float(np.float32(eps))
+                want = 1.0 / np.sqrt(np.square(x.double().numpy()).mean(1) + eps32)
+            g = got.scale.cpu().double().numpy()
+            assert np.array_equal(np.isnan(g), np.isnan(want))
+            far = want > float(np.finfo(np.float32).max)  # 1 / 0 among them
+            assert np.array_equal(np.isposinf(g), far)
+            fine = ~np.isnan(want) & ~far
+            # half a step of the numbers below the normal ones
+            bound = ref.scale_bound(width) * want + 2.0 ** -149
+            assert (np.abs(g - want)[fine] <= bound[fine]).all(), (eps, fmt)
+            q, exps, _, _ = ref.rms_norm_q8(x, w, None, eps, fmt, block)
+            assert np.array_equal(got.exps.cpu().numpy(), exps)
+            if fmt == "int8":
+                assert torch.equal(got.q.cpu(), q)
