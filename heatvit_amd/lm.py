@@ -244,7 +244,10 @@ def log_probs(logits, tokens=None, *, scale_exp=0, temperature=1.0, top=0, live_
         raise ValueError(f"top {top} outside [0, {_lib.HV_LOG_PROBS_MAX_TOP}] or over the width")
     if not 0 < temperature < math.inf:
         raise ValueError("temperature must be positive and finite")
-    scale = math.ldexp(1.0, scale_exp) / temperature
+    try:
+        scale = math.ldexp(1.0, scale_exp) / temperature
+    except OverflowError:
+        raise ValueError(f"2^{scale_exp} / temperature is out of range") from None
     count = 0
     if tokens is not None:
         if not isinstance(tokens, torch.Tensor) or tokens.dtype != torch.int32:

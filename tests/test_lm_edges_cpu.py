@@ -5,6 +5,7 @@ import math
 import pytest
 import torch
 
+from heatvit_amd import lm
 from heatvit_amd.device import DeviceF8Weight, quantise_f8_weight
 
 
@@ -34,3 +35,9 @@ def test_weight_not_finite_stays_alone(value):
     finite = w.isfinite()
     assert q.float()[~finite].isnan().all()
     assert torch.equal(q.view(torch.uint8)[finite], want.view(torch.uint8)[finite])
+
+
+@pytest.mark.parametrize("scale_exp,temperature", ((2000, 1.0), (1024, 3.0), (10 ** 30, 1.0)))
+def test_answer_scale_out_of_range(scale_exp, temperature):
+    with pytest.raises(ValueError, match="out of range"):
+        lm.log_probs(torch.zeros(3, 50), scale_exp=scale_exp, temperature=temperature)
