@@ -65,13 +65,19 @@ struct Logit {
   // below every finite logit's place in a sum, and finite
   static __device__ __forceinline__ float lowest() { return -3.402823466e38f; }
   static __device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
-  static __device__ __forceinline__ float below(float x, float m) { return x - m; }
+  // x - m in halves: the type's largest and lowest numbers lie twice the largest
+  // float apart.
+  static constexpr float kUnit = 2.f;
+  static __device__ __forceinline__ float below(float x, float m) {
+    return __builtin_fmaf(x, .5f, -.5f * m);
+  }
 };
 template <>
 struct Logit<int> {
   typedef int type;
   static __device__ __forceinline__ int lowest() { return INT32_MIN; }
   static __device__ __forceinline__ int larger(int a, int b) { return max(a, b); }
+  static constexpr float kUnit = 1.f;
   static __device__ __forceinline__ float below(int x, int m) {
     return -(float)((unsigned)m - (unsigned)x);
   }
@@ -93,8 +99,14 @@ __device__ __forceinline__ typename Logit<T>::type wave_max(typename Logit<T>::t
   return L::larger(L::larger(of(0), of(16)), L::larger(of(32), of(48)));
 }
 
-// Sum of 2^d and of 2^d d over logits, d = c (x - max), c = scale log2(e),
-// and the maximum they are relative to.
+// What makes a below() an exponent of 2: scale log2(e), in its units.
+template <typename T>
+__device__ __forceinline__ float factor_of(const AnswerArgs &a) {
+  return a.scale * (1.44269504089f * Logit<T>::kUnit);
+}
+
+// Sum of 2^d and of 2^d d over logits, d = c below(x, max), and the maximum
+// they are relative to.
 template <typename T>
 struct Sums {
   typedef Logit<T> L;
@@ -241,7 +253,7 @@ __device__ void write_answer(const AnswerArgs &a, int64_t row, const T *x, const
   const float log2_sum = log2f(s.sum), log_sum = log2_sum * kLn2;
   if (tid == 0) a.entropy[row] = none ? 0.f : (log2_sum - s.weighted / s.sum) * kLn2;
   auto logp = [&](V v) {
-    return none ? -__builtin_inff() : L::below(v, s.max) * a.scale - log_sum;
+    return none ? -__builtin_inff() : L::below(v, s.max) * (a.scale * L::kUnit) - log_sum;
   };
   for (int i = tid; i < a.n_tokens; i += kThreads) {
     const int t = i == tid ? given.token : a.tokens[row * a.tokens_ld + i];
@@ -273,7 +285,7 @@ __global__ __launch_bounds__(kThreads) void k_log_probs(AnswerArgs a) {
   const int part = blockIdx.x % a.parts;
   if (row >= rows) return;
   const T *x = (const T *)a.logits + row * a.logits_ld;
-  const float c = a.scale * 1.44269504089f;
+  const float c = factor_of<T>(a);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   __shared__ V slots[TOP ? kSlots * kThreads : 1];
   __shared__ u64 keys[TOP ? kKeep : 1];
@@ -456,7 +468,7 @@ __global__ __launch_bounds__(kThreads) void k_log_probs_join(AnswerArgs a) {
     }
     bound = least ? least : 1;
   }
-  s.join_lanes(a.scale * 1.44269504089f);
+  s.join_lanes(factor_of<T>(a));
   if (TOP) {
     __syncthreads();
     for (int i = tid; i < n; i += kThreads)

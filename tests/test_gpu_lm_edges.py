@@ -119,3 +119,25 @@ def test_norm_squares_outside_float32(size, kind, residual):
             assert np.array_equal(got.exps.cpu().numpy(), exps)
             if fmt == "int8":
                 assert torch.equal(got.q.cpu(), q)
+
+
+# ------------------------------------------------------------------ log_probs
+
+@pytest.mark.parametrize("kind", ("bf16", "f32"))
+@pytest.mark.parametrize("size", ((1, 131072), (3, 900), (600, 3000)), ids=str)
+def test_answer_differences_beyond_the_largest_number(size, kind):
+    """Logits over the whole range of their type with a scale that brings them
+    near each other: their differences are twice the largest number."""
+    from heatvit_amd import lm
+    rows, width = size
+    x = (torch.rand(rows, width, generator=_gen(rows)) * 2 - 1) * 3.38e38
+    x = x.to(TYPES[kind])
+    x[0, 5], x[0, 9] = torch.finfo(TYPES[kind]).max, torch.finfo(TYPES[kind]).min
+    t = torch.randint(0, width, (rows, 2), generator=_gen(1)).to(torch.int32)
+    t[0, 0], t[0, 1] = 5, 9
+    got = lm.log_probs(x.cuda(), t.cuda(), scale_exp=-126, top=7)
+    want = ref.log_probs(x.double().numpy(), t.numpy().astype(np.int64), 2.0 ** -126, 7)
+    for name in ("entropy", "logp", "top_logp"):
+        off = np.abs(getattr(got, name).cpu().double().numpy() - want[name])
+        assert (off <= want[name + "_bound"]).all(), name
+    assert np.array_equal(got.top_index.cpu().numpy(), want["top_index"])
