@@ -1,0 +1,228 @@
+"""Every kernel of the e4m3 block product (heatvit_amd.lm.gemm_f8) at its own
+hazards: live rows on the borders of its tiles, strides, what lies behind k,
+far rows, refills of its exponents, the whole range of exponents, and values
+that are not finite."""
+
+import pytest
+import torch
+
+import lm_reference as ref
+from lm_kernels import F16, F32, kernel_of
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+ROWS = {"rows16": 16, "rows16x2": 16, "rows32": 32, "rows64": 64, "tile64": 64,
+        "tile128deep": 128, "tile128": 128, "tile256": 256}
+# rows and channels that take each kernel, of 16-bit and of float32 outputs
+SIZES16 = {"rows16": (40, 300), "rows16x2": (13, 4200), "rows32": (30, 2100), "tile64": (260, 4200),
+           "tile128deep": (500, 4100), "tile128": (1000, 4100), "tile256": (4100, 2000)}
+SIZES32 = {"rows16": (40, 300), "rows16x2": (13, 4200), "rows32": (40, 2000), "rows64": (90, 2000),
+           "tile64": (260, 4200), "tile128": (500, 4100)}
+CALLS = [(kind, name) for kind in TYPES for name in (F32 if kind == "f32" else F16)]
+
+
+def _size(kind, name, lda):
+    """The kernel's rows and channels: the call takes that kernel indeed."""
+    m, n = (SIZES32 if kind == "f32" else SIZES16)[name]
+    assert kernel_of(kind == "f32", m, n, lda) == name
+    print(f"gemm {kind} {name} {m} x {n}", flush=True)
+    return m, n
+
+
+def _gen(seed, device="cuda"):
+    return torch.Generator(device).manual_seed(seed)
+
+
+def _whole(shape, seed, high=3):
+    """Small whole numbers as e4m3: every partial sum is exact in 32 bits."""
+    return torch.randint(-high, high + 1, shape, generator=_gen(seed), device="cuda").float().to(
+        torch.float8_e4m3fn)
+
+
+def _exps(shape, seed, low, high):
+    return torch.randint(low, high + 1, shape, generator=_gen(seed), device="cuda").to(torch.int8)
+
+
+def _exact(a, ae, w, we):
+    """The product in float32, where it is exact."""
+    k, n = w.shape
+    s = torch.exp2(ae.float()).repeat_interleave(128, 1)[:, :k]
+    t = torch.exp2(we.float()).repeat_interleave(128, 0)[:k].repeat_interleave(128, 1)[:, :n]
+    return (a.float() * s) @ (w.float() * t)
+
+
+@pytest.mark.parametrize("call", CALLS, ids="-".join)
+def test_strides_live_rows_and_nothing_outside(call):
+    """Rows of k values followed by NaN, exponents between others, outputs at
+    any element, live counts on both sides of a tile's borders."""
+    from heatvit_amd import lm
+    from heatvit_amd.device import DeviceF8Weight
+    kind, name = call
+    dtype = TYPES[kind]
+    for k in (400, 240):  # ending in a block's first 16 bytes and in its last but one
+        m, n = _size(kind, name, k + 48)
+        kb, nb = -(-k // 128), -(-n // 128)
+        a, w = _whole((m, k), 1), _whole((k, n), 2)
+        ae, we = _exps((m, kb), 3, -2, 0), _exps((kb, nb), 4, -3, 0)
+        want = _exact(a, ae, w, we).to(dtype)
+        dw = DeviceF8Weight(w, we)
+        da = torch.full((m, k + 48), 0x7F, dtype=torch.uint8, device="cuda")
+        da[:, 16:16 + k] = a.view(torch.uint8)
+        da = da.view(torch.float8_e4m3fn)[:, 16:16 + k]
+        de = torch.full((m, kb + 3), 100, dtype=torch.int8, device="cuda")
+        de[:, 2:2 + kb] = ae
+        de = de[:, 2:2 + kb]
+        edge = ROWS[name]
+        counts = sorted({0, 1, min(edge - 1, m), min(edge, m), min(edge + 1, m), m - 1, m, m + 9})
+        for i, live in enumerate(counts):
+            pad = (0, 1, 4)[i % 3]
+            c = torch.full((m, n + 8), 55.0, dtype=dtype, device="cuda")
+            lm.gemm_f8(da, de, dw, out_dtype=dtype, out=c[:, pad:pad + n],
+                       live_rows=torch.tensor([live], dtype=torch.int32, device="cuda"))
+            rows = min(live, m)
+            assert torch.equal(c[:rows, pad:pad + n], want[:rows]), (k, live, pad)
+            assert (c[rows:] == 55).all()
+            assert (c[:, :pad] == 55).all() and (c[:, pad + n:] == 55).all()
+
+
+@pytest.mark.parametrize("call", CALLS, ids="-".join)
+def test_nan_behind_k_and_in_a_row(call):
+    """NaN in what follows k in memory reaches nothing, NaN at the last of k
+    its row alone, NaN in a weight its channel alone."""
+    from heatvit_amd import lm
+    from heatvit_amd.device import DeviceF8Weight
+    kind, name = call
+    dtype = TYPES[kind]
+    for k in (144, 272, 368):
+        m, n = _size(kind, name, k + 112)
+        a, w = _whole((m, k + 112), 1), _whole((k, n), 2)
+        a.view(torch.uint8)[:, k:] = 0x7F
+        kb = -(-k // 128)
+        ae, we = _exps((m, kb), 3, -2, 0), _exps((kb, -(-n // 128)), 4, -3, 0)
+        want = _exact(a[:, :k], ae, w, we).to(dtype)
+        a.view(torch.uint8)[m // 2, k - 1] = 0x7F
+        w.view(torch.uint8)[k - 2, n - 3] = 0x7F
+        got = lm.gemm_f8(a[:, :k], ae, DeviceF8Weight(w, we), out_dtype=dtype)
+        assert got[m // 2].isnan().all() and got[:, n - 3].isnan().all()
+        keep = torch.arange(m, device="cuda") != m // 2
+        got, want = got[keep], want[keep]
+        got[:, n - 3] = want[:, n - 3] = 0
+        assert torch.equal(got, want), k
+
+
+@pytest.mark.parametrize("call", [c for c in CALLS if c[1].startswith("tile")], ids="-".join)
+def test_far_rows_in_tiles(call):
+    """Rows 2^22 - 16 bytes apart, the last whose offsets a tile holds, and
+    2^22, which the kernel for few rows takes."""
+    from heatvit_amd import lm
+    from heatvit_amd.device import DeviceF8Weight
+    kind, name = call
+    k = 400
+    m, n = {"tile64": (70, 4200), "tile256": (400, 32700)}.get(name) or _size(kind, name, k)
+    a, w = _whole((m, k), 1), _whole((k, n), 2)
+    ae, we = _exps((m, 4), 3, -2, 0), _exps((4, -(-n // 128)), 4, -3, 0)
+    want = _exact(a, ae, w, we).to(TYPES[kind])
+    dw = DeviceF8Weight(w, we)
+    far = torch.zeros(m << 22, dtype=torch.uint8, device="cuda")
+    for ld, taken in (((1 << 22) - 16, name), (1 << 22, "rows16x2")):
+        assert kernel_of(kind == "f32", m, n, ld) == taken
+        rows = far[:m * ld].view(m, ld)[:, :k]
+        rows.copy_(a.view(torch.uint8))
+        got = lm.gemm_f8(rows.view(torch.float8_e4m3fn), ae, dw, out_dtype=TYPES[kind])
+        assert torch.equal(got, want), ld
+        rows.zero_()
+
+
+@pytest.mark.parametrize("call", CALLS, ids="-".join)
+def test_numbers_of_blocks(call):
+    """One block and a few, and so many that a tile's exponents are refilled
+    (64 blocks), at every number of blocks modulo the stages; the values are
+    exact."""
+    from heatvit_amd import lm
+    from heatvit_amd.device import DeviceF8Weight
+    kind, name = call
+    for k in (16, 128, 272, 640, 8192, 8208, 8448, 8464, 16528):
+        m, n = _size(kind, name, k)
+        kb, nb = -(-k // 128), -(-n // 128)
+        a, w = _whole((m, k), 1, 1), _whole((k, n), 2, 1)
+        # |sum| <= k < 2^24 units of 2^-4
+        ae, we = _exps((m, kb), 3, -2, 0), _exps((kb, nb), 4, -2, 0)
+        got = lm.gemm_f8(a, ae, DeviceF8Weight(w, we), out_dtype=TYPES[kind])
+        assert torch.equal(got, _exact(a, ae, w, we).to(TYPES[kind])), k
+
+
+@pytest.mark.parametrize("call", CALLS, ids="-".join)
+def test_every_exponent(call):
+    """Exponents over their whole range, of the rows and of the weight: the
+    factors are powers of two, and sums within float32's normal numbers are
+    exact. row_scale takes the factor back, so that every type can show them."""
+    from heatvit_amd import lm
+    from heatvit_amd.device import DeviceF8Weight
+    kind, name = call
+    m, n = _size(kind, name, 128)
+    a, w = _whole((m, 128), 1), _whole((128, n), 2)
+    sums = a.float() @ w.float()  # below 2^11: exact in float16 too
+    for first, e in ((-127, -127), (-127, -1), (-20, -60), (-90, 60), (0, 0), (-127, 120),
+                     (-m // 2, 1), (113 - m, 0), (127 - m, -13), (0, -127)):
+        ae = (first + torch.arange(m)).clamp(-127, 127)
+        total = ae + e
+        fine = ((total >= -126) & (total <= 114)).cuda()
+        scale = torch.exp2(-total.clamp(-126, 114).double()).float().cuda()
+        dw = DeviceF8Weight(w, torch.full((1, -(-n // 128)), e, dtype=torch.int8))
+        got = lm.gemm_f8(a, ae.to(torch.int8)[:, None].cuda(), dw, row_scale=scale,
+                         out_dtype=TYPES[kind])
+        assert torch.equal(got[fine], sums[fine].to(TYPES[kind])), (first, e)
+
+
+@pytest.mark.parametrize("call", CALLS, ids="-".join)
+def test_far_blocks_beside_near_ones(call):
+    """A block whose factor is far from its neighbours': the sum is that of
+    the formula within 264 additions of 2^-23 each and the output's rounding."""
+    from heatvit_amd import lm
+    from heatvit_amd.device import DeviceF8Weight
+    kind, name = call
+    dtype = TYPES[kind]
+    m, n = _size(kind, name, 256)
+    a, w = _whole((m, 256), 1), _whole((256, n), 2)
+    x, y = a.double(), w.double()
+    first, second = x[:, :128] @ y[:128], x[:, 128:] @ y[128:]
+    size1, size2 = x[:, :128].abs() @ y[:128].abs(), x[:, 128:].abs() @ y[128:].abs()
+    del x, y
+    nb = -(-n // 128)
+    for e, f in ((0, -14), (0, -30), (0, -127), (-100, -127), (3, 5)):
+        ae = torch.tensor([[e, f]], dtype=torch.int8).repeat(m, 1).cuda()
+        for we in ((0, 0), (-13, 6)):
+            dw = DeviceF8Weight(w, torch.tensor(we, dtype=torch.int8)[:, None].repeat(1, nb))
+            one, two = 2.0 ** (e + we[0]), 2.0 ** (f + we[1])
+            # brought near 1 for float16, whose smallest steps count as errors
+            back = 2.0 ** -max(e + we[0], f + we[1])
+            scale = torch.full((m,), back, device="cuda")
+            got = lm.gemm_f8(a, ae, dw, row_scale=scale, out_dtype=dtype)
+            want = (first * one + second * two) * back
+            bound = (size1 * one + size2 * two) * back * 264 * 2.0 ** -23
+            bound += (want.abs() + bound) * ref.HALF[dtype] + 2.0 ** -24
+            assert ((got.double() - want).abs() <= bound).all(), (e, f, we)
+
+
+@pytest.mark.parametrize("call", CALLS, ids="-".join)
+def test_factors_and_addends_not_finite(call):
+    """Infinities and NaN in row_scale and bias stay in their row and their
+    channel, as the formula has them."""
+    from heatvit_amd import lm
+    from heatvit_amd.device import DeviceF8Weight
+    kind, name = call
+    k, inf = 144, float("inf")
+    m, n = _size(kind, name, k)
+    a, w = _whole((m, k), 1), _whole((k, n), 2)
+    a.view(torch.uint8)[1] = 0  # 0 times an infinity
+    ae, we = _exps((m, 2), 3, -2, 0), _exps((2, -(-n // 128)), 4, -3, 0)
+    scale, bias = torch.ones(m), torch.zeros(n)
+    scale[0], scale[1], scale[m - 1], scale[m // 2] = inf, inf, float("nan"), -inf
+    bias[0], bias[n - 1], bias[n // 2] = inf, -inf, float("nan")
+    scale, bias = scale.cuda(), bias.cuda()
+    want = (_exact(a, ae, w, we) * scale[:, None] + bias).to(TYPES[kind])
+    got = lm.gemm_f8(a, ae, DeviceF8Weight(w, we), row_scale=scale, bias=bias,
+                     out_dtype=TYPES[kind])
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got.nan_to_num(7.0, inf, -inf), want.nan_to_num(7.0, inf, -inf))

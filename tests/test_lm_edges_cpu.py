@@ -5,6 +5,7 @@ import math
 import pytest
 import torch
 
+import lm_kernels
 from heatvit_amd import lm
 from heatvit_amd.device import DeviceF8Weight, quantise_f8_weight
 
@@ -41,3 +42,17 @@ def test_weight_not_finite_stays_alone(value):
 def test_answer_scale_out_of_range(scale_exp, temperature):
     with pytest.raises(ValueError, match="out of range"):
         lm.log_probs(torch.zeros(3, 50), scale_exp=scale_exp, temperature=temperature)
+
+
+def test_product_kernels_by_size():
+    """The rule that picks a product's kernel: the sizes that the GPU tests
+    hold each kernel to take it, and rows too far apart for a tile do not."""
+    import test_gpu_lm_kernels as gpu
+    assert {n for k, n in gpu.CALLS if k != "f32"} == set(gpu.SIZES16)
+    assert {n for k, n in gpu.CALLS if k == "f32"} == set(gpu.SIZES32)
+    assert set(gpu.SIZES16) | set(gpu.SIZES32) == set(lm_kernels.NAMES)
+    for f32, sizes in ((False, gpu.SIZES16), (True, gpu.SIZES32)):
+        for name, (m, n) in sizes.items():
+            for lda in (16, 400, (1 << 22) - 16):
+                assert lm_kernels.kernel_of(f32, m, n, lda) == name
+            assert lm_kernels.kernel_of(f32, m, n, 1 << 22) in ("rows16", "rows16x2")
