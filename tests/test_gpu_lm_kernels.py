@@ -1,7 +1,7 @@
 """Every kernel of the e4m3 block product (heatvit_amd.lm.gemm_f8) at its own
 hazards: live rows on the borders of its tiles, strides, what lies behind k,
-far rows, refills of its exponents, the whole range of exponents, and values
-that are not finite."""
+far rows, refills of its exponents, the whole range of exponents, values that
+are not finite, and what the 8-bit matrix cores cut off."""
 
 import pytest
 import torch
@@ -226,3 +226,86 @@ def test_factors_and_addends_not_finite(call):
                      out_dtype=TYPES[kind])
     assert torch.equal(got.isnan(), want.isnan())
     assert torch.equal(got.nan_to_num(7.0, inf, -inf), want.nan_to_num(7.0, inf, -inf))
+
+
+# ------------------------------------------------------------------ what is cut off
+
+def _operands(inputs, k, n, seed):
+    """One row and a weight, both e4m3; the row in blocks as a norm leaves it."""
+    g = _gen(seed, "cpu")
+    a, w = torch.randn(k, generator=g), torch.randn(k, n, generator=g)
+    if inputs == "same sign":
+        a, w = a.abs(), w.abs()
+    if inputs.startswith("outlier"):  # a channel in each block far above the others
+        a[::128] *= 64
+        if inputs.endswith("same sign"):
+            a, w = a.abs(), w.abs()
+    top = a.view(-1, 128).abs().amax(1, keepdim=True)
+    e = torch.ceil(torch.log2(top / 448))
+    q = (a.view(-1, 128) / torch.exp2(e)).view(1, -1).to(torch.float8_e4m3fn)
+    return q, e.to(torch.int8).view(1, -1), (w * 64).clamp(-448, 448).to(torch.float8_e4m3fn)
+
+
+@pytest.mark.parametrize("inputs", ("normal", "same sign", "outlier", "outlier same sign"))
+@pytest.mark.parametrize("call", (("f16", "rows16"), ("bf16", "tile64"), ("f16", "tile128deep"),
+                                  ("bf16", "tile256"), ("f32", "rows16"), ("f32", "tile128")),
+                         ids="-".join)
+def test_what_the_matrix_cores_cut_off(call, inputs):
+    """The accumulators' own error. All rows are the same one and the bias is
+    the negated result, so that the output is the error and nothing else is
+    rounded away.
+
+    The 8-bit matrix cores cut a product at u = 2^-13 of the power of two under
+    the largest one beside it (of the block at most); a product that is a
+    multiple of u loses nothing.  So an output is off by at most the sum of u
+    over the others, and by k + 8 additions of 2^-23 of the sum of sizes.
+
+    Norm over the channels: what is cut, spread evenly over [0, u) towards
+    zero, has the expected square sum u^2 / 12 + (sum +-u / 2)^2; a block adds
+    one 2^-23 of the largest partial sum, and the matrix cores 16 within a
+    block, independent of each other.  The error has to stay within twice
+    that."""
+    from heatvit_amd import lm
+    from heatvit_amd.device import DeviceF8Weight
+    kind, name = call
+    fast = kind != "f32"
+    for k in (128, 1024, 4096):
+        m, _ = _size(kind, name, k)
+        n = (SIZES16 if fast else SIZES32)[name][1]
+        q, e, w = _operands(inputs, k, n, k)
+        qd, wd = q.double().cuda()[0], w.double().cuda()
+        exact = torch.zeros(n, dtype=torch.float64, device="cuda")
+        worst, mean, square, size, peak = (torch.zeros_like(exact) for _ in range(5))
+        for b in range(k // 128):
+            p = qd[b * 128:b * 128 + 128, None] * wd[b * 128:b * 128 + 128]
+            unit = torch.exp2(torch.floor(torch.log2(p.abs().amax(0).clamp(min=1e-30))) - 13)
+            u = torch.where(torch.remainder(p, unit) != 0, unit, 0.0) * 2.0 ** int(e[0, b])
+            p *= 2.0 ** int(e[0, b])
+            peak = torch.maximum(peak, exact.abs() + p.abs().sum(0))
+            exact += p.sum(0)
+            size += p.abs().sum(0)
+            worst += u.sum(0)
+            mean += (u * p.sign()).sum(0) / 2
+            square += (u * u).sum(0) / 12
+        # the result near 2^9, so that float16 holds the errors as normal numbers
+        back = 2.0 ** (9 - round(float(torch.log2(exact.abs().max()))))
+        bias = (-exact * back).float()
+        rows = q.view(torch.uint8).repeat(m, 1).cuda().view(torch.float8_e4m3fn)
+        got = lm.gemm_f8(rows, e.repeat(m, 1).cuda(),
+                         DeviceF8Weight(w, torch.zeros((k // 128, -(-n // 128)), dtype=torch.int8)),
+                         row_scale=torch.full((m,), back, device="cuda"), bias=bias,
+                         out_dtype=TYPES[kind])
+        assert torch.equal(got, got[:1].expand(m, n))
+        off = got[0].double() - (exact * back + bias.double())
+        ends = bias.double().abs() * ref.U32 + 2.0 ** -24
+        ends += (off.abs() + ends) * (ref.HALF[TYPES[kind]] + ref.U32)
+        bound = ends + size * back * (k + 8) * 2.0 ** -23 + (worst * back if fast else 0)
+        assert (off.abs() <= bound).all(), (k, float((off.abs() / bound).max()))
+        expected = (k // 128 + 16) * (2.0 ** -23 * peak).square()
+        if fast:
+            expected += square + mean * mean
+        norm, expected = (float(v / (exact * back).norm())
+                          for v in (off.norm(), expected.sum().sqrt() * back))
+        print(f"  {inputs} k {k}: error {norm:.2e} of the result's norm, expected {expected:.2e}, "
+              f"worst {float((off.abs() / (size * back)).max()):.2e} of the sizes' sum", flush=True)
+        assert norm <= 2 * expected + float(ends.norm() / (exact * back).norm())
