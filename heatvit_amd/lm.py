@@ -143,7 +143,9 @@ def rms_norm_q8(x, weight, *, residual=None, eps=1e-6, fmt="e4m3", block=F8_BLOC
 
     x, residual [R][C] and weight [C] of one type (float32, float16,
     bfloat16); fmt "e4m3" or "int8"; block 128 columns, or 0 for one exponent
-    a row.  `out`: the Q8Rows to write; its residual may be `residual` or `x`
+    a row (gemm_f8 takes the first).  A NaN or an infinity is NaN in e4m3; int8
+    has the end of its range for an infinity and 0 for NaN, and the row's scale
+    is 0 or NaN.  `out`: the Q8Rows to write; its residual may be `residual` or `x`
     itself.  Returns Q8Rows(q, exps, scale, residual)."""
     rows, width, x_ld = _matrix("x", x, _TYPES)
     if fmt not in _FORMATS:
@@ -197,8 +199,9 @@ def gemm_f8(a, a_exps, w, *, row_scale=None, bias=None, out_dtype=torch.bfloat16
     times the others: where that counts, ask for float32).
 
     a [M][K] float8_e4m3fn and a_exps [M][ceil(K/128)] int8 (rms_norm_q8
-    writes both, and row_scale) in [-127, 127] (-128 makes the row NaN); w a DeviceF8Weight [K][N]; row_scale [M] and
-    bias [N] float32.  The rows of `a` start at multiples of 16 bytes.
+    writes both, and row_scale) in [-127, 127] (-128 makes the row NaN); w a
+    DeviceF8Weight [K][N]; row_scale [M] and bias [N] float32.  The rows of `a`
+    start at multiples of 16 bytes.
     Returns [M][N] (`out` if given)."""
     if not isinstance(w, DeviceF8Weight):
         raise TypeError("w must be a DeviceF8Weight")

@@ -121,6 +121,35 @@ def test_norm_squares_outside_float32(size, kind, residual):
                 assert torch.equal(got.q.cpu(), q)
 
 
+def test_int8_rows_through_the_int8_product():
+    """int8 rows of very different sizes through hv_gemm_i8 on the device: its
+    sums, times 2^exps and scale of each row, are the normalised rows' product.
+    q is off by half a step of 2^exps, scale by its roundings."""
+    from heatvit_amd import _lib, lm
+    from heatvit_amd.device import pack_mfma32
+    m, n, k = 70, 40, 192
+    x = torch.randn(m, k, generator=_gen(3)) * torch.exp2(torch.arange(m) % 23 - 11.0)[:, None]
+    x, w = x.to(torch.bfloat16), (1 + 0.3 * torch.randn(k, generator=_gen(4))).to(torch.bfloat16)
+    rows = lm.rms_norm_q8(x.cuda(), w.cuda(), fmt="int8", block=0)
+    assert rows.exps.unique().numel() > 10
+    b = np.random.default_rng(2).integers(-128, 128, (k, n)).astype(np.int8)
+    packed = torch.from_numpy(pack_mfma32(b)).cuda()
+    sums = torch.empty((m, n), dtype=torch.int32, device="cuda")
+    d = _lib.GemmDesc()
+    d.a, d.b_packed, d.c = rows.q.data_ptr(), packed.data_ptr(), sums.data_ptr()
+    d.m, d.n, d.k, d.lda, d.ldc, d.ldr = m, n, k, k, n, n
+    d.a_mode, d.epilogue = _lib.HV_A_ROWS, _lib.HV_EPI_I32
+    _lib.check(_lib.lib().hv_gemm_i8(d, torch.cuda.current_stream().cuda_stream), "gemm")
+    step = torch.exp2(rows.exps[:, 0].double().cpu()) * rows.scale.double().cpu()
+    got = sums.cpu().double() * step[:, None]
+    h = x.double()
+    normal = h * w.double() / torch.sqrt(h.square().mean(1, keepdim=True) + 1e-6)
+    want = normal @ torch.from_numpy(b).double()
+    size = normal.abs() @ torch.from_numpy(b).double().abs()
+    half = step[:, None] / 2 * torch.from_numpy(b).double().abs().sum(0)
+    assert ((got - want).abs() <= (half + size * ref.scale_bound(k)) * (1 + 2.0 ** -20)).all()
+
+
 # ------------------------------------------------------------------ log_probs
 
 @pytest.mark.parametrize("kind", ("bf16", "f32"))
