@@ -211,7 +211,8 @@ def pack_f8x64(w):
 class DeviceF8Weight:
     """A weight W[K][N] of heatvit_amd.lm.gemm_f8, laid out once: a float
     matrix, quantised here in 128 x 128 blocks, or float8_e4m3fn values with
-    their int8 exponents [ceil(K/128)][ceil(N/128)] in [-127, 127].  Either
+    their int8 exponents [ceil(K/128)][ceil(N/128)] in [-127, 127] (-128 is
+    refused on the host; on a GPU it makes its block's channels NaN).  Either
     order of storage is taken (a checkpoint's [N][K] as `w.t()`)."""
 
     def __init__(self, w, exps=None, device=None):
@@ -230,7 +231,7 @@ class DeviceF8Weight:
             raise TypeError("a quantised weight is float8_e4m3fn with int8 exponents")
         elif tuple(exps.shape) != (-(-k // F8_BLOCK), -(-n // F8_BLOCK)):
             raise ValueError(f"exponents of a {k} x {n} weight are [ceil(K/128)][ceil(N/128)]")
-        elif (exps == -128).any():
+        elif not exps.is_cuda and (exps == -128).any():  # no wait for a GPU's
             raise ValueError("exponents lie in [-127, 127]")
         self.inner, self.width = k, n
         self.packed = pack_f8x64(w.to(device))
