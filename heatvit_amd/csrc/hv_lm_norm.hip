@@ -28,7 +28,7 @@ struct NormArgs {
   const int32_t *rows_dev;
   int64_t x_ld, residual_ld, residual_out_ld, q_ld, exps_ld;
   int rows, width;
-  float eps;
+  float eps, low;  // low: under it a sum of squares has lost bits that eps does not hide
 };
 
 static constexpr int kNormBlock = 128;  // columns that share an exponent
@@ -170,10 +170,9 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void k_rms_norm_q8(NormA
   }
   // Every thread reads again what it read or wrote itself.
   const T *kept = out ? out : x;
-  const float mean = sum / (float)a.width + a.eps;
   // Squares above float32's numbers, or below its normal ones where eps does
   // not hide that, are summed again in 64 bits. (A float16's never are.)
-  if (!std::is_same<T, f16>::value && (mean < 0x1p-100f || mean == __builtin_inff())) {
+  if (!std::is_same<T, f16>::value && (sum < a.low || sum >= 0x1p120f)) {
     double again = 0.;
     for (int c0 = tid * 8; c0 < a.width; c0 += LANES * 8) {
       const v8 t = Eight<T>::load(kept + c0, min(8, a.width - c0));
@@ -183,7 +182,7 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void k_rms_norm_q8(NormA
     again = row_sum<LANES>(again, tid);
     if (live && tid == 0) a.scale[row] = (float)(1. / sqrt(again / a.width + (double)a.eps));
   } else if (live && tid == 0) {
-    a.scale[row] = 1.f / sqrtf(mean);
+    a.scale[row] = 1.f / sqrtf(sum / (float)a.width + a.eps);
   }
   if (!ROW || !live) return;
   const int e = block_exp<FMT>(amax);
@@ -268,6 +267,7 @@ extern "C" int hv_rms_norm_q8(const hv_rms_norm_desc *d, hv_stream_t stream) {
   a.x_ld = d->x_ld; a.residual_ld = d->residual_ld; a.residual_out_ld = d->residual_out_ld;
   a.q_ld = d->q_ld; a.exps_ld = d->exps_ld;
   a.rows = d->rows; a.width = d->width; a.eps = d->eps;
+  a.low = d->eps < 0x1p-100f ? (0x1p-100f - d->eps) * (float)d->width : 0.f;
   const hipStream_t s = (hipStream_t)stream;
   if (d->type == HV_T_F32) norm_launch<float>(a, d->format, d->block == 0, s);
   else if (d->type == HV_T_F16) norm_launch<f16>(a, d->format, d->block == 0, s);
