@@ -72,23 +72,6 @@ __device__ __forceinline__ void store_q8(uint8_t *q, int n, const float *p, floa
   Eight<uint8_t>::store(q, n, b);
 }
 
-// Sum over a row's LANES threads, in every one of them; all of the row's
-// threads have to be here.
-template <int LANES>
-__device__ __forceinline__ double row_sum(double v, int tid) {
-#pragma unroll
-  for (int o = 1; o < (LANES < 64 ? LANES : 64); o *= 2) v += __shfl_xor(v, o);
-  if (LANES > 64) {
-    __shared__ double part[LANES / 64 > 0 ? LANES / 64 : 1];
-    if ((tid & 63) == 0) part[tid >> 6] = v;
-    __syncthreads();
-    v = 0.;
-#pragma unroll
-    for (int w = 0; w < LANES / 64; ++w) v += part[w];
-  }
-  return v;
-}
-
 // LANES threads a row (16: sixteen rows a workgroup, 64: four, else one); each
 // takes eight columns at a time, so a block of 128 is 16 adjacent lanes.
 template <typename T, int FMT, bool ROW, int LANES>
@@ -161,33 +144,37 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void k_rms_norm_q8(NormA
       part[1][tid >> 6] = amax;
     }
     __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) amax = fmaxf(amax, part[1][w]);
     sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      sum += part[0][w];
-      amax = fmaxf(amax, part[1][w]);
-    }
+    for (int w = 0; w < kWaves; ++w) sum += part[0][w];
   }
-  // Every thread reads again what it read or wrote itself.
   const T *kept = out ? out : x;
   // Squares above float32's numbers, or below its normal ones where eps does
-  // not hide that, are summed again in 64 bits. (A float16's never are.)
-  if (!std::is_same<T, f16>::value && (sum < a.low || sum >= 0x1p120f)) {
-    double again = 0.;
-    for (int c0 = tid * 8; c0 < a.width; c0 += LANES * 8) {
-      const v8 t = Eight<T>::load(kept + c0, min(8, a.width - c0));
+  // not hide that, are summed again in 64 bits, by the row's first wavefront.
+  // (A float16's never are.)
+  constexpr int kAgain = LANES < 64 ? LANES : 64;
+  if (tid < kAgain) {
+    if (!std::is_same<T, f16>::value && (sum < a.low || sum >= 0x1p120f)) {
+      double again = 0.;
+      for (int c0 = tid * 8; c0 < a.width; c0 += kAgain * 8) {
+        const v8 t = Eight<T>::load(kept + c0, min(8, a.width - c0));
 #pragma unroll
-      for (int i = 0; i < 8; ++i) again += (double)(float)t[i] * (double)(float)t[i];
+        for (int i = 0; i < 8; ++i) again += (double)(float)t[i] * (double)(float)t[i];
+      }
+#pragma unroll
+      for (int o = 1; o < kAgain; o *= 2) again += __shfl_xor(again, o);
+      if (live && tid == 0) a.scale[row] = (float)(1. / sqrt(again / a.width + (double)a.eps));
+    } else if (live && tid == 0) {
+      a.scale[row] = 1.f / sqrtf(sum / (float)a.width + a.eps);
     }
-    again = row_sum<LANES>(again, tid);
-    if (live && tid == 0) a.scale[row] = (float)(1. / sqrt(again / a.width + (double)a.eps));
-  } else if (live && tid == 0) {
-    a.scale[row] = 1.f / sqrtf(sum / (float)a.width + a.eps);
   }
   if (!ROW || !live) return;
   const int e = block_exp<FMT>(amax);
   const float inv = __builtin_bit_cast(float, (127 - e) << 23);
   if (tid == 0) exps[0] = (int8_t)e;
+  // Every thread reads again what it read or wrote itself.
   for (int c0 = tid * 8; c0 < a.width; c0 += LANES * 8) {
     const int n = min(8, a.width - c0);
     const v8 t = Eight<T>::load(kept + c0, n), g = Eight<T>::load(w + c0, n);

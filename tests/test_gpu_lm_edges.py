@@ -121,6 +121,31 @@ def test_norm_squares_outside_float32(size, kind, residual):
                 assert torch.equal(got.q.cpu(), q)
 
 
+@pytest.mark.parametrize("size", ((3, 200), (3, 700), (3, 1500), (600, 3000), (2, 20000)), ids=str)
+def test_norm_squares_outside_float32_in_place(size):
+    """The same with the residual's sum in its place: what is squared a second
+    time is what the row's other threads have written."""
+    from heatvit_amd import lm
+    rows, width = size
+    for power in (-100, 80):
+        g = _gen(width)
+        x, r = (torch.ldexp(torch.randn(rows, width, generator=g).double(),
+                            torch.tensor(power)).to(torch.bfloat16) for _ in range(2))
+        h = (x.float() + r.float()).to(torch.bfloat16)
+        kept = r.cuda()
+        out = lm.Q8Rows(torch.empty((rows, width), dtype=torch.int8, device="cuda"),
+                        torch.empty((rows, 1), dtype=torch.int8, device="cuda"),
+                        torch.empty(rows, device="cuda"), kept)
+        lm.rms_norm_q8(x.cuda(), torch.ones(width, dtype=torch.bfloat16).cuda(), residual=kept,
+                       eps=0.0, fmt="int8", block=0, out=out)
+        assert torch.equal(kept.cpu(), h)
+        want = 1.0 / np.sqrt(np.square(h.double().numpy()).mean(1))
+        off = np.abs(out.scale.cpu().double().numpy() - want)
+        assert (off <= ref.scale_bound(width) * want).all(), power
+        q, exps, _, _ = ref.rms_norm_q8(h, torch.ones(width).to(h.dtype), None, 0.0, "int8", 0)
+        assert np.array_equal(out.exps.cpu().numpy(), exps) and torch.equal(out.q.cpu(), q)
+
+
 def test_int8_rows_through_the_int8_product():
     """int8 rows of very different sizes through hv_gemm_i8 on the device: its
     sums, times 2^exps and scale of each row, are the normalised rows' product.
