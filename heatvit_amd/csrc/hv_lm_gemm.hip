@@ -312,12 +312,12 @@ constexpr int wait_loads(int vm) { return 0x70 | (vm & 15) | (vm >> 4) << 14; }
 // memory pipeline has taken them (8192^3: all at once 502 us, spread 438).
 // The exponents of kExpSteps blocks wait in LDS too: a load of theirs in the
 // loop would have to wait for the stage's loads in front of it.
-// The matrix cores bound a long k: 8192^3 takes 413 us (2.66 PFLOP/s), the matrix
-// cores busy for 64 to 68 % of it at the 1.93 GHz that such a load leaves. A
-// tile's loads at the start and its stores bound a short one: 11 us a round of
-// 256 x 256 tiles and 1.1 a block of k (50432 x 768 by k = 192: 32.5 us, where the
-// stores alone take 19.3 and all but the stores 19.9). Weights alone bound few
-// rows: 48 x 14336 by k = 4096 takes 12.2 us, 60 MB at a copy's rate.
+// The matrix cores bound a long k: 8192^3 takes 410 to 438 us by card (2.5 to 2.7
+// PFLOP/s), the matrix cores busy for 64 to 68 % of it at the 1.93 GHz that such
+// a load leaves. A tile's loads at the start and its stores bound a short one: 11
+// us a round of 256 x 256 tiles and 1.1 a block of k (50432 x 768 by k = 192: 32.5
+// us, where the stores alone take 19.3 and all but the stores 19.9). Weights alone
+// bound few rows: 48 x 14336 by k = 4096 takes 12.2 us, 60 MB at a copy's rate.
 template <typename T, int BM, int BN, int WM, int WN, int S>
 __global__ __launch_bounds__(64 * WM * WN) void k_gemm_f8_tile(GemmF8Args g) {
   typedef typename std::conditional<std::is_same<T, float>::value, Exact, Fast>::type Mma;

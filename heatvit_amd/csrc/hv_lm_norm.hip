@@ -9,9 +9,9 @@
 // e come from p alone, need no sum over the row, and are the same bits in any
 // order of work; a product over q multiplies its rows by `scale` in the end.
 //
-// HBM bounds it: 16384 x 8192 bf16 with a residual (950 MB) take 165 us, 4096 x
+// HBM bounds it: 16384 x 8192 bf16 with a residual (950 MB) take 166 us, 4096 x
 // 5120 f16 with one exponent a row (147 MB, the row read again from the L2)
-// 33 us, 5.8 and 4.4 TB/s. One row of 4096 takes 2.5 us, 1003 x 1000 f32 3.8:
+// 33 us, 5.7 and 4.4 TB/s. One row of 4096 takes 2.5 us, 1003 x 1000 f32 3.9:
 // a load's latency, the reduction and the stores.
 #include <type_traits>
 

@@ -21,9 +21,9 @@ enum class F8Kernel {
 inline F8Kernel f8_kernel(bool f32, int m, int n, int64_t lda) {
   // Up to 16 rows (us at k = 4096): the weights' bytes bound them, and parts of
   // 16 channels leave a CU a workgroup up to 4096 channels; wider weights take two
-  // parts a workgroup (1 row by 2048 channels 3.6, two parts 3.8; by 4096 5.2, 5.0;
-  // by 8192 9.0, 7.2; by 131072 104, 91; 16 rows to float32 by 2048 5.1, 5.6; by
-  // 8192 9.9, 8.5).
+  // parts a workgroup (1 row by 2048 channels 3.6, two parts 3.8; by 4096 5.2, 5.0,
+  // and with weights from memory 6.4, 6.6, 16 rows 7.4, 8.3; by 8192 9.0, 7.2; by
+  // 131072 104, 91; 16 rows to float32 by 2048 5.1, 5.6; by 8192 9.9, 8.5).
   const int parts = (n + 63) / 64 * 4;
   const bool near = lda < (int64_t)1 << 22;  // a tile's offsets into the rows are 32-bit
   if (m <= 16 || !near) return parts <= 256 ? F8Kernel::kRows16 : F8Kernel::kRows16x2;
