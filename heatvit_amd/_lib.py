@@ -27,6 +27,11 @@ HV_FWD_PIPELINED = 1
 HV_T_F32, HV_T_F16, HV_T_BF16, HV_T_I32 = 0, 1, 2, 3
 HV_Q_E4M3, HV_Q_I8 = 0, 1
 HV_LOG_PROBS_MAX_TOP = 64
+HV_ROTARY_HALF, HV_ROTARY_INTERLEAVED = 0, 1
+HV_ROTARY_MAX_WIDTH = 1024
+HV_CACHE_SAME, HV_CACHE_E4M3 = 0, 1
+HV_CACHE_MIN_PAGE, HV_CACHE_MAX_PAGE = 16, 4096
+HV_ATTENTION_MAX_WIDTH = 256
 ABI_VERSION = 5
 PROF_CLASSES = ("patch", "layernorm", "gemm_qkv", "attention", "gemm_proj", "gemm_ffn1",
                 "gemm_ffn2", "selector", "head", "other", "ffn")
@@ -131,6 +136,41 @@ class LogProbsDesc(C.Structure):
         (n, _i32) for n in ("rows", "width", "type", "n_tokens", "top")] + [("scale", C.c_float)]
 
 
+class RotaryDesc(C.Structure):
+    _fields_ = [(n, _vp) for n in ("q", "k", "q_weight", "k_weight", "q_out", "k_out", "positions",
+                                   "freqs", "rows_dev")] + [
+        (n, C.c_int64) for n in ("q_ld", "q_head_ld", "k_ld", "k_head_ld", "q_out_ld",
+                                 "q_out_head_ld", "k_out_ld", "k_out_head_ld")] + [
+        (n, _i32) for n in ("rows", "q_heads", "k_heads", "width", "rotated", "type", "layout")] + [
+        ("eps", C.c_float), ("scale", C.c_float), ("reserved", _i32)]
+
+
+# The structures that the descriptors below hold, field by field.
+_CACHE_FIELDS = [(n, _vp) for n in ("cache_k", "cache_v", "cache_k_exps", "cache_v_exps", "table",
+                                    "lengths")] + [("table_ld", C.c_int64)] + [
+    (n, _i32) for n in ("pages", "page", "max_pages", "format")]
+_ROWS_FIELDS = [(n, _vp) for n in ("q", "out", "lse", "starts")] + [
+    (n, C.c_int64) for n in ("q_ld", "q_head_ld", "out_ld", "out_head_ld")] + [
+    (n, _i32) for n in ("rows", "batch", "heads", "kv_heads", "width", "type", "causal",
+                        "window")] + [("scale", C.c_float), ("reserved", _i32)]
+
+
+class CacheWriteDesc(C.Structure):
+    _fields_ = _CACHE_FIELDS + [(n, _vp) for n in ("k", "v", "starts")] + [
+        (n, C.c_int64) for n in ("k_ld", "k_head_ld", "v_ld", "v_head_ld")] + [
+        (n, _i32) for n in ("rows", "batch", "kv_heads", "width", "type", "reserved")]
+
+
+class AttentionDesc(C.Structure):
+    _fields_ = _ROWS_FIELDS + [(n, _vp) for n in ("k", "v", "k_starts")] + [
+        (n, C.c_int64) for n in ("k_ld", "k_head_ld", "v_ld", "v_head_ld")] + [
+        ("k_rows", _i32), ("k_reserved", _i32)]
+
+
+class PagedAttentionDesc(C.Structure):
+    _fields_ = _ROWS_FIELDS + _CACHE_FIELDS
+
+
 def packer(desc):
     """pack(*values): a descriptor's bytes, which an entry point takes as its
     address (0.6 us a call where making the structure takes 1.4)."""
@@ -205,6 +245,12 @@ def _declare(L):
     L.hv_log_probs_workspace_bytes.restype = C.c_size_t
     L.hv_log_probs_workspace_bytes.argtypes = [C.c_int, C.c_int, C.c_int]
     L.hv_log_probs.argtypes = [_vp, _vp, C.c_size_t, _vp]
+    L.hv_rotary_qk.argtypes = [_vp, _vp]
+    L.hv_cache_write.argtypes = [_vp, _vp]
+    L.hv_attention_workspace_bytes.restype = C.c_size_t
+    L.hv_attention_workspace_bytes.argtypes = [C.c_int] * 5
+    L.hv_attention.argtypes = [_vp, _vp, C.c_size_t, _vp]
+    L.hv_paged_attention.argtypes = [_vp, _vp, C.c_size_t, _vp]
     L.hv_profile_enable.argtypes = [C.c_int]
     L.hv_profile_read.argtypes = [_vp, _vp, C.c_int]
 
@@ -235,4 +281,5 @@ def exported_symbols():
             "hv_model_forward_ex", "hv_model_forward_f32_ex",
             "hv_quantize_images", "hv_schedule_compile", "hv_schedule_packed_bytes",
             "hv_schedule_bind", "hv_rms_norm_q8", "hv_gemm_f8",
-            "hv_log_probs_workspace_bytes", "hv_log_probs")
+            "hv_log_probs_workspace_bytes", "hv_log_probs", "hv_rotary_qk", "hv_cache_write",
+            "hv_attention_workspace_bytes", "hv_attention", "hv_paged_attention")

@@ -32,45 +32,6 @@ struct NormArgs {
 };
 
 static constexpr int kNormBlock = 128;  // columns that share an exponent
-static constexpr int kMinExp = -127;    // the matrix cores' smallest scale, 2^-127
-
-// Smallest e >= -127 with amax <= L 2^e, L = 448 = 1.75 2^8 (e4m3) or
-// 127 = 1.984375 2^6 (int8): adding the complement of L's mantissa to the
-// float's bits carries into the exponent exactly when the mantissa is larger.
-// An infinite amax gives 120 or 122.
-template <int FMT>
-__device__ __forceinline__ int block_exp(float amax) {
-  const int bits = __builtin_bit_cast(int, amax);
-  const int e = FMT == HV_Q_E4M3 ? ((bits + (0x7FFFFF - 0x600000)) >> 23) - 127 - 8
-                                 : ((bits + (0x7FFFFF - 0x7E0000)) >> 23) - 127 - 6;
-  return e < kMinExp ? kMinExp : e;
-}
-
-// Four values p 2^-e in 8 bits (round to nearest even); the products by a
-// power of two are exact, or far below the smallest step.
-template <int FMT>
-__device__ __forceinline__ int quant4(const float *p, float inv) {
-  if (FMT == HV_Q_E4M3) {
-    int r = __builtin_amdgcn_cvt_pk_fp8_f32(p[0] * inv, p[1] * inv, 0, false);
-    return __builtin_amdgcn_cvt_pk_fp8_f32(p[2] * inv, p[3] * inv, r, true);
-  }
-  int r = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float v = rintf(p[i] * inv);
-    const int q = v != v ? 0 : (int)fminf(fmaxf(v, -127.f), 127.f);
-    r |= (q & 0xFF) << (8 * i);
-  }
-  return r;
-}
-
-template <int FMT>
-__device__ __forceinline__ void store_q8(uint8_t *q, int n, const float *p, float inv) {
-  const v2i t = {quant4<FMT>(p, inv), quant4<FMT>(p + 4, inv)};
-  Eight<uint8_t>::v8 b;
-  __builtin_memcpy(&b, &t, sizeof b);
-  Eight<uint8_t>::store(q, n, b);
-}
 
 // LANES threads a row (16: sixteen rows a workgroup, 64: four, else one); each
 // takes eight columns at a time, so a block of 128 is 16 adjacent lanes.

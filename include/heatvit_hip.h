@@ -511,6 +511,135 @@ int hv_log_probs(const hv_log_probs_desc *d, void *workspace, size_t workspace_b
                  hv_stream_t stream);
 
 /* ------------------------------------------------------------------ */
+/* Attention of language models (no counterpart in the reference):       */
+/* between the product that makes queries, keys and values and the one    */
+/* behind the attention.  Heads lie in rows of [rows][heads][width]       */
+/* tensors: `ld` elements from row to row, `head_ld` from head to head,   */
+/* a head's elements adjacent.                                            */
+/* ------------------------------------------------------------------ */
+
+#define HV_LM_MAX_HEADS 4096
+
+/* Norms of the heads of queries and keys and the rotation by position:
+ *   y = x / sqrt(mean of x^2 over the head + eps) * weight (no norm where the
+ *       weight is NULL)
+ *   pairs (a, b) of y's first `rotated` elements become
+ *       scale * (a cos t - b sin t, a sin t + b cos t), t = position * freqs[pair]
+ * in 32 bits, the angle in 64, rounded once to the type.  Pair i is elements
+ * i and rotated/2 + i (HV_ROTARY_HALF) or 2i and 2i + 1
+ * (HV_ROTARY_INTERLEAVED); elements from `rotated` on are the norm's alone.
+ * k_heads 0: queries alone.  An output may be its input (same strides) and
+ * overlaps nothing else.  rows_dev as above.  Pointers are aligned to their
+ * elements. */
+#define HV_ROTARY_HALF 0
+#define HV_ROTARY_INTERLEAVED 1
+#define HV_ROTARY_MAX_WIDTH 1024
+
+typedef struct {
+  const void *q, *k;
+  const void *q_weight, *k_weight; /* [width] or NULL              */
+  void *q_out, *k_out;
+  const int32_t *positions;        /* [rows]                       */
+  const float *freqs;              /* [rotated/2] radians a position */
+  const int32_t *rows_dev;
+  int64_t q_ld, q_head_ld, k_ld, k_head_ld, q_out_ld, q_out_head_ld, k_out_ld, k_out_head_ld;
+  int32_t rows, q_heads, k_heads, width, rotated, type, layout;
+  float eps, scale;
+  int32_t reserved;
+} hv_rotary_desc;
+
+int hv_rotary_qk(const hv_rotary_desc *d, hv_stream_t stream);
+
+/* A cache of keys and values in pages of 16 to 4096 keys (a power of two):
+ * k and v are [pages][kv_heads][page][width] of the call's type
+ * (HV_CACHE_SAME) or of e4m3 (HV_CACHE_E4M3: value * 2^exps, with
+ * k_exps and v_exps [pages][kv_heads][page]), rounded to the call's type where
+ * they are read.  Sequence b has lengths[b] keys, key j in page
+ * table[b][j / page].  Widths are multiples of 8 (e4m3: 16) up to 256, k and v
+ * 16-byte aligned. */
+#define HV_CACHE_SAME 0
+#define HV_CACHE_E4M3 1
+#define HV_CACHE_MIN_PAGE 16
+#define HV_CACHE_MAX_PAGE 4096
+#define HV_ATTENTION_MAX_WIDTH 256
+
+typedef struct {
+  void *k, *v;
+  int8_t *k_exps, *v_exps;
+  const int32_t *table;   /* [batch][table_ld], max_pages of a row used */
+  const int32_t *lengths; /* [batch]                                    */
+  int64_t table_ld;
+  int32_t pages, page, max_pages, format;
+} hv_cache_desc;
+
+/* New keys and values into a cache: rows starts[b] .. starts[b+1] - 1 are the
+ * last keys of sequence b, whose lengths count them (starts NULL: a row for
+ * each sequence).  Heads of e4m3 get the smallest exponent e >= -127 with
+ * |x| <= 448 * 2^e and are rounded to nearest, ties to even; what would round
+ * past the type's numbers (240 * 2^8 in float16, 240 * 2^120 in bfloat16) stays
+ * at that, and an infinity or NaN is NaN.  A row whose place is before the
+ * sequence's first key, past the table or in a page outside the cache is not
+ * written, nor are rows before starts[0] and from starts[batch] on.  Sequences
+ * that share a page must not both write it. */
+typedef struct {
+  hv_cache_desc cache;
+  const void *k, *v;
+  const int32_t *starts; /* [batch + 1] or NULL */
+  int64_t k_ld, k_head_ld, v_ld, v_head_ld;
+  int32_t rows, batch, kv_heads, width, type, reserved;
+} hv_cache_write_desc;
+
+int hv_cache_write(const hv_cache_write_desc *d, hv_stream_t stream);
+
+/* Attention of packed sequences (hv_attention), or of new rows over a paged
+ * cache (hv_paged_attention):
+ *   out = sum over the keys j that a row sees of softmax(scale * q.k_j) v_j
+ * for each head, query head h with key head h / (heads / kv_heads).  The rows
+ * of sequence b are starts[b] .. starts[b+1] - 1 (NULL, paged alone: a row for
+ * each sequence), its keys k_starts[b] .. k_starts[b+1] - 1 (NULL: starts) or
+ * the cache's.  `causal`: row i of n sees the first keys - n + i + 1 keys, the
+ * last `window` of those where that is not 0.  A row that sees nothing gets
+ * zeros, and -infinity in lse, which (optional) is [rows][heads], the natural
+ * logarithm of the sum of exponentials.  What a row does not see leaves no
+ * trace, infinities and NaN among it; a sequence whose table has no room for
+ * its keys, or a page outside the cache among those that are read, gets NaN.
+ * Sums are held in 32 bits, the softmax's terms rounded to the type for
+ * the product with v.  Rows outside all sequences are left as they were.
+ * Widths are multiples of 8 up to 256, strides multiples of 8, pointers 16-byte
+ * aligned (lse 4); type HV_T_F16 or HV_T_BF16.  The workspace (16-byte aligned) holds
+ * what the parts of a long axis leave, for the call alone; calls that overlap
+ * need one each. */
+typedef struct {
+  const void *q;
+  void *out;
+  float *lse;
+  const int32_t *starts; /* [batch + 1] */
+  int64_t q_ld, q_head_ld, out_ld, out_head_ld;
+  int32_t rows, batch, heads, kv_heads, width, type, causal, window;
+  float scale;
+  int32_t reserved;
+} hv_attention_rows;
+
+typedef struct {
+  hv_attention_rows rows;
+  const void *k, *v;
+  const int32_t *k_starts; /* [batch + 1] or NULL */
+  int64_t k_ld, k_head_ld, v_ld, v_head_ld;
+  int32_t k_rows, reserved;
+} hv_attention_desc;
+
+typedef struct {
+  hv_attention_rows rows;
+  hv_cache_desc cache;
+} hv_paged_attention_desc;
+
+size_t hv_attention_workspace_bytes(int rows, int batch, int heads, int kv_heads, int width);
+int hv_attention(const hv_attention_desc *d, void *workspace, size_t workspace_bytes,
+                 hv_stream_t stream);
+int hv_paged_attention(const hv_paged_attention_desc *d, void *workspace, size_t workspace_bytes,
+                       hv_stream_t stream);
+
+/* ------------------------------------------------------------------ */
 /* Kernel-class timing with HIP events (for benchmarks).  While enabled, */
 /* every kernel the forwards launch carries a start/stop event pair      */
 /* recorded by its own dispatch; hv_profile_read() waits for them and    */

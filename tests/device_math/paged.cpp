@@ -1,0 +1,26 @@
+// Where rows and keys of a paged cache lie, for the tests.
+#include "hv_lm_paged.h"
+
+using namespace hv;
+
+extern "C" {
+void seq_rows_of(const int32_t *starts, int b, int rows, int32_t *out) {
+  const SeqRows r = seq_rows(starts, b, rows);
+  out[0] = r.first;
+  out[1] = r.count;
+}
+int keys_of(int pages, int shift, int max_pages, int length) {
+  return paged_keys({pages, shift, max_pages}, length);
+}
+int page_at(int pages, int shift, int max_pages, const int32_t *table, long long position) {
+  return page_of({pages, shift, max_pages}, table, position);
+}
+long long row_at(int pages, int shift, int heads, int page, int head, long long position) {
+  return cache_row({pages, shift, 0}, heads, page, head, position);
+}
+void seen_at(int i, int n, int keys, int causal, int window, int32_t *out) {
+  const Seen s = seen_by(i, n, keys, causal != 0, window);
+  out[0] = s.from;
+  out[1] = s.to;
+}
+}
