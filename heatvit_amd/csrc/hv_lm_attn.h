@@ -66,97 +66,102 @@ __device__ __forceinline__ float factor_of(int e) {
   return __builtin_bit_cast(float, e == -128 ? 0x7FC00000 : (e + 127) << 23);
 }
 
-// Keys and values of one head of a sequence, element by element.
-template <typename T, bool PAGED, bool Q8>
-struct HeadKeys {
-  const LmAttnArgs &a;
-  Sequence s;
-  int head;  // of the keys
+// Workgroups that keep the card busy: two a CU.
+static constexpr int kTarget = 512;
 
-  // Row of key j: an element offset of the packed rows (of k, and of v), or a
-  // row of the cache; false where its page is none.
-  struct Place {
-    int64_t k, v;
-    bool ok;
-  };
-  __device__ __forceinline__ Place place(int j) const {
-    if (PAGED) {
-      const int page = page_of(a.map, s.table, j);
-      const int64_t row = cache_row(a.map, a.kv_heads, max(page, 0), head, j);
-      return {row, row, page >= 0};
-    }
-    const int64_t row = (int64_t)s.k_first + j;
-    return {row * a.k_ld + head * a.k_head_ld, row * a.v_ld + head * a.v_head_ld, true};
-  }
-  // Eight elements from d on, of k (value false) or v.
-  __device__ __forceinline__ void eight(const Place &p, bool value, int d, float (&x)[8]) const {
-    const int64_t at = value ? p.v : p.k;
-    const void *base = value ? a.v : a.k;
-    if (Q8) {
-      v2i w;
-      __builtin_memcpy(&w, (const uint8_t *)base + at * a.width + d, 8);
-      const float f = factor_of((value ? a.v_exps : a.k_exps)[at]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const auto t = Pair8<T>::of(w[i / 2], f, i % 2);
-        x[2 * i] = (float)t[0];
-        x[2 * i + 1] = (float)t[1];
-      }
-    } else {
-      const auto t = Eight<T>::load((const T *)base + (PAGED ? at * a.width : at) + d, 8);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = (float)t[i];
-    }
-  }
+// Tiles that a call's sequences have at most, and whether their keys are cut into parts:
+// where the tiles alone would leave CUs idle.
+inline int64_t most_tiles(int rows, int batch, int group, int tile_rows) {
+  return (int64_t)rows * group / tile_rows + batch;
+}
+inline int64_t most_slots(int64_t tiles, int kv_heads) {
+  return (tiles + (kTarget + kv_heads - 1) / kv_heads) * kv_heads;
+}
+struct Shape {
+  int tile_rows;
+  bool split;
+};
+inline Shape shape_of(int rows, int batch, int heads, int kv_heads) {
+  const int64_t tiles = most_tiles(rows, batch, heads / kv_heads, 128);
+  return {128, tiles * kv_heads < kTarget};
+}
+inline size_t workspace_of(int rows, int batch, int heads, int kv_heads, int width) {
+  const Shape shape = shape_of(rows, batch, heads, kv_heads);
+  if (!shape.split) return 0;
+  const int64_t slots =
+      most_slots(most_tiles(rows, batch, heads / kv_heads, shape.tile_rows), kv_heads);
+  return (size_t)slots * shape.tile_rows * (width * 4 + 8);
+}
+
+// The kernels of either type. The workspace is looked at here.
+int attend_f16(const LmAttnArgs &a, bool paged, bool q8, void *workspace, size_t bytes, hipStream_t s);
+int attend_bf16(const LmAttnArgs &a, bool paged, bool q8, void *workspace, size_t bytes,
+                hipStream_t s);
+
+// Items of a launch: a sequence's tiles of `rows` rows (of a key head's group:
+// token r / group, head r % group of it), each over `parts` parts of its keys.
+struct Item {
+  int b, tile, part;
+  int slot;  // of all items' parts, of the first part
 };
 
-// One row of queries over keys [from, to), by a wavefront: 64 keys at a time, a
-// key to a lane for the scores and eight elements to a lane for the sums. A
-// key that is not seen is not read, so nothing of it is in the result.
-// m and l: the largest score (to a power of two) and the sum of the terms
-// relative to it; lane i < width / 8 has elements 8 i .. 8 i + 7 of the sum of
-// terms times values.
-struct RowState {
-  float m, l, o[8];
+// The index-th of the items that count(b) says sequence b has, by all threads of
+// the workgroup: (sequence, index in it, items before the sequence); b -1: fewer
+// than that. count is asked for every sequence once.
+struct Found {
+  int b, rest, before;
 };
-template <typename T, bool PAGED, bool Q8>
-__device__ RowState attend_row(const LmAttnArgs &a, const Sequence &s, int row, int head, int from,
-                               int to) {
-  const int lane = threadIdx.x & 63;
-  const HeadKeys<T, PAGED, Q8> keys{a, s, head / a.group};
-  const T *q = (const T *)a.q + row * a.q_ld + head * a.q_head_ld;
-  RowState r{-__builtin_inff(), 0.f, {}};
-  for (int j0 = from; j0 < to; j0 += 64) {
-    const int n = min(64, to - j0), j = j0 + min(lane, n - 1);
-    const auto at = keys.place(j);
-    float score = 0.f;
-    for (int d = 0; d < a.width; d += 8) {
-      float x[8];
-      keys.eight(at, false, d, x);
-      const auto y = Eight<T>::load(q + d, 8);
+template <int THREADS, typename Count>
+__device__ __forceinline__ Found find_item(int batch, int index, Count count) {
+  __shared__ int sums[THREADS / 64], found[2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (batch == 1) return {index < count(0) ? 0 : -1, index, 0};
+  int before = 0;
+  for (int base = 0; base < batch; base += THREADS) {
+    const int b = base + tid, mine = b < batch ? count(b) : 0;
+    int upto = mine;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) score = __builtin_fmaf(x[i], (float)y[i], score);
+    for (int o = 1; o < 64; o *= 2) {
+      const int t = __shfl_up(upto, o);
+      if (lane >= o) upto += t;
     }
-    score = lane < n ? score * a.scale : -__builtin_inff();
-    if (!at.ok) score = __builtin_nanf("");
-    const float m = fmaxf(r.m, max64(score));
-    const bool none = m == -__builtin_inff();  // nothing but scores of -infinity (or NaN) so far
-    const float p = none ? score == score ? 0.f : score : __builtin_amdgcn_exp2f(score - m);
-    const float f = none ? 1.f : __builtin_amdgcn_exp2f(r.m - m);
-    r.m = m;
-    r.l = r.l * f + sum64(p);
+    if (lane == 63) sums[wave] = upto;
+    if (tid == 0) found[0] = -1;
+    __syncthreads();
+    int total = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r.o[i] *= f;
-    for (int i = 0; i < n; ++i) {
-      const float t = __shfl(p, i);
-      if (t == 0.f || lane * 8 >= a.width) continue;
-      float x[8];
-      keys.eight(keys.place(j0 + i), true, lane * 8, x);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) r.o[k] = __builtin_fmaf(t, x[k], r.o[k]);
+    for (int w = 0; w < THREADS / 64; ++w) {
+      if (w < wave) upto += sums[w];
+      total += sums[w];
     }
+    upto += before;
+    if (index < upto && index >= upto - mine) {
+      found[0] = b;
+      found[1] = upto - mine;
+    }
+    __syncthreads();
+    if (found[0] >= 0) return {found[0], index - found[1], found[1]};
+    before += total;
+    __syncthreads();
   }
-  return r;
+  return {-1, 0, 0};
+}
+
+// Sum of value(b) over the sequences, by all threads of the workgroup.
+template <int THREADS, typename Value>
+__device__ __forceinline__ int64_t sum_over(int batch, Value value) {
+  __shared__ int64_t sums[THREADS / 64];
+  if (batch == 1) return value(0);
+  int64_t s = 0;
+  for (int b = threadIdx.x; b < batch; b += THREADS) s += value(b);
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) s += __shfl_xor(s, o);
+  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
+  __syncthreads();
+  s = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) s += sums[w];
+  return s;
 }
 
 }  // namespace hv

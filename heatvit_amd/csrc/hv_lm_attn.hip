@@ -1,51 +1,15 @@
-// hv_lm_attn.hip -- attention of packed sequences and over a paged cache.
-//
-//   out = sum_j p_j v_j / sum_j p_j,  p_j = 2^(scale log2(e) q.k_j - m),  m the largest
+// hv_lm_attn.hip -- attention of packed sequences and over a paged cache: the entry
+// points, and what they refuse.
 #include "hv_lm_attn.h"
 
 namespace hv {
-
-// A row of one head to a wavefront.
-template <typename T, bool PAGED, bool Q8>
-__global__ __launch_bounds__(256) void k_attention_rows(LmAttnArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (item >= (int64_t)a.rows * a.heads) return;
-  const int row = (int)(item / a.heads), head = (int)(item - (int64_t)row * a.heads);
-  int b = row;
-  if (a.starts) {
-    for (b = 0; b < a.batch && a.starts[b + 1] <= row; ++b) {}
-    if (b == a.batch || a.starts[b] > row) return;
-  }
-  const Sequence s = sequence_of<PAGED>(a, b);
-  RowState r{-__builtin_inff(), __builtin_nanf(""), {}};
-  if (s.keys >= 0) {
-    const Seen seen = seen_by(row - s.first, s.count, s.keys, a.causal, a.window);
-    r = attend_row<T, PAGED, Q8>(a, s, row, head, seen.from, seen.to);
-  }
-  if (lane == 0 && a.lse)
-    a.lse[(int64_t)row * a.heads + head] =
-        r.l == 0.f ? -__builtin_inff() : (r.m + log2f(r.l)) * 0.69314718055994531f;
-  if (lane * 8 >= a.width) return;
-  typename Eight<T>::v8 t;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) t[i] = (T)(r.l == 0.f ? 0.f : r.o[i] / r.l);
-  Eight<T>::store((T *)a.out + row * a.out_ld + head * a.out_head_ld + lane * 8, 8, t);
-}
-
-template <typename T, bool PAGED, bool Q8>
-static int attend(const LmAttnArgs &a, hipStream_t s) {
-  const dim3 grid((unsigned)(((int64_t)a.rows * a.heads + 3) / 4)), block(256);
-  hv_launch(k_attention_rows<T, PAGED, Q8>, grid, block, 0, s, a);
-  return check_hip(hipGetLastError(), "k_attention_rows launch");
-}
 
 static int check_rows(const char *what, const hv_attention_rows &r, bool need_starts) {
   if (r.type != HV_T_F16 && r.type != HV_T_BF16)
     return fail(HV_EVALUE, HV_ERR_OPCODE, "%s: bad element type %d", what, r.type);
   if (r.rows < 0 || r.rows > HV_LM_MAX_ROWS || r.batch < 0 || r.batch > HV_LM_MAX_ROWS ||
       r.heads < 1 || r.heads > HV_LM_MAX_HEADS || r.kv_heads < 1 || r.heads % r.kv_heads ||
-      ((int64_t)r.rows + r.batch) * r.heads > 1 << 26)
+      (int64_t)r.rows * r.heads > 1 << 26 || (int64_t)r.batch * r.kv_heads > 1 << 22)
     return fail(HV_EVALUE, HV_ERR_DIMENSION, "%s: %d rows of %d heads, %d of keys, %d sequences",
                 what, r.rows, r.heads, r.kv_heads, r.batch);
   if (r.width < 8 || r.width > HV_ATTENTION_MAX_WIDTH || r.width % 8)
@@ -88,7 +52,8 @@ using namespace hv;
 extern "C" {
 
 size_t hv_attention_workspace_bytes(int rows, int batch, int heads, int kv_heads, int width) {
-  return 0;
+  if (rows <= 0 || batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || width <= 0) return 0;
+  return workspace_of(rows, batch, heads, kv_heads, width);
 }
 
 int hv_attention(const hv_attention_desc *d, void *workspace, size_t workspace_bytes,
@@ -111,8 +76,8 @@ int hv_attention(const hv_attention_desc *d, void *workspace, size_t workspace_b
   LmAttnArgs a = args_of(d->rows);
   a.k = d->k; a.v = d->v; a.k_starts = d->k_starts; a.k_rows = d->k_rows;
   a.k_ld = d->k_ld; a.k_head_ld = d->k_head_ld; a.v_ld = d->v_ld; a.v_head_ld = d->v_head_ld;
-  return d->rows.type == HV_T_F16 ? attend<f16, false, false>(a, (hipStream_t)stream)
-                                  : attend<bf16, false, false>(a, (hipStream_t)stream);
+  const auto attend = d->rows.type == HV_T_F16 ? attend_f16 : attend_bf16;
+  return attend(a, false, false, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
 int hv_paged_attention(const hv_paged_attention_desc *d, void *workspace, size_t workspace_bytes,
@@ -129,11 +94,9 @@ int hv_paged_attention(const hv_paged_attention_desc *d, void *workspace, size_t
   a.k = d->cache.k; a.v = d->cache.v; a.k_exps = d->cache.k_exps; a.v_exps = d->cache.v_exps;
   a.table = d->cache.table; a.lengths = d->cache.lengths; a.table_ld = d->cache.table_ld;
   a.map = {d->cache.pages, __builtin_ctz(d->cache.page), d->cache.max_pages};
-  const hipStream_t s = (hipStream_t)stream;
-  const bool q8 = d->cache.format == HV_CACHE_E4M3;
-  if (d->rows.type == HV_T_F16)
-    return q8 ? attend<f16, true, true>(a, s) : attend<f16, true, false>(a, s);
-  return q8 ? attend<bf16, true, true>(a, s) : attend<bf16, true, false>(a, s);
+  const auto attend = d->rows.type == HV_T_F16 ? attend_f16 : attend_bf16;
+  return attend(a, true, d->cache.format == HV_CACHE_E4M3, workspace, workspace_bytes,
+                (hipStream_t)stream);
 }
 
 }  // extern "C"
