@@ -20,12 +20,18 @@ struct Mma<bf16> {
   static __device__ __forceinline__ v16f wide(frag a, frag b, v16f c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
+  static __device__ __forceinline__ v4f small(frag a, frag b, v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
 };
 template <>
 struct Mma<f16> {
   typedef v8h frag;
   static __device__ __forceinline__ v16f wide(frag a, frag b, v16f c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ v4f small(frag a, frag b, v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
 };
 
@@ -59,8 +65,7 @@ __device__ __forceinline__ v4s read_column(const void *p) {
       (__attribute__((address_space(3))) v4s *)(__attribute__((address_space(3))) void *)p);
 }
 
-static constexpr int kKeys = 64;         // of a tile
-static constexpr int kMinPartTiles = 4;  // of a part, at least
+static constexpr float kRise = 8.f;      // over a row's reference, to a power of two
 
 // Where 16-byte chunk c of a tile's row lies in that row, so that the reads of
 // a tile meet no bank twice: of keys, one chunk of 32 rows at a time; of
@@ -80,6 +85,34 @@ __device__ __forceinline__ void to_lds(const void *from, void *to) {
   __builtin_amdgcn_global_load_lds(
       (const __attribute__((address_space(1))) void *)from,
       (__attribute__((address_space(3))) void *)to, 16, 0, 0);
+}
+
+// Element d of key j's value, as the products take it.
+template <typename T, bool PAGED, bool Q8>
+__device__ __forceinline__ float value_at(const LmAttnArgs &a, const Sequence &s, int head, int j, int d) {
+  if (!PAGED) return (float)((const T *)a.v)[((int64_t)s.k_first + j) * a.v_ld + head * a.v_head_ld + d];
+  const int page = page_of(a.map, s.table, j);
+  if (page < 0) return 0.f;
+  const int64_t row = cache_row(a.map, a.kv_heads, page, head, j);
+  if (!Q8) return (float)((const T *)a.v)[row * a.width + d];
+  const auto x = Pair8<T>::of(((const uint8_t *)a.v)[row * a.width + d], factor_of(a.v_exps[row]), false);
+  return (float)x[0];
+}
+
+// Of eight values in LDS, those that are no numbers become zeros; whether there were any.
+template <typename T>
+__device__ __forceinline__ bool take_out(void *at) {
+  typedef T eight __attribute__((ext_vector_type(8)));
+  eight v = *reinterpret_cast<const eight *>(at);
+  bool any = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const bool fine = fabsf((float)v[i]) < __builtin_inff();
+    any |= !fine;
+    v[i] = fine ? v[i] : (T)0.f;
+  }
+  if (any) *reinterpret_cast<eight *>(at) = v;
+  return any;
 }
 
 // What is loaded behind a head's width.
@@ -178,34 +211,6 @@ struct TileLoader {
   }
 };
 
-// What a launch's parts of the keys are: every sequence's keys in parts of so many
-// tiles of 64 that all of them together are about `target` workgroups' work.
-struct Split {
-  float *o;    // [slots][rows of a tile][width], sums relative to m
-  float2 *ml;  // [slots][rows of a tile]
-  int target;
-};
-
-template <bool PAGED>
-__device__ __forceinline__ int tiles_of(const LmAttnArgs &a, int b, int tile_rows) {
-  const int64_t n = (int64_t)seq_rows(a.starts, b, a.rows).count * a.group;
-  return (int)((n + tile_rows - 1) / tile_rows);
-}
-__device__ __forceinline__ int key_tiles(int keys) { return keys > 0 ? (keys + kKeys - 1) / kKeys : 0; }
-
-// Tiles of 64 keys of a part.
-template <bool PAGED, int THREADS>
-__device__ __forceinline__ int part_tiles(const LmAttnArgs &a, int tile_rows, int target) {
-  const int64_t all = sum_over<THREADS>(a.batch, [&](int b) {
-    return (int64_t)tiles_of<PAGED>(a, b, tile_rows) * key_tiles(sequence_of<PAGED>(a, b).keys);
-  });
-  const int64_t n = (all * a.kv_heads + target - 1) / target;
-  return (int)max((int64_t)kMinPartTiles, min(n, (int64_t)1 << 26));
-}
-__device__ __forceinline__ int parts_of(int keys, int part) {
-  return max(1, (key_tiles(keys) + part - 1) / part);
-}
-
 // NW x 32 rows by all keys that they see (SPLIT: by a part of them), 64 keys at
 // a time through LDS, two tiles of which take turns.
 //
@@ -224,35 +229,13 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void k_attention_tile(L
   __shared__ __attribute__((aligned(16))) T k1[kKeys * DP];
   __shared__ __attribute__((aligned(16))) T v0[kKeys * DP];
   __shared__ __attribute__((aligned(16))) T v1[kKeys * DP];
+  __shared__ unsigned long long odd_keys;
 
-  const int head = blockIdx.x % a.kv_heads, index = blockIdx.x / a.kv_heads;
-  Found f;
-  int part_len = 0;
-  if (SPLIT) {
-    part_len = part_tiles<PAGED, kThreads>(a, kRows, split.target);
-    f = find_item<kThreads>(a.batch, index, [&](int b) {
-      return tiles_of<PAGED>(a, b, kRows) * parts_of(sequence_of<PAGED>(a, b).keys, part_len);
-    });
-  } else {
-    f = find_item<kThreads>(a.batch, index, [&](int b) { return tiles_of<PAGED>(a, b, kRows); });
-  }
-  if (f.b < 0) return;
-  const Sequence s = sequence_of<PAGED>(a, f.b);
-  const int keys = max(s.keys, 0), parts = SPLIT ? parts_of(keys, part_len) : 1;
-  const int n_rows = s.count * a.group;
-  // The last tiles, which see the most keys, go first.
-  const int tile = tiles_of<PAGED>(a, f.b, kRows) - 1 - f.rest / parts, part = f.rest % parts;
-  const int r0 = tile * kRows;
-  const Seen first = seen_by(r0 / a.group, s.count, keys, a.causal, a.window);
-  const Seen final = seen_by(min(r0 + kRows - 1, n_rows - 1) / a.group, s.count, keys, a.causal,
-                             a.window);
-  int t0 = first.from / kKeys, t1 = max(t0, key_tiles(final.to)), used = 1;
-  if (SPLIT) {
-    used = max(1, (t1 - t0 + part_len - 1) / part_len);
-    if (part >= used) return;
-    t0 += part * part_len;
-    t1 = min(t1, t0 + part_len);
-  }
+  const int head = blockIdx.x % a.kv_heads;
+  const Work w = locate<kThreads, PAGED, SPLIT>(a, kRows, split.target, blockIdx.x / a.kv_heads);
+  if (!w.used) return;
+  const Sequence &s = w.s;
+  const int keys = w.keys, n_rows = w.n_rows, r0 = w.r0, t0 = w.t0, t1 = w.t1;
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
@@ -274,7 +257,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void k_attention_tile(L
       q[i] = d < a.width ? *reinterpret_cast<const frag *>(from + d) : frag{};
     }
   }
-  TileLoader<T, DP, PAGED, Q8, NW> loader(a, s, head, final.to - 1);
+  TileLoader<T, DP, PAGED, Q8, NW> loader(a, s, head, w.last);
   v16f o[kD];
   float m, l;
 
@@ -286,11 +269,16 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void k_attention_tile(L
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
-  // CAREFUL: with values that are no numbers among the tile's, of keys that
-  // not all rows see. They count as zeros in the sums, and what they make of the
-  // rows that do see them is found by a product of its own.
+  // Values that are no numbers, of keys that not all rows see, are taken out of a
+  // tile (careful), and added to the sums of the rows that do see them.
+  auto take = [&](T *v) __attribute__((always_inline)) {
+    if (threadIdx.x == 0) odd_keys = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < kKeys * DP / 8; i += kThreads)
+      if (take_out<T>(v + 8 * i)) atomicOr(&odd_keys, 1ull << i / (DP / 8));
+    __syncthreads();
+  };
   auto compute = [&](int t, const T *k, const T *v, auto careful) __attribute__((always_inline)) {
-    constexpr bool CAREFUL = decltype(careful)::value;
     if (idle || t * kKeys >= end.to || (t + 1) * kKeys <= top.from) return;
     v16f x[2] = {};
     const T *kr = k + col * DP;
@@ -313,11 +301,11 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void k_attention_tile(L
     float most = x[0][0];
 #pragma unroll
     for (int i = 1; i < 32; ++i) most = fmaxf(most, x[i / 16][i % 16]);
-    most = max_of_halves(most) * a.scale;
     // A row's reference rises only when a score passes it by 2^8: what is summed
     // is the same but for its exponent.
-    const bool rise = most > m + 8.f;
-    if (__builtin_amdgcn_ballot_w64(rise)) {
+    if (__builtin_amdgcn_ballot_w64(most * a.scale > m + kRise)) {
+      most = max_of_halves(most) * a.scale;
+      const bool rise = most > m + kRise;
       const float by = rise ? __builtin_amdgcn_exp2f(m - most) : 1.f;
       m = rise ? most : m;
       l *= by;
@@ -332,50 +320,34 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void k_attention_tile(L
       l += e;
       p[i / 8][i % 8] = (T)e;
     }
-    frag seen_keys[CAREFUL ? 4 : 1];
-    if (CAREFUL) {
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        seen_keys[i / 8][i % 8] =
-            (T)(sees(32 * (i / 16) + 8 * (i % 16 / 4) + i % 4) ? 1.f : 0.f);
-    }
     const int vr = 4 * half + (lane >> 2 & 3);
 #pragma unroll
     for (int d = 0; d < kD; ++d) {
       const int c = v_place<DP>(vr, 4 * d + (lane >> 4 & 1) * 2 + (lane >> 1 & 1)) * 8 + (lane & 1) * 4;
       const T *vc = v + vr * DP + c;
-      v16f odd = {};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const v4s lo = read_column(vc + 16 * i * DP), hi = read_column(vc + (16 * i + 8) * DP);
-        v8s both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        if (CAREFUL) {
-          // 1 for a NaN, 2^7 and 2^14 for the infinities, times 1 where the row sees the key
-          frag kind;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float val = (float)__builtin_bit_cast(T, (short)both[e]);
-            const bool fine = fabsf(val) < __builtin_inff();
-            kind[e] = (T)(fine ? 0.f : val != val ? 1.f : val > 0.f ? 128.f : 16384.f);
-            if (!fine) both[e] = 0;
-          }
-          odd = Mma<T>::wide(kind, seen_keys[i], odd);
-        }
+        const v8s both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         o[d] = Mma<T>::wide(__builtin_bit_cast(frag, both), p[i], o[d]);
       }
-      if (CAREFUL) {
+    }
+    if (!decltype(careful)::value) return;
+    for (uint64_t left = odd_keys; left; left &= left - 1) {
+      const int j = t * kKeys + __builtin_ctzll(left);
+      if (j < seen.from || j >= seen.to) continue;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int code = (int)odd[i];
-          const float up = code >> 7 & 127 ? __builtin_inff() : 0.f;
-          const float down = code >> 14 ? -__builtin_inff() : 0.f;
-          o[d][i] += code & 127 ? __builtin_nanf("") : up + down;
-        }
+      for (int i = 0; i < 16 * kD; ++i) {
+        const int e = 32 * (i / 16) + 8 * (i % 16 / 4) + 4 * half + i % 4;
+        const float x = e < a.width ? value_at<T, PAGED, Q8>(a, s, head, j, e) : 0.f;
+        o[i / 16][i % 16] += fabsf(x) < __builtin_inff() ? 0.f : x;
+        asm volatile("" ::: "memory");  // one after another, in few registers
       }
     }
   };
   auto step = [&](int t, T *k, T *v, T *nk, T *nv, auto careful) __attribute__((always_inline)) {
     meet();
+    if (decltype(careful)::value) take(v);
     if (t + 1 < t1) {
       loader.load(t + 1, nk, nv);
       loader.find(t + 2);
@@ -400,20 +372,18 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void k_attention_tile(L
     }
   };
   pass(std::false_type());
-  // NaN or infinities in what was summed: from values of keys that a row may not
-  // see, since 0 times those is a NaN.
+  // NaN or infinities in what was summed may be of keys that a row does not see,
+  // since 0 times those is a NaN: once more, with care.
   float sum = 0.f;
 #pragma unroll
-  for (int d = 0; d < kD; ++d)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) sum = __builtin_fmaf(o[d][i], 0.f, sum);
+  for (int i = 0; i < 16 * kD; ++i) sum = __builtin_fmaf(o[i / 16][i % 16], 0.f, sum);
   if (__syncthreads_or(sum != 0.f)) pass(std::true_type());
 
   l = sum_of_halves(l);
   if (PAGED && __syncthreads_or(s.keys < 0 || loader.bad)) l = __builtin_nanf("");
   if (idle || w0 + col >= n_rows) return;
-  if (SPLIT && used > 1) {
-    const int64_t at = ((int64_t)(f.before + f.rest) * a.kv_heads + head) * kRows + wave * 32 + col;
+  if (SPLIT && w.used > 1) {
+    const int64_t at = ((int64_t)(w.slot + w.part) * a.kv_heads + head) * kRows + wave * 32 + col;
     if (half == 0) split.ml[at] = make_float2(m, l);
     float *to = split.o + at * a.width;
 #pragma unroll
@@ -451,101 +421,396 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void k_attention_tile(L
     }
 }
 
-// Joins the parts of a tile's rows, of one key head: sixteen rows a workgroup, a row
-// to a wavefront, LANES lanes to a part of four elements a lane.
-template <typename T, bool PAGED, int LANES>
-__global__ __launch_bounds__(256) void k_attention_join(LmAttnArgs a, Split split, int tile_rows) {
-  const int head = blockIdx.x % a.kv_heads, index = blockIdx.x / a.kv_heads;
-  const int part_len = part_tiles<PAGED, 256>(a, tile_rows, split.target);
-  // The parts of all tiles before this one's: items are counted in tiles here.
-  const Found f =
-      find_item<256>(a.batch, index, [&](int b) { return tiles_of<PAGED>(a, b, tile_rows); });
-  if (f.b < 0) return;
-  const Sequence s = sequence_of<PAGED>(a, f.b);
-  const int keys = max(s.keys, 0), parts = parts_of(keys, part_len);
-  if (parts == 1) return;
-  const int64_t before = sum_over<256>(a.batch, [&](int b) {
-    return b < f.b ? (int64_t)tiles_of<PAGED>(a, b, tile_rows) *
-                         parts_of(sequence_of<PAGED>(a, b).keys, part_len)
-                   : 0;
-  });
-  const int n_rows = s.count * a.group, tiles = (n_rows + tile_rows - 1) / tile_rows;
-  const int tile = tiles - 1 - f.rest, r0 = tile * tile_rows;
-  const Seen first = seen_by(r0 / a.group, s.count, keys, a.causal, a.window);
-  const Seen final = seen_by(min(r0 + tile_rows - 1, n_rows - 1) / a.group, s.count, keys, a.causal,
-                             a.window);
-  const int used = (max(first.from / kKeys, key_tiles(final.to)) - first.from / kKeys + part_len - 1) /
-                   part_len;
-  if (used <= 1) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int e = lane % LANES * 4, sub = lane / LANES;
-  for (int i = blockIdx.y * 16 + wave; i < min(tile_rows, blockIdx.y * 16 + 16); i += 4) {
-    const int r = r0 + i;
-    if (r >= n_rows) return;
-    const int64_t at0 = ((before + (int64_t)f.rest * parts) * a.kv_heads + head) * tile_rows + i;
-    const int64_t step = (int64_t)a.kv_heads * tile_rows;
-    float m = -__builtin_inff(), l = 0.f;
-    for (int p = lane; p < used; p += 64) m = fmaxf(m, split.ml[at0 + p * step].x);
-    m = max64(m);
-    const float ref = m == -__builtin_inff() ? 0.f : m;
-    v4f o = {};
-    for (int p0 = 0; p0 < used; p0 += 64) {
-      float w = 0.f;
-      if (p0 + lane < used) {
-        const float2 ml = split.ml[at0 + (p0 + lane) * step];
-        w = __builtin_amdgcn_exp2f(ml.x - ref);
-        l = __builtin_fmaf(w, ml.y, l);
-      }
-      const int n = min(64, used - p0);
-      for (int p = 0; p < n; p += 64 / LANES) {
-        const int mine = p + sub;
-        const float wp = __shfl(w, mine & 63);
-        if (mine < n && e < a.width) {
-          const v4f x = *reinterpret_cast<const v4f *>(split.o + (at0 + (p0 + mine) * step) * a.width + e);
+// Where 16-byte chunk c of a row of values lies, where sixteen rows' 32 bytes are
+// read by columns at a time.
+template <int DP>
+__device__ __forceinline__ int few_place(int row, int c) {
+  return c ^ (DP == 64 ? (row >> 1 & 3) * 2 : (row & 7) * 2);
+}
+
+// Sixteen bytes of e4m3 times 2^e as two operands.
+template <typename T>
+__device__ __forceinline__ void wide_of(v4i w, float f, typename Mma<T>::frag (&x)[2]) {
+  typename Pair8<T>::type t[8];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) o[k] = __builtin_fmaf(wp, x[k], o[k]);
+  for (int i = 0; i < 4; ++i) {
+    t[2 * i] = Pair8<T>::of(w[i], f, false);
+    t[2 * i + 1] = Pair8<T>::of(w[i], f, true);
+  }
+  __builtin_memcpy(x, t, sizeof t);
+}
+
+// Sixteen rows by a part of the keys. Four wavefronts take 32 keys each in turn, for
+// themselves: keys come from memory as the lanes multiply them, values go through LDS
+// of the wavefront's own to be read by columns; the next 32 are on their way
+// meanwhile. In the end the wavefronts' sums are joined at their common reference.
+//
+//   S^T = K Q^T   16x16x32 MFMA: lane l has row l % 16, keys 4 (l / 16) + i of sixteen
+//   O^T += V^T P^T  with k slot 8 g + i as key 16 (i / 4) + 4 g + i % 4, as in the tiles
+template <typename T, int DP, bool PAGED, bool Q8, bool SPLIT>
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attention_few(LmAttnArgs a, Split split) {
+  typedef typename Mma<T>::frag frag;
+  constexpr int kRows = 16, kStep = 32, kD = DP / 16, kSteps = DP / 32;
+  // Loads of 16 bytes a lane: of keys, sixteen keys by 4 chunks; of values, 1 KiB of rows.
+  constexpr int kChunks = Q8 ? DP / 16 : DP / 8, kLoads = kChunks / 2, kRowsOf = 64 / kChunks;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kStep * DP * 2];
+  __shared__ float2 ml[4][kRows];
+
+  const int head = blockIdx.x % a.kv_heads;
+  const Work work = locate<256, PAGED, SPLIT>(a, kRows, split.target, blockIdx.x / a.kv_heads);
+  if (!work.used) return;
+  const Sequence &s = work.s;
+  const int keys = work.keys, n_rows = work.n_rows, r0 = work.r0, t0 = work.t0;
+  const int last = work.last, end = min(work.t1 * kKeys, last + 1);
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, grp = lane >> 4;
+  const int row = min(r0 + col, n_rows - 1), token = row / a.group;
+  const Seen seen = seen_by(token, s.count, keys, a.causal, a.window);
+  frag q[kSteps];
+  {
+    const T *from = (const T *)a.q + (int64_t)(s.first + token) * a.q_ld +
+                    (head * a.group + row - token * a.group) * a.q_head_ld;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      const int d = Q8 ? 64 * (i / 2) + 16 * grp + 8 * (i % 2) : 32 * i + 8 * grp;
+      q[i] = d < a.width ? *reinterpret_cast<const frag *>(from + d) : frag{};
+    }
+  }
+  T *const mine = reinterpret_cast<T *>(lds) + wave * kStep * DP;
+  const int width_chunks = Q8 ? a.width / 16 : a.width / 8;
+
+  bool bad = false;
+  v4i kr[2][kLoads / 2 > 0 ? kLoads / 2 : 1], vr[kLoads];
+  int ke[2], ve[Q8 ? kLoads : 1];
+  int page[2];
+  // Sixteen keys from a multiple of sixteen on lie in one page.
+  auto group_of = [&](int key0, int i) { return min(key0 + 16 * i, last & ~15); };
+  auto find = [&](int key0) __attribute__((always_inline)) {
+    if (!PAGED) return;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      page[i] = __builtin_amdgcn_readfirstlane(s.table[group_of(key0, i) >> a.map.shift]);
+  };
+  auto load = [&](int key0) __attribute__((always_inline)) {
+    constexpr int kSize = Q8 ? 1 : 2;
+    int64_t base[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (PAGED) {
+        const bool none = (unsigned)page[i] >= (unsigned)a.map.pages;
+        bad |= none;
+        base[i] = cache_row(a.map, a.kv_heads, none ? 0 : page[i], head, group_of(key0, i));
+      } else {
+        base[i] = (int64_t)s.k_first + group_of(key0, i);
+      }
+    }
+    // Of key n of sixteen, the last one for those behind it.
+    auto row_in = [&](int i, int n) { return min(n, last - group_of(key0, i)); };
+    const uint8_t *k = (const uint8_t *)a.k, *v = (const uint8_t *)a.v;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int64_t at = base[i] + row_in(i, col);
+      const uint8_t *from = PAGED ? k + at * a.width * kSize : k + (at * a.k_ld + head * a.k_head_ld) * 2;
+      if (Q8) ke[i] = a.k_exps[at];
+#pragma unroll
+      for (int c = 0; c < kLoads / 2; ++c) {
+        const int chunk = 4 * c + grp;
+        kr[i][c] = *reinterpret_cast<const v4i *>(chunk < width_chunks ? from + chunk * 16
+                                                                       : (const uint8_t *)kZeros);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < kLoads; ++c) {
+      const int n = c * kRowsOf + lane / kChunks, i = c * kRowsOf / 16, chunk = lane % kChunks;
+      const int64_t at = base[i] + row_in(i, n & 15);
+      const uint8_t *from = PAGED ? v + at * a.width * kSize : v + (at * a.v_ld + head * a.v_head_ld) * 2;
+      if (Q8) ve[c] = a.v_exps[at];
+      vr[c] = *reinterpret_cast<const v4i *>(chunk < width_chunks ? from + chunk * 16
+                                                                  : (const uint8_t *)kZeros);
+    }
+  };
+  // The values that came into LDS.
+  auto put = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < kLoads; ++c) {
+      const int n = c * kRowsOf + lane / kChunks, chunk = lane % kChunks;
+      if (Q8) {
+        frag x[2];
+        wide_of<T>(vr[c], factor_of(ve[c]), x);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          *reinterpret_cast<frag *>(mine + n * DP + few_place<DP>(n, 2 * chunk + i) * 8) = x[i];
+      } else {
+        *reinterpret_cast<v4i *>(mine + n * DP + few_place<DP>(n, chunk) * 8) = vr[c];
+      }
+    }
+  };
+
+  v4f o[kD];
+  float m, l;
+  auto pass = [&](auto careful) __attribute__((always_inline)) {  // as in k_attention_tile
+    m = -__builtin_inff();
+    l = 0.f;
+#pragma unroll
+    for (int i = 0; i < kD; ++i) o[i] = v4f{};
+    int key0 = t0 * kKeys + wave * kStep;
+    if (key0 >= end) return;
+    find(key0);
+    load(key0);
+    find(key0 + 4 * kStep);
+#pragma unroll 1
+    for (; key0 < end; key0 += 4 * kStep) {
+      v4f x[2] = {};
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float fk = Q8 ? factor_of(ke[i]) : 0.f;
+#pragma unroll
+        for (int c = 0; c < kLoads / 2; ++c) {
+          if (Q8) {
+            frag y[2];
+            wide_of<T>(kr[i][c], fk, y);
+            x[i] = Mma<T>::small(y[0], q[2 * c], x[i]);
+            x[i] = Mma<T>::small(y[1], q[2 * c + 1], x[i]);
+          } else {
+            x[i] = Mma<T>::small(__builtin_bit_cast(frag, kr[i][c]), q[c], x[i]);
+          }
+        }
+      }
+      put();
+      unsigned odd = 0;
+      if (decltype(careful)::value) {
+#pragma unroll 1
+        for (int i = lane; i < kStep * DP / 8; i += 64) {
+          const bool any = take_out<T>(mine + 8 * i);
+          // which of the rows that 64 lanes look at
+          const uint64_t lanes = __builtin_amdgcn_ballot_w64(any);
+          constexpr int kPer = DP / 8;
+#pragma unroll
+          for (int r = 0; r < 64 / kPer; ++r)
+            if (lanes >> r * kPer & ((kPer < 64 ? 1ull << kPer % 64 : 0ull) - 1)) odd |= 1u << ((i - lane) / kPer + r);
+        }
+      }
+      if (key0 + 4 * kStep < end) {
+        load(key0 + 4 * kStep);
+        find(key0 + 8 * kStep);
+      }
+      const unsigned below = key0 + 4 * grp - seen.from, span = seen.to - seen.from;
+      auto sees = [&](int i) { return below + (i / 4 * 16 + i % 4) < span; };
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (!sees(i)) x[i / 4][i % 4] = -__builtin_inff();
+      float most = x[0][0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) most = fmaxf(most, x[i / 4][i % 4]);
+      if (__builtin_amdgcn_ballot_w64(most * a.scale > m + kRise)) {
+        most = fmaxf(most, __shfl_xor(most, 16));
+        most = fmaxf(most, __shfl_xor(most, 32)) * a.scale;
+        const bool rise = most > m + kRise;
+        const float by = rise ? __builtin_amdgcn_exp2f(m - most) : 1.f;
+        m = rise ? most : m;
+        l *= by;
+#pragma unroll
+        for (int i = 0; i < kD; ++i) o[i] *= by;
+      }
+      const float ref = m == -__builtin_inff() ? 0.f : m;
+      frag p;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i / 4][i % 4], a.scale, -ref));
+        l += e;
+        p[i] = (T)e;
+      }
+      const int n = 4 * grp + (lane >> 2 & 3);
+#pragma unroll
+      for (int d = 0; d < kD; ++d) {
+        const int c = few_place<DP>(n, 2 * d + (lane >> 1 & 1)) * 8 + (lane & 1) * 4;
+        const v4s lo = read_column(mine + n * DP + c), hi = read_column(mine + (n + 16) * DP + c);
+        const v8s both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        o[d] = Mma<T>::small(__builtin_bit_cast(frag, both), p, o[d]);
+      }
+      for (; odd; odd &= odd - 1) {
+        const int j = key0 + __builtin_ctz(odd);
+        if (j < seen.from || j >= seen.to) continue;
+#pragma unroll
+        for (int i = 0; i < 4 * kD; ++i) {
+          const int e = 16 * (i / 4) + 4 * grp + i % 4;
+          const float x = e < a.width ? value_at<T, PAGED, Q8>(a, s, head, j, e) : 0.f;
+          o[i / 4][i % 4] += fabsf(x) < __builtin_inff() ? 0.f : x;
+          asm volatile("" ::: "memory");
         }
       }
     }
-    l = sum64(l);
+  };
+  pass(std::false_type());
+  float sum = 0.f;
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
+  for (int i = 0; i < 4 * kD; ++i) sum = __builtin_fmaf(o[i / 4][i % 4], 0.f, sum);
+  if (__builtin_amdgcn_ballot_w64(sum != 0.f)) pass(std::true_type());
+
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  if (PAGED && __builtin_amdgcn_ballot_w64(s.keys < 0 || bad)) l = __builtin_nanf("");
+  if (grp == 0) ml[wave][col] = make_float2(m, l);
+  __syncthreads();
+  float all = ml[0][col].x;
 #pragma unroll
-      for (int x = LANES; x < 64; x *= 2) o[k] += __shfl_xor(o[k], x);
-    const int token = r / a.group, q_head = head * a.group + r - token * a.group;
-    if (a.lse && lane == 0)
-      a.lse[(int64_t)(s.first + token) * a.heads + q_head] =
-          l == 0.f ? -__builtin_inff() : (m + log2f(l)) * 0.69314718055994531f;
-    if (sub == 0 && e < a.width) {
-      const float by = l == 0.f ? 0.f : 1.f / l;
-      typedef T four __attribute__((ext_vector_type(4)));
-      four t;
+  for (int w = 1; w < 4; ++w) all = fmaxf(all, ml[w][col].x);
+  const float by = __builtin_amdgcn_exp2f(m - (all == -__builtin_inff() ? 0.f : all));
+  // A wavefront's sums lie where its values did: [row][element], 32 bits.
+  float *sums = reinterpret_cast<float *>(lds);
+  constexpr int kLd = DP;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) t[k] = (T)(o[k] * by);
-      *reinterpret_cast<four *>((T *)a.out + (int64_t)(s.first + token) * a.out_ld +
-                                q_head * a.out_head_ld + e) = t;
+  for (int d = 0; d < kD; ++d) {
+    const v4f x = o[d] * by;
+    const int e = 16 * d + 4 * grp;
+    *reinterpret_cast<v4f *>(sums + (wave * kRows + col) * kLd + (e ^ (col & 7) * 4)) = x;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < kRows * DP / 4; i += 256) {
+    const int r = i / (DP / 4), e = i % (DP / 4) * 4;
+    if (r0 + r >= n_rows || e >= a.width) continue;
+    float top = ml[0][r].x, total = 0.f;
+#pragma unroll
+    for (int w = 1; w < 4; ++w) top = fmaxf(top, ml[w][r].x);
+    const float ref = top == -__builtin_inff() ? 0.f : top;
+    v4f x = {};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      total = __builtin_fmaf(__builtin_amdgcn_exp2f(ml[w][r].x - ref), ml[w][r].y, total);
+      x += *reinterpret_cast<const v4f *>(sums + (w * kRows + r) * kLd + (e ^ (r & 7) * 4));
     }
+    if (SPLIT && work.used > 1) {
+      const int64_t at = ((int64_t)(work.slot + work.part) * a.kv_heads + head) * kRows + r;
+      if (e == 0) split.ml[at] = make_float2(top, total);
+      *reinterpret_cast<v4f *>(split.o + at * a.width + e) = x;
+      continue;
+    }
+    const int tok = (r0 + r) / a.group, q_head = head * a.group + r0 + r - tok * a.group;
+    if (a.lse && e == 0)
+      a.lse[(int64_t)(s.first + tok) * a.heads + q_head] =
+          total == 0.f ? -__builtin_inff() : (top + log2f(total)) * 0.69314718055994531f;
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    typedef T four __attribute__((ext_vector_type(4)));
+    four t;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) t[k] = (T)(x[k] * inv);
+    *reinterpret_cast<four *>((T *)a.out + (int64_t)(s.first + tok) * a.out_ld +
+                              q_head * a.out_head_ld + e) = t;
+  }
+}
+
+// Joins the parts of a tile's rows, sixteen of them a workgroup. A thread takes four
+// elements of a row and every n-th part, eight on their way at a time; threads of the
+// same elements are joined through LDS.
+template <typename T, bool PAGED, int DP>
+__global__ __launch_bounds__(512) void k_attention_join(LmAttnArgs a, Split split, int tile_rows) {
+  constexpr int kLanes = DP / 4, kThreads = 512;
+  __shared__ v4f sums[kThreads];
+  __shared__ float2 mls[kThreads];
+  const int head = blockIdx.x % a.kv_heads;
+  const Work w = locate<kThreads, PAGED, true>(a, tile_rows, split.target, blockIdx.x / a.kv_heads);
+  const int r0 = w.r0 + blockIdx.y * 16, rows = min(min(16, tile_rows), w.n_rows - r0);
+  if (w.used <= 1 || w.part || rows <= 0) return;
+  int span = kLanes;  // threads that take a part
+  while (span < kThreads && span < rows * kLanes) span *= 2;
+  const int n = kThreads / span, sub = threadIdx.x / span;
+  const int e = threadIdx.x % kLanes * 4;
+  const int64_t step = (int64_t)a.kv_heads * tile_rows;
+  for (int i0 = 0; i0 < rows; i0 += span / kLanes) {
+    const int i = i0 + threadIdx.x % span / kLanes;
+    const bool live = i < rows && e < a.width;
+    const int64_t at0 = ((int64_t)w.slot * a.kv_heads + head) * tile_rows + blockIdx.y * 16 + min(i, rows - 1);
+    const int el = min(e, a.width - 4);
+    float m = -__builtin_inff(), l = 0.f;
+    v4f o = {};
+    for (int p0 = sub; p0 < w.used; p0 += 8 * n) {
+      float2 ml[8];
+      v4f x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int64_t at = at0 + min(p0 + u * n, w.used - 1) * step;
+        ml[u] = split.ml[at];
+        x[u] = *reinterpret_cast<const v4f *>(split.o + at * a.width + el);
+      }
+      float top = m;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        if (p0 + u * n >= w.used) {
+          ml[u] = make_float2(-__builtin_inff(), 0.f);
+          x[u] = v4f{};
+        }
+        top = fmaxf(top, ml[u].x);
+      }
+      const float ref = top == -__builtin_inff() ? 0.f : top;
+      const float f = __builtin_amdgcn_exp2f(m - ref);
+      m = top;
+      l *= f;
+      o *= f;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float by = __builtin_amdgcn_exp2f(ml[u].x - ref);
+        l = __builtin_fmaf(by, ml[u].y, l);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] = __builtin_fmaf(by, x[u][k], o[k]);
+      }
+    }
+    if (n > 1) {
+      __syncthreads();
+      sums[threadIdx.x] = o;
+      mls[threadIdx.x] = make_float2(m, l);
+      __syncthreads();
+      if (sub == 0) {
+        for (int u = 1; u < n; ++u) {
+          const float2 ml = mls[threadIdx.x + u * span];
+          const v4f x = sums[threadIdx.x + u * span];
+          const float top = fmaxf(m, ml.x), ref = top == -__builtin_inff() ? 0.f : top;
+          const float f = __builtin_amdgcn_exp2f(m - ref), g = __builtin_amdgcn_exp2f(ml.x - ref);
+          m = top;
+          l = l * f + ml.y * g;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) o[k] = o[k] * f + x[k] * g;
+        }
+      }
+    }
+    if (sub || !live) continue;
+    const int r = r0 + i, token = r / a.group, q_head = head * a.group + r - token * a.group;
+    if (a.lse && e == 0)
+      a.lse[(int64_t)(w.s.first + token) * a.heads + q_head] =
+          l == 0.f ? -__builtin_inff() : (m + log2f(l)) * 0.69314718055994531f;
+    const float by = l == 0.f ? 0.f : 1.f / l;
+    typedef T four __attribute__((ext_vector_type(4)));
+    four t;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) t[k] = (T)(o[k] * by);
+    *reinterpret_cast<four *>((T *)a.out + (int64_t)(w.s.first + token) * a.out_ld +
+                              q_head * a.out_head_ld + e) = t;
   }
 }
 
 template <typename T, bool PAGED, bool Q8, int DP>
 static void attend_launch(const LmAttnArgs &a, const Split &split, const Shape &shape, hipStream_t s) {
   const int64_t tiles = most_tiles(a.rows, a.batch, a.group, shape.tile_rows);
+  const bool few = shape.tile_rows == kFewRows;
+  const dim3 block(256);
   if (!shape.split) {
-    hv_launch(k_attention_tile<T, DP, PAGED, Q8, 4, false>, dim3((unsigned)(tiles * a.kv_heads)),
-              dim3(256), 0, s, a, split);
+    const dim3 grid((unsigned)(tiles * a.kv_heads));
+    if (few) hv_launch(k_attention_few<T, DP, PAGED, Q8, false>, grid, block, 0, s, a, split);
+    else hv_launch(k_attention_tile<T, DP, PAGED, Q8, 4, false>, grid, block, 0, s, a, split);
     return;
   }
-  hv_launch(k_attention_tile<T, DP, PAGED, Q8, 4, true>,
-            dim3((unsigned)most_slots(tiles, a.kv_heads)), dim3(256), 0, s, a, split);
-  hv_launch(k_attention_join<T, PAGED, DP / 4>,
-            dim3((unsigned)(tiles * a.kv_heads), (shape.tile_rows + 15) / 16), dim3(256), 0, s, a,
+  const dim3 grid((unsigned)most_slots(tiles, a.kv_heads, split.target));
+  if (few) hv_launch(k_attention_few<T, DP, PAGED, Q8, true>, grid, block, 0, s, a, split);
+  else hv_launch(k_attention_tile<T, DP, PAGED, Q8, 4, true>, grid, block, 0, s, a, split);
+  hv_launch(k_attention_join<T, PAGED, DP>, dim3(grid.x, shape.tile_rows / 16), dim3(512), 0, s, a,
             split, shape.tile_rows);
 }
 
 template <typename T, bool PAGED, bool Q8>
 static int attend(const LmAttnArgs &a, void *workspace, size_t bytes, hipStream_t s) {
-  const Shape shape = shape_of(a.rows, a.batch, a.heads, a.kv_heads);
+  Shape shape = shape_of(a.rows, a.batch, a.heads, a.kv_heads);
+  const int64_t most_keys = PAGED ? (int64_t)a.map.max_pages << a.map.shift : a.k_rows;
+  if (shape.tile_rows == kFewRows && most_keys <= 1024) shape.split = false;
   Split split{};
   if (shape.split) {
     const size_t need = workspace_of(a.rows, a.batch, a.heads, a.kv_heads, a.width);
@@ -553,10 +818,10 @@ static int attend(const LmAttnArgs &a, void *workspace, size_t bytes, hipStream_
       return fail(HV_EVALUE, HV_ERR_ADDRESS, "attention: a workspace of %zu bytes, %zu needed", bytes,
                   need);
     const int64_t slots =
-        most_slots(most_tiles(a.rows, a.batch, a.group, shape.tile_rows), a.kv_heads);
+        most_slots(most_tiles(a.rows, a.batch, a.group, shape.tile_rows), a.kv_heads, shape.target);
     split.o = (float *)workspace;
     split.ml = (float2 *)(split.o + slots * shape.tile_rows * a.width);
-    split.target = kTarget;
+    split.target = shape.target;
   }
   if (a.width <= 64) attend_launch<T, PAGED, Q8, 64>(a, split, shape, s);
   else if (a.width <= 128) attend_launch<T, PAGED, Q8, 128>(a, split, shape, s);

@@ -119,7 +119,7 @@ int hv::check_cache(const char *what, const hv_cache_desc &c, int type, int batc
     return fail(HV_EVALUE, HV_ERR_OPCODE, "%s: bad cache format %d", what, c.format);
   if (c.page < HV_CACHE_MIN_PAGE || c.page > HV_CACHE_MAX_PAGE || (c.page & (c.page - 1)))
     return fail(HV_EVALUE, HV_ERR_DIMENSION, "%s: pages of %d keys", what, c.page);
-  if (c.pages < 1 || c.max_pages < 0 || (int64_t)c.max_pages * c.page > 0x7FFFFFFF ||
+  if (c.pages < 1 || c.max_pages < 0 || (int64_t)c.max_pages * c.page > HV_CACHE_MAX_KEYS ||
       c.table_ld < c.max_pages)
     return fail(HV_EVALUE, HV_ERR_DIMENSION, "%s: %d pages, a table of %d in rows of %lld", what,
                 c.pages, c.max_pages, (long long)c.table_ld);

@@ -561,6 +561,7 @@ int hv_rotary_qk(const hv_rotary_desc *d, hv_stream_t stream);
 #define HV_CACHE_E4M3 1
 #define HV_CACHE_MIN_PAGE 16
 #define HV_CACHE_MAX_PAGE 4096
+#define HV_CACHE_MAX_KEYS (1 << 30) /* that a row of the table has room for */
 #define HV_ATTENTION_MAX_WIDTH 256
 
 typedef struct {
