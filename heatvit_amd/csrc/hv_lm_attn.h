@@ -70,32 +70,25 @@ __device__ __forceinline__ float factor_of(int e) {
 inline int64_t most_tiles(int rows, int batch, int group, int tile_rows) {
   return (int64_t)rows * group / tile_rows + batch;
 }
-// Parts of them that there are at most where the keys are cut into about `target`
-// workgroups' work.
-inline int64_t most_slots(int64_t tiles, int kv_heads, int target) {
-  return (tiles + (target + kv_heads - 1) / kv_heads) * kv_heads;
-}
 
-// Rows of a tile (of k_attention_few, or of k_attention_tile), and whether the keys
-// are cut into parts.
+// Rows of a tile (of k_attention_few, or of k_attention_tile), and whether the tiles' work
+// is cut into `workgroups` shares.
 static constexpr int kFewRows = 16, kTileRows = 128;
 struct Shape {
-  int tile_rows, target;
+  int tile_rows, workgroups;
   bool split;
 };
-inline Shape shape_of(int rows, int batch, int heads, int kv_heads) {
+inline Shape shape_of(int rows, int batch, int heads, int kv_heads, int width) {
   const int group = heads / kv_heads;
   const bool few = (int64_t)rows * group <= (int64_t)batch * kFewRows;
-  const int tile_rows = few ? kFewRows : kTileRows, target = few ? 1024 : 512;
+  const int tile_rows = few ? kFewRows : kTileRows;
   const int64_t items = most_tiles(rows, batch, group, tile_rows) * kv_heads;
-  return {tile_rows, target, items < (few ? 4 * target : target)};
+  return {tile_rows, width <= 128 ? 512 : 256, items < (few ? 4096 : 512)};
 }
-inline size_t workspace_of(int rows, int batch, int heads, int kv_heads, int width) {
-  const Shape shape = shape_of(rows, batch, heads, kv_heads);
-  if (!shape.split) return 0;
-  const int64_t slots = most_slots(most_tiles(rows, batch, heads / kv_heads, shape.tile_rows),
-                                   kv_heads, shape.target);
-  return (size_t)slots * shape.tile_rows * (width * 4 + 8);
+// Two partial results a workgroup: of a tile that an earlier one began, and of one that a
+// later one ends.
+inline size_t workspace_of(const Shape &shape, int width) {
+  return shape.split ? (size_t)shape.workgroups * (2 * shape.tile_rows * (width * 4 + 8) + 32) : 0;
 }
 
 // The kernels of either type. The workspace is looked at here.
@@ -103,136 +96,301 @@ int attend_f16(const LmAttnArgs &a, bool paged, bool q8, void *workspace, size_t
 int attend_bf16(const LmAttnArgs &a, bool paged, bool q8, void *workspace, size_t bytes,
                 hipStream_t s);
 
-// What a launch's parts of the keys are: every sequence's keys in parts of so many
-// tiles of 64 that all of them together are about `target` workgroups' work.
+// Shares of a launch's work where there are too few tiles to fill the card, or where whole
+// tiles would leave the last round of them on a part of it.
+// A tile that a share begins and a later one ends: rows r0 .. of n_rows of a sequence's group,
+// from row `first` of the call on, in the partial results 2 share + 1, 2 (share + 1), ..
+struct Cut {
+  int first, n_rows, r0, head, parts;  // parts 0: none
+  int unused[3];
+};
 struct Split {
-  float *o;    // [slots][rows of a tile][width], sums relative to m
-  float2 *ml;  // [slots][rows of a tile]: m, and the sum of the terms
-  int target;
+  float *o;    // [2 * workgroups][rows of a tile][width], sums relative to m
+  float2 *ml;  // [2 * workgroups][rows of a tile]: m, and the sum of the terms
+  Cut *cuts;   // [workgroups]
+  int workgroups;
 };
 
-static constexpr int kKeys = 64;         // of a tile
-static constexpr int kMinPartTiles = 4;  // of a part, at least
+static constexpr int kKeys = 64;  // of a tile
 
-__device__ __forceinline__ int key_tiles(int keys) {
-  return keys > 0 ? (int)(((int64_t)keys + kKeys - 1) / kKeys) : 0;
+__device__ __forceinline__ int key_tiles(int keys) { return keys > 0 ? (keys - 1) / kKeys + 1 : 0; }
+
+// a / b, rounded down, of numbers below 2^52.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  int64_t q = (int64_t)((double)a / (double)b);
+  const int64_t r = a - q * b;
+  return q + (r >= b) - (r < 0);
 }
 
-// A workgroup's work: a tile of a sequence's rows (of a key head's group: token r /
-// group, head r % group of it) over a part of the tiles of 64 keys that they see.
-struct Work {
-  Sequence s;
-  int keys;     // that the sequence has, 0 where its table has no room
-  int n_rows;   // s.count * group
-  int r0;       // the tile's first row
-  int t0, t1;   // tiles of keys
-  int last;     // the last key that the rows see, -1: none
-  int part, used;  // of the tile's parts; used 0: no work
-  int slot;     // of the tile's first part, among all items
+// What a sequence's tiles cost, in keys times the group: tile i (of `count`) first + step (i + 1).
+struct Cost {
+  int64_t first, step;
+  int count;
+  __device__ __forceinline__ int64_t before(int i) const {
+    return first * i + step * ((int64_t)i * (i + 1) / 2);
+  }
+  __device__ __forceinline__ int64_t all() const { return before(count); }
+  // The tile that a cost in [0, all()) lies in.
+  __device__ __forceinline__ int tile_at(int64_t at) const {
+    const double f = (double)first + .5 * (double)step;
+    int i = step ? (int)((sqrt(f * f + 2. * (double)step * (double)at) - f) / (double)step)
+                 : (int)quotient(at, first);
+    i = min(max(i, 0), count - 1);
+    while (i > 0 && before(i) > at) --i;
+    while (i < count - 1 && before(i + 1) <= at) ++i;
+    return i;
+  }
+};
+__device__ __forceinline__ Cost cost_of(const LmAttnArgs &a, const Sequence &s, int tile_rows) {
+  const int keys = max(s.keys, 0);
+  const int count = (int)(((int64_t)s.count * a.group + tile_rows - 1) / tile_rows);
+  const int64_t base = (int64_t)kKeys * a.group;  // a tile costs one of keys by itself
+  if (a.causal && !a.window)
+    return {base + (int64_t)a.group * max(keys - s.count, 0), tile_rows, count};
+  const int seen = a.window ? min(keys, a.window) : keys;
+  return {base + tile_rows + (int64_t)a.group * seen, 0, count};
+}
+
+// Shares of a launch's cost, n of them: the first `more` are one longer than the others.
+struct Shares {
+  int64_t each, more;
+  int n;
+  __device__ __forceinline__ Shares(int64_t cost, int workgroups, int group)
+      : n((int)max((int64_t)1, min((int64_t)workgroups, quotient(cost, 4 * kKeys * group)))) {
+    each = quotient(cost, n);
+    more = cost - each * n;
+  }
+  __device__ __forceinline__ int64_t start(int i) const { return each * i + min((int64_t)i, more); }
+  __device__ __forceinline__ int of(int64_t at) const {
+    const int64_t longer = more * (each + 1);
+    return (int)(at < longer ? quotient(at, each + 1) : more + quotient(at - longer, each));
+  }
 };
 
-// Work `index` of a launch of THREADS threads a workgroup, found by all of them: sequences'
-// tiles, the last ones first (which see the most keys), each by its parts.
-template <int THREADS, bool PAGED, bool SPLIT>
-__device__ __forceinline__ Work locate(const LmAttnArgs &a, int tile_rows, int target, int index) {
-  __shared__ int64_t all[THREADS / 64];
-  __shared__ int sums[THREADS / 64], found[8];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  auto tiles_of = [&](const Sequence &s) {
-    return (int)(((int64_t)s.count * a.group + tile_rows - 1) / tile_rows);
-  };
-  auto sequence = [&](int b) { return b < a.batch ? sequence_of<PAGED>(a, b) : Sequence{}; };
-  Sequence s = sequence(a.batch == 1 ? 0 : tid);
-  int part_len = 1 << 26;  // tiles of a part
-  if (SPLIT) {
-    int64_t work = (int64_t)tiles_of(s) * key_tiles(s.keys);
-    if (a.batch > 1) {
-      for (int b = tid + THREADS; b < a.batch; b += THREADS) {
-        const Sequence t = sequence(b);
-        work += (int64_t)tiles_of(t) * key_tiles(t.keys);
-      }
-#pragma unroll
-      for (int o = 1; o < 64; o *= 2) work += __shfl_xor(work, o);
-      if (lane == 0) all[wave] = work;
-      __syncthreads();
-      work = 0;
-#pragma unroll
-      for (int w = 0; w < THREADS / 64; ++w) work += all[w];
-    }
-    const int64_t n = (work * a.kv_heads + target - 1) / target;
-    part_len = (int)max((int64_t)kMinPartTiles, min(n, (int64_t)part_len));
+// How many of a tile's n tiles of keys lie before `at` of its cost.
+__device__ __forceinline__ int tiles_at(int n, int64_t at, int64_t cost) {
+  return min(n, (int)((double)n * ((double)at / (double)cost)));
+}
+
+// A tile of a sequence's rows (of a key head's group: token r / group, head r % group of it)
+// over some of the tiles of 64 keys that they see.
+struct Work {
+  Sequence s;
+  int keys;    // that the sequence has, 0 where its table has no room
+  int n_rows;  // s.count * group
+  int r0;      // the tile's first row
+  int t0, t1;  // tiles of keys
+  int last;    // the last key that the rows see, -1: none
+  int head;    // of the keys
+  int slot;    // of the partial result, -1: the result is whole
+};
+
+// A number that all lanes have, in scalar registers.
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  const unsigned lo = __builtin_amdgcn_readfirstlane((int)v);
+  return (int64_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | lo;
+}
+
+// Where a launch's work lies among the sequences, by all THREADS threads of a workgroup.
+template <int THREADS, bool PAGED>
+struct Finder {
+  const LmAttnArgs &a;
+  int tile_rows;
+  v4i *held;    // in LDS: sequence threadIdx.x, of more than one
+  int64_t all;  // cost of all sequences, for one head
+
+  __device__ __forceinline__ Sequence sequence(int b) const {
+    return b < a.batch ? sequence_of<PAGED>(a, b) : Sequence{};
   }
-  auto parts_of = [&](const Sequence &t) {
-    return SPLIT ? max(1, (key_tiles(t.keys) + part_len - 1) / part_len) : 1;
-  };
-  int rest = index, before = 0;
-  if (a.batch == 1) {
-    if (index >= tiles_of(s) * parts_of(s)) return {};
-  } else {
-    for (int base = 0;; base += THREADS) {
-      if (base >= a.batch) return {};
-      if (base) s = sequence(base + tid);
-      const int mine = tiles_of(s) * parts_of(s);
-      int upto = mine;
+  __device__ __forceinline__ Finder(const LmAttnArgs &args, int rows, bool costs)
+      : a(args), tile_rows(rows), all(0) {
+    __shared__ v4i sequences[THREADS];
+    __shared__ int64_t sums[THREADS / 64];
+    held = sequences;
+    const Sequence mine = sequence(a.batch == 1 ? 0 : threadIdx.x);
+    held[threadIdx.x] = v4i{mine.first, mine.count, mine.keys, mine.k_first};
+    if (!costs) return;
+    all = cost_of(a, mine, tile_rows).all();
+    if (a.batch == 1) return;
+    for (int b = threadIdx.x + THREADS; b < a.batch; b += THREADS)
+      all += cost_of(a, sequence(b), tile_rows).all();
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) all += __shfl_xor(all, o);
+    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = all;
+    __syncthreads();
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) all += sums[w];
+    all = uniform(all);
+  }
+  __device__ __forceinline__ Sequence mine() const {
+    if (a.batch == 1) return sequence(0);
+    const v4i t = held[threadIdx.x];
+    return {t[0], t[1], t[2], t[3], nullptr};
+  }
+
+  // The sequence whose part of the sums of count(sequence) `at` lies in, and what is before
+  // it. False: none.
+  template <typename Count>
+  __device__ __forceinline__ bool find(int64_t at, Count count, Sequence &s, int64_t &before) const {
+    before = 0;
+    if (a.batch == 1) {
+      s = mine();
+      return at < count(s);
+    }
+    __shared__ int64_t sums[THREADS / 64], found;
+    __shared__ int which, fields[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int base = 0; base < a.batch; base += THREADS) {
+      const Sequence t = base ? sequence(base + threadIdx.x) : mine();
+      const int64_t n = count(t);
+      int64_t upto = n;
 #pragma unroll
       for (int o = 1; o < 64; o *= 2) {
-        const int t = __shfl_up(upto, o);
-        if (lane >= o) upto += t;
+        const int64_t x = __shfl_up(upto, o);
+        if (lane >= o) upto += x;
       }
-      if (lane == 63) sums[wave] = upto;
-      if (tid == 0) found[0] = -1;
       __syncthreads();
-      int total = 0;
+      if (lane == 63) sums[wave] = upto;
+      if (threadIdx.x == 0) which = -1;
+      __syncthreads();
+      int64_t total = 0;
 #pragma unroll
       for (int w = 0; w < THREADS / 64; ++w) {
         if (w < wave) upto += sums[w];
         total += sums[w];
       }
-      upto += before;
-      if (index < upto && index >= upto - mine) {
-        found[0] = base + tid;
-        found[1] = upto - mine;
-        found[2] = s.first;
-        found[3] = s.count;
-        found[4] = s.keys;
-        found[5] = s.k_first;
+      const int64_t from = before + upto - n;
+      if (at >= from && at < from + n) {
+        which = base + threadIdx.x;
+        found = from;
+        fields[0] = t.first;
+        fields[1] = t.count;
+        fields[2] = t.keys;
+        fields[3] = t.k_first;
       }
       __syncthreads();
-      const int b = __builtin_amdgcn_readfirstlane(found[0]);
+      const int b = __builtin_amdgcn_readfirstlane(which);
       if (b >= 0) {
-        before = __builtin_amdgcn_readfirstlane(found[1]);
-        s = {__builtin_amdgcn_readfirstlane(found[2]), __builtin_amdgcn_readfirstlane(found[3]),
-             __builtin_amdgcn_readfirstlane(found[4]), __builtin_amdgcn_readfirstlane(found[5]),
+        before = uniform(found);
+        s = {__builtin_amdgcn_readfirstlane(fields[0]), __builtin_amdgcn_readfirstlane(fields[1]),
+             __builtin_amdgcn_readfirstlane(fields[2]), __builtin_amdgcn_readfirstlane(fields[3]),
              PAGED ? a.table + b * a.table_ld : nullptr};
-        rest = index - before;
-        break;
+        return true;
       }
-      before += total;
-      __syncthreads();
+      before += uniform(total);
     }
+    return false;
   }
-  Work w;
-  w.s = s;
-  w.keys = max(s.keys, 0);
-  w.n_rows = s.count * a.group;
-  const int parts = parts_of(s);
-  w.r0 = (tiles_of(s) - 1 - rest / parts) * tile_rows;
-  w.part = rest % parts;
-  w.slot = before + rest - w.part;
-  const Seen first = seen_by(w.r0 / a.group, s.count, w.keys, a.causal, a.window);
-  const Seen final = seen_by(min(w.r0 + tile_rows - 1, w.n_rows - 1) / a.group, s.count, w.keys,
-                             a.causal, a.window);
-  w.last = final.to - 1;
-  w.t0 = first.from / kKeys;
-  w.t1 = max(w.t0, key_tiles(final.to));
-  w.used = 1;
-  if (SPLIT) {
-    w.used = max(1, (w.t1 - w.t0 + part_len - 1) / part_len);
-    w.t0 += w.part * part_len;
-    w.t1 = min(w.t1, w.t0 + part_len);
-    if (w.part >= w.used) w.used = 0;
+
+  // Tile `tile` of a sequence, over all keys that its rows see.
+  __device__ __forceinline__ Work work_of(const Sequence &s, int tile, int head) const {
+    Work w;
+    w.s = s;
+    w.keys = max(s.keys, 0);
+    w.n_rows = s.count * a.group;
+    w.r0 = tile * tile_rows;
+    w.head = head;
+    w.slot = -1;
+    const Seen first = seen_by(w.r0 / a.group, s.count, w.keys, a.causal, a.window);
+    const Seen final = seen_by(min(w.r0 + tile_rows - 1, w.n_rows - 1) / a.group, s.count, w.keys,
+                               a.causal, a.window);
+    w.last = final.to - 1;
+    w.t0 = first.from / kKeys;
+    w.t1 = max(w.t0, key_tiles(final.to));
+    return w;
   }
-  return w;
+  // Tile `index` of all sequences', the last ones of each first, which see the most keys.
+  // False: there are fewer.
+  __device__ __forceinline__ bool whole(int index, int head, Work &w) const {
+    Sequence s;
+    int64_t before;
+    if (!find(index, [&](const Sequence &t) { return (int64_t)cost_of(a, t, tile_rows).count; }, s,
+              before))
+      return false;
+    w = work_of(s, cost_of(a, s, tile_rows).count - 1 - (int)(index - before), head);
+    return true;
+  }
+  // The tile that `at` of all heads' cost lies in, whose own starts at `from`.
+  __device__ __forceinline__ bool at(int64_t at, Work &w, int64_t &from, int64_t &cost) const {
+    const int head = (int)quotient(at, all);
+    Sequence s;
+    int64_t before;
+    if (!find(at - head * all, [&](const Sequence &t) { return cost_of(a, t, tile_rows).all(); }, s,
+              before))
+      return false;
+    before += head * all;
+    const Cost c = cost_of(a, s, tile_rows);
+    const int tile = c.tile_at(at - before);
+    from = before + c.before(tile);
+    cost = c.first + c.step * (tile + 1);
+    w = work_of(s, tile, head);
+    return true;
+  }
+};
+
+// The same work, its numbers in scalar registers.
+__device__ __forceinline__ void make_uniform(Work &w) {
+  int *const n[] = {&w.s.first, &w.s.count, &w.s.keys, &w.s.k_first, &w.keys, &w.n_rows, &w.r0,
+                    &w.t0,      &w.t1,      &w.last,   &w.head,      &w.slot};
+#pragma unroll
+  for (int i = 0; i < 12; ++i) *n[i] = __builtin_amdgcn_readfirstlane(*n[i]);
+  w.s.table = (const int32_t *)uniform((int64_t)w.s.table);
+}
+
+// The work of a workgroup: one tile, or a share of all tiles' cost, from which next() cuts
+// what it has of one tile after another. Shares that the same XCD takes lie side by side,
+// heads apart, so that they meet in its L2.
+template <int THREADS, bool PAGED, bool SPLIT>
+struct Walk {
+  Finder<THREADS, PAGED> finder;
+  const Split &split;
+  int64_t at, end;
+  int share;
+  __device__ __forceinline__ Shares shares() const {
+    return Shares(finder.all * finder.a.kv_heads, split.workgroups, finder.a.group);
+  }
+  __device__ __forceinline__ Walk(const LmAttnArgs &a, const Split &parts, int tile_rows)
+      : finder(a, tile_rows, SPLIT), split(parts), at(0), end(0), share(0) {
+    if (!SPLIT) return;
+    const Shares all = shares();
+    share = blockIdx.x;
+    if (all.n == split.workgroups) share = share % 8 * (split.workgroups / 8) + share / 8;
+    if (threadIdx.x == 0) split.cuts[share] = Cut{};
+    if (share >= all.n || !finder.all) return;
+    at = uniform(all.start(share));
+    end = uniform(all.start(share + 1));
+  }
+  __device__ __forceinline__ bool next(Work &w) {
+    if (!SPLIT) {
+      const int kv_heads = finder.a.kv_heads;
+      const bool some = finder.whole(blockIdx.x / kv_heads, blockIdx.x % kv_heads, w);
+      make_uniform(w);
+      return some;
+    }
+    int64_t from, cost;
+    if (at >= end || !finder.at(at, w, from, cost)) return false;
+    const int t0 = w.t0;
+    const int n = w.t1 - t0;
+    const bool starts = at == from, ends = end >= from + cost;
+    if (!starts) w.t0 = t0 + tiles_at(n, at - from, cost);
+    if (!ends) w.t1 = t0 + tiles_at(n, end - from, cost);
+    if (!starts || !ends) w.slot = 2 * share + starts;
+    if (starts && !ends && threadIdx.x == 0)
+      split.cuts[share] =
+          Cut{w.s.first, w.n_rows, w.r0, w.head, shares().of(from + cost - 1) - share + 1, {}};
+    at = ends ? uniform(from + cost) : end;
+    make_uniform(w);
+    return true;
+  }
+};
+
+// The thread's number, found again wherever it is asked for: what hangs on it in one stretch of
+// a kernel is not held in registers all through the others.
+__device__ __forceinline__ int thread_again() {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t;
 }
 
 }  // namespace hv

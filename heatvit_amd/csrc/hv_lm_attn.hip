@@ -53,7 +53,7 @@ extern "C" {
 
 size_t hv_attention_workspace_bytes(int rows, int batch, int heads, int kv_heads, int width) {
   if (rows <= 0 || batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || width <= 0) return 0;
-  return workspace_of(rows, batch, heads, kv_heads, width);
+  return workspace_of(shape_of(rows, batch, heads, kv_heads, width), width);
 }
 
 int hv_attention(const hv_attention_desc *d, void *workspace, size_t workspace_bytes,

@@ -137,9 +137,10 @@ struct TileLoader {
   __device__ __forceinline__ int row_of(int u) const {
     return (u * NW + wave) * kRowsOf + lane / kChunks;
   }
-  __device__ __forceinline__ TileLoader(const LmAttnArgs &args, const Sequence &seq, int h, int last_key)
-      : a(args), s(seq), head(h), lane(threadIdx.x & 63),
-        wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), last(last_key), bad(false) {}
+  __device__ __forceinline__ TileLoader(const LmAttnArgs &args, const Sequence &seq, int h, int last_key,
+                                        int tid)
+      : a(args), s(seq), head(h), lane(tid & 63), wave(__builtin_amdgcn_readfirstlane(tid >> 6)),
+        last(last_key), bad(false) {}
   // The pages of tile t's keys, which the loads of it need.
   __device__ __forceinline__ void find(int t) {
     if (!PAGED) return;
@@ -225,19 +226,23 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void k_attention_tile(L
                                                                                 Split split) {
   typedef typename Mma<T>::frag frag;
   constexpr int kRows = 32 * NW, kD = DP / 32, kSteps = DP / 16, kThreads = 64 * NW;
-  __shared__ __attribute__((aligned(16))) T k0[kKeys * DP];
-  __shared__ __attribute__((aligned(16))) T k1[kKeys * DP];
-  __shared__ __attribute__((aligned(16))) T v0[kKeys * DP];
-  __shared__ __attribute__((aligned(16))) T v1[kKeys * DP];
+  // The two tiles' keys and values: variables of their own where loads go straight to
+  // LDS, so that the compiler sees that a read of one need not wait for loads into
+  // another; one variable otherwise, whose parts share the lanes' addresses.
+  constexpr int kSize = kKeys * DP, kOwn = Q8 ? 1 : kSize;
+  __shared__ __attribute__((aligned(16))) T lds0[Q8 ? 4 * kSize : kSize], lds1[kOwn], lds2[kOwn], lds3[kOwn];
+  T *const k0 = lds0, *const k1 = Q8 ? lds0 + kSize : lds1;
+  T *const v0 = Q8 ? lds0 + 2 * kSize : lds2, *const v1 = Q8 ? lds0 + 3 * kSize : lds3;
   __shared__ unsigned long long odd_keys;
 
-  const int head = blockIdx.x % a.kv_heads;
-  const Work w = locate<kThreads, PAGED, SPLIT>(a, kRows, split.target, blockIdx.x / a.kv_heads);
-  if (!w.used) return;
+  Walk<kThreads, PAGED, SPLIT> walk(a, split, kRows);
+  Work w;
+  if (!walk.next(w)) return;
+  do {
   const Sequence &s = w.s;
-  const int keys = w.keys, n_rows = w.n_rows, r0 = w.r0, t0 = w.t0, t1 = w.t1;
+  const int head = w.head, keys = w.keys, n_rows = w.n_rows, r0 = w.r0, t0 = w.t0, t1 = w.t1;
 
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tid = thread_again(), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int w0 = r0 + wave * 32;  // the wavefront's first row
   const bool idle = w0 >= n_rows;
@@ -257,7 +262,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void k_attention_tile(L
       q[i] = d < a.width ? *reinterpret_cast<const frag *>(from + d) : frag{};
     }
   }
-  TileLoader<T, DP, PAGED, Q8, NW> loader(a, s, head, w.last);
+  TileLoader<T, DP, PAGED, Q8, NW> loader(a, s, head, w.last, tid);
   v16f o[kD];
   float m, l;
 
@@ -336,9 +341,11 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void k_attention_tile(L
     for (uint64_t left = odd_keys; left; left &= left - 1) {
       const int j = t * kKeys + __builtin_ctzll(left);
       if (j < seen.from || j >= seen.to) continue;
+      int e0 = 4 * half;
+      asm volatile("" : "+v"(e0));  // found here, and not held all along
 #pragma unroll
       for (int i = 0; i < 16 * kD; ++i) {
-        const int e = 32 * (i / 16) + 8 * (i % 16 / 4) + 4 * half + i % 4;
+        const int e = 32 * (i / 16) + 8 * (i % 16 / 4) + e0 + i % 4;
         const float x = e < a.width ? value_at<T, PAGED, Q8>(a, s, head, j, e) : 0.f;
         o[i / 16][i % 16] += fabsf(x) < __builtin_inff() ? 0.f : x;
         asm volatile("" ::: "memory");  // one after another, in few registers
@@ -379,11 +386,15 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void k_attention_tile(L
   for (int i = 0; i < 16 * kD; ++i) sum = __builtin_fmaf(o[i / 16][i % 16], 0.f, sum);
   if (__syncthreads_or(sum != 0.f)) pass(std::true_type());
 
+  // (Again, so that it is not held all along.)
+  int at_row = min(w0 + col, n_rows - 1);
+  asm volatile("" : "+v"(at_row));
+  const int out_token = at_row / a.group, out_head = head * a.group + at_row - out_token * a.group;
   l = sum_of_halves(l);
   if (PAGED && __syncthreads_or(s.keys < 0 || loader.bad)) l = __builtin_nanf("");
-  if (idle || w0 + col >= n_rows) return;
-  if (SPLIT && w.used > 1) {
-    const int64_t at = ((int64_t)(w.slot + w.part) * a.kv_heads + head) * kRows + wave * 32 + col;
+  if (idle || w0 + col >= n_rows) continue;
+  if (SPLIT && w.slot >= 0) {
+    const int64_t at = (int64_t)w.slot * kRows + wave * 32 + col;
     if (half == 0) split.ml[at] = make_float2(m, l);
     float *to = split.o + at * a.width;
 #pragma unroll
@@ -394,13 +405,13 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void k_attention_tile(L
         const v4f x = {o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
         if (e < a.width) *reinterpret_cast<v4f *>(to + e) = x;
       }
-    return;
+    continue;
   }
   const float by = l == 0.f ? 0.f : 1.f / l;
   if (a.lse && half == 0)
-    a.lse[(int64_t)(s.first + token) * a.heads + q_head] =
+    a.lse[(int64_t)(s.first + out_token) * a.heads + out_head] =
         l == 0.f ? -__builtin_inff() : (m + log2f(l)) * 0.69314718055994531f;
-  T *to = (T *)a.out + (int64_t)(s.first + token) * a.out_ld + q_head * a.out_head_ld;
+  T *to = (T *)a.out + (int64_t)(s.first + out_token) * a.out_ld + out_head * a.out_head_ld;
 #pragma unroll
   for (int d = 0; d < kD; ++d)
 #pragma unroll
@@ -419,6 +430,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void k_attention_tile(L
       const int e = 32 * d + 16 * i + 8 * half;
       if (e < a.width) *reinterpret_cast<v4i *>(to + e) = out;
     }
+  } while (SPLIT && walk.next(w));
 }
 
 // Where 16-byte chunk c of a row of values lies, where sixteen rows' 32 bytes are
@@ -456,14 +468,15 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attention_few(LmAttn
   __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kStep * DP * 2];
   __shared__ float2 ml[4][kRows];
 
-  const int head = blockIdx.x % a.kv_heads;
-  const Work work = locate<256, PAGED, SPLIT>(a, kRows, split.target, blockIdx.x / a.kv_heads);
-  if (!work.used) return;
+  Walk<256, PAGED, SPLIT> walk(a, split, kRows);
+  Work work;
+  if (!walk.next(work)) return;
+  do {
   const Sequence &s = work.s;
-  const int keys = work.keys, n_rows = work.n_rows, r0 = work.r0, t0 = work.t0;
+  const int head = work.head, keys = work.keys, n_rows = work.n_rows, r0 = work.r0, t0 = work.t0;
   const int last = work.last, end = min(work.t1 * kKeys, last + 1);
 
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tid = thread_again(), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
   const int row = min(r0 + col, n_rows - 1), token = row / a.group;
   const Seen seen = seen_by(token, s.count, keys, a.causal, a.window);
@@ -632,9 +645,11 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attention_few(LmAttn
       for (; odd; odd &= odd - 1) {
         const int j = key0 + __builtin_ctz(odd);
         if (j < seen.from || j >= seen.to) continue;
+        int e0 = 4 * grp;
+        asm volatile("" : "+v"(e0));
 #pragma unroll
         for (int i = 0; i < 4 * kD; ++i) {
-          const int e = 16 * (i / 4) + 4 * grp + i % 4;
+          const int e = 16 * (i / 4) + e0 + i % 4;
           const float x = e < a.width ? value_at<T, PAGED, Q8>(a, s, head, j, e) : 0.f;
           o[i / 4][i % 4] += fabsf(x) < __builtin_inff() ? 0.f : x;
           asm volatile("" ::: "memory");
@@ -680,8 +695,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attention_few(LmAttn
       total = __builtin_fmaf(__builtin_amdgcn_exp2f(ml[w][r].x - ref), ml[w][r].y, total);
       x += *reinterpret_cast<const v4f *>(sums + (w * kRows + r) * kLd + (e ^ (r & 7) * 4));
     }
-    if (SPLIT && work.used > 1) {
-      const int64_t at = ((int64_t)(work.slot + work.part) * a.kv_heads + head) * kRows + r;
+    if (SPLIT && work.slot >= 0) {
+      const int64_t at = (int64_t)work.slot * kRows + r;
       if (e == 0) split.ml[at] = make_float2(top, total);
       *reinterpret_cast<v4f *>(split.o + at * a.width + e) = x;
       continue;
@@ -698,45 +713,47 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attention_few(LmAttn
     *reinterpret_cast<four *>((T *)a.out + (int64_t)(s.first + tok) * a.out_ld +
                               q_head * a.out_head_ld + e) = t;
   }
+  __syncthreads();  // before the sums make room for the next values
+  } while (SPLIT && walk.next(work));
 }
 
-// Joins the parts of a tile's rows, sixteen of them a workgroup. A thread takes four
+// Joins the parts of the tiles that are cut, sixteen rows of one a workgroup. A thread takes four
 // elements of a row and every n-th part, eight on their way at a time; threads of the
 // same elements are joined through LDS.
-template <typename T, bool PAGED, int DP>
+template <typename T, int DP>
 __global__ __launch_bounds__(512) void k_attention_join(LmAttnArgs a, Split split, int tile_rows) {
   constexpr int kLanes = DP / 4, kThreads = 512;
   __shared__ v4f sums[kThreads];
   __shared__ float2 mls[kThreads];
-  const int head = blockIdx.x % a.kv_heads;
-  const Work w = locate<kThreads, PAGED, true>(a, tile_rows, split.target, blockIdx.x / a.kv_heads);
-  const int r0 = w.r0 + blockIdx.y * 16, rows = min(min(16, tile_rows), w.n_rows - r0);
-  if (w.used <= 1 || w.part || rows <= 0) return;
+  const Cut c = split.cuts[blockIdx.x];
+  const int r0 = c.r0 + blockIdx.y * 16, rows = min(16, c.n_rows - r0);
+  if (c.parts < 2 || rows <= 0) return;
+  const int share = blockIdx.x, parts = c.parts, head = c.head;
   int span = kLanes;  // threads that take a part
   while (span < kThreads && span < rows * kLanes) span *= 2;
   const int n = kThreads / span, sub = threadIdx.x / span;
   const int e = threadIdx.x % kLanes * 4;
-  const int64_t step = (int64_t)a.kv_heads * tile_rows;
   for (int i0 = 0; i0 < rows; i0 += span / kLanes) {
     const int i = i0 + threadIdx.x % span / kLanes;
     const bool live = i < rows && e < a.width;
-    const int64_t at0 = ((int64_t)w.slot * a.kv_heads + head) * tile_rows + blockIdx.y * 16 + min(i, rows - 1);
+    const int64_t row = blockIdx.y * 16 + min(i, rows - 1);
     const int el = min(e, a.width - 4);
     float m = -__builtin_inff(), l = 0.f;
     v4f o = {};
-    for (int p0 = sub; p0 < w.used; p0 += 8 * n) {
+    for (int p0 = sub; p0 < parts; p0 += 8 * n) {
       float2 ml[8];
       v4f x[8];
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        const int64_t at = at0 + min(p0 + u * n, w.used - 1) * step;
+        const int p = min(p0 + u * n, parts - 1);
+        const int64_t at = (int64_t)(2 * (share + p) + (p == 0)) * tile_rows + row;
         ml[u] = split.ml[at];
         x[u] = *reinterpret_cast<const v4f *>(split.o + at * a.width + el);
       }
       float top = m;
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        if (p0 + u * n >= w.used) {
+        if (p0 + u * n >= parts) {
           ml[u] = make_float2(-__builtin_inff(), 0.f);
           x[u] = v4f{};
         }
@@ -776,57 +793,55 @@ __global__ __launch_bounds__(512) void k_attention_join(LmAttnArgs a, Split spli
     if (sub || !live) continue;
     const int r = r0 + i, token = r / a.group, q_head = head * a.group + r - token * a.group;
     if (a.lse && e == 0)
-      a.lse[(int64_t)(w.s.first + token) * a.heads + q_head] =
+      a.lse[(int64_t)(c.first + token) * a.heads + q_head] =
           l == 0.f ? -__builtin_inff() : (m + log2f(l)) * 0.69314718055994531f;
     const float by = l == 0.f ? 0.f : 1.f / l;
     typedef T four __attribute__((ext_vector_type(4)));
     four t;
 #pragma unroll
     for (int k = 0; k < 4; ++k) t[k] = (T)(o[k] * by);
-    *reinterpret_cast<four *>((T *)a.out + (int64_t)(w.s.first + token) * a.out_ld +
+    *reinterpret_cast<four *>((T *)a.out + (int64_t)(c.first + token) * a.out_ld +
                               q_head * a.out_head_ld + e) = t;
   }
 }
 
 template <typename T, bool PAGED, bool Q8, int DP>
 static void attend_launch(const LmAttnArgs &a, const Split &split, const Shape &shape, hipStream_t s) {
-  const int64_t tiles = most_tiles(a.rows, a.batch, a.group, shape.tile_rows);
   const bool few = shape.tile_rows == kFewRows;
-  const dim3 block(256);
+  const unsigned items =
+      (unsigned)(most_tiles(a.rows, a.batch, a.group, shape.tile_rows) * a.kv_heads);
+  const dim3 grid(shape.split ? shape.workgroups : items), block(256);
   if (!shape.split) {
-    const dim3 grid((unsigned)(tiles * a.kv_heads));
     if (few) hv_launch(k_attention_few<T, DP, PAGED, Q8, false>, grid, block, 0, s, a, split);
     else hv_launch(k_attention_tile<T, DP, PAGED, Q8, 4, false>, grid, block, 0, s, a, split);
     return;
   }
-  const dim3 grid((unsigned)most_slots(tiles, a.kv_heads, split.target));
   if (few) hv_launch(k_attention_few<T, DP, PAGED, Q8, true>, grid, block, 0, s, a, split);
   else hv_launch(k_attention_tile<T, DP, PAGED, Q8, 4, true>, grid, block, 0, s, a, split);
-  hv_launch(k_attention_join<T, PAGED, DP>, dim3(grid.x, shape.tile_rows / 16), dim3(512), 0, s, a,
+  hv_launch(k_attention_join<T, DP>, dim3(shape.workgroups, shape.tile_rows / 16), dim3(512), 0, s, a,
             split, shape.tile_rows);
 }
 
 template <typename T, bool PAGED, bool Q8>
 static int attend(const LmAttnArgs &a, void *workspace, size_t bytes, hipStream_t s) {
-  Shape shape = shape_of(a.rows, a.batch, a.heads, a.kv_heads);
-  const int64_t most_keys = PAGED ? (int64_t)a.map.max_pages << a.map.shift : a.k_rows;
-  if (shape.tile_rows == kFewRows && most_keys <= 1024) shape.split = false;
+  Shape shape = shape_of(a.rows, a.batch, a.heads, a.kv_heads, a.width);
   Split split{};
   if (shape.split) {
-    const size_t need = workspace_of(a.rows, a.batch, a.heads, a.kv_heads, a.width);
+    const size_t need = workspace_of(shape, a.width);
     if (!workspace || bytes < need || ((uintptr_t)workspace & 15))
       return fail(HV_EVALUE, HV_ERR_ADDRESS, "attention: a workspace of %zu bytes, %zu needed", bytes,
                   need);
-    const int64_t slots =
-        most_slots(most_tiles(a.rows, a.batch, a.group, shape.tile_rows), a.kv_heads, shape.target);
     split.o = (float *)workspace;
-    split.ml = (float2 *)(split.o + slots * shape.tile_rows * a.width);
-    split.target = shape.target;
+    split.ml = (float2 *)(split.o + (int64_t)2 * shape.workgroups * shape.tile_rows * a.width);
+    split.cuts = (Cut *)(split.ml + (int64_t)2 * shape.workgroups * shape.tile_rows);
+    split.workgroups = shape.workgroups;
+    const int64_t most_keys = PAGED ? (int64_t)a.map.max_pages << a.map.shift : a.k_rows;
+    if (most_keys <= 1024) shape.split = false;
   }
   if (a.width <= 64) attend_launch<T, PAGED, Q8, 64>(a, split, shape, s);
   else if (a.width <= 128) attend_launch<T, PAGED, Q8, 128>(a, split, shape, s);
   else attend_launch<T, PAGED, Q8, 256>(a, split, shape, s);
-  return check_hip(hipGetLastError(), "k_attention_tile launch");
+  return check_hip(hipGetLastError(), "k_attention launch");
 }
 
 template <typename T>
