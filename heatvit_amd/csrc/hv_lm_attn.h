@@ -87,8 +87,12 @@ inline Shape shape_of(int rows, int batch, int heads, int kv_heads, int width) {
 }
 // Two partial results a workgroup: of a tile that an earlier one began, and of one that a
 // later one ends.
+inline int slot_floats_of(const Shape &shape, int width) {
+  // 64 more than it takes: slots a power of two apart meet in the same memory channels.
+  return shape.tile_rows * (width + 2) + 64;
+}
 inline size_t workspace_of(const Shape &shape, int width) {
-  return shape.split ? (size_t)shape.workgroups * (2 * shape.tile_rows * (width * 4 + 8) + 32) : 0;
+  return shape.split ? (size_t)shape.workgroups * (8 * slot_floats_of(shape, width) + 32) : 0;
 }
 
 // The kernels of either type. The workspace is looked at here.
@@ -105,37 +109,34 @@ struct Cut {
   int unused[3];
 };
 struct Split {
-  float *o;    // [2 * workgroups][rows of a tile][width], sums relative to m
-  float2 *ml;  // [2 * workgroups][rows of a tile]: m, and the sum of the terms
-  Cut *cuts;   // [workgroups]
-  int workgroups;
+  Cut *cuts;      // [workgroups]
+  float *slots;   // [2 * workgroups][slot_floats]: partial results
+  int workgroups, tile_rows, slot_floats;
+  // Row r of a partial result: m and the sum of the terms, and the sums relative to m.
+  __device__ __forceinline__ float2 *ml(int slot, int r) const {
+    return reinterpret_cast<float2 *>(slots + (int64_t)slot * slot_floats) + r;
+  }
+  __device__ __forceinline__ float *sums(int slot, int r, int width) const {
+    return slots + (int64_t)slot * slot_floats + 2 * tile_rows + r * width;
+  }
 };
 
 static constexpr int kKeys = 64;  // of a tile
 
 __device__ __forceinline__ int key_tiles(int keys) { return keys > 0 ? (keys - 1) / kKeys + 1 : 0; }
 
-// a / b, rounded down, of numbers below 2^52.
-__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
-  int64_t q = (int64_t)((double)a / (double)b);
-  const int64_t r = a - q * b;
-  return q + (r >= b) - (r < 0);
-}
-
-// What a sequence's tiles cost, in keys times the group: tile i (of `count`) first + step (i + 1).
+// What a sequence's tiles cost, in sixteenths of a tile of keys: tile i (of `count`) first +
+// step (i + 1). Sums over a launch's tiles, 4096 at most where shares are taken, fit 32 bits.
+static constexpr int kCostlyTiles = 1 << 14;  // of keys: more count as so many
 struct Cost {
-  int64_t first, step;
-  int count;
-  __device__ __forceinline__ int64_t before(int i) const {
-    return first * i + step * ((int64_t)i * (i + 1) / 2);
-  }
-  __device__ __forceinline__ int64_t all() const { return before(count); }
+  int first, step, count;
+  __device__ __forceinline__ int before(int i) const { return first * i + step * (i * (i + 1) / 2); }
+  __device__ __forceinline__ int all() const { return before(count); }
   // The tile that a cost in [0, all()) lies in.
-  __device__ __forceinline__ int tile_at(int64_t at) const {
-    const double f = (double)first + .5 * (double)step;
-    int i = step ? (int)((sqrt(f * f + 2. * (double)step * (double)at) - f) / (double)step)
-                 : (int)quotient(at, first);
-    i = min(max(i, 0), count - 1);
+  __device__ __forceinline__ int tile_at(int at) const {
+    const float f = first + .5f * step;
+    int i = step ? (int)((sqrtf(f * f + 2.f * step * at) - f) / step) : at / first;
+    i = clamp_to(i, 0, count - 1);
     while (i > 0 && before(i) > at) --i;
     while (i < count - 1 && before(i + 1) <= at) ++i;
     return i;
@@ -144,32 +145,31 @@ struct Cost {
 __device__ __forceinline__ Cost cost_of(const LmAttnArgs &a, const Sequence &s, int tile_rows) {
   const int keys = max(s.keys, 0);
   const int count = (int)(((int64_t)s.count * a.group + tile_rows - 1) / tile_rows);
-  const int64_t base = (int64_t)kKeys * a.group;  // a tile costs one of keys by itself
-  if (a.causal && !a.window)
-    return {base + (int64_t)a.group * max(keys - s.count, 0), tile_rows, count};
-  const int seen = a.window ? min(keys, a.window) : keys;
-  return {base + tile_rows + (int64_t)a.group * seen, 0, count};
+  // A tile costs one of keys by itself.
+  auto cost = [](int seen) { return 16 * min(1 + key_tiles(seen), kCostlyTiles); };
+  if (a.causal && !a.window) return {cost(max(keys - s.count, 0)), tile_rows / (4 * a.group), count};
+  return {cost(a.window ? min(keys, a.window) : keys), 0, count};
 }
 
-// Shares of a launch's cost, n of them: the first `more` are one longer than the others.
+// Shares of a launch's cost, n of them of four tiles of keys at least: the first `more` are one
+// longer than the others.
 struct Shares {
-  int64_t each, more;
-  int n;
-  __device__ __forceinline__ Shares(int64_t cost, int workgroups, int group)
-      : n((int)max((int64_t)1, min((int64_t)workgroups, quotient(cost, 4 * kKeys * group)))) {
-    each = quotient(cost, n);
+  int n, each, more;
+  __device__ __forceinline__ Shares(int cost, int workgroups) {
+    n = clamp_to(cost / 64, 1, workgroups);
+    each = cost / n;
     more = cost - each * n;
   }
-  __device__ __forceinline__ int64_t start(int i) const { return each * i + min((int64_t)i, more); }
-  __device__ __forceinline__ int of(int64_t at) const {
-    const int64_t longer = more * (each + 1);
-    return (int)(at < longer ? quotient(at, each + 1) : more + quotient(at - longer, each));
+  __device__ __forceinline__ int start(int i) const { return each * i + min(i, more); }
+  __device__ __forceinline__ int of(int at) const {
+    const int longer = more * (each + 1);
+    return at < longer ? at / (each + 1) : more + (at - longer) / each;
   }
 };
 
 // How many of a tile's n tiles of keys lie before `at` of its cost.
-__device__ __forceinline__ int tiles_at(int n, int64_t at, int64_t cost) {
-  return min(n, (int)((double)n * ((double)at / (double)cost)));
+__device__ __forceinline__ int tiles_at(int n, int at, int cost) {
+  return min(n, (int)((float)n * ((float)at / (float)cost)));
 }
 
 // A tile of a sequence's rows (of a key head's group: token r / group, head r % group of it)
@@ -185,19 +185,16 @@ struct Work {
   int slot;    // of the partial result, -1: the result is whole
 };
 
-// A number that all lanes have, in scalar registers.
-__device__ __forceinline__ int64_t uniform(int64_t v) {
-  const unsigned lo = __builtin_amdgcn_readfirstlane((int)v);
-  return (int64_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | lo;
-}
+// A number that all lanes have, in a scalar register.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // Where a launch's work lies among the sequences, by all THREADS threads of a workgroup.
 template <int THREADS, bool PAGED>
 struct Finder {
   const LmAttnArgs &a;
   int tile_rows;
-  v4i *held;    // in LDS: sequence threadIdx.x, of more than one
-  int64_t all;  // cost of all sequences, for one head
+  v4i *held;  // in LDS: sequence threadIdx.x, of more than one
+  int all;    // cost of all sequences, for one head
 
   __device__ __forceinline__ Sequence sequence(int b) const {
     return b < a.batch ? sequence_of<PAGED>(a, b) : Sequence{};
@@ -205,13 +202,16 @@ struct Finder {
   __device__ __forceinline__ Finder(const LmAttnArgs &args, int rows, bool costs)
       : a(args), tile_rows(rows), all(0) {
     __shared__ v4i sequences[THREADS];
-    __shared__ int64_t sums[THREADS / 64];
+    __shared__ int sums[THREADS / 64];
     held = sequences;
-    const Sequence mine = sequence(a.batch == 1 ? 0 : threadIdx.x);
-    held[threadIdx.x] = v4i{mine.first, mine.count, mine.keys, mine.k_first};
+    if (a.batch == 1) {
+      if (costs) all = uniform(cost_of(a, sequence(0), tile_rows).all());
+      return;
+    }
+    const Sequence first = sequence(threadIdx.x);
+    held[threadIdx.x] = v4i{first.first, first.count, first.keys, first.k_first};
     if (!costs) return;
-    all = cost_of(a, mine, tile_rows).all();
-    if (a.batch == 1) return;
+    all = cost_of(a, first, tile_rows).all();
     for (int b = threadIdx.x + THREADS; b < a.batch; b += THREADS)
       all += cost_of(a, sequence(b), tile_rows).all();
 #pragma unroll
@@ -223,58 +223,57 @@ struct Finder {
     for (int w = 0; w < THREADS / 64; ++w) all += sums[w];
     all = uniform(all);
   }
-  __device__ __forceinline__ Sequence mine() const {
-    if (a.batch == 1) return sequence(0);
-    const v4i t = held[threadIdx.x];
-    return {t[0], t[1], t[2], t[3], nullptr};
-  }
 
   // The sequence whose part of the sums of count(sequence) `at` lies in, and what is before
   // it. False: none.
   template <typename Count>
-  __device__ __forceinline__ bool find(int64_t at, Count count, Sequence &s, int64_t &before) const {
+  __device__ __forceinline__ bool find(int at, Count count, Sequence &s, int &before) const {
     before = 0;
     if (a.batch == 1) {
-      s = mine();
+      s = sequence(0);
       return at < count(s);
     }
-    __shared__ int64_t sums[THREADS / 64], found;
-    __shared__ int which, fields[4];
+    __shared__ int sums[THREADS / 64], found[6];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int base = 0; base < a.batch; base += THREADS) {
-      const Sequence t = base ? sequence(base + threadIdx.x) : mine();
-      const int64_t n = count(t);
-      int64_t upto = n;
+      Sequence t;
+      if (base) {
+        t = sequence(base + threadIdx.x);
+      } else {
+        const v4i x = held[threadIdx.x];
+        t = {x[0], x[1], x[2], x[3], nullptr};
+      }
+      const int n = count(t);
+      int upto = n;
 #pragma unroll
       for (int o = 1; o < 64; o *= 2) {
-        const int64_t x = __shfl_up(upto, o);
+        const int x = __shfl_up(upto, o);
         if (lane >= o) upto += x;
       }
       __syncthreads();
       if (lane == 63) sums[wave] = upto;
-      if (threadIdx.x == 0) which = -1;
+      if (threadIdx.x == 0) found[0] = -1;
       __syncthreads();
-      int64_t total = 0;
+      int total = 0;
 #pragma unroll
       for (int w = 0; w < THREADS / 64; ++w) {
         if (w < wave) upto += sums[w];
         total += sums[w];
       }
-      const int64_t from = before + upto - n;
+      const int from = before + upto - n;
       if (at >= from && at < from + n) {
-        which = base + threadIdx.x;
-        found = from;
-        fields[0] = t.first;
-        fields[1] = t.count;
-        fields[2] = t.keys;
-        fields[3] = t.k_first;
+        found[0] = base + threadIdx.x;
+        found[1] = from;
+        found[2] = t.first;
+        found[3] = t.count;
+        found[4] = t.keys;
+        found[5] = t.k_first;
       }
       __syncthreads();
-      const int b = __builtin_amdgcn_readfirstlane(which);
+      const int b = uniform(found[0]);
       if (b >= 0) {
-        before = uniform(found);
-        s = {__builtin_amdgcn_readfirstlane(fields[0]), __builtin_amdgcn_readfirstlane(fields[1]),
-             __builtin_amdgcn_readfirstlane(fields[2]), __builtin_amdgcn_readfirstlane(fields[3]),
+        before = uniform(found[1]);
+        s = {uniform(found[2]), uniform(found[3]), uniform(found[4]), uniform(found[5]),
              PAGED ? a.table + b * a.table_ld : nullptr};
         return true;
       }
@@ -304,18 +303,17 @@ struct Finder {
   // False: there are fewer.
   __device__ __forceinline__ bool whole(int index, int head, Work &w) const {
     Sequence s;
-    int64_t before;
-    if (!find(index, [&](const Sequence &t) { return (int64_t)cost_of(a, t, tile_rows).count; }, s,
-              before))
+    int before;
+    if (!find(index, [&](const Sequence &t) { return cost_of(a, t, tile_rows).count; }, s, before))
       return false;
-    w = work_of(s, cost_of(a, s, tile_rows).count - 1 - (int)(index - before), head);
+    w = work_of(s, cost_of(a, s, tile_rows).count - 1 - (index - before), head);
     return true;
   }
   // The tile that `at` of all heads' cost lies in, whose own starts at `from`.
-  __device__ __forceinline__ bool at(int64_t at, Work &w, int64_t &from, int64_t &cost) const {
-    const int head = (int)quotient(at, all);
+  __device__ __forceinline__ bool at(int at, Work &w, int &from, int &cost) const {
+    const int head = at / all;
     Sequence s;
-    int64_t before;
+    int before;
     if (!find(at - head * all, [&](const Sequence &t) { return cost_of(a, t, tile_rows).all(); }, s,
               before))
       return false;
@@ -334,8 +332,10 @@ __device__ __forceinline__ void make_uniform(Work &w) {
   int *const n[] = {&w.s.first, &w.s.count, &w.s.keys, &w.s.k_first, &w.keys, &w.n_rows, &w.r0,
                     &w.t0,      &w.t1,      &w.last,   &w.head,      &w.slot};
 #pragma unroll
-  for (int i = 0; i < 12; ++i) *n[i] = __builtin_amdgcn_readfirstlane(*n[i]);
-  w.s.table = (const int32_t *)uniform((int64_t)w.s.table);
+  for (int i = 0; i < 12; ++i) *n[i] = uniform(*n[i]);
+  const uint64_t table = (uint64_t)w.s.table;
+  w.s.table = (const int32_t *)((uint64_t)(unsigned)uniform((int)(table >> 32)) << 32 |
+                                (unsigned)uniform((int)table));
 }
 
 // The work of a workgroup: one tile, or a share of all tiles' cost, from which next() cuts
@@ -345,10 +345,9 @@ template <int THREADS, bool PAGED, bool SPLIT>
 struct Walk {
   Finder<THREADS, PAGED> finder;
   const Split &split;
-  int64_t at, end;
-  int share;
+  int at, end, share;
   __device__ __forceinline__ Shares shares() const {
-    return Shares(finder.all * finder.a.kv_heads, split.workgroups, finder.a.group);
+    return Shares(finder.all * finder.a.kv_heads, split.workgroups);
   }
   __device__ __forceinline__ Walk(const LmAttnArgs &a, const Split &parts, int tile_rows)
       : finder(a, tile_rows, SPLIT), split(parts), at(0), end(0), share(0) {
@@ -357,7 +356,7 @@ struct Walk {
     share = blockIdx.x;
     if (all.n == split.workgroups) share = share % 8 * (split.workgroups / 8) + share / 8;
     if (threadIdx.x == 0) split.cuts[share] = Cut{};
-    if (share >= all.n || !finder.all) return;
+    if (share >= all.n || finder.all <= 0) return;
     at = uniform(all.start(share));
     end = uniform(all.start(share + 1));
   }
@@ -368,10 +367,9 @@ struct Walk {
       make_uniform(w);
       return some;
     }
-    int64_t from, cost;
+    int from, cost;
     if (at >= end || !finder.at(at, w, from, cost)) return false;
-    const int t0 = w.t0;
-    const int n = w.t1 - t0;
+    const int t0 = w.t0, n = w.t1 - t0;
     const bool starts = at == from, ends = end >= from + cost;
     if (!starts) w.t0 = t0 + tiles_at(n, at - from, cost);
     if (!ends) w.t1 = t0 + tiles_at(n, end - from, cost);
@@ -379,7 +377,9 @@ struct Walk {
     if (starts && !ends && threadIdx.x == 0)
       split.cuts[share] =
           Cut{w.s.first, w.n_rows, w.r0, w.head, shares().of(from + cost - 1) - share + 1, {}};
-    at = ends ? uniform(from + cost) : end;
+    const int then = ends ? from + cost : end;
+    if (then <= at) return false;  // offsets that run backwards: sums past 32 bits
+    at = uniform(then);
     make_uniform(w);
     return true;
   }

@@ -394,9 +394,8 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void k_attention_tile(L
   if (PAGED && __syncthreads_or(s.keys < 0 || loader.bad)) l = __builtin_nanf("");
   if (idle || w0 + col >= n_rows) continue;
   if (SPLIT && w.slot >= 0) {
-    const int64_t at = (int64_t)w.slot * kRows + wave * 32 + col;
-    if (half == 0) split.ml[at] = make_float2(m, l);
-    float *to = split.o + at * a.width;
+    if (half == 0) *split.ml(w.slot, wave * 32 + col) = make_float2(m, l);
+    float *to = split.sums(w.slot, wave * 32 + col, a.width);
 #pragma unroll
     for (int d = 0; d < kD; ++d)
 #pragma unroll
@@ -696,9 +695,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attention_few(LmAttn
       x += *reinterpret_cast<const v4f *>(sums + (w * kRows + r) * kLd + (e ^ (r & 7) * 4));
     }
     if (SPLIT && work.slot >= 0) {
-      const int64_t at = (int64_t)work.slot * kRows + r;
-      if (e == 0) split.ml[at] = make_float2(top, total);
-      *reinterpret_cast<v4f *>(split.o + at * a.width + e) = x;
+      if (e == 0) *split.ml(work.slot, r) = make_float2(top, total);
+      *reinterpret_cast<v4f *>(split.sums(work.slot, r, a.width) + e) = x;
       continue;
     }
     const int tok = (r0 + r) / a.group, q_head = head * a.group + r0 + r - tok * a.group;
@@ -721,14 +719,17 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attention_few(LmAttn
 // elements of a row and every n-th part, eight on their way at a time; threads of the
 // same elements are joined through LDS.
 template <typename T, int DP>
-__global__ __launch_bounds__(512) void k_attention_join(LmAttnArgs a, Split split, int tile_rows) {
+__global__ __launch_bounds__(512) void k_attention_join(LmAttnArgs a, Split split) {
   constexpr int kLanes = DP / 4, kThreads = 512;
   __shared__ v4f sums[kThreads];
   __shared__ float2 mls[kThreads];
-  const Cut c = split.cuts[blockIdx.x];
+  // Neighbouring workgroups, which lie on different XCDs, take shares that are far apart:
+  // those that cut a tile may be every n-th.
+  const int share = blockIdx.x % 8 * (split.workgroups / 8) + blockIdx.x / 8;
+  const Cut c = split.cuts[share];
   const int r0 = c.r0 + blockIdx.y * 16, rows = min(16, c.n_rows - r0);
   if (c.parts < 2 || rows <= 0) return;
-  const int share = blockIdx.x, parts = c.parts, head = c.head;
+  const int parts = c.parts, head = c.head;
   int span = kLanes;  // threads that take a part
   while (span < kThreads && span < rows * kLanes) span *= 2;
   const int n = kThreads / span, sub = threadIdx.x / span;
@@ -736,7 +737,7 @@ __global__ __launch_bounds__(512) void k_attention_join(LmAttnArgs a, Split spli
   for (int i0 = 0; i0 < rows; i0 += span / kLanes) {
     const int i = i0 + threadIdx.x % span / kLanes;
     const bool live = i < rows && e < a.width;
-    const int64_t row = blockIdx.y * 16 + min(i, rows - 1);
+    const int row = blockIdx.y * 16 + min(i, rows - 1);
     const int el = min(e, a.width - 4);
     float m = -__builtin_inff(), l = 0.f;
     v4f o = {};
@@ -746,9 +747,9 @@ __global__ __launch_bounds__(512) void k_attention_join(LmAttnArgs a, Split spli
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         const int p = min(p0 + u * n, parts - 1);
-        const int64_t at = (int64_t)(2 * (share + p) + (p == 0)) * tile_rows + row;
-        ml[u] = split.ml[at];
-        x[u] = *reinterpret_cast<const v4f *>(split.o + at * a.width + el);
+        const int slot = 2 * (share + p) + (p == 0);
+        ml[u] = *split.ml(slot, row);
+        x[u] = *reinterpret_cast<const v4f *>(split.sums(slot, row, a.width) + el);
       }
       float top = m;
 #pragma unroll
@@ -819,7 +820,7 @@ static void attend_launch(const LmAttnArgs &a, const Split &split, const Shape &
   if (few) hv_launch(k_attention_few<T, DP, PAGED, Q8, true>, grid, block, 0, s, a, split);
   else hv_launch(k_attention_tile<T, DP, PAGED, Q8, 4, true>, grid, block, 0, s, a, split);
   hv_launch(k_attention_join<T, DP>, dim3(shape.workgroups, shape.tile_rows / 16), dim3(512), 0, s, a,
-            split, shape.tile_rows);
+            split);
 }
 
 template <typename T, bool PAGED, bool Q8>
@@ -831,10 +832,11 @@ static int attend(const LmAttnArgs &a, void *workspace, size_t bytes, hipStream_
     if (!workspace || bytes < need || ((uintptr_t)workspace & 15))
       return fail(HV_EVALUE, HV_ERR_ADDRESS, "attention: a workspace of %zu bytes, %zu needed", bytes,
                   need);
-    split.o = (float *)workspace;
-    split.ml = (float2 *)(split.o + (int64_t)2 * shape.workgroups * shape.tile_rows * a.width);
-    split.cuts = (Cut *)(split.ml + (int64_t)2 * shape.workgroups * shape.tile_rows);
+    split.cuts = (Cut *)workspace;
+    split.slots = (float *)(split.cuts + shape.workgroups);
     split.workgroups = shape.workgroups;
+    split.tile_rows = shape.tile_rows;
+    split.slot_floats = slot_floats_of(shape, a.width);
     const int64_t most_keys = PAGED ? (int64_t)a.map.max_pages << a.map.shift : a.k_rows;
     if (most_keys <= 1024) shape.split = false;
   }
