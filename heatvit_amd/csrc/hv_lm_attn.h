@@ -60,10 +60,10 @@ struct Pair8<f16> {
   }
 };
 
-// 2^e of an exponent in [-127, 127], NaN for -128. (The conversion's factor is
-// taken by its exponent alone, which 2^-127 still has.)
-__device__ __forceinline__ float factor_of(int e) {
-  return __builtin_bit_cast(float, e == -128 ? 0x7FC00000 : (e + 127) << 23);
+// 2^e of an exponent's byte. (The conversion takes its factor by the exponent alone, which 2^-127
+// still has.) A byte is taken as it was loaded: to extend its sign there would wait for it.
+__device__ __forceinline__ float factor_of(int byte) {
+  return __builtin_bit_cast(float, ((byte ^ 0x80) - 1) << 23);
 }
 
 // Tiles of `tile_rows` rows that a call's sequences have at most.
@@ -87,6 +87,16 @@ inline Shape shape_of(int rows, int batch, int heads, int kv_heads, int width) {
 }
 // Two partial results a workgroup: of a tile that an earlier one began, and of one that a
 // later one ends.
+// Shares cost a launch and the partial results' way through memory. Few rows: 8 sequences
+// of up to 1000 keys take 13.5 us whole, 13.7 in shares; one of 2048 16. Tiles: 14 + 15
+// us, where whole tiles take 2 us for each 64 keys and leave the card's 512 workgroups short
+// of (512 - items) of them (one prompt of 1536 tokens, 384 items: 64 us in shares).
+inline bool worth_sharing(const Shape &shape, int rows, int batch, int kv_heads, int group,
+                          int64_t most_keys) {
+  if (shape.tile_rows == kFewRows) return most_keys > 1024;
+  return most_keys * (512 - most_tiles(rows, batch, group, shape.tile_rows) * kv_heads) > 1 << 19;
+}
+
 inline int slot_floats_of(const Shape &shape, int width) {
   // 64 more than it takes: slots a power of two apart meet in the same memory channels.
   return shape.tile_rows * (width + 2) + 64;

@@ -95,7 +95,7 @@ __device__ __forceinline__ float value_at(const LmAttnArgs &a, const Sequence &s
   if (page < 0) return 0.f;
   const int64_t row = cache_row(a.map, a.kv_heads, page, head, j);
   if (!Q8) return (float)((const T *)a.v)[row * a.width + d];
-  const auto x = Pair8<T>::of(((const uint8_t *)a.v)[row * a.width + d], factor_of(a.v_exps[row]), false);
+  const auto x = Pair8<T>::of(((const uint8_t *)a.v)[row * a.width + d], factor_of((uint8_t)a.v_exps[row]), false);
   return (float)x[0];
 }
 
@@ -113,6 +113,12 @@ __device__ __forceinline__ bool take_out(void *at) {
   }
   if (any) *reinterpret_cast<eight *>(at) = v;
   return any;
+}
+
+// A pointer to global memory, said so to the compiler.
+template <typename P>
+__device__ __forceinline__ const __attribute__((address_space(1))) P *global(const P *p) {
+  return (const __attribute__((address_space(1))) P *)p;
 }
 
 // What is loaded behind a head's width.
@@ -146,7 +152,7 @@ struct TileLoader {
     if (!PAGED) return;
 #pragma unroll
     for (int u = 0; u < kUnits; ++u)
-      page[u] = s.table[min(t * kKeys + row_of(u), last) >> a.map.shift];
+      page[u] = global(s.table)[min(t * kKeys + row_of(u), last) >> a.map.shift];
   }
   // Tile t on its way into k and v (Q8: into registers).
   __device__ __forceinline__ void load(int t, T *k, T *v) {
@@ -160,8 +166,8 @@ struct TileLoader {
         bad |= none;
         at_k = cache_row(a.map, a.kv_heads, none ? 0 : page[u], head, key);
         if (Q8) {
-          exps[2 * u] = a.k_exps[at_k];
-          exps[2 * u + 1] = a.v_exps[at_k];
+          exps[2 * u] = (uint8_t)a.k_exps[at_k];
+          exps[2 * u + 1] = (uint8_t)a.v_exps[at_k];
         }
         at_k = at_v = at_k * a.width;
       } else {
@@ -171,8 +177,8 @@ struct TileLoader {
       }
       if (Q8) {
         const int64_t off = at_k + min(c, chunks - 1) * 16;
-        held[2 * u] = *reinterpret_cast<const v4i *>((const uint8_t *)a.k + off);
-        held[2 * u + 1] = *reinterpret_cast<const v4i *>((const uint8_t *)a.v + off);
+        held[2 * u] = *global((const v4i *)((const uint8_t *)a.k + off));
+        held[2 * u + 1] = *global((const v4i *)((const uint8_t *)a.v + off));
       } else {
         const int kc = k_place<DP>(row, c), vc = v_place<DP>(row, c);
         to_lds(kc < chunks ? (const T *)a.k + at_k + kc * 8 : (const T *)kZeros,
@@ -479,6 +485,9 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attention_few(LmAttn
   const int col = lane & 15, grp = lane >> 4;
   const int row = min(r0 + col, n_rows - 1), token = row / a.group;
   const Seen seen = seen_by(token, s.count, keys, a.causal, a.window);
+  // What all rows see starts at fin.from and ends at top.to.
+  const Seen top = seen_by(r0 / a.group, s.count, keys, a.causal, a.window);
+  const Seen fin = seen_by(min(r0 + kRows - 1, n_rows - 1) / a.group, s.count, keys, a.causal, a.window);
   frag q[kSteps];
   {
     const T *from = (const T *)a.q + (int64_t)(s.first + token) * a.q_ld +
@@ -493,7 +502,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attention_few(LmAttn
   const int width_chunks = Q8 ? a.width / 16 : a.width / 8;
 
   bool bad = false;
-  v4i kr[2][kLoads / 2 > 0 ? kLoads / 2 : 1], vr[kLoads];
+  v4i kr[2][kLoads / 2], vr[kLoads];
   int ke[2], ve[Q8 ? kLoads : 1];
   int page[2];
   // Sixteen keys from a multiple of sixteen on lie in one page.
@@ -501,45 +510,43 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attention_few(LmAttn
   auto find = [&](int key0) __attribute__((always_inline)) {
     if (!PAGED) return;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      page[i] = __builtin_amdgcn_readfirstlane(s.table[group_of(key0, i) >> a.map.shift]);
+    for (int i = 0; i < 2; ++i) page[i] = global(s.table)[group_of(key0, i) >> a.map.shift];
   };
   auto load = [&](int key0) __attribute__((always_inline)) {
     constexpr int kSize = Q8 ? 1 : 2;
-    int64_t base[2];
+    int64_t base[2];  // the groups' first rows
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if (PAGED) {
-        const bool none = (unsigned)page[i] >= (unsigned)a.map.pages;
+        const int p = uniform(page[i]);
+        const bool none = (unsigned)p >= (unsigned)a.map.pages;
         bad |= none;
-        base[i] = cache_row(a.map, a.kv_heads, none ? 0 : page[i], head, group_of(key0, i));
+        base[i] = cache_row(a.map, a.kv_heads, none ? 0 : p, head, group_of(key0, i));
       } else {
         base[i] = (int64_t)s.k_first + group_of(key0, i);
       }
     }
-    // Of key n of sixteen, the last one for those behind it.
-    auto row_in = [&](int i, int n) { return min(n, last - group_of(key0, i)); };
-    const uint8_t *k = (const uint8_t *)a.k, *v = (const uint8_t *)a.v;
+    // Where chunk c of key n of sixteen lies (of the last key's, behind it), from a row on.
+    auto at = [&](const void *from, int64_t ld, int64_t head_ld, int i, int n, int c) {
+      const int row = min(n, last - group_of(key0, i));
+      const uint8_t *p = (const uint8_t *)from;
+      if (PAGED) return p + base[i] * a.width * kSize + (__umul24(row, a.width * kSize) + c * 16);
+      return p + ((base[i] + row) * ld + head * head_ld) * 2 + c * 16;
+    };
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int64_t at = base[i] + row_in(i, col);
-      const uint8_t *from = PAGED ? k + at * a.width * kSize : k + (at * a.k_ld + head * a.k_head_ld) * 2;
-      if (Q8) ke[i] = a.k_exps[at];
 #pragma unroll
-      for (int c = 0; c < kLoads / 2; ++c) {
-        const int chunk = 4 * c + grp;
-        kr[i][c] = *reinterpret_cast<const v4i *>(chunk < width_chunks ? from + chunk * 16
-                                                                       : (const uint8_t *)kZeros);
-      }
+      for (int c = 0; c < kLoads / 2; ++c)
+        kr[i][c] = *global((const v4i *)at(a.k, a.k_ld, a.k_head_ld, i, col,
+                                           min(4 * c + grp, width_chunks - 1)));
+      if (Q8) ke[i] = *global((const uint8_t *)a.k_exps + base[i] + min(col, last - group_of(key0, i)));
     }
 #pragma unroll
     for (int c = 0; c < kLoads; ++c) {
-      const int n = c * kRowsOf + lane / kChunks, i = c * kRowsOf / 16, chunk = lane % kChunks;
-      const int64_t at = base[i] + row_in(i, n & 15);
-      const uint8_t *from = PAGED ? v + at * a.width * kSize : v + (at * a.v_ld + head * a.v_head_ld) * 2;
-      if (Q8) ve[c] = a.v_exps[at];
-      vr[c] = *reinterpret_cast<const v4i *>(chunk < width_chunks ? from + chunk * 16
-                                                                  : (const uint8_t *)kZeros);
+      const int n = c * kRowsOf + lane / kChunks, i = c * kRowsOf / 16;
+      vr[c] = *global((const v4i *)at(a.v, a.v_ld, a.v_head_ld, i, n & 15,
+                                      min(lane % kChunks, width_chunks - 1)));
+      if (Q8) ve[c] = *global((const uint8_t *)a.v_exps + base[i] + min(n & 15, last - group_of(key0, i)));
     }
   };
   // The values that came into LDS.
@@ -574,6 +581,11 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attention_few(LmAttn
 #pragma unroll 1
     for (; key0 < end; key0 += 4 * kStep) {
       v4f x[2] = {};
+      if (a.width < DP) {  // nothing behind a head's width
+#pragma unroll
+        for (int c = 0; c < kLoads / 2; ++c)
+          if (4 * c + grp >= width_chunks) kr[0][c] = kr[1][c] = v4i{};
+      }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const float fk = Q8 ? factor_of(ke[i]) : 0.f;
@@ -609,9 +621,11 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attention_few(LmAttn
       }
       const unsigned below = key0 + 4 * grp - seen.from, span = seen.to - seen.from;
       auto sees = [&](int i) { return below + (i / 4 * 16 + i % 4) < span; };
+      if (key0 < fin.from || key0 + kStep > top.to) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (!sees(i)) x[i / 4][i % 4] = -__builtin_inff();
+        for (int i = 0; i < 8; ++i)
+          if (!sees(i)) x[i / 4][i % 4] = -__builtin_inff();
+      }
       float most = x[0][0];
 #pragma unroll
       for (int i = 1; i < 8; ++i) most = fmaxf(most, x[i / 4][i % 4]);
@@ -838,7 +852,7 @@ static int attend(const LmAttnArgs &a, void *workspace, size_t bytes, hipStream_
     split.tile_rows = shape.tile_rows;
     split.slot_floats = slot_floats_of(shape, a.width);
     const int64_t most_keys = PAGED ? (int64_t)a.map.max_pages << a.map.shift : a.k_rows;
-    if (most_keys <= 1024) shape.split = false;
+    if (!worth_sharing(shape, a.rows, a.batch, a.kv_heads, a.group, most_keys)) shape.split = false;
   }
   if (a.width <= 64) attend_launch<T, PAGED, Q8, 64>(a, split, shape, s);
   else if (a.width <= 128) attend_launch<T, PAGED, Q8, 128>(a, split, shape, s);
