@@ -8,6 +8,8 @@
 // float32 angle of a far position has lost the turn it lies in; what is left
 // of a turn is a float32 to half a step. All heads of a token share its angles:
 // a workgroup computes those of its tokens once and keeps them in LDS.
+#include <type_traits>
+
 #include "hv_lm.h"
 
 namespace hv {
@@ -21,10 +23,27 @@ struct RotaryArgs {
   int64_t ld[2], head_ld[2], out_ld[2], out_head_ld[2];
   int rows, heads[2], width, pairs, interleaved;
   int tokens;  // of a workgroup
-  float eps, scale, low;  // low: under it a sum of squares has lost bits
+  float eps, scale, inv_width, low;  // low: under it a sum of squares has lost bits
 };
 
 static constexpr int kMaxPairs = HV_ROTARY_MAX_WIDTH / 2;
+
+// Sum over LANES lanes side by side, which all of them get.
+template <int LANES>
+__device__ __forceinline__ float sum_of(float v) {
+  auto moved = [](float x, auto ctrl) {
+    const int b = __builtin_bit_cast(int, x);
+    return __builtin_bit_cast(
+        float, __builtin_amdgcn_update_dpp(b, b, decltype(ctrl)::value, 0xf, 0xf, false));
+  };
+  v += moved(v, std::integral_constant<int, 0xB1>());                  // lane ^ 1
+  v += moved(v, std::integral_constant<int, 0x4E>());                  // lane ^ 2
+  if (LANES > 4) v += moved(v, std::integral_constant<int, 0x141>());  // 7 - lane, of eight
+  if (LANES > 8) v += moved(v, std::integral_constant<int, 0x140>());  // 15 - lane, of sixteen
+  if (LANES > 16) v += __shfl_xor(v, 16);
+  if (LANES > 32) v += __shfl_xor(v, 32);
+  return v;
+}
 
 // LANES lanes a head; each takes 16 of its elements as two runs of eight: the
 // two halves of eight pairs (or eight interleaved pairs), or what follows the
@@ -38,15 +57,16 @@ __global__ __launch_bounds__(256) void k_rotary_qk(RotaryArgs a) {
   const int64_t row0 = (int64_t)blockIdx.x * a.tokens;
   if (row0 >= rows) return;
   const int tokens = (int)min((int64_t)a.tokens, rows - row0);
-  for (int i = threadIdx.x; i < tokens * a.pairs; i += 256) {
-    const int t = i / a.pairs, p = i - t * a.pairs;
-    const double turns =
-        (double)a.positions[row0 + t] * (double)a.freqs[p] * 0.15915494309189533577;
-    float sin_, cos_;
-    sincospif((float)(2. * (turns - rint(turns))), &sin_, &cos_);
-    turn[i] = make_float2(cos_ * a.scale, sin_ * a.scale);
-  }
-  __syncthreads();
+  auto turns = [&]() {
+    for (int i = threadIdx.x; i < tokens * a.pairs; i += 256) {
+      const int t = i / a.pairs, p = i - t * a.pairs;
+      const double turns =
+          (double)a.positions[row0 + t] * (double)a.freqs[p] * 0.15915494309189533577;
+      float sin_, cos_;
+      sincospif((float)(2. * (turns - rint(turns))), &sin_, &cos_);
+      turn[i] = make_float2(cos_ * a.scale, sin_ * a.scale);
+    }
+  };
 
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
   const int heads = a.heads[0] + a.heads[1], rotated = 2 * a.pairs;
@@ -65,30 +85,56 @@ __global__ __launch_bounds__(256) void k_rotary_qk(RotaryArgs a) {
     n[1] = max(0, min(8, left - 8));
   }
   const int items = tokens * heads;
+  // Where item i's head lies, and what is loaded of it: the next one's is on its way while
+  // one is worked on.
+  v8 next[2];
+  auto load = [&](int t, int h) {
+    const int which = h >= a.heads[0], head = which ? h - a.heads[0] : h;
+    const T *x = (const T *)a.x[which] + (row0 + t) * a.ld[which] + head * a.head_ld[which];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) next[r] = n[r] > 0 ? Eight<T>::load(x + at[r], n[r]) : v8{};
+  };
+  const int step_t = kGroups / heads, step_h = kGroups - step_t * heads;
+  int t = min(group, items - 1) / heads, h = min(group, items - 1) - t * heads;
+  load(t, h);
+  v8 weight[2][2] = {};  // of queries and of keys
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+      if (a.weight[k] && n[r] > 0) weight[k][r] = Eight<T>::load((const T *)a.weight[k] + at[r], n[r]);
+  turns();
+  __syncthreads();
   // Every lane of a wavefront takes part in its reductions: a group past the
   // last item repeats it and writes nothing.
   for (int i0 = 0; i0 < items; i0 += kGroups) {
     const bool live = i0 + group < items;
-    const int item = live ? i0 + group : items - 1;
-    const int t = item / heads, h = item - t * heads;
-    const int which = h >= a.heads[0], head = which ? h - a.heads[0] : h;
-    const T *x = (const T *)a.x[which] + (row0 + t) * a.ld[which] + head * a.head_ld[which];
+    const int token = t, which = h >= a.heads[0], head = which ? h - a.heads[0] : h;
     float v[2][8];
     float sum = 0.f;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const v8 e = n[r] > 0 ? Eight<T>::load(x + at[r], n[r]) : v8{};
+    for (int r = 0; r < 2; ++r)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        v[r][i] = (float)e[i];
+        v[r][i] = (float)next[r][i];
         sum = __builtin_fmaf(v[r][i], v[r][i], sum);
       }
+    if (i0 + kGroups < items) {
+      t += step_t;
+      h += step_h;
+      if (h >= heads) {
+        h -= heads;
+        ++t;
+      }
+      if (t >= tokens) {
+        t = tokens - 1;
+        h = heads - 1;
+      }
+      load(t, h);
     }
-    const T *w = (const T *)a.weight[which];
-    if (w) {
-#pragma unroll
-      for (int o = 1; o < LANES; o *= 2) sum += __shfl_xor(sum, o);
-      float f = 1.f / sqrtf(sum / (float)a.width + a.eps);
+    if (a.weight[which]) {
+      sum = sum_of<LANES>(sum);
+      float f = __builtin_amdgcn_rsqf(sum * a.inv_width + a.eps);
       // Squares outside float32's normal numbers are summed again in 64 bits.
       const bool again = sum < a.low || !(sum < 0x1p120f);
       if (__builtin_amdgcn_ballot_w64(again)) {
@@ -111,13 +157,13 @@ __global__ __launch_bounds__(256) void k_rotary_qk(RotaryArgs a) {
       }
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const v8 g = n[r] > 0 ? Eight<T>::load(w + at[r], n[r]) : v8{};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[r][i] = v[r][i] * f * (float)g[i];
+        for (int i = 0; i < 8; ++i)
+          v[r][i] = v[r][i] * f * (float)(which ? weight[1][r][i] : weight[0][r][i]);
       }
     }
     if (pair) {
-      const float2 *cs = turn + t * a.pairs + 8 * lane;
+      const float2 *cs = turn + token * a.pairs + 8 * lane;
       const int count = min(8, a.pairs - 8 * lane);
       if (!a.interleaved) {
 #pragma unroll
@@ -139,7 +185,7 @@ __global__ __launch_bounds__(256) void k_rotary_qk(RotaryArgs a) {
       }
     }
     if (live) {
-      T *out = (T *)a.out[which] + (row0 + t) * a.out_ld[which] + head * a.out_head_ld[which];
+      T *out = (T *)a.out[which] + (row0 + token) * a.out_ld[which] + head * a.out_head_ld[which];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         v8 e;
@@ -210,7 +256,7 @@ extern "C" int hv_rotary_qk(const hv_rotary_desc *d, hv_stream_t stream) {
   a.out_head_ld[0] = d->q_out_head_ld; a.out_head_ld[1] = d->k_out_head_ld;
   a.rows = d->rows; a.heads[0] = d->q_heads; a.heads[1] = d->k_heads; a.width = d->width;
   a.pairs = d->rotated / 2; a.interleaved = d->layout == HV_ROTARY_INTERLEAVED;
-  a.eps = d->eps; a.scale = d->scale;
+  a.eps = d->eps; a.scale = d->scale; a.inv_width = 1.f / (float)d->width;
   a.low = d->eps < 0x1p-100f ? (0x1p-100f - d->eps) * (float)d->width : 0.f;
   const hipStream_t s = (hipStream_t)stream;
   if (d->type == HV_T_F32) rotary_launch<float>(a, s);
