@@ -22,26 +22,27 @@ struct RotaryArgs {
   const int32_t *rows_dev;
   int64_t ld[2], head_ld[2], out_ld[2], out_head_ld[2];
   int rows, heads[2], width, pairs, interleaved;
-  int tokens;  // of a workgroup
+  int tokens[2];  // of a workgroup, of queries or of keys
+  int least_exp;
   float eps, scale, inv_width, low;  // low: under it a sum of squares has lost bits
 };
 
 static constexpr int kMaxPairs = HV_ROTARY_MAX_WIDTH / 2;
 
-// Sum over LANES lanes side by side, which all of them get.
-template <int LANES>
-__device__ __forceinline__ float sum_of(float v) {
+// Sum, or largest, of LANES lanes side by side, which all of them get.
+template <int LANES, typename Op>
+__device__ __forceinline__ float all_of(float v, Op op) {
   auto moved = [](float x, auto ctrl) {
     const int b = __builtin_bit_cast(int, x);
     return __builtin_bit_cast(
         float, __builtin_amdgcn_update_dpp(b, b, decltype(ctrl)::value, 0xf, 0xf, false));
   };
-  v += moved(v, std::integral_constant<int, 0xB1>());                  // lane ^ 1
-  v += moved(v, std::integral_constant<int, 0x4E>());                  // lane ^ 2
-  if (LANES > 4) v += moved(v, std::integral_constant<int, 0x141>());  // 7 - lane, of eight
-  if (LANES > 8) v += moved(v, std::integral_constant<int, 0x140>());  // 15 - lane, of sixteen
-  if (LANES > 16) v += __shfl_xor(v, 16);
-  if (LANES > 32) v += __shfl_xor(v, 32);
+  v = op(v, moved(v, std::integral_constant<int, 0xB1>()));                  // lane ^ 1
+  v = op(v, moved(v, std::integral_constant<int, 0x4E>()));                  // lane ^ 2
+  if (LANES > 4) v = op(v, moved(v, std::integral_constant<int, 0x141>()));  // 7 - lane, of eight
+  if (LANES > 8) v = op(v, moved(v, std::integral_constant<int, 0x140>()));  // 15 - lane, of 16
+  if (LANES > 16) v = op(v, __shfl_xor(v, 16));
+  if (LANES > 32) v = op(v, __shfl_xor(v, 32));
   return v;
 }
 
@@ -49,14 +50,18 @@ __device__ __forceinline__ float sum_of(float v) {
 // two halves of eight pairs (or eight interleaved pairs), or what follows the
 // rotated part.
 template <typename T, int LANES>
-__global__ __launch_bounds__(256) void k_rotary_qk(RotaryArgs a) {
+__global__ __launch_bounds__(256, 5) void k_rotary_qk(RotaryArgs a) {
   constexpr int kGroups = 256 / LANES;
   typedef typename Eight<T>::v8 v8;
   extern __shared__ float2 turn[];  // [tokens][pairs]
   const int rows = a.rows_dev ? min(a.rows, *a.rows_dev) : a.rows;
-  const int64_t row0 = (int64_t)blockIdx.x * a.tokens;
+  const int which = blockIdx.y, heads = a.heads[which];
+  const int64_t row0 = (int64_t)blockIdx.x * a.tokens[which];
   if (row0 >= rows) return;
-  const int tokens = (int)min((int64_t)a.tokens, rows - row0);
+  const int tokens = (int)min((int64_t)a.tokens[which], rows - row0);
+  const T *const x0 = (const T *)a.x[which] + row0 * a.ld[which];
+  T *const out0 = (T *)a.out[which] + row0 * a.out_ld[which];
+  const T *const w = (const T *)a.weight[which];
   auto turns = [&]() {
     for (int i = threadIdx.x; i < tokens * a.pairs; i += 256) {
       const int t = i / a.pairs, p = i - t * a.pairs;
@@ -69,7 +74,7 @@ __global__ __launch_bounds__(256) void k_rotary_qk(RotaryArgs a) {
   };
 
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
-  const int heads = a.heads[0] + a.heads[1], rotated = 2 * a.pairs;
+  const int rotated = 2 * a.pairs;
   const int pair_lanes = (a.pairs + 7) / 8;
   const bool pair = lane < pair_lanes;
   int at[2], n[2];  // the lane's two runs
@@ -89,27 +94,24 @@ __global__ __launch_bounds__(256) void k_rotary_qk(RotaryArgs a) {
   // one is worked on.
   v8 next[2];
   auto load = [&](int t, int h) {
-    const int which = h >= a.heads[0], head = which ? h - a.heads[0] : h;
-    const T *x = (const T *)a.x[which] + (row0 + t) * a.ld[which] + head * a.head_ld[which];
+    const T *x = x0 + t * a.ld[which] + h * a.head_ld[which];
 #pragma unroll
     for (int r = 0; r < 2; ++r) next[r] = n[r] > 0 ? Eight<T>::load(x + at[r], n[r]) : v8{};
   };
   const int step_t = kGroups / heads, step_h = kGroups - step_t * heads;
   int t = min(group, items - 1) / heads, h = min(group, items - 1) - t * heads;
   load(t, h);
-  v8 weight[2][2] = {};  // of queries and of keys
+  v8 weight[2] = {};
 #pragma unroll
-  for (int k = 0; k < 2; ++k)
-#pragma unroll
-    for (int r = 0; r < 2; ++r)
-      if (a.weight[k] && n[r] > 0) weight[k][r] = Eight<T>::load((const T *)a.weight[k] + at[r], n[r]);
+  for (int r = 0; r < 2; ++r)
+    if (w && n[r] > 0) weight[r] = Eight<T>::load(w + at[r], n[r]);
   turns();
   __syncthreads();
   // Every lane of a wavefront takes part in its reductions: a group past the
   // last item repeats it and writes nothing.
   for (int i0 = 0; i0 < items; i0 += kGroups) {
     const bool live = i0 + group < items;
-    const int token = t, which = h >= a.heads[0], head = which ? h - a.heads[0] : h;
+    const int token = t, head = h;
     float v[2][8];
     float sum = 0.f;
 #pragma unroll
@@ -132,34 +134,34 @@ __global__ __launch_bounds__(256) void k_rotary_qk(RotaryArgs a) {
       }
       load(t, h);
     }
-    if (a.weight[which]) {
-      sum = sum_of<LANES>(sum);
+    if (w) {
+      auto add = [](float p, float q) { return p + q; };
+      sum = all_of<LANES>(sum, add);
       float f = __builtin_amdgcn_rsqf(sum * a.inv_width + a.eps);
-      // Squares outside float32's normal numbers are summed again in 64 bits.
+      // Squares outside float32's normal numbers are summed again, of the values times a
+      // power of two, which the root of the scaled sum takes out.
       const bool again = sum < a.low || !(sum < 0x1p120f);
       if (__builtin_amdgcn_ballot_w64(again)) {
-        double s = 0.;
+        float most = 0.f;
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
+        for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(v[i / 8][i % 8]));
+        most = all_of<LANES>(most, [](float p, float q) { return fmaxf(p, q); });
+        // (eps by that power squared stays a number)
+        const int e = again ? max(__builtin_amdgcn_frexp_expf(most), a.least_exp) : 0;
+        float s = 0.f;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) s += (double)v[r][i] * (double)v[r][i];
-#pragma unroll
-        for (int o = 1; o < LANES; o *= 2) s += __shfl_xor(s, o);
-        const double d = 1. / sqrt(s / a.width + (double)a.eps);
-        if (again) {
-          // x f in 64 bits: f may lie outside float32's numbers where x f does not
-#pragma unroll
-          for (int r = 0; r < 2; ++r)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[r][i] = (float)((double)v[r][i] * d);
-          f = 1.f;
+        for (int i = 0; i < 16; ++i) {
+          float &x = v[i / 8][i % 8];
+          x = ldexpf(x, -e);
+          s = __builtin_fmaf(x, x, s);
         }
+        s = all_of<LANES>(s, add);
+        if (again) f = __builtin_amdgcn_rsqf(s * a.inv_width + ldexpf(a.eps, -2 * e));
       }
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          v[r][i] = v[r][i] * f * (float)(which ? weight[1][r][i] : weight[0][r][i]);
+        for (int i = 0; i < 8; ++i) v[r][i] = v[r][i] * f * (float)weight[r][i];
       }
     }
     if (pair) {
@@ -185,7 +187,7 @@ __global__ __launch_bounds__(256) void k_rotary_qk(RotaryArgs a) {
       }
     }
     if (live) {
-      T *out = (T *)a.out[which] + (row0 + token) * a.out_ld[which] + head * a.out_head_ld[which];
+      T *out = out0 + token * a.out_ld[which] + head * a.out_head_ld[which];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         v8 e;
@@ -201,11 +203,15 @@ template <typename T>
 static void rotary_launch(RotaryArgs a, hipStream_t s) {
   const int lanes = (a.pairs + 7) / 8 + (a.width - 2 * a.pairs + 15) / 16;
   // Tokens a workgroup: its threads compute an angle each, while there are
-  // workgroups enough.
-  a.tokens = a.pairs ? max(1, min(16, 256 / a.pairs)) : 16;
-  while (a.tokens > 1 && (a.rows + a.tokens - 1) / a.tokens < 1024) a.tokens /= 2;
-  const dim3 grid((unsigned)((a.rows + a.tokens - 1) / a.tokens)), block(256);
-  const uint32_t lds = (uint32_t)(a.tokens * a.pairs * sizeof(float2));
+  // workgroups enough; keys, whose heads are fewer, take more of them.
+  const int keys = a.heads[1] ? 1 : 0;
+  int most = a.pairs ? max(1, min(16, 256 / a.pairs)) : 16;
+  while (most > 1 && (a.rows + most - 1) / most < 1024) most /= 2;
+  a.tokens[0] = a.tokens[1] = most;
+  if (keys)
+    a.tokens[1] = max(most, min(most * a.heads[0] / a.heads[1], min(16, 1024 / max(1, a.pairs))));
+  const dim3 grid((unsigned)((a.rows + most - 1) / most), 1 + keys), block(256);
+  const uint32_t lds = (uint32_t)(max(a.tokens[0], a.tokens[1]) * a.pairs * sizeof(float2));
   if (lanes <= 4) hv_launch(k_rotary_qk<T, 4>, grid, block, lds, s, a);
   else if (lanes <= 8) hv_launch(k_rotary_qk<T, 8>, grid, block, lds, s, a);
   else if (lanes <= 16) hv_launch(k_rotary_qk<T, 16>, grid, block, lds, s, a);
@@ -257,6 +263,9 @@ extern "C" int hv_rotary_qk(const hv_rotary_desc *d, hv_stream_t stream) {
   a.rows = d->rows; a.heads[0] = d->q_heads; a.heads[1] = d->k_heads; a.width = d->width;
   a.pairs = d->rotated / 2; a.interleaved = d->layout == HV_ROTARY_INTERLEAVED;
   a.eps = d->eps; a.scale = d->scale; a.inv_width = 1.f / (float)d->width;
+  int e = 0;
+  frexpf(d->eps, &e);  // eps <= 2^e
+  a.least_exp = d->eps > 0.f ? (e - 100) / 2 : -200;
   a.low = d->eps < 0x1p-100f ? (0x1p-100f - d->eps) * (float)d->width : 0.f;
   const hipStream_t s = (hipStream_t)stream;
   if (d->type == HV_T_F32) rotary_launch<float>(a, s);
