@@ -68,6 +68,9 @@ int hv_attention(const hv_attention_desc *d, void *workspace, size_t workspace_b
   for (int64_t l : ld)
     if (l < 0 || l % 8)
       return fail(HV_EVALUE, HV_ERR_DIMENSION, "attention: a stride is no multiple of 8");
+  if (d->k_ld > HV_ATTENTION_MAX_STRIDE || d->v_ld > HV_ATTENTION_MAX_STRIDE)
+    return fail(HV_EVALUE, HV_ERR_DIMENSION, "attention: rows of keys or values %lld and %lld apart",
+                (long long)d->k_ld, (long long)d->v_ld);
   if (d->rows.rows == 0 || d->rows.batch == 0) return HV_OK;
   if (d->k_rows && (!d->k || !d->v))
     return fail(HV_EVALUE, HV_ERR_ADDRESS, "attention: null argument");

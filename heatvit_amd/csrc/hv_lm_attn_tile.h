@@ -121,70 +121,86 @@ __device__ __forceinline__ const __attribute__((address_space(1))) P *global(con
   return (const __attribute__((address_space(1))) P *)p;
 }
 
-// What is loaded behind a head's width.
-static __device__ const v4i kZeros[1] = {};
-
 // Keys and values of a workgroup's tile, loaded by NW wavefronts.
 template <typename T, int DP, bool PAGED, bool Q8, int NW>
 struct TileLoader {
-  // A unit is what a wavefront loads at once: 1 KiB of the source.
+  // A unit is what a wavefront loads at once: 1 KiB of the source, up to sixteen rows from a
+  // multiple of as many on, which lie in one page.
   static constexpr int kChunks = Q8 ? DP / 16 : DP / 8;  // 16-byte chunks of a row's source
   static constexpr int kRowsOf = 64 / kChunks, kUnits = kKeys / kRowsOf / NW;
-  static_assert(kUnits * NW * kRowsOf == kKeys, "whole units");
+  static constexpr int kBytes = Q8 ? 1 : 2;
+  static_assert(kUnits * NW * kRowsOf == kKeys && kRowsOf <= 16, "whole units");
   const LmAttnArgs &a;
   const Sequence &s;
   int head, lane, wave, last;  // last: the last key that is there
   int page[kUnits];
-  int chunk[kUnits];
+  unsigned k_off[kUnits], v_off[kUnits];
   bool bad;
   v4i held[Q8 ? 2 * kUnits : 1];
   int exps[Q8 ? 2 * kUnits : 1];
 
+  __device__ __forceinline__ TileLoader(const LmAttnArgs &args, const Sequence &seq, int h, int last_key,
+                                        int tid)
+      : a(args), s(seq), head(h), lane(tid & 63), wave(uniform(tid >> 6)), last(last_key), bad(false) {
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      k_off[u] = offset(u, lane / kChunks, false);
+      v_off[u] = offset(u, lane / kChunks, true);
+    }
+  }
   __device__ __forceinline__ int row_of(int u) const {
     return (u * NW + wave) * kRowsOf + lane / kChunks;
   }
-  __device__ __forceinline__ TileLoader(const LmAttnArgs &args, const Sequence &seq, int h, int last_key,
-                                        int tid)
-      : a(args), s(seq), head(h), lane(tid & 63), wave(__builtin_amdgcn_readfirstlane(tid >> 6)),
-        last(last_key), bad(false) {}
+  // The first key of a unit of tile t: of the last one that there is, for those behind it.
+  __device__ __forceinline__ int first_of(int t, int u) const {
+    return min(t * kKeys + (u * NW + wave) * kRowsOf, last & ~(kRowsOf - 1));
+  }
   // The pages of tile t's keys, which the loads of it need.
   __device__ __forceinline__ void find(int t) {
     if (!PAGED) return;
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u)
-      page[u] = global(s.table)[min(t * kKeys + row_of(u), last) >> a.map.shift];
+    for (int u = 0; u < kUnits; ++u) page[u] = global(s.table)[first_of(t, u) >> a.map.shift];
   }
-  // Tile t on its way into k and v (Q8: into registers).
+  // Where a lane's chunk lies in a unit, in bytes from the unit's first row on: row n's.
+  __device__ __forceinline__ unsigned offset(int u, int n, bool value) const {
+    const int c = lane % kChunks;
+    const int chunk = Q8 ? min(c, a.width / 16 - 1)
+                         : value ? v_place<DP>(row_of(u), c) : k_place<DP>(row_of(u), c);
+    const unsigned stride = PAGED ? a.width * kBytes : (unsigned)(value ? a.v_ld : a.k_ld) * 2u;
+    return (unsigned)n * stride + chunk * 16u;
+  }
+  // Tile t on its way into k and v (Q8: into registers). A unit's place is a scalar, a lane's
+  // in it the same for all tiles but the one that the last key cuts.
   __device__ __forceinline__ void load(int t, T *k, T *v) {
-    const int chunks = Q8 ? a.width / 16 : a.width / 8, c = lane % kChunks;
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
-      const int row = row_of(u), key = min(t * kKeys + row, last);
-      int64_t at_k, at_v;
-      if (PAGED) {
-        const bool none = (unsigned)page[u] >= (unsigned)a.map.pages;
-        bad |= none;
-        at_k = cache_row(a.map, a.kv_heads, none ? 0 : page[u], head, key);
-        if (Q8) {
-          exps[2 * u] = (uint8_t)a.k_exps[at_k];
-          exps[2 * u + 1] = (uint8_t)a.v_exps[at_k];
-        }
-        at_k = at_v = at_k * a.width;
-      } else {
-        const int64_t r = (int64_t)s.k_first + key;
-        at_k = r * a.k_ld + head * a.k_head_ld;
-        at_v = r * a.v_ld + head * a.v_head_ld;
+      const int first = first_of(t, u), r = lane / kChunks;
+      int n = r;
+      unsigned ko = k_off[u], vo = v_off[u];
+      if (last - first < kRowsOf - 1) {
+        n = min(r, last - first);
+        ko = offset(u, n, false);
+        vo = offset(u, n, true);
       }
+      int64_t row = (int64_t)s.k_first + first;
+      if (PAGED) {
+        const int p = uniform(page[u]);
+        const bool none = (unsigned)p >= (unsigned)a.map.pages;
+        bad |= none;
+        row = cache_row(a.map, a.kv_heads, none ? 0 : p, head, first);
+      }
+      const int64_t k_at = PAGED ? row * a.width * kBytes : (row * a.k_ld + head * a.k_head_ld) * 2;
+      const int64_t v_at = PAGED ? k_at : (row * a.v_ld + head * a.v_head_ld) * 2;
+      const uint8_t *ks = (const uint8_t *)a.k + k_at, *vs = (const uint8_t *)a.v + v_at;
       if (Q8) {
-        const int64_t off = at_k + min(c, chunks - 1) * 16;
-        held[2 * u] = *global((const v4i *)((const uint8_t *)a.k + off));
-        held[2 * u + 1] = *global((const v4i *)((const uint8_t *)a.v + off));
+        exps[2 * u] = *global((const uint8_t *)a.k_exps + row + (unsigned)n);
+        exps[2 * u + 1] = *global((const uint8_t *)a.v_exps + row + (unsigned)n);
+        held[2 * u] = *global((const v4i *)(ks + ko));
+        held[2 * u + 1] = *global((const v4i *)(vs + vo));
       } else {
-        const int kc = k_place<DP>(row, c), vc = v_place<DP>(row, c);
-        to_lds(kc < chunks ? (const T *)a.k + at_k + kc * 8 : (const T *)kZeros,
-               k + (u * NW + wave) * 512);
-        to_lds(vc < chunks ? (const T *)a.v + at_v + vc * 8 : (const T *)kZeros,
-               v + (u * NW + wave) * 512);
+        const int chunks = a.width / 8, c = lane % kChunks;
+        if (k_place<DP>(row_of(u), c) < chunks) to_lds(ks + ko, k + (u * NW + wave) * 512);
+        if (v_place<DP>(row_of(u), c) < chunks) to_lds(vs + vo, v + (u * NW + wave) * 512);
       }
     }
   }
@@ -228,7 +244,7 @@ struct TileLoader {
 //                 of a product is key 16 s + 8 (i / 4) + 4 h + i % 4, and V^T
 //                 is read from LDS by columns in that order
 template <typename T, int DP, bool PAGED, bool Q8, int NW, bool SPLIT>
-__global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void k_attention_tile(LmAttnArgs a,
+__global__ __launch_bounds__(64 * NW, DP == 64 ? 3 : DP == 128 ? 2 : 1) void k_attention_tile(LmAttnArgs a,
                                                                                 Split split) {
   typedef typename Mma<T>::frag frag;
   constexpr int kRows = 32 * NW, kD = DP / 32, kSteps = DP / 16, kThreads = 64 * NW;
@@ -267,6 +283,13 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void k_attention_tile(L
       const int d = 16 * i + 8 * half;
       q[i] = d < a.width ? *reinterpret_cast<const frag *>(from + d) : frag{};
     }
+  }
+  if (!Q8 && a.width < DP) {  // zeros behind a head's width, where no load writes
+    __syncthreads();
+    for (int i = tid; i < kKeys * DP / 8; i += kThreads)
+      reinterpret_cast<v4i *>(k0)[i] = reinterpret_cast<v4i *>(k1)[i] =
+          reinterpret_cast<v4i *>(v0)[i] = reinterpret_cast<v4i *>(v1)[i] = v4i{};
+    __syncthreads();
   }
   TileLoader<T, DP, PAGED, Q8, NW> loader(a, s, head, w.last, tid);
   v16f o[kD];
