@@ -79,14 +79,6 @@ __device__ __forceinline__ int v_place(int row, int c) {
   return c ^ (DP == 64 ? (row >> 1 & 1) * 4 : (row & 3) * 4);
 }
 
-// 16 bytes a lane from memory straight to LDS, the wavefront's lanes one after
-// another from `to` on (the same in all lanes).
-__device__ __forceinline__ void to_lds(const void *from, void *to) {
-  __builtin_amdgcn_global_load_lds(
-      (const __attribute__((address_space(1))) void *)from,
-      (__attribute__((address_space(3))) void *)to, 16, 0, 0);
-}
-
 // Element d of key j's value, as the products take it.
 template <typename T, bool PAGED, bool Q8>
 __device__ __forceinline__ float value_at(const LmAttnArgs &a, const Sequence &s, int head, int j, int d) {
@@ -129,79 +121,98 @@ struct TileLoader {
   static constexpr int kChunks = Q8 ? DP / 16 : DP / 8;  // 16-byte chunks of a row's source
   static constexpr int kRowsOf = 64 / kChunks, kUnits = kKeys / kRowsOf / NW;
   static constexpr int kBytes = Q8 ? 1 : 2;
+  static constexpr int kBehind = 0x7FFFFFF0;  // an offset that no buffer has: it reads zeros
   static_assert(kUnits * NW * kRowsOf == kKeys && kRowsOf <= 16, "whole units");
   const LmAttnArgs &a;
   const Sequence &s;
   int head, lane, wave, last;  // last: the last key that is there
-  int page[kUnits];
-  unsigned k_off[kUnits], v_off[kUnits];
+  int page[PAGED ? kUnits : 1];
+  int k_off[kUnits], v_off[kUnits];  // a lane's, from a unit's first row on
   bool bad;
   v4i held[Q8 ? 2 * kUnits : 1];
   int exps[Q8 ? 2 * kUnits : 1];
 
-  __device__ __forceinline__ TileLoader(const LmAttnArgs &args, const Sequence &seq, int h, int last_key,
-                                        int tid)
-      : a(args), s(seq), head(h), lane(tid & 63), wave(uniform(tid >> 6)), last(last_key), bad(false) {
-#pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-      k_off[u] = offset(u, lane / kChunks, false);
-      v_off[u] = offset(u, lane / kChunks, true);
-    }
-  }
   __device__ __forceinline__ int row_of(int u) const {
     return (u * NW + wave) * kRowsOf + lane / kChunks;
   }
-  // The first key of a unit of tile t: of the last one that there is, for those behind it.
-  __device__ __forceinline__ int first_of(int t, int u) const {
-    return min(t * kKeys + (u * NW + wave) * kRowsOf, last & ~(kRowsOf - 1));
+  __device__ __forceinline__ TileLoader(const LmAttnArgs &args, const Sequence &seq, int h, int last_key,
+                                        int tid)
+      : a(args), s(seq), head(h), lane(tid & 63), wave(uniform(tid >> 6)), last(last_key), bad(false) {
+    const int chunks = a.width * kBytes / 16, c = lane % kChunks, r = lane / kChunks;
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const int kc = Q8 ? c : k_place<DP>(row_of(u), c), vc = Q8 ? c : v_place<DP>(row_of(u), c);
+      k_off[u] = kc < chunks ? r * k_stride() + kc * 16 : kBehind;
+      v_off[u] = vc < chunks ? r * v_stride() + vc * 16 : kBehind;
+    }
   }
+  // Bytes from row to row.
+  __device__ __forceinline__ int k_stride() const { return PAGED ? a.width * kBytes : (int)a.k_ld * 2; }
+  __device__ __forceinline__ int v_stride() const { return PAGED ? a.width * kBytes : (int)a.v_ld * 2; }
+  // Whether a tile's keys lie side by side: in rows of a tensor, or in one page.
+  __device__ __forceinline__ bool together() const { return !PAGED || a.map.shift >= 6; }
   // The pages of tile t's keys, which the loads of it need.
   __device__ __forceinline__ void find(int t) {
     if (!PAGED) return;
+    if (together()) {
+      page[0] = global(s.table)[min(t * kKeys, last) >> a.map.shift];
+      return;
+    }
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u) page[u] = global(s.table)[first_of(t, u) >> a.map.shift];
+    for (int u = 0; u < kUnits; ++u)
+      page[u] = global(s.table)[min(t * kKeys + (u * NW + wave) * kRowsOf, last) >> a.map.shift];
   }
-  // Where a lane's chunk lies in a unit, in bytes from the unit's first row on: row n's.
-  __device__ __forceinline__ unsigned offset(int u, int n, bool value) const {
-    const int c = lane % kChunks;
-    const int chunk = Q8 ? min(c, a.width / 16 - 1)
-                         : value ? v_place<DP>(row_of(u), c) : k_place<DP>(row_of(u), c);
-    const unsigned stride = PAGED ? a.width * kBytes : (unsigned)(value ? a.v_ld : a.k_ld) * 2u;
-    return (unsigned)n * stride + chunk * 16u;
+  // Unit u of a tile, `row` of whose rows it is, from the row of key `first` on: rows behind the
+  // last key read as zeros.
+  __device__ __forceinline__ void load_unit(int u, int row, int64_t at, int first, T *k, T *v) {
+    const int left = last - first;  // rows behind the first
+    const int k_size = min(left, kKeys) * k_stride() + a.width * kBytes;
+    const int v_size = min(left, kKeys) * v_stride() + a.width * kBytes;
+    const uint8_t *ks = (const uint8_t *)a.k + (PAGED ? at * a.width * kBytes
+                                                      : (at * a.k_ld + head * a.k_head_ld) * 2);
+    const uint8_t *vs = (const uint8_t *)a.v + (PAGED ? at * a.width * kBytes
+                                                      : (at * a.v_ld + head * a.v_head_ld) * 2);
+    if (Q8) {
+      auto buffer = [](const void *p, int size) {
+        return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, size, 0x00020000);
+      };
+      const int r = lane / kChunks;
+      exps[2 * u] = __builtin_amdgcn_raw_buffer_load_b8(buffer(a.k_exps + at, left + 1), r, row, 0);
+      exps[2 * u + 1] = __builtin_amdgcn_raw_buffer_load_b8(buffer(a.v_exps + at, left + 1), r, row, 0);
+      held[2 * u] = __builtin_amdgcn_raw_buffer_load_b128(buffer(ks, k_size), k_off[u], row * k_stride(), 0);
+      held[2 * u + 1] =
+          __builtin_amdgcn_raw_buffer_load_b128(buffer(vs, v_size), v_off[u], row * v_stride(), 0);
+    } else {
+      auto to_lds = [](const void *p, int size, int lane_at, int unit_at, T *to) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, size, 0x00020000),
+            (__attribute__((address_space(3))) void *)to, 16, lane_at, unit_at, 0, 0);
+      };
+      to_lds(ks, k_size, k_off[u], row * k_stride(), k + (u * NW + wave) * 512);
+      to_lds(vs, v_size, v_off[u], row * v_stride(), v + (u * NW + wave) * 512);
+    }
   }
-  // Tile t on its way into k and v (Q8: into registers). A unit's place is a scalar, a lane's
-  // in it the same for all tiles but the one that the last key cuts.
+  // The row of a key, which starts a tile or a unit.
+  __device__ __forceinline__ int64_t place(int key, int page_of_it) {
+    if (!PAGED) return (int64_t)s.k_first + key;
+    const int p = uniform(page_of_it);
+    const bool none = (unsigned)p >= (unsigned)a.map.pages;
+    bad |= none;
+    return cache_row(a.map, a.kv_heads, none ? 0 : p, head, key);
+  }
+  // Tile t on its way into k and v (Q8: into registers).
   __device__ __forceinline__ void load(int t, T *k, T *v) {
+    if (together()) {
+      const int64_t at = place(t * kKeys, page[0]);
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) load_unit(u, (u * NW + wave) * kRowsOf, at, t * kKeys, k, v);
+      return;
+    }
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
-      const int first = first_of(t, u), r = lane / kChunks;
-      int n = r;
-      unsigned ko = k_off[u], vo = v_off[u];
-      if (last - first < kRowsOf - 1) {
-        n = min(r, last - first);
-        ko = offset(u, n, false);
-        vo = offset(u, n, true);
-      }
-      int64_t row = (int64_t)s.k_first + first;
-      if (PAGED) {
-        const int p = uniform(page[u]);
-        const bool none = (unsigned)p >= (unsigned)a.map.pages;
-        bad |= none;
-        row = cache_row(a.map, a.kv_heads, none ? 0 : p, head, first);
-      }
-      const int64_t k_at = PAGED ? row * a.width * kBytes : (row * a.k_ld + head * a.k_head_ld) * 2;
-      const int64_t v_at = PAGED ? k_at : (row * a.v_ld + head * a.v_head_ld) * 2;
-      const uint8_t *ks = (const uint8_t *)a.k + k_at, *vs = (const uint8_t *)a.v + v_at;
-      if (Q8) {
-        exps[2 * u] = *global((const uint8_t *)a.k_exps + row + (unsigned)n);
-        exps[2 * u + 1] = *global((const uint8_t *)a.v_exps + row + (unsigned)n);
-        held[2 * u] = *global((const v4i *)(ks + ko));
-        held[2 * u + 1] = *global((const v4i *)(vs + vo));
-      } else {
-        const int chunks = a.width / 8, c = lane % kChunks;
-        if (k_place<DP>(row_of(u), c) < chunks) to_lds(ks + ko, k + (u * NW + wave) * 512);
-        if (v_place<DP>(row_of(u), c) < chunks) to_lds(vs + vo, v + (u * NW + wave) * 512);
-      }
+      const int first = t * kKeys + (u * NW + wave) * kRowsOf;
+      // A unit behind the last key reads the last one's row again, all of whose scores are masked.
+      load_unit(u, 0, place(min(first, last), page[u]), min(first, last), k, v);
     }
   }
   // Q8: what `load` brought, into k and v.
@@ -220,9 +231,6 @@ struct TileLoader {
           x[2 * i] = Pair8<T>::of(w[i], f, false);
           x[2 * i + 1] = Pair8<T>::of(w[i], f, true);
         }
-        if (c * 8 >= a.width)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = typename Pair8<T>::type{};
         T *to = (which ? v : k) + row * DP;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -284,13 +292,6 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 3 : DP == 128 ? 2 : 1) void k_a
       q[i] = d < a.width ? *reinterpret_cast<const frag *>(from + d) : frag{};
     }
   }
-  if (!Q8 && a.width < DP) {  // zeros behind a head's width, where no load writes
-    __syncthreads();
-    for (int i = tid; i < kKeys * DP / 8; i += kThreads)
-      reinterpret_cast<v4i *>(k0)[i] = reinterpret_cast<v4i *>(k1)[i] =
-          reinterpret_cast<v4i *>(v0)[i] = reinterpret_cast<v4i *>(v1)[i] = v4i{};
-    __syncthreads();
-  }
   TileLoader<T, DP, PAGED, Q8, NW> loader(a, s, head, w.last, tid);
   v16f o[kD];
   float m, l;
@@ -316,14 +317,41 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 3 : DP == 128 ? 2 : 1) void k_a
     if (idle || t * kKeys >= end.to || (t + 1) * kKeys <= top.from) return;
     v16f x[2] = {};
     const T *kr = k + col * DP;
+    // Keys are read four fragments ahead of their products, and values eight: the compiler
+    // by itself reads one and waits for it.
+    frag kf[2][4];
+    auto read_keys = [&](int g) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      const int c = k_place<DP>(col, 2 * i + half) * 8;
-      const frag a0 = *reinterpret_cast<const frag *>(kr + c);
-      const frag a1 = *reinterpret_cast<const frag *>(kr + 32 * DP + c);
-      x[0] = Mma<T>::wide(a0, q[i], x[0]);
-      x[1] = Mma<T>::wide(a1, q[i], x[1]);
+      for (int i = 0; i < 2; ++i) {
+        const T *at = kr + k_place<DP>(col, 2 * (2 * g + i) + half) * 8;
+        kf[g & 1][2 * i] = *reinterpret_cast<const frag *>(at);
+        kf[g & 1][2 * i + 1] = *reinterpret_cast<const frag *>(at + 32 * DP);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    v4s vf[2][8];
+    const int vr = 4 * half + (lane >> 2 & 3);
+    auto read_values = [&](int d) __attribute__((always_inline)) {
+      const T *at = v + vr * DP + v_place<DP>(vr, 4 * d + (lane >> 4 & 1) * 2 + (lane >> 1 & 1)) * 8 +
+                    (lane & 1) * 4;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) vf[d & 1][i] = read_column(at + 8 * i * DP);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    read_keys(0);
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int g = 0; g < kSteps / 2; ++g) {
+      if (g + 1 < kSteps / 2) read_keys(g + 1);
+      else read_values(0);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        x[0] = Mma<T>::wide(kf[g & 1][2 * i], q[2 * g + i], x[0]);
+        x[1] = Mma<T>::wide(kf[g & 1][2 * i + 1], q[2 * g + i], x[1]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_s_setprio(0);
     // Whether the row sees the tile's key 4 half + i.
     const unsigned below = t * kKeys + 4 * half - seen.from, span = seen.to - seen.from;
     auto sees = [&](int i) { return below + i < span; };
@@ -354,18 +382,19 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 3 : DP == 128 ? 2 : 1) void k_a
       l += e;
       p[i / 8][i % 8] = (T)e;
     }
-    const int vr = 4 * half + (lane >> 2 & 3);
+    __builtin_amdgcn_s_setprio(1);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int d = 0; d < kD; ++d) {
-      const int c = v_place<DP>(vr, 4 * d + (lane >> 4 & 1) * 2 + (lane >> 1 & 1)) * 8 + (lane & 1) * 4;
-      const T *vc = v + vr * DP + c;
+      if (d + 1 < kD) read_values(d + 1);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const v4s lo = read_column(vc + 16 * i * DP), hi = read_column(vc + (16 * i + 8) * DP);
-        const v8s both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        const v8s both = __builtin_shufflevector(vf[d & 1][2 * i], vf[d & 1][2 * i + 1], 0, 1, 2, 3, 4, 5, 6, 7);
         o[d] = Mma<T>::wide(__builtin_bit_cast(frag, both), p[i], o[d]);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_s_setprio(0);
     if (!decltype(careful)::value) return;
     for (uint64_t left = odd_keys; left; left &= left - 1) {
       const int j = t * kKeys + __builtin_ctzll(left);

@@ -563,7 +563,7 @@ int hv_rotary_qk(const hv_rotary_desc *d, hv_stream_t stream);
 #define HV_CACHE_MAX_PAGE 4096
 #define HV_CACHE_MAX_KEYS (1 << 30) /* that a row of the table has room for */
 #define HV_ATTENTION_MAX_WIDTH 256
-#define HV_ATTENTION_MAX_STRIDE ((int64_t)1 << 26) /* of rows of packed keys and values */
+#define HV_ATTENTION_MAX_STRIDE (1 << 23) /* of rows of packed keys and values */
 
 typedef struct {
   void *k, *v;
