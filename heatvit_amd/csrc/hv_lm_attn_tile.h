@@ -331,15 +331,19 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 3 : DP == 128 ? 2 : 1) void k_a
     };
     v4s vf[2][8];
     const int vr = 4 * half + (lane >> 2 & 3);
-    auto read_values = [&](int d) __attribute__((always_inline)) {
-      const T *at = v + vr * DP + v_place<DP>(vr, 4 * d + (lane >> 4 & 1) * 2 + (lane >> 1 & 1)) * 8 +
-                    (lane & 1) * 4;
+    // Of two runs of 32 elements, half of the tile's keys: four fragments.
+    auto read_values = [&](int g) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) vf[d & 1][i] = read_column(at + 8 * i * DP);
+      for (int e = 0; e < 2; ++e) {
+        const int d = g / 2 * 2 + e;
+        const T *at = v + (vr + 32 * (g % 2)) * DP +
+                      v_place<DP>(vr, 4 * d + (lane >> 4 & 1) * 2 + (lane >> 1 & 1)) * 8 + (lane & 1) * 4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) vf[g & 1][4 * e + i] = read_column(at + 8 * i * DP);
+      }
       __builtin_amdgcn_sched_barrier(0);
     };
     read_keys(0);
-    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int g = 0; g < kSteps / 2; ++g) {
       if (g + 1 < kSteps / 2) read_keys(g + 1);
@@ -351,7 +355,6 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 3 : DP == 128 ? 2 : 1) void k_a
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-    __builtin_amdgcn_s_setprio(0);
     // Whether the row sees the tile's key 4 half + i.
     const unsigned below = t * kKeys + 4 * half - seen.from, span = seen.to - seen.from;
     auto sees = [&](int i) { return below + i < span; };
@@ -382,19 +385,18 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 3 : DP == 128 ? 2 : 1) void k_a
       l += e;
       p[i / 8][i % 8] = (T)e;
     }
-    __builtin_amdgcn_s_setprio(1);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int d = 0; d < kD; ++d) {
-      if (d + 1 < kD) read_values(d + 1);
+    for (int g = 0; g < kD; ++g) {
+      if (g + 1 < kD) read_values(g + 1);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const v8s both = __builtin_shufflevector(vf[d & 1][2 * i], vf[d & 1][2 * i + 1], 0, 1, 2, 3, 4, 5, 6, 7);
-        o[d] = Mma<T>::wide(__builtin_bit_cast(frag, both), p[i], o[d]);
+        const int d = g / 2 * 2 + i % 2, n = 4 * (i % 2) + i / 2 * 2;
+        const v8s both = __builtin_shufflevector(vf[g & 1][n], vf[g & 1][n + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+        o[d] = Mma<T>::wide(__builtin_bit_cast(frag, both), p[2 * (g % 2) + i / 2], o[d]);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-    __builtin_amdgcn_s_setprio(0);
     if (!decltype(careful)::value) return;
     for (uint64_t left = odd_keys; left; left &= left - 1) {
       const int j = t * kKeys + __builtin_ctzll(left);
