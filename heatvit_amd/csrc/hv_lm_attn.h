@@ -5,6 +5,7 @@
 #include <type_traits>
 
 #include "hv_lm.h"
+#include "hv_lm_attn_plan.h"
 #include "hv_lm_paged.h"
 
 namespace hv {
@@ -64,45 +65,6 @@ struct Pair8<f16> {
 // still has.) A byte is taken as it was loaded: to extend its sign there would wait for it.
 __device__ __forceinline__ float factor_of(int byte) {
   return __builtin_bit_cast(float, ((byte ^ 0x80) - 1) << 23);
-}
-
-// Tiles of `tile_rows` rows that a call's sequences have at most.
-inline int64_t most_tiles(int rows, int batch, int group, int tile_rows) {
-  return (int64_t)rows * group / tile_rows + batch;
-}
-
-// Rows of a tile (of k_attention_few, or of k_attention_tile), and whether the tiles' work
-// is cut into `workgroups` shares.
-static constexpr int kFewRows = 16, kTileRows = 128;
-struct Shape {
-  int tile_rows, workgroups;
-  bool split;
-};
-inline Shape shape_of(int rows, int batch, int heads, int kv_heads, int width) {
-  const int group = heads / kv_heads;
-  const bool few = (int64_t)rows * group <= (int64_t)batch * kFewRows;
-  const int tile_rows = few ? kFewRows : kTileRows;
-  const int64_t items = most_tiles(rows, batch, group, tile_rows) * kv_heads;
-  return {tile_rows, width <= 128 ? 512 : 256, items < (few ? 4096 : 512)};
-}
-// Two partial results a workgroup: of a tile that an earlier one began, and of one that a
-// later one ends.
-// Shares cost a launch and the partial results' way through memory. Few rows: 8 sequences
-// of up to 1000 keys take 13.5 us whole, 13.7 in shares; one of 2048 16. Tiles: 14 + 15
-// us, where whole tiles take 2 us for each 64 keys and leave the card's 512 workgroups short
-// of (512 - items) of them (one prompt of 1536 tokens, 384 items: 64 us in shares).
-inline bool worth_sharing(const Shape &shape, int rows, int batch, int kv_heads, int group,
-                          int64_t most_keys) {
-  if (shape.tile_rows == kFewRows) return most_keys > 1024;
-  return most_keys * (512 - most_tiles(rows, batch, group, shape.tile_rows) * kv_heads) > 1 << 19;
-}
-
-inline int slot_floats_of(const Shape &shape, int width) {
-  // 64 more than it takes: slots a power of two apart meet in the same memory channels.
-  return shape.tile_rows * (width + 2) + 64;
-}
-inline size_t workspace_of(const Shape &shape, int width) {
-  return shape.split ? (size_t)shape.workgroups * (8 * slot_floats_of(shape, width) + 32) : 0;
 }
 
 // The kernels of either type. The workspace is looked at here.

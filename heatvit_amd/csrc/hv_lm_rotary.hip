@@ -207,6 +207,7 @@ static void rotary_launch(RotaryArgs a, hipStream_t s) {
   const int keys = a.heads[1] ? 1 : 0;
   int most = a.pairs ? max(1, min(16, 256 / a.pairs)) : 16;
   while (most > 1 && (a.rows + most - 1) / most < 1024) most /= 2;
+  while ((a.rows + most - 1) / most > 1 << 22) most *= 2;  // a launch has less than 2^32 threads
   a.tokens[0] = a.tokens[1] = most;
   if (keys)
     a.tokens[1] = max(most, min(most * a.heads[0] / a.heads[1], min(16, 1024 / max(1, a.pairs))));

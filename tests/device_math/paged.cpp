@@ -24,3 +24,16 @@ void seen_at(int i, int n, int keys, int causal, int window, int32_t *out) {
   out[1] = s.to;
 }
 }
+
+// Which kernels a call takes.
+#include "hv_lm_attn_plan.h"
+extern "C" {
+int attention_shape(int rows, int batch, int heads, int kv_heads, int width, long long most_keys) {
+  const Shape s = shape_of(rows, batch, heads, kv_heads, width);
+  const bool shares = s.split && worth_sharing(s, rows, batch, kv_heads, heads / kv_heads, most_keys);
+  return (s.tile_rows == kFewRows ? 0 : 2) + shares;
+}
+long long attention_workspace(int rows, int batch, int heads, int kv_heads, int width) {
+  return (long long)workspace_of(shape_of(rows, batch, heads, kv_heads, width), width);
+}
+}

@@ -9,6 +9,7 @@ import numpy as np
 import pytest
 import torch
 
+import lm_attention_kernels
 import lm_attention_reference as ref
 
 pytestmark = pytest.mark.gpu
@@ -639,6 +640,100 @@ def test_paged_far_pages(e4m3):
     for a, b in ((got[0], got[2]), (got[1], got[3])):
         assert a.out.isfinite().all()
         assert torch.equal(a.out, b.out) and torch.equal(a.lse, b.lse)
+
+
+# ------------------------------------------------------------------ shares of the work
+
+def _room(lengths, page):
+    return (max(-(-n // page) for n in lengths) + 1) * page
+
+
+@pytest.mark.parametrize("e4m3", (False, True))
+@pytest.mark.parametrize("kind", HALVES)
+def test_paged_tiles_in_shares(kind, e4m3):
+    """Tiles whose keys are cut into shares: one sequence, a few of very
+    different lengths (none and one key among them), windows, wide heads."""
+    for new, lengths, heads, kv, width, page, window, causal in (
+            ([40], [3000], 4, 1, 64, 64, 0, True), ([130, 20, 1, 0], [2500, 20, 1, 900], 4, 2, 128, 16, 0, True),
+            ([64], [2600], 2, 2, 96, 128, 0, False), ([150], [2500], 3, 1, 64, 16, 700, True),
+            ([33], [2200], 4, 4, 256, 64, 0, True), ([60, 60], [1900, 2100], 2, 1, 32, 32, 0, True)):
+        assert lm_attention_kernels.kernel_of(sum(new), len(new), heads, kv, width,
+                                              _room(lengths, page)) == "tiles in shares"
+        _run_paged(new, lengths, heads, kv, width, page, kind, e4m3, window, causal, seed=8)
+
+
+@pytest.mark.parametrize("kind", HALVES)
+def test_paged_few_rows_in_shares(kind):
+    """Few rows in shares beyond a workgroup's threads of sequences, in groups
+    that take two tiles, and whole where sequences are many."""
+    lengths = [(37 * b) % 50 for b in range(300)]
+    lengths[7], lengths[290] = 1200, 1100
+    for lengths, heads, kv, want in ((lengths, 2, 2, "few in shares"), ([900, 30, 1200], 16, 1, "few in shares"),
+                                     ([1 + b % 40 for b in range(1200)], 4, 4, "few"),
+                                     ([1500, 2], 12, 1, "few in shares")):
+        assert lm_attention_kernels.kernel_of(len(lengths), len(lengths), heads, kv, 64,
+                                              _room(lengths, 16)) == want
+        _run_paged([1] * len(lengths), lengths, heads, kv, 64, 16, kind, False, starts=False, seed=2)
+
+
+def test_attention_tiles_in_shares():
+    """Packed keys of their own, cut into shares."""
+    assert lm_attention_kernels.kernel_of(180, 2, 4, 2, 64, 3300) == "tiles in shares"
+    _run_attention([100, 80], 4, 2, 64, "bf16", True, 0, 5, [2500, 800])
+    _run_attention([100, 80], 4, 2, 128, "f16", False, 0, 5, [2500, 800])
+    assert lm_attention_kernels.kernel_of(6, 2, 4, 2, 64, 3300) == "few in shares"
+    _run_attention([4, 2], 4, 2, 64, "f16", True, 0, 5, [2500, 800])
+
+
+@pytest.mark.parametrize("new", ([2, 1], [90, 45]))
+def test_shares_leave_out_what_is_not_seen(new):
+    """NaN and infinities that a row does not see leave no trace where the keys
+    are cut into shares, and a bad page makes its own sequence NaN alone."""
+    from heatvit_amd import lm
+    lengths, kv = [2500, 800], 2
+    book = _filled(lengths, kv, 64, 64, torch.bfloat16, False, 3)
+    q = torch.randn(sum(new), 4, 64, generator=_gen(1)).to(torch.bfloat16).cuda()
+    assert lm_attention_kernels.kernel_of(sum(new), 2, 4, kv, 64, _room(lengths, 64)).endswith("shares")
+    at = _starts(new)
+    s, n, table = _i32(at).cuda(), _i32(lengths).cuda(), book.table.cuda()
+    for window in (0, 400):
+        clean = lm.paged_attention(q, book.cache, table, n, starts=s, window=window, lse=True)
+        for position, value in ((2499, math.nan), (2499, math.inf), (50, math.nan), (50, math.inf)):
+            for t in (book.cache.k, book.cache.v):
+                page, i = book.place(0, position)
+                old = t[page, :, i].clone()
+                t[page, :, i] = value
+                got = lm.paged_attention(q, book.cache, table, n, starts=s, window=window, lse=True)
+                t[page, :, i] = old
+                rows = torch.arange(sum(new))
+                row_at = 2500 - new[0] + rows  # places of the first sequence's rows
+                sees = (rows < new[0]) & (position <= row_at) & \
+                    ((position > row_at - window) if window else True)
+                same = (~sees).cuda()
+                assert torch.equal(got.out[same], clean.out[same]), (window, position, value)
+                assert torch.equal(got.lse[same], clean.lse[same]), (window, position, value)
+                if value != value and sees.any():
+                    assert got.out[sees.cuda()].isnan().any(-1).all()
+    bad = table.clone()
+    bad[0, 20] = book.cache.pages
+    clean = lm.paged_attention(q, book.cache, table, n, starts=s, lse=True)
+    got = lm.paged_attention(q, book.cache, bad, n, starts=s, lse=True)
+    assert got.out[:at[1]].isnan().all() and got.lse[:at[1]].isnan().all()
+    assert torch.equal(got.out[at[1]:], clean.out[at[1]:])
+
+
+def test_attention_bad_offsets_in_shares():
+    """Offsets that run backwards or leave the tensors where the work is cut
+    into shares: nothing outside the rows is written, and the call ends."""
+    from heatvit_amd import lm
+    q, k, v = (t.cuda() for t in _packed([300], 2, 1, 64, torch.bfloat16, 2, [3000]))
+    assert lm_attention_kernels.kernel_of(300, 5, 2, 1, 64, 3000) == "tiles in shares"
+    for starts, ks in (([0, 300, 0, 300, 0, 300], [0, 3000, 0, 3000, 0, 3000]),
+                       ([2 ** 31 - 1, -2 ** 31, 7, 7, 300, 2 ** 31 - 1], [-5, 9, 4000, 0, 3, 2 ** 31 - 1])):
+        out = lm.Attended(torch.full_like(q, 7.0), torch.full((300, 2), 7.0, device="cuda"))
+        lm.attention(q, k, v, _i32(starts).cuda(), k_starts=_i32(ks).cuda(), lse=True, out=out)
+        torch.cuda.synchronize()
+        assert out.out.isfinite().all()
 
 
 # ------------------------------------------------------------------ streams, graphs, workspaces

@@ -5,13 +5,13 @@ launch)."""
 
 import ctypes as C
 import math
-import subprocess
 from pathlib import Path
 
 import numpy as np
 import pytest
 import torch
 
+import lm_attention_kernels
 from heatvit_amd import _lib, lm
 
 ROOT = Path(__file__).resolve().parents[1]
@@ -23,18 +23,8 @@ F8 = torch.float8_e4m3fn
 # ------------------------------------------------------------------ places
 
 @pytest.fixture(scope="module")
-def places(tmp_path_factory):
-    so = tmp_path_factory.mktemp("paged") / "paged.so"
-    subprocess.run(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", "-o", str(so), "-I",
-                    str(ROOT / "heatvit_amd" / "csrc"),
-                    str(ROOT / "tests" / "device_math" / "paged.cpp")], check=True)
-    L = C.CDLL(str(so))
-    L.row_at.restype = C.c_longlong
-    L.page_at.argtypes = [C.c_int] * 3 + [C.c_void_p, C.c_longlong]
-    L.row_at.argtypes = [C.c_int] * 5 + [C.c_longlong]
-    L.seq_rows_of.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_void_p]
-    L.seen_at.argtypes = [C.c_int] * 5 + [C.c_void_p]
-    return L
+def places():
+    return lm_attention_kernels.library()
 
 
 def test_rows_stay_inside(places):
@@ -88,6 +78,26 @@ def test_what_a_row_sees(places):
                     assert list(range(*out)) == want
     places.seen_at(0, 2 ** 24, 2 ** 31 - 1, 1, 0, out.ctypes.data)
     assert out.tolist() == [0, 2 ** 31 - 1 - 2 ** 24 + 1]
+
+
+def test_kernels():
+    """Few rows a sequence, or tiles; shares where tiles leave the card idle and
+    the keys are many; a workspace where there may be shares, and only there."""
+    of = lm_attention_kernels.kernel_of
+    assert of(1, 1, 32, 8, 128, 32768) == "few in shares"
+    assert of(8, 8, 16, 16, 64, 1008) == "few"
+    assert of(4096, 4096, 8, 8, 64, 4096) == "few"
+    assert of(8192, 1, 32, 8, 128, 8192) == "tiles"
+    assert of(50432, 256, 3, 3, 64, 50432) == "tiles"
+    assert of(100, 1, 4, 1, 64, 100) == "tiles"
+    assert of(648, 4, 32, 8, 128, 16384) == "tiles in shares"
+    for rows, batch, heads, kv, width in ((1, 1, 1, 1, 8), (4096, 4096, 8, 8, 64), (648, 4, 32, 8, 128),
+                                          (8192, 1, 32, 8, 128), (300, 1, 4, 4, 256)):
+        size = lm_attention_kernels.library().attention_workspace(rows, batch, heads, kv, width)
+        if "shares" in of(rows, batch, heads, kv, width, 1 << 30):
+            assert 0 < size < 1 << 28
+        else:
+            assert size == 0
 
 
 # ------------------------------------------------------------------ frequencies
@@ -315,7 +325,7 @@ CACHE = dict(cache_k=PTR, cache_v=PTR, table=PTR, lengths=PTR, table_ld=4, pages
              max_pages=4, format=_lib.HV_CACHE_SAME)
 CACHE_DIMENSION = (dict(page=8), dict(page=24), dict(page=8192), dict(page=0), dict(page=-16),
                    dict(pages=0), dict(max_pages=-1), dict(table_ld=3), dict(width=0),
-                   dict(max_pages=1 << 28, table_ld=1 << 28),
+                   dict(max_pages=1 << 28, table_ld=1 << 28), dict(max_pages=(1 << 26) + 1, table_ld=1 << 27),
                    dict(width=20), dict(width=264), dict(width=24, format=_lib.HV_CACHE_E4M3))
 CACHE_ADDRESS = (dict(cache_k=None), dict(cache_v=None), dict(table=None), dict(lengths=None),
                  dict(format=_lib.HV_CACHE_E4M3), dict(cache_k=PTR + 8), dict(table=PTR + 2),
@@ -364,7 +374,7 @@ def test_attention_c_refusals(library):
     _refused(L, L.hv_attention(None, None, 0, None), _lib.HV_ERR_ADDRESS)
     _check(L, call, (dict(type=0), dict(type=3)), ROWS_DIMENSION + (
         dict(k_rows=5), dict(k_rows=-1), dict(k_rows=1 << 24, k_starts=PTR), dict(k_ld=60),
-        dict(v_head_ld=-8)), ROWS_ADDRESS + (
+        dict(v_head_ld=-8), dict(k_ld=(1 << 23) + 8), dict(v_ld=(1 << 23) + 8)), ROWS_ADDRESS + (
         dict(k=None), dict(v=None), dict(starts=None), dict(k=PTR + 8), dict(k_starts=PTR + 1)))
     assert call(batch=0) == _lib.HV_OK
 
