@@ -26,14 +26,15 @@ inline Shape shape_of(int rows, int batch, int heads, int kv_heads, int width) {
   const int64_t items = most_tiles(rows, batch, group, tile_rows) * kv_heads;
   return {tile_rows, width <= 128 ? 512 : 256, items < (few ? 4096 : 512)};
 }
-// Shares cost a launch and the partial results' way through memory. Few rows: 8 sequences
-// of up to 1000 keys take 13.5 us whole, 13.7 in shares; one of 2048 keys 16 in shares. Tiles:
-// shares cost 30 us, and whole tiles take 2 us for each 64 keys while the card's 512
-// workgroups lack (512 - items) of them (one prompt of 1536 tokens, 392 items: whole 44 us, in
-// shares 64; 4 sequences of up to 16384 keys with 512 new rows: 192 items, 430 and 195).
+// Shares cost a launch and the partial results' way through memory (us, whole and in shares).
+// Few rows: one row of 32 heads over 1024 keys in e4m3 12.5 and 17.9, 2048 18.3 and 18.8, 4096
+// 30.9 and 18.8, 32768 213 and 28. Tiles: the more keys and the fewer of the card's 512
+// workgroups have a tile, the better (64 rows of 32 heads over 1024 keys, 24 items: 30.3 and
+// 34.5, 2048 54 and 40; 1024 rows, 264 items, over 2048 64 and 68, 4096 116 and 102; a prompt
+// of 1536, 392 items, 38 and 59).
 inline bool worth_sharing(const Shape &shape, int rows, int batch, int kv_heads, int group,
                           int64_t most_keys) {
-  if (shape.tile_rows == kFewRows) return most_keys > 1024;
+  if (shape.tile_rows == kFewRows) return most_keys > 2048;
   return most_keys * (512 - most_tiles(rows, batch, group, shape.tile_rows) * kv_heads) > 1 << 19;
 }
 

@@ -694,12 +694,15 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attention_few(LmAttn
         for (int i = 0; i < kD; ++i) o[i] *= by;
       }
       const float ref = m == -__builtin_inff() ? 0.f : m;
-      frag p;
+      // A term as the sum of two of the type: with few rows the rounding of one is no longer
+      // averaged out, and the products cost nothing beside the loads.
+      frag p, rest;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i / 4][i % 4], a.scale, -ref));
         l += e;
         p[i] = (T)e;
+        rest[i] = (T)(e - (float)p[i]);
       }
       const int n = 4 * grp + (lane >> 2 & 3);
 #pragma unroll
@@ -707,6 +710,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attention_few(LmAttn
         const int c = few_place<DP>(n, 2 * d + (lane >> 1 & 1)) * 8 + (lane & 1) * 4;
         const v4s lo = read_column(mine + n * DP + c), hi = read_column(mine + (n + 16) * DP + c);
         const v8s both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        o[d] = Mma<T>::small(__builtin_bit_cast(frag, both), rest, o[d]);
         o[d] = Mma<T>::small(__builtin_bit_cast(frag, both), p, o[d]);
       }
       for (; odd; odd &= odd - 1) {
