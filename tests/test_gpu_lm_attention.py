@@ -667,10 +667,10 @@ def test_paged_few_rows_in_shares(kind):
     """Few rows in shares beyond a workgroup's threads of sequences, in groups
     that take two tiles, and whole where sequences are many."""
     lengths = [(37 * b) % 50 for b in range(300)]
-    lengths[7], lengths[290] = 1200, 1100
-    for lengths, heads, kv, want in ((lengths, 2, 2, "few in shares"), ([900, 30, 1200], 16, 1, "few in shares"),
+    lengths[7], lengths[290] = 2300, 2100
+    for lengths, heads, kv, want in ((lengths, 2, 2, "few in shares"), ([900, 30, 2200], 16, 1, "few in shares"),
                                      ([1 + b % 40 for b in range(1200)], 4, 4, "few"),
-                                     ([1500, 2], 12, 1, "few in shares")):
+                                     ([2500, 2], 12, 1, "few in shares")):
         assert lm_attention_kernels.kernel_of(len(lengths), len(lengths), heads, kv, 64,
                                               _room(lengths, 16)) == want
         _run_paged([1] * len(lengths), lengths, heads, kv, 64, 16, kind, False, starts=False, seed=2)
