@@ -36,7 +36,7 @@ __device__ __forceinline__ Sequence sequence_of(const LmAttnArgs &a, int b) {
   const SeqRows r = seq_rows(a.starts, b, a.rows);
   if (PAGED)
     return {r.first, r.count, paged_keys(a.map, a.lengths[b]), 0, a.table + b * a.table_ld};
-  const SeqRows k = a.k_starts ? seq_rows(a.k_starts, b, a.k_rows) : seq_rows(a.starts, b, a.k_rows);
+  const SeqRows k = seq_rows(a.k_starts ? a.k_starts : a.starts, b, a.k_rows);
   return {r.first, r.count, k.count, k.first, nullptr};
 }
 
@@ -68,7 +68,8 @@ __device__ __forceinline__ float factor_of(int byte) {
 }
 
 // The kernels of either type. The workspace is looked at here.
-int attend_f16(const LmAttnArgs &a, bool paged, bool q8, void *workspace, size_t bytes, hipStream_t s);
+int attend_f16(const LmAttnArgs &a, bool paged, bool q8, void *workspace, size_t bytes,
+               hipStream_t s);
 int attend_bf16(const LmAttnArgs &a, bool paged, bool q8, void *workspace, size_t bytes,
                 hipStream_t s);
 
@@ -102,7 +103,9 @@ __device__ __forceinline__ int key_tiles(int keys) { return keys > 0 ? (keys - 1
 static constexpr int kCostlyTiles = 1 << 14;  // of keys: more count as so many
 struct Cost {
   int first, step, count;
-  __device__ __forceinline__ int before(int i) const { return first * i + step * (i * (i + 1) / 2); }
+  __device__ __forceinline__ int before(int i) const {
+    return first * i + step * (i * (i + 1) / 2);
+  }
   __device__ __forceinline__ int all() const { return before(count); }
   // The tile that a cost in [0, all()) lies in.
   __device__ __forceinline__ int tile_at(int at) const {
@@ -119,7 +122,8 @@ __device__ __forceinline__ Cost cost_of(const LmAttnArgs &a, const Sequence &s, 
   const int count = (int)(((int64_t)s.count * a.group + tile_rows - 1) / tile_rows);
   // A tile costs one of keys by itself.
   auto cost = [](int seen) { return 16 * min(1 + key_tiles(seen), kCostlyTiles); };
-  if (a.causal && !a.window) return {cost(max(keys - s.count, 0)), tile_rows / (4 * a.group), count};
+  if (a.causal && !a.window)
+    return {cost(max(keys - s.count, 0)), tile_rows / (4 * a.group), count};
   return {cost(a.window ? min(keys, a.window) : keys), 0, count};
 }
 

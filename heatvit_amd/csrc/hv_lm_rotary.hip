@@ -8,6 +8,11 @@
 // float32 angle of a far position has lost the turn it lies in; what is left
 // of a turn is a float32 to half a step. All heads of a token share its angles:
 // a workgroup computes those of its tokens once and keeps them in LDS.
+//
+// HBM bounds it: 16384 rows of 32 and 8 heads of 128 in bf16 (336 MB) take 61 us, 5.4 TB/s,
+// in float32 126. One row takes 3.3 us: its loads, the angles, a barrier and the stores. What
+// cost most on the way there (84 us at first): reductions through LDS and the weights loaded
+// for every head (76), and registers, of which five wavefronts a SIMD leave 96 (63).
 #include <type_traits>
 
 #include "hv_lm.h"

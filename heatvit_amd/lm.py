@@ -592,7 +592,8 @@ def attention(q, k, v, starts, *, k_starts=None, scale=None, causal=True, window
     1 / sqrt(D) if None.  causal: the last row of a sequence sees all of its
     keys, each row before it one less; window > 0: the last `window` of those.
     A row that sees nothing gets zeros (and -inf in lse); what a row does not
-    see leaves no trace in it.  Returns Attended(out, lse), lse [T][Hq] the
+    see leaves no trace in it.  Sequences may be empty; offsets that leave the
+    tensors are taken at their ends.  Returns Attended(out, lse), lse [T][Hq] the
     logarithm of the sum of exponentials where asked for."""
     if not isinstance(k, torch.Tensor) or not isinstance(q, torch.Tensor):
         raise TypeError("q and k must be torch tensors")
@@ -627,8 +628,8 @@ def paged_attention(q, cache, table, lengths, *, starts=None, scale=None, causal
     over the lengths[b] keys of sequence b, key j in page table[b][j / page].
 
     q [T][Hq][D] of the cache's dtype; the rest as in attention.  A sequence
-    whose table has no room for its keys, or names a page that the cache does
-    not have among those it reads, gets NaN."""
+    whose table has no room for its keys gets NaN, and so does a row that sees a
+    page that the cache does not have (and perhaps others of its sequence)."""
     if not isinstance(cache, KvCache):
         raise TypeError("cache must be a KvCache")
     if not isinstance(q, torch.Tensor) or q.dtype != cache.dtype:

@@ -603,10 +603,13 @@ int hv_cache_write(const hv_cache_write_desc *d, hv_stream_t stream);
  * last `window` of those where that is not 0.  A row that sees nothing gets
  * zeros, and -infinity in lse, which (optional) is [rows][heads], the natural
  * logarithm of the sum of exponentials.  What a row does not see leaves no
- * trace, infinities and NaN among it; a sequence whose table has no room for
- * its keys, or a page outside the cache among those that are read, gets NaN.
- * Sums are held in 32 bits, the softmax's terms rounded to the type for
- * the product with v.  Rows outside all sequences are left as they were.
+ * trace in it, infinities and NaN among it; an infinity that it does see may
+ * come out as NaN.  A sequence whose table has no room for its keys gets NaN,
+ * and so does a row that sees a page outside the cache (other rows of its
+ * sequence may).  Sums are held in 32 bits.  The softmax's terms are rounded to
+ * the type for the product with v, as the sum of two of the type where a call
+ * has at most 16 rows a sequence and key head.  Rows outside all sequences are
+ * left as they were.
  * Widths are multiples of 8 up to 256, strides multiples of 8, pointers 16-byte
  * aligned (lse 4); type HV_T_F16 or HV_T_BF16.  The workspace (16-byte aligned) holds
  * what the parts of a long axis leave, for the call alone; calls that overlap
