@@ -98,25 +98,6 @@ static constexpr int kKeys = 64;  // of a tile
 
 __device__ __forceinline__ int key_tiles(int keys) { return keys > 0 ? (keys - 1) / kKeys + 1 : 0; }
 
-// What a sequence's tiles cost, in sixteenths of a tile of keys: tile i (of `count`) first +
-// step (i + 1). Sums over a launch's tiles, 4096 at most where shares are taken, fit 32 bits.
-static constexpr int kCostlyTiles = 1 << 14;  // of keys: more count as so many
-struct Cost {
-  int first, step, count;
-  __device__ __forceinline__ int before(int i) const {
-    return first * i + step * (i * (i + 1) / 2);
-  }
-  __device__ __forceinline__ int all() const { return before(count); }
-  // The tile that a cost in [0, all()) lies in.
-  __device__ __forceinline__ int tile_at(int at) const {
-    const float f = first + .5f * step;
-    int i = step ? (int)((sqrtf(f * f + 2.f * step * at) - f) / step) : at / first;
-    i = clamp_to(i, 0, count - 1);
-    while (i > 0 && before(i) > at) --i;
-    while (i < count - 1 && before(i + 1) <= at) ++i;
-    return i;
-  }
-};
 __device__ __forceinline__ Cost cost_of(const LmAttnArgs &a, const Sequence &s, int tile_rows) {
   const int keys = max(s.keys, 0);
   const int count = (int)(((int64_t)s.count * a.group + tile_rows - 1) / tile_rows);
@@ -125,27 +106,6 @@ __device__ __forceinline__ Cost cost_of(const LmAttnArgs &a, const Sequence &s, 
   if (a.causal && !a.window)
     return {cost(max(keys - s.count, 0)), tile_rows / (4 * a.group), count};
   return {cost(a.window ? min(keys, a.window) : keys), 0, count};
-}
-
-// Shares of a launch's cost, n of them of four tiles of keys at least: the first `more` are one
-// longer than the others.
-struct Shares {
-  int n, each, more;
-  __device__ __forceinline__ Shares(int cost, int workgroups) {
-    n = clamp_to(cost / 64, 1, workgroups);
-    each = cost / n;
-    more = cost - each * n;
-  }
-  __device__ __forceinline__ int start(int i) const { return each * i + min(i, more); }
-  __device__ __forceinline__ int of(int at) const {
-    const int longer = more * (each + 1);
-    return at < longer ? at / (each + 1) : more + (at - longer) / each;
-  }
-};
-
-// How many of a tile's n tiles of keys lie before `at` of its cost.
-__device__ __forceinline__ int tiles_at(int n, int at, int cost) {
-  return min(n, (int)((float)n * ((float)at / (float)cost)));
 }
 
 // A tile of a sequence's rows (of a key head's group: token r / group, head r % group of it)
@@ -348,11 +308,11 @@ struct Walk {
     const int t0 = w.t0, n = w.t1 - t0;
     const bool starts = at == from, ends = end >= from + cost;
     if (!starts) w.t0 = t0 + tiles_at(n, at - from, cost);
-    if (!ends) w.t1 = t0 + tiles_at(n, end - from, cost);
+    if (!ends) w.t1 = max(w.t0, t0 + tiles_at(n, end - from, cost));
     if (!starts || !ends) w.slot = 2 * share + starts;
     if (starts && !ends && threadIdx.x == 0)
       split.cuts[share] =
-          Cut{w.s.first, w.n_rows, w.r0, w.head, shares().of(from + cost - 1) - share + 1, {}};
+          Cut{w.s.first, w.n_rows, w.r0, w.head, shares().parts(share, from + cost), {}};
     const int then = ends ? from + cost : end;
     if (then <= at) return false;  // offsets that run backwards: sums past 32 bits
     at = uniform(then);

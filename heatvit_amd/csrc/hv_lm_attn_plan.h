@@ -1,9 +1,12 @@
-// hv_lm_attn_plan.h -- which kernels an attention call takes. Host code without HIP, so
-// that tests can ask which kernel their sizes reach.
+// hv_lm_attn_plan.h -- which kernels an attention call takes, and how the work is cut into
+// shares. Code without HIP, so that tests can run it on the host.
 #pragma once
 
+#include <cmath>
 #include <cstddef>
 #include <cstdint>
+
+#include "hv_lm_paged.h"
 
 namespace hv {
 
@@ -43,6 +46,51 @@ inline bool worth_sharing(const Shape &shape, int rows, int batch, int kv_heads,
 inline int slot_floats_of(const Shape &shape, int width) { return shape.tile_rows * (width + 2); }
 inline size_t workspace_of(const Shape &shape, int width) {
   return shape.split ? (size_t)shape.workgroups * (8 * slot_floats_of(shape, width) + 32) : 0;
+}
+
+// What a sequence's tiles cost, in sixteenths of a tile of keys: tile i (of `count`) first +
+// step (i + 1). Sums over a launch's tiles, 4096 at most where shares are taken, fit 32 bits,
+// but for offsets that run backwards, whose sequences overlap: numbers that left 32 bits then
+// still give tiles, parts and shares that there are.
+static constexpr int kCostlyTiles = 1 << 14;  // of keys: more count as so many
+struct Cost {
+  int first, step, count;
+  HV_HD int before(int i) const { return first * i + step * (i * (i + 1) / 2); }
+  HV_HD int all() const { return before(count); }
+  // The tile that a cost in [0, all()) lies in.
+  HV_HD int tile_at(int at) const {
+    const float f = first + .5f * step;
+    int i = step ? (int)((sqrtf(f * f + 2.f * step * at) - f) / step) : at / first;
+    i = clamp_to(i, 0, count - 1);
+    while (i > 0 && before(i) > at) --i;
+    while (i < count - 1 && before(i + 1) <= at) ++i;
+    return i;
+  }
+};
+
+// Shares of a launch's cost, n of them of four tiles of keys at least: the first `more` are one
+// longer than the others.
+struct Shares {
+  int n, each, more;
+  HV_HD Shares(int cost, int workgroups) {
+    n = clamp_to(cost / 64, 1, workgroups);
+    each = cost / n;
+    more = cost - each * n;
+  }
+  HV_HD int start(int i) const { return each * i + (i < more ? i : more); }
+  HV_HD int of(int at) const {
+    const int longer = more * (each + 1);
+    return at < longer ? at / (each + 1) : more + (at - longer) / each;
+  }
+  // How many shares, from `share` on, have a part of a tile whose cost ends at `end`.
+  HV_HD int parts(int share, int end) const {
+    return clamp_to(of(end - 1) - share + 1, 1, n - share);
+  }
+};
+
+// How many of a tile's n tiles of keys lie before `at` of its cost.
+HV_HD int tiles_at(int n, int at, int cost) {
+  return (int)fminf(fmaxf((float)n * ((float)at / (float)cost), 0.f), (float)n);
 }
 
 }  // namespace hv

@@ -593,8 +593,10 @@ def attention(q, k, v, starts, *, k_starts=None, scale=None, causal=True, window
     keys, each row before it one less; window > 0: the last `window` of those.
     A row that sees nothing gets zeros (and -inf in lse); what a row does not
     see leaves no trace in it.  Sequences may be empty; offsets that leave the
-    tensors are taken at their ends.  Returns Attended(out, lse), lse [T][Hq] the
-    logarithm of the sum of exponentials where asked for."""
+    tensors are taken at their ends, and rows that several sequences claim hold
+    any values.  `out`: the Attended to write, its tensor q itself if wanted, and
+    apart from k and v.  Returns Attended(out, lse), lse [T][Hq] the logarithm of
+    the sum of exponentials where asked for."""
     if not isinstance(k, torch.Tensor) or not isinstance(q, torch.Tensor):
         raise TypeError("q and k must be torch tensors")
     if q.dtype not in _HEAD_TYPES:

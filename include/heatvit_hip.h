@@ -609,7 +609,8 @@ int hv_cache_write(const hv_cache_write_desc *d, hv_stream_t stream);
  * sequence may).  Sums are held in 32 bits.  The softmax's terms are rounded to
  * the type for the product with v, as the sum of two of the type where a call
  * has at most 16 rows a sequence and key head.  Rows outside all sequences are
- * left as they were.
+ * left as they were; those that several sequences claim hold any values.  out
+ * may be q itself (same strides) and overlaps nothing else.
  * Widths are multiples of 8 up to 256, strides multiples of 8, pointers 16-byte
  * aligned (lse 4); type HV_T_F16 or HV_T_BF16.  The workspace (16-byte aligned) holds
  * what the parts of a long axis leave, for the call alone; calls that overlap

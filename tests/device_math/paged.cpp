@@ -36,4 +36,19 @@ int attention_shape(int rows, int batch, int heads, int kv_heads, int width, lon
 long long attention_workspace(int rows, int batch, int heads, int kv_heads, int width) {
   return (long long)workspace_of(shape_of(rows, batch, heads, kv_heads, width), width);
 }
+int tile_of_cost(int first, int step, int count, int at) {
+  return Cost{first, step, count}.tile_at(at);
+}
+int cost_before(int first, int step, int count, int tile) {
+  return Cost{first, step, count}.before(tile);
+}
+int part_of_tiles(int n, int at, int cost) { return tiles_at(n, at, cost); }
+// n, start(share), of(at), parts(share, end)
+void share_numbers(int cost, int workgroups, int share, int at, int end, int32_t *out) {
+  const Shares s(cost, workgroups);
+  out[0] = s.n;
+  out[1] = s.start(share);
+  out[2] = s.of(at);
+  out[3] = s.parts(share, end);
+}
 }

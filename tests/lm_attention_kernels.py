@@ -15,7 +15,7 @@ NAMES = ("few", "few in shares", "tiles", "tiles in shares")
 def library():
     with tempfile.TemporaryDirectory() as d:
         so = Path(d) / "paged.so"
-        subprocess.run(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", "-o", str(so),
+        subprocess.run(["g++", "-O1", "-fwrapv", "-std=c++17", "-shared", "-fPIC", "-o", str(so),
                         "-I", str(ROOT / "heatvit_amd" / "csrc"),
                         str(ROOT / "tests" / "device_math" / "paged.cpp")], check=True)
         L = C.CDLL(str(so))
@@ -29,6 +29,9 @@ def library():
     L.attention_shape.argtypes = [i] * 5 + [n]
     L.attention_workspace.argtypes = [i] * 5
     L.attention_workspace.restype = n
+    L.tile_of_cost.argtypes = L.cost_before.argtypes = [i] * 4
+    L.part_of_tiles.argtypes = [i] * 3
+    L.share_numbers.argtypes = [i] * 5 + [p]
     return L
 
 

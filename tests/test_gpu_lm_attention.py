@@ -736,6 +736,24 @@ def test_attention_bad_offsets_in_shares():
         assert out.out.isfinite().all()
 
 
+@pytest.mark.parametrize("last", (1, 8128))
+def test_attention_overlapping_sequences_in_shares(last):
+    """Offsets that run back and forth, of sequences whose cost leaves 32 bits:
+    nothing outside their rows is written, and the call ends."""
+    from heatvit_amd import lm
+    book = _filled([64], 1, 16, 4096, torch.bfloat16, False, 1)
+    batch, rows = 2049, 256
+    lengths = [2 ** 20] * (batch - 1) + [last]
+    assert lm_attention_kernels.kernel_of(300, batch, 1, 1, 16, 2 ** 20) == "few in shares"
+    q = torch.randn(300, 1, 16, generator=_gen(2)).to(torch.bfloat16).cuda()
+    out = lm.Attended(torch.full_like(q, 7.0), torch.full((300, 1), 7.0, device="cuda"))
+    lm.paged_attention(q, book.cache, torch.zeros(batch, 256, dtype=torch.int32, device="cuda"),
+                       _i32(lengths).cuda(), starts=_i32([0, rows] * (batch // 2 + 1)).cuda(),
+                       causal=False, lse=True, out=out)
+    torch.cuda.synchronize()
+    assert (out.out[rows:] == 7).all() and (out.lse[rows:] == 7).all()
+
+
 # ------------------------------------------------------------------ streams, graphs, workspaces
 
 def test_streams_graphs_and_workspaces():
@@ -821,6 +839,20 @@ def test_same_bits_again():
     for _ in range(3):
         again = lm.paged_attention(*args, lse=True)
         assert torch.equal(first.out, again.out) and torch.equal(first.lse, again.lse)
+
+
+@pytest.mark.parametrize("new, lengths", (([1, 1], [300, 90]), ([1, 1], [2500, 90]),
+                                          ([90, 45], [300, 90]), ([90, 45], [2500, 90])))
+def test_attention_in_place(new, lengths):
+    """Results over the queries, of few rows and of tiles, whole and in shares."""
+    from heatvit_amd import lm
+    book = _filled(lengths, 2, 128, 16, torch.bfloat16, False, 1)
+    q = torch.randn(sum(new), 6, 128, generator=_gen(1)).to(torch.bfloat16).cuda()
+    args = book.cache, book.table.cuda(), _i32(lengths).cuda()
+    starts = _i32(_starts(new)).cuda()
+    want = lm.paged_attention(q, *args, starts=starts)
+    got = lm.paged_attention(q, *args, starts=starts, out=lm.Attended(q, None))
+    assert got.out is q and torch.equal(q, want.out)
 
 
 # ------------------------------------------------------------------ a run of them

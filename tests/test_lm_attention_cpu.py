@@ -100,6 +100,59 @@ def test_kernels():
             assert size == 0
 
 
+def test_shares():
+    """Shares of the work cover it, one behind the other, and a tile's parts are
+    the shares that it reaches into."""
+    L = lm_attention_kernels.library()
+    out = np.zeros(4, np.int32)
+
+    def numbers(cost, groups, share=0, at=0, end=1):
+        L.share_numbers(cost, groups, share, at, end, out.ctypes.data)
+        return out.tolist()
+
+    for cost in (16, 63, 64, 640, 512 * 64 - 1, 512 * 64, 1000003, (1 << 30) + (1 << 28) + 7):
+        for groups in (256, 512):
+            n = numbers(cost, groups)[0]
+            assert n == min(max(cost // 64, 1), groups)
+            starts = [numbers(cost, groups, i)[1] for i in range(n + 1)]
+            assert starts[0] == 0 and starts[n] == cost and min(np.diff(starts)) >= min(64, cost)
+            for i in range(n):
+                assert numbers(cost, groups, at=starts[i])[2] == i
+                assert numbers(cost, groups, at=starts[i + 1] - 1)[2] == i
+                last = min(i + 3, n)
+                assert numbers(cost, groups, i, end=starts[last])[3] == last - i
+    for first, step, count in ((16, 0, 1), (48, 0, 300), (32, 8, 4000), (1 << 18, 32, 4096)):
+        for tile in sorted({0, count // 3, count - 1}):
+            lo, hi = (L.cost_before(first, step, count, t) for t in (tile, tile + 1))
+            for at in (lo, (lo + hi) // 2, hi - 1):
+                assert L.tile_of_cost(first, step, count, at) == tile
+    for n in (0, 1, 7, 1 << 24):
+        assert L.part_of_tiles(n, 0, 64) == 0 and L.part_of_tiles(n, 64, 64) == n
+
+
+def test_shares_of_numbers_past_32_bits():
+    """What sums of overlapping sequences may wrap to still gives tiles, parts
+    and shares that there are."""
+    L = lm_attention_kernels.library()
+    out = np.zeros(4, np.int32)
+    rng = np.random.default_rng(0)
+    edges = [-2 ** 31, -2 ** 31 + 1, -1, 0, 1, 31, 2 ** 18, 2 ** 30, 2 ** 31 - 1]
+    some = edges + rng.integers(-2 ** 31, 2 ** 31 - 1, 40).tolist()
+    for cost in (1, 32, 100, 2 ** 18, 2 ** 31 - 1):
+        for at in some:
+            for n in (0, 1, 5, 1 << 24):
+                assert 0 <= L.part_of_tiles(n, at, cost) <= n
+            for groups in (256, 512):
+                L.share_numbers(cost, groups, 0, 0, 1, out.ctypes.data)
+                n = int(out[0])
+                for share in (0, n // 2, n - 1):
+                    L.share_numbers(cost, groups, share, 0, at, out.ctypes.data)
+                    assert 1 <= out[3] <= n - share
+    for first, step, count in ((16, 0, 5), (1 << 18, 0, 1 << 14), (1 << 18, 32, 4096), (1 << 18, 32, 30000)):
+        for at in some:
+            assert 0 <= L.tile_of_cost(first, step, count, max(at, 0)) < count
+
+
 # ------------------------------------------------------------------ frequencies
 
 def test_frequencies():
