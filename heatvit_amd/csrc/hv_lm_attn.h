@@ -21,6 +21,7 @@ struct LmAttnArgs {
   int64_t k_ld, k_head_ld, v_ld, v_head_ld;  // packed keys
   int64_t table_ld;
   int rows, k_rows, batch, heads, kv_heads, group, width, causal, window;
+  int run;  // run_of
   PageMap map;
   float scale;  // of q.k, to a power of two: scale log2(e)
 };
@@ -299,7 +300,8 @@ struct Walk {
   __device__ __forceinline__ bool next(Work &w) {
     if (!SPLIT) {
       const int kv_heads = finder.a.kv_heads;
-      const bool some = finder.whole(blockIdx.x / kv_heads, blockIdx.x % kv_heads, w);
+      const int run = finder.a.run, at = run ? place_of(blockIdx.x, run) : (int)blockIdx.x;
+      const bool some = finder.whole(at / kv_heads, at % kv_heads, w);
       make_uniform(w);
       return some;
     }

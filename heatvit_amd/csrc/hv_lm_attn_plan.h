@@ -41,6 +41,26 @@ inline bool worth_sharing(const Shape &shape, int rows, int batch, int kv_heads,
   return most_keys * (512 - most_tiles(rows, batch, group, shape.tile_rows) * kv_heads) > 1 << 19;
 }
 
+// Tiles of a short sequence run on one XCD, whose L2 then has their keys once. Workgroup b runs on
+// XCD b % 8: with a multiple of eight heads of keys a head's tiles meet there by themselves;
+// otherwise each XCD takes the tiles of a run of the list, all heads' of as many tiles as a
+// sequence has, four at most. (us, without runs and with them: 256 sequences of 197 tokens and 3
+// heads of 64, two tiles, 31.5 and 28.7; of 577, five tiles, 130.8 and 128.0; of 400, causal,
+// 64.1 and 61.2. Long causal sequences gain nothing, as their neighbours run at the same time
+// anyway, and lose where the longest tiles come in runs: 8192 tokens and 4 heads of 128 525 and
+// 543.) 0: no runs.
+inline int run_of(const Shape &shape, int rows, int batch, int kv_heads, int group) {
+  const int64_t tiles = ((int64_t)rows * group + (int64_t)batch * shape.tile_rows - 1) /
+                        ((int64_t)batch * shape.tile_rows);
+  if (shape.split || kv_heads % 8 == 0 || tiles < 2 || tiles > 8) return 0;
+  return (int)(tiles < 4 ? tiles : 4) * kv_heads;
+}
+// The place in the list of workgroup b of a launch of a multiple of eight runs.
+HV_HD int place_of(int b, int run) {
+  const int turn = b / 8 / run;
+  return (turn * 8 + b % 8) * run + b / 8 - turn * run;
+}
+
 // Two partial results a workgroup, of a tile that an earlier one began and of one that a later
 // one ends: for each row the reference, the sum of the terms and the sums relative to it.
 inline int slot_floats_of(const Shape &shape, int width) { return shape.tile_rows * (width + 2); }

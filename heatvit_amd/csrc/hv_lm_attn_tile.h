@@ -920,7 +920,8 @@ static void attend_launch(const LmAttnArgs &a, const Split &split, const Shape &
   const bool few = shape.tile_rows == kFewRows;
   const unsigned items =
       (unsigned)(most_tiles(a.rows, a.batch, a.group, shape.tile_rows) * a.kv_heads);
-  const dim3 grid(shape.split ? shape.workgroups : items), block(256);
+  const unsigned unit = a.run ? 8 * a.run : 1;
+  const dim3 grid(shape.split ? shape.workgroups : (items + unit - 1) / unit * unit), block(256);
   if (!shape.split) {
     if (few) hv_launch(k_attention_few<T, DP, PAGED, Q8, false>, grid, block, 0, s, a, split);
     else hv_launch(k_attention_tile<T, DP, PAGED, Q8, 4, false>, grid, block, 0, s, a, split);
@@ -933,7 +934,7 @@ static void attend_launch(const LmAttnArgs &a, const Split &split, const Shape &
 }
 
 template <typename T, bool PAGED, bool Q8>
-static int attend(const LmAttnArgs &a, void *workspace, size_t bytes, hipStream_t s) {
+static int attend(LmAttnArgs a, void *workspace, size_t bytes, hipStream_t s) {
   Shape shape = shape_of(a.rows, a.batch, a.heads, a.kv_heads, a.width);
   Split split{};
   if (shape.split) {
@@ -949,6 +950,7 @@ static int attend(const LmAttnArgs &a, void *workspace, size_t bytes, hipStream_
     const int64_t most_keys = PAGED ? (int64_t)a.map.max_pages << a.map.shift : a.k_rows;
     if (!worth_sharing(shape, a.rows, a.batch, a.kv_heads, a.group, most_keys)) shape.split = false;
   }
+  a.run = run_of(shape, a.rows, a.batch, a.kv_heads, a.group);
   if (a.width <= 64) attend_launch<T, PAGED, Q8, 64>(a, split, shape, s);
   else if (a.width <= 128) attend_launch<T, PAGED, Q8, 128>(a, split, shape, s);
   else attend_launch<T, PAGED, Q8, 256>(a, split, shape, s);

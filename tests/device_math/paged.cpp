@@ -51,4 +51,10 @@ void share_numbers(int cost, int workgroups, int share, int at, int end, int32_t
   out[2] = s.of(at);
   out[3] = s.parts(share, end);
 }
+int attention_run(int rows, int batch, int heads, int kv_heads, int width, int split) {
+  Shape s = shape_of(rows, batch, heads, kv_heads, width);
+  s.split = split != 0;
+  return run_of(s, rows, batch, kv_heads, heads / kv_heads);
+}
+int place_in_runs(int b, int run) { return place_of(b, run); }
 }

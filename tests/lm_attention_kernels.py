@@ -31,6 +31,8 @@ def library():
     L.attention_workspace.restype = n
     L.tile_of_cost.argtypes = L.cost_before.argtypes = [i] * 4
     L.part_of_tiles.argtypes = [i] * 3
+    L.attention_run.argtypes = [i] * 6
+    L.place_in_runs.argtypes = [i] * 2
     L.share_numbers.argtypes = [i] * 5 + [p]
     return L
 

@@ -676,6 +676,16 @@ def test_paged_few_rows_in_shares(kind):
         _run_paged([1] * len(lengths), lengths, heads, kv, 64, 16, kind, False, starts=False, seed=2)
 
 
+@pytest.mark.parametrize("causal", (True, False))
+def test_attention_in_runs(causal):
+    """More tiles than the card takes at once, of short sequences (empty ones
+    among them) and heads that are no multiple of eight."""
+    for new, kv, kind in (([0, 400, 1] * 100, 3, "f16"), ([140 + 3 * (b % 40) for b in range(300)], 2, "bf16")):
+        assert lm_attention_kernels.kernel_of(sum(new), len(new), kv, kv, 64, sum(new)) == "tiles"
+        assert lm_attention_kernels.library().attention_run(sum(new), len(new), kv, kv, 64, 0) == 2 * kv
+        _run_attention(new, kv, kv, 64, kind, causal, 0, 3)
+
+
 def test_attention_tiles_in_shares():
     """Packed keys of their own, cut into shares."""
     assert lm_attention_kernels.kernel_of(180, 2, 4, 2, 64, 3300) == "tiles in shares"

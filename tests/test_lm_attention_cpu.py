@@ -100,6 +100,22 @@ def test_kernels():
             assert size == 0
 
 
+def test_runs():
+    """Workgroups in runs take every place once, and an XCD's are side by side."""
+    L = lm_attention_kernels.library()
+    for run in (2, 6, 9, 12, 20):
+        places = np.array([L.place_in_runs(b, run) for b in range(3 * 8 * run)])
+        assert (np.sort(places) == np.arange(places.size)).all()
+        for xcd in range(8):
+            assert (places[xcd::8].reshape(3, run) ==
+                    np.arange(3)[:, None] * 8 * run + xcd * run + np.arange(run)).all()
+    assert L.attention_run(256 * 197, 256, 3, 3, 64, 0) == 6
+    assert L.attention_run(256 * 577, 256, 3, 3, 64, 0) == 12
+    for none in ((256 * 197, 256, 16, 8, 64, 0), (4096, 4096, 12, 3, 64, 0), (8192, 1, 4, 4, 128, 0),
+                 (256 * 197, 256, 3, 3, 64, 1)):
+        assert L.attention_run(*none) == 0
+
+
 def test_shares():
     """Shares of the work cover it, one behind the other, and a tile's parts are
     the shares that it reaches into."""
