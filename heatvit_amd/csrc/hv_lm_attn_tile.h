@@ -263,12 +263,12 @@ struct TileLoader {
 //                 is read from LDS by columns in that order
 //
 // The matrix cores bound long prompts, with the exponentials beside them: 8192 causal tokens of
-// 32 heads over 8 of 128 in bf16 take 500 to 535 us by card (1030 to 1100 TFLOP/s; a library
+// 32 heads over 8 of 128 in bf16 take 500 to 542 us by card (1015 to 1100 TFLOP/s; a library
 // product of 8192^3 reaches 1210), the matrix cores busy for 56 % of it at the 1.7 GHz that such a
 // load leaves. A wavefront's 32 products of a tile take 1024 cycles, its 32 exponentials a lane
 // 512 and what else it does with the scores as many; two wavefronts a SIMD, of workgroups that
 // share no barrier, run one beside the other. A lone tile of keys takes 1.3 us, and a workgroup
-// 7 us around its tiles: 256 sequences of 197 tokens, 3 heads of 64, 30 us, are four tiles in
+// 7 us around its tiles: 256 sequences of 197 tokens, 3 heads of 64, 29 us, are four tiles in
 // two rounds of that.
 // (Terms are rounded to the type for the second product: of the result's norm 1.1e-3 in bf16,
 // 1.4e-4 in f16, where the result's own rounding takes 1.6e-3 and 2.1e-4.)

@@ -208,7 +208,9 @@ template <typename T>
 static void rotary_launch(RotaryArgs a, hipStream_t s) {
   const int lanes = (a.pairs + 7) / 8 + (a.width - 2 * a.pairs + 15) / 16;
   // Tokens a workgroup: its threads compute an angle each, while there are
-  // workgroups enough; keys, whose heads are fewer, take more of them.
+  // workgroups enough; keys, whose heads are fewer, take more of them. (4096 rows of 32 and 8
+  // heads of 128 take 15.6 us by 1024 workgroups, 18.4 by 4096 of a token each; 4000 rows of
+  // 20 and 20 of 100 33.3 by 1000 of four tokens, 36.2 by 400 of ten.)
   const int keys = a.heads[1] ? 1 : 0;
   int most = a.pairs ? max(1, min(16, 256 / a.pairs)) : 16;
   while (most > 1 && (a.rows + most - 1) / most < 1024) most /= 2;
