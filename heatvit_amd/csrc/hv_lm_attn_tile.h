@@ -469,7 +469,10 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 3 : DP == 128 ? 2 : 1) void k_a
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 16 * kD; ++i) sum = __builtin_fmaf(o[i / 16][i % 16], 0.f, sum);
-    if (__syncthreads_or(sum != 0.f)) pass(std::true_type());
+    if (__syncthreads_or(sum != 0.f)) {
+      pass(std::true_type());
+      __syncthreads();  // before the next tile's first loads take the place of its last values
+    }
 
     // (Again, so that it is not held all along.)
     int at_row = min(w0 + col, n_rows - 1);

@@ -732,6 +732,31 @@ def test_shares_leave_out_what_is_not_seen(new):
     assert torch.equal(got.out[at[1]:], clean.out[at[1]:])
 
 
+@pytest.mark.parametrize("value", (math.nan, math.inf))
+@pytest.mark.parametrize("rows, keys, heads, kv, width", ((4096, 4096, 8, 8, 128), (64, 2500, 4, 2, 64),
+                                                          (2048, 2048, 4, 4, 64), (700, 3100, 2, 2, 256)))
+def test_one_packed_sequence_in_shares_with_a_bad_value(rows, keys, heads, kv, width, value):
+    """One element of one value that is no number, where shares of one packed
+    sequence hold parts of several tiles: every other element of every row has
+    the clean call's bits."""
+    from heatvit_amd import lm
+    assert lm_attention_kernels.kernel_of(rows, 1, heads, kv, width, keys) == "tiles in shares"
+    q, k, v = (t.cuda() for t in _packed([rows], heads, kv, width, torch.bfloat16, 6, [keys]))
+    args = dict(k_starts=_i32([0, keys]).cuda(), lse=True)
+    starts = _i32([0, rows]).cuda()
+    clean = lm.attention(q, k, v, starts, **args)
+    row_at = keys - rows + torch.arange(rows, device="cuda")
+    for position in (keys - 1, keys - 70, keys - rows // 2, 3):
+        x = v.clone()
+        x[position, 0, 5] = value
+        got = lm.attention(q, k, x, starts, **args)
+        touched = torch.zeros(rows, heads, width, dtype=torch.bool, device="cuda")
+        touched[row_at >= position, :heads // kv, 5] = True
+        assert torch.equal(got.out[~touched], clean.out[~touched]), position
+        assert not got.out[touched].isfinite().any(), position
+        assert torch.equal(got.lse, clean.lse), position
+
+
 def test_attention_bad_offsets_in_shares():
     """Offsets that run backwards or leave the tensors where the work is cut
     into shares: nothing outside the rows is written, and the call ends."""
