@@ -16,6 +16,7 @@
 #include <type_traits>
 
 #include "hv_lm.h"
+#include "hv_lm_rotary_plan.h"
 
 namespace hv {
 
@@ -53,8 +54,8 @@ __device__ __forceinline__ float all_of(float v, Op op) {
 
 // LANES lanes a head; each takes 16 of its elements as two runs of eight: the
 // two halves of eight pairs (or eight interleaved pairs), or what follows the
-// rotated part.
-template <typename T, int LANES>
+// rotated part. MORE: a head of 65 lanes, of whose last one's elements 64 take one each.
+template <typename T, int LANES, bool MORE>
 __global__ __launch_bounds__(256, 5) void k_rotary_qk(RotaryArgs a) {
   constexpr int kGroups = 256 / LANES;
   typedef typename Eight<T>::v8 v8;
@@ -80,7 +81,7 @@ __global__ __launch_bounds__(256, 5) void k_rotary_qk(RotaryArgs a) {
 
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
   const int rotated = 2 * a.pairs;
-  const int pair_lanes = (a.pairs + 7) / 8;
+  const int pair_lanes = rotary_pair_lanes(a.pairs);
   const bool pair = lane < pair_lanes;
   int at[2], n[2];  // the lane's two runs
   if (pair && !a.interleaved) {
@@ -98,10 +99,14 @@ __global__ __launch_bounds__(256, 5) void k_rotary_qk(RotaryArgs a) {
   // Where item i's head lies, and what is loaded of it: the next one's is on its way while
   // one is worked on.
   v8 next[2];
+  const int more_at = rotated + 16 * (LANES - pair_lanes) + lane;
+  const bool more = MORE && more_at < a.width;
+  T next_more = (T)0.f;
   auto load = [&](int t, int h) {
     const T *x = x0 + t * a.ld[which] + h * a.head_ld[which];
 #pragma unroll
     for (int r = 0; r < 2; ++r) next[r] = n[r] > 0 ? Eight<T>::load(x + at[r], n[r]) : v8{};
+    if (more) next_more = x[more_at];
   };
   const int step_t = kGroups / heads, step_h = kGroups - step_t * heads;
   int t = min(group, items - 1) / heads, h = min(group, items - 1) - t * heads;
@@ -110,6 +115,7 @@ __global__ __launch_bounds__(256, 5) void k_rotary_qk(RotaryArgs a) {
 #pragma unroll
   for (int r = 0; r < 2; ++r)
     if (w && n[r] > 0) weight[r] = Eight<T>::load(w + at[r], n[r]);
+  const float weight_more = w && more ? (float)w[more_at] : 0.f;
   turns();
   __syncthreads();
   // Every lane of a wavefront takes part in its reductions: a group past the
@@ -126,6 +132,8 @@ __global__ __launch_bounds__(256, 5) void k_rotary_qk(RotaryArgs a) {
         v[r][i] = (float)next[r][i];
         sum = __builtin_fmaf(v[r][i], v[r][i], sum);
       }
+    float v_more = (float)next_more;
+    if (MORE) sum = __builtin_fmaf(v_more, v_more, sum);
     if (i0 + kGroups < items) {
       t += step_t;
       h += step_h;
@@ -150,6 +158,7 @@ __global__ __launch_bounds__(256, 5) void k_rotary_qk(RotaryArgs a) {
         float most = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(v[i / 8][i % 8]));
+        if (MORE) most = fmaxf(most, fabsf(v_more));
         most = all_of<LANES>(most, [](float p, float q) { return fmaxf(p, q); });
         // (eps by that power squared stays a number)
         const int e = again ? max(__builtin_amdgcn_frexp_expf(most), a.least_exp) : 0;
@@ -160,6 +169,10 @@ __global__ __launch_bounds__(256, 5) void k_rotary_qk(RotaryArgs a) {
           x = ldexpf(x, -e);
           s = __builtin_fmaf(x, x, s);
         }
+        if (MORE) {
+          v_more = ldexpf(v_more, -e);
+          s = __builtin_fmaf(v_more, v_more, s);
+        }
         s = all_of<LANES>(s, add);
         if (again) f = __builtin_amdgcn_rsqf(s * a.inv_width + ldexpf(a.eps, -2 * e));
       }
@@ -168,6 +181,7 @@ __global__ __launch_bounds__(256, 5) void k_rotary_qk(RotaryArgs a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[r][i] = v[r][i] * f * (float)weight[r][i];
       }
+      v_more = v_more * f * weight_more;
     }
     if (pair) {
       const float2 *cs = turn + token * a.pairs + 8 * lane;
@@ -200,13 +214,14 @@ __global__ __launch_bounds__(256, 5) void k_rotary_qk(RotaryArgs a) {
         for (int i = 0; i < 8; ++i) e[i] = (T)v[r][i];
         if (n[r] > 0) Eight<T>::store(out + at[r], n[r], e);
       }
+      if (more) out[more_at] = (T)v_more;
     }
   }
 }
 
 template <typename T>
 static void rotary_launch(RotaryArgs a, hipStream_t s) {
-  const int lanes = (a.pairs + 7) / 8 + (a.width - 2 * a.pairs + 15) / 16;
+  const int lanes = rotary_lanes(a.pairs, a.width);
   // Tokens a workgroup: its threads compute an angle each, while there are
   // workgroups enough; keys, whose heads are fewer, take more of them. (4096 rows of 32 and 8
   // heads of 128 take 15.6 us by 1024 workgroups, 18.4 by 4096 of a token each; 4000 rows of
@@ -220,11 +235,12 @@ static void rotary_launch(RotaryArgs a, hipStream_t s) {
     a.tokens[1] = max(most, min(most * a.heads[0] / a.heads[1], min(16, 1024 / max(1, a.pairs))));
   const dim3 grid((unsigned)((a.rows + most - 1) / most), 1 + keys), block(256);
   const uint32_t lds = (uint32_t)(max(a.tokens[0], a.tokens[1]) * a.pairs * sizeof(float2));
-  if (lanes <= 4) hv_launch(k_rotary_qk<T, 4>, grid, block, lds, s, a);
-  else if (lanes <= 8) hv_launch(k_rotary_qk<T, 8>, grid, block, lds, s, a);
-  else if (lanes <= 16) hv_launch(k_rotary_qk<T, 16>, grid, block, lds, s, a);
-  else if (lanes <= 32) hv_launch(k_rotary_qk<T, 32>, grid, block, lds, s, a);
-  else hv_launch(k_rotary_qk<T, 64>, grid, block, lds, s, a);
+  if (lanes <= 4) hv_launch(k_rotary_qk<T, 4, false>, grid, block, lds, s, a);
+  else if (lanes <= 8) hv_launch(k_rotary_qk<T, 8, false>, grid, block, lds, s, a);
+  else if (lanes <= 16) hv_launch(k_rotary_qk<T, 16, false>, grid, block, lds, s, a);
+  else if (lanes <= 32) hv_launch(k_rotary_qk<T, 32, false>, grid, block, lds, s, a);
+  else if (lanes <= 64) hv_launch(k_rotary_qk<T, 64, false>, grid, block, lds, s, a);
+  else hv_launch(k_rotary_qk<T, 64, true>, grid, block, lds, s, a);
 }
 
 }  // namespace hv

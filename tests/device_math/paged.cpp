@@ -58,3 +58,7 @@ int attention_run(int rows, int batch, int heads, int kv_heads, int width, int s
 }
 int place_in_runs(int b, int run) { return place_of(b, run); }
 }
+
+// Lanes of a head of the rotary kernels.
+#include "hv_lm_rotary_plan.h"
+extern "C" int lanes_of_head(int pairs, int width) { return rotary_lanes(pairs, width); }

@@ -71,6 +71,46 @@ def test_rotary_sizes(kind, norm, layout):
         _check_rotary(got, q, k, w, p, f, 1e-5, layout, 1.25)
 
 
+@pytest.mark.parametrize("layout", ("half", "interleaved"))
+@pytest.mark.parametrize("norm", (False, True))
+@pytest.mark.parametrize("kind", TYPES)
+def test_rotary_heads_of_65_lanes(kind, norm, layout):
+    """Heads both parts of which end within a lane: all elements count in the
+    norm and are written, and nothing else is.  (A lane adds 17 squares in a row
+    here, half a step of float32 after the root that the bound's 21 have: the
+    mean's and eps' steps are halved by the root too.)"""
+    from heatvit_amd import lm
+    for width, rotated in ((1024, 2), (1024, 1022), (1011, 2), (1024, 500), (1020, 1002), (1024, 0)):
+        assert rotated == 0 or lm_attention_kernels.library().lanes_of_head(rotated // 2, width) == 65
+        q, k, w, p, f = _rotary_inputs(5, 3, 2, width, rotated, TYPES[kind], norm, rotated, 77)
+        q[1, :, -1], q[2, :, :-1] = 100, 0  # a last element that the norm hangs on
+        print(f"rotary {kind} {layout} {width}/{rotated}", flush=True)
+        buf = [torch.full((5, n, width + 3), 9.0, dtype=q.dtype, device="cuda") for n in (3, 2)]
+        out = lm.QK(*(t[..., 1:1 + width] for t in buf))
+        args = dict(q_weight=_dev(w[0]), k_weight=_dev(w[1]), eps=1e-5, layout=layout)
+        got = lm.rotary_qk(q.cuda(), k.cuda(), p.cuda(), f.cuda(), out=out, **args)
+        _check_rotary(got, q, k, w, p, f, 1e-5, layout, 1.0)
+        assert all((t[..., 0] == 9).all() and (t[..., 1 + width:] == 9).all() for t in buf)
+        qv, kv = (t.cuda() for t in (q, k))
+        lm.rotary_qk(qv, kv, p.cuda(), f.cuda(), out=lm.QK(qv, kv), **args)
+        assert torch.equal(qv, got.q) and torch.equal(kv, got.k)
+
+
+def test_rotary_heads_of_65_lanes_at_the_edges():
+    """Squares that leave float32, of such heads' last elements."""
+    from heatvit_amd import lm
+    q, k, w, p, f = _rotary_inputs(4, 2, 1, 1024, 998, torch.float32, True, 1)
+    info = torch.finfo(torch.float32)
+    q[0, 0], q[0, 0, -1] = 0, info.max / 4
+    q[1, 1] = 0
+    q[2, 0], q[2, 0, -1] = 0, info.smallest_normal
+    for eps in (1e-6, 0.0):
+        with np.errstate(all="ignore"):
+            got = lm.rotary_qk(q.cuda(), k.cuda(), p.cuda(), f.cuda(), q_weight=w[0].cuda(),
+                               k_weight=w[1].cuda(), eps=eps)
+            _check_rotary(got, q, k, w, p, f, eps, "half", 1.0)
+
+
 @pytest.mark.parametrize("rows", (63, 1025, 5000))
 def test_rotary_many_rows(rows):
     from heatvit_amd import lm

@@ -169,6 +169,21 @@ def test_shares_of_numbers_past_32_bits():
             assert 0 <= L.tile_of_cost(first, step, count, max(at, 0)) < count
 
 
+def test_lanes_of_a_head():
+    """Every head that rotary_qk takes has 65 lanes at most, the last of which
+    then has up to 16 elements, none of them rotated."""
+    L = lm_attention_kernels.library()
+    wide = 0
+    for width in range(1, _lib.HV_ROTARY_MAX_WIDTH + 1):
+        for pairs in range(width // 2 + 1):
+            lanes, of_pairs = L.lanes_of_head(pairs, width), -(-pairs // 8)
+            assert lanes <= 65 and lanes * 16 >= width
+            if lanes == 65:
+                wide += 1
+                assert of_pairs <= 64 and 0 < width - 2 * pairs - 16 * (64 - of_pairs) <= 16
+    assert wide
+
+
 # ------------------------------------------------------------------ frequencies
 
 def test_frequencies():
