@@ -117,7 +117,8 @@ struct Work {
   int n_rows;  // s.count * group
   int r0;      // the tile's first row
   int t0, t1;  // tiles of keys
-  int last;    // the last key that the rows see, -1: none
+  int from;    // the first key that the rows see
+  int last;    // the last one, -1: none
   int head;    // of the keys
   int slot;    // of the partial result, -1: the result is whole
 };
@@ -231,6 +232,7 @@ struct Finder {
     const Seen first = seen_by(w.r0 / a.group, s.count, w.keys, a.causal, a.window);
     const Seen final = seen_by(min(w.r0 + tile_rows - 1, w.n_rows - 1) / a.group, s.count, w.keys,
                                a.causal, a.window);
+    w.from = first.from;
     w.last = final.to - 1;
     w.t0 = first.from / kKeys;
     w.t1 = max(w.t0, key_tiles(final.to));
@@ -267,9 +269,9 @@ struct Finder {
 // The same work, its numbers in scalar registers.
 __device__ __forceinline__ void make_uniform(Work &w) {
   int *const n[] = {&w.s.first, &w.s.count, &w.s.keys, &w.s.k_first, &w.keys, &w.n_rows, &w.r0,
-                    &w.t0,      &w.t1,      &w.last,   &w.head,      &w.slot};
+                    &w.t0,      &w.t1,      &w.from,   &w.last,      &w.head, &w.slot};
 #pragma unroll
-  for (int i = 0; i < 12; ++i) *n[i] = uniform(*n[i]);
+  for (int i = 0; i < 13; ++i) *n[i] = uniform(*n[i]);
   const uint64_t table = (uint64_t)w.s.table;
   w.s.table = (const int32_t *)((uint64_t)(unsigned)uniform((int)(table >> 32)) << 32 |
                                 (unsigned)uniform((int)table));

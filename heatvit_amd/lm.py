@@ -631,7 +631,9 @@ def paged_attention(q, cache, table, lengths, *, starts=None, scale=None, causal
 
     q [T][Hq][D] of the cache's dtype; the rest as in attention.  A sequence
     whose table has no room for its keys gets NaN, and so does a row that sees a
-    page that the cache does not have (and perhaps others of its sequence)."""
+    page that the cache does not have (and perhaps others of its sequence);
+    table entries of pages that no row sees, as those that a window has left
+    behind, may be anything."""
     if not isinstance(cache, KvCache):
         raise TypeError("cache must be a KvCache")
     if not isinstance(q, torch.Tensor) or q.dtype != cache.dtype:

@@ -606,7 +606,8 @@ int hv_cache_write(const hv_cache_write_desc *d, hv_stream_t stream);
  * trace in it, infinities and NaN among it; an infinity that it does see may
  * come out as NaN.  A sequence whose table has no room for its keys gets NaN,
  * and so does a row that sees a page outside the cache (other rows of its
- * sequence may).  Sums are held in 32 bits.  The softmax's terms are rounded to
+ * sequence may); pages that no row of it sees may be anything, as those are
+ * that a window has left behind.  Sums are held in 32 bits.  The softmax's terms are rounded to
  * the type for the product with v, as the sum of two of the type where a call
  * has at most 16 rows a sequence and key head.  Rows outside all sequences are
  * left as they were; those that several sequences claim hold any values.  out

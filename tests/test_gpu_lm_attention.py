@@ -637,6 +637,37 @@ def test_paged_bad_pages(e4m3):
         assert (got.out[at[1]:at[2]] == 0).all() and (got.lse[at[1]:at[2]] == -math.inf).all()
 
 
+@pytest.mark.parametrize("e4m3", (False, True))
+@pytest.mark.parametrize("page", (16, 32, 64))
+def test_paged_pages_before_a_window(page, e4m3):
+    """Pages that lie before what any row sees may be gone: the same bits. The
+    first page that a row does see may not."""
+    from heatvit_amd import lm
+    for new, lengths, width, window, kernel in (
+            ([1], [1000], 64, 80, "few"), ([1, 1], [1000, 333], 128, 17, "few"),
+            ([1, 1], [2500, 71], 64, 1500, "few in shares"), ([6], [2613], 128, 2200, "few in shares"),
+            ([70, 40], [301, 290], 64, 101, "tiles"), ([33], [455], 256, 60, "tiles"),
+            ([70], [2601], 64, 933, "tiles in shares"), ([40, 60], [2601, 2222], 128, 700, "tiles in shares")):
+        book = _filled(lengths, 2, width, page, torch.bfloat16, e4m3, 5)
+        assert lm_attention_kernels.kernel_of(sum(new), len(new), 4, 2, width,
+                                              book.table.shape[1] * page) == kernel
+        print(f"pages of {page} before a window: {new} of {lengths}, {width}, {window}", flush=True)
+        q = torch.randn(sum(new), 4, width, generator=_gen(1)).to(torch.bfloat16).cuda()
+        args = dict(starts=_i32(_starts(new)).cuda(), window=window, lse=True)
+        n = _i32(lengths).cuda()
+        clean = lm.paged_attention(q, book.cache, book.table.cuda(), n, **args)
+        assert clean.out.isfinite().all() and clean.lse.isfinite().all()
+        table = book.table.clone()
+        first = [max(length - rows + 1 - window, 0) // page for length, rows in zip(lengths, new)]
+        for b, count in enumerate(first):
+            table[b, :count] = _i32([(-1, 2 ** 30, -2 ** 31)[i % 3] for i in range(count)])
+        got = lm.paged_attention(q, book.cache, table.cuda(), n, **args)
+        assert torch.equal(got.out, clean.out) and torch.equal(got.lse, clean.lse)
+        table[0, first[0]] = -1
+        got = lm.paged_attention(q, book.cache, table.cuda(), n, **args)
+        assert got.out[0].isnan().all() and got.lse[0].isnan().all()
+
+
 def test_paged_smallest_exponent():
     """Heads of the smallest exponent, as zeros have, beside ordinary ones."""
     from heatvit_amd import lm
