@@ -1,6 +1,7 @@
 // hv_lm_attn_tile.h -- the attention kernels, for the file of each element type.
 //
-//   out = sum_j p_j v_j / sum_j p_j,  p_j = 2^(scale log2(e) q.k_j - m),  m the largest
+//   out = sum_j p_j v_j / sum_j p_j,  p_j = 2^(scale log2(e) q.k_j - m),  m a reference near the
+//   largest
 #pragma once
 
 #include "hv_lm_attn.h"
@@ -65,7 +66,15 @@ __device__ __forceinline__ v4s read_column(const void *p) {
       (__attribute__((address_space(3))) v4s *)(__attribute__((address_space(3))) void *)p);
 }
 
-static constexpr float kRise = 8.f;  // over a row's reference, to a power of two
+// A row's reference lies kLift under its largest score when it rises, and rises when a score is
+// kRise above it, to powers of two. f16's terms are up to 2^15 so, of 65504, as its smallest
+// numbers are near: a term 2^-25 of the largest would be none with a reference at the largest
+// score, though the sum counts it (1000 terms of 2^-26 beside one of a value of zero, in tiles:
+// nothing left of the result; so 2^-32 is lost). It costs no time.
+template <typename T>
+static constexpr float kLift = std::is_same<T, f16>::value ? 7.f : 0.f;
+template <typename T>
+static constexpr float kRise = 8.f + kLift<T>;
 
 // Where 16-byte chunk c of a tile's row lies in that row, so that the reads of
 // a tile meet no bank twice: of keys, one chunk of 32 rows at a time; of
@@ -390,13 +399,13 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 3 : DP == 128 ? 2 : 1) void k_a
       float most = x[0][0];
 #pragma unroll
       for (int i = 1; i < 32; ++i) most = fmaxf(most, x[i / 16][i % 16]);
-      // A row's reference rises only when a score passes it by 2^8: what is summed
+      // A row's reference rises only when a score passes it by kRise: what is summed
       // is the same but for its exponent.
-      if (__builtin_amdgcn_ballot_w64(most * a.scale > m + kRise)) {
+      if (__builtin_amdgcn_ballot_w64(most * a.scale > m + kRise<T>)) {
         most = max_of_halves(most) * a.scale;
-        const bool rise = most > m + kRise;
-        const float by = rise ? __builtin_amdgcn_exp2f(m - most) : 1.f;
-        m = rise ? most : m;
+        const bool rise = most > m + kRise<T>;
+        const float by = rise ? __builtin_amdgcn_exp2f(m - (most - kLift<T>)) : 1.f;
+        m = rise ? most - kLift<T> : m;
         l *= by;
 #pragma unroll
         for (int i = 0; i < kD; ++i) o[i] *= by;
@@ -723,12 +732,12 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attention_few(LmAttn
         float most = x[0][0];
 #pragma unroll
         for (int i = 1; i < 8; ++i) most = fmaxf(most, x[i / 4][i % 4]);
-        if (__builtin_amdgcn_ballot_w64(most * a.scale > m + kRise)) {
+        if (__builtin_amdgcn_ballot_w64(most * a.scale > m + kRise<T>)) {
           most = fmaxf(most, __shfl_xor(most, 16));
           most = fmaxf(most, __shfl_xor(most, 32)) * a.scale;
-          const bool rise = most > m + kRise;
-          const float by = rise ? __builtin_amdgcn_exp2f(m - most) : 1.f;
-          m = rise ? most : m;
+          const bool rise = most > m + kRise<T>;
+          const float by = rise ? __builtin_amdgcn_exp2f(m - (most - kLift<T>)) : 1.f;
+          m = rise ? most - kLift<T> : m;
           l *= by;
 #pragma unroll
           for (int i = 0; i < kD; ++i) o[i] *= by;

@@ -609,7 +609,8 @@ int hv_cache_write(const hv_cache_write_desc *d, hv_stream_t stream);
  * sequence may); pages that no row of it sees may be anything, as those are
  * that a window has left behind.  Sums are held in 32 bits.  The softmax's terms are rounded to
  * the type for the product with v, as the sum of two of the type where a call
- * has at most 16 rows a sequence and key head.  Rows outside all sequences are
+ * has at most 16 rows a sequence and key head; in f16 a term within 2^-21 of the
+ * row's largest keeps all of its bits, and one under 2^-32 of it none.  Rows outside all sequences are
  * left as they were; those that several sequences claim hold any values.  out
  * may be q itself (same strides) and overlaps nothing else.
  * Widths are multiples of 8 up to 256, strides multiples of 8, pointers 16-byte

@@ -482,6 +482,33 @@ def test_attention_scores(kind):
                          dtype, f"{kind} {form}")
 
 
+@pytest.mark.parametrize("rows", (1, 40))
+@pytest.mark.parametrize("below", (20, 24, 26, 28))
+@pytest.mark.parametrize("kind", HALVES)
+def test_attention_many_small_terms_beside_a_large_one(kind, below, rows, monkeypatch):
+    """One key far above 1000 others, whose values alone count as its own is
+    zero.  (A term 2^-below of the largest is rounded relative to itself or, in
+    float16, by half of its smallest step at most, which is 2^-25 where the
+    largest term is 2^7 or more: 2^-32 of that.  The results are normal numbers.)"""
+    from heatvit_amd import lm
+    monkeypatch.setitem(ref.TINY, torch.float16, 2.0 ** -32)
+    dtype, width, keys, g = TYPES[kind], 64, 1001, _gen(3)
+    # (whole: a share without the large key would have a reference of its own)
+    assert lm_attention_kernels.kernel_of(rows, 1, 1, 1, width, keys) == ("few" if rows == 1 else "tiles")
+    for at in (0, 500, 1000):
+        q, k = torch.ones(rows, 1, width, dtype=dtype), torch.zeros(keys, 1, width)
+        k[:, 0, :4] = torch.randn(keys, 4, generator=g) / 16
+        k[at] = below * math.log(2) / 8
+        v = 100 * (1 + torch.rand(keys, 1, width, generator=g))
+        v[at] = 0
+        k, v = k.to(dtype), v.to(dtype)
+        got = lm.attention(q.cuda(), k.cuda(), v.cuda(), _i32([0, rows]).cuda(),
+                           k_starts=_i32([0, keys]).cuda(), causal=False, lse=True)
+        assert (got.out[..., 0] >= 2.0 ** -14).all()
+        _check_attention(got, q, [(k.double().numpy(), v.double().numpy())], [0, rows], 0.125, False, 0,
+                         dtype, f"{kind} 2^-{below} at {at}")
+
+
 @pytest.mark.parametrize("width", (64, 128))
 @pytest.mark.parametrize("kind", HALVES)
 def test_attention_leaves_out_what_is_not_seen(kind, width):
