@@ -152,7 +152,7 @@ _CACHE_FIELDS = [(n, _vp) for n in ("cache_k", "cache_v", "cache_k_exps", "cache
 _ROWS_FIELDS = [(n, _vp) for n in ("q", "out", "lse", "starts")] + [
     (n, C.c_int64) for n in ("q_ld", "q_head_ld", "out_ld", "out_head_ld")] + [
     (n, _i32) for n in ("rows", "batch", "heads", "kv_heads", "width", "type", "causal",
-                        "window")] + [("scale", C.c_float), ("reserved", _i32)]
+                        "window")] + [("scale", C.c_float), ("most_keys", _i32)]
 
 
 class CacheWriteDesc(C.Structure):

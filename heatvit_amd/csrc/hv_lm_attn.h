@@ -21,7 +21,8 @@ struct LmAttnArgs {
   int64_t k_ld, k_head_ld, v_ld, v_head_ld;  // packed keys
   int64_t table_ld;
   int rows, k_rows, batch, heads, kv_heads, group, width, causal, window;
-  int run;  // run_of
+  int most_keys;  // of a sequence, 0: unknown
+  int run;        // run_of
   PageMap map;
   float scale;  // of q.k, to a power of two: scale log2(e)
 };

@@ -18,6 +18,8 @@ static int check_rows(const char *what, const hv_attention_rows &r, bool need_st
   if (r.window < 0 || (r.window && !r.causal))
     return fail(HV_EVALUE, HV_ERR_DIMENSION, "%s: a window of %d without the causal order", what,
                 r.window);
+  if (r.most_keys < 0)
+    return fail(HV_EVALUE, HV_ERR_DIMENSION, "%s: at most %d keys", what, r.most_keys);
   if (!(r.scale > 0.f) || r.scale > 1e30f)
     return fail(HV_EVALUE, HV_ERR_DIMENSION, "%s: scale must lie in (0, 1e30]", what);
   if (!need_starts && !r.starts && r.rows != r.batch)
@@ -41,6 +43,7 @@ static LmAttnArgs args_of(const hv_attention_rows &r) {
   a.q_ld = r.q_ld; a.q_head_ld = r.q_head_ld; a.out_ld = r.out_ld; a.out_head_ld = r.out_head_ld;
   a.rows = r.rows; a.batch = r.batch; a.heads = r.heads; a.kv_heads = r.kv_heads;
   a.group = r.heads / r.kv_heads; a.width = r.width; a.causal = r.causal; a.window = r.window;
+  a.most_keys = r.most_keys;
   a.scale = r.scale * 1.4426950408889634f;
   return a;
 }

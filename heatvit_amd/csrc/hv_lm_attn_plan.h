@@ -35,10 +35,29 @@ inline Shape shape_of(int rows, int batch, int heads, int kv_heads, int width) {
 // workgroups have a tile, the better (64 rows of 32 heads over 1024 keys, 24 items: 30.3 and
 // 34.5, 2048 54 and 40; 1024 rows, 264 items, over 2048 64 and 68, 4096 116 and 102; a prompt
 // of 1536, 392 items, 38 and 59).
+// most_keys: of the longest sequence, by keys_of_table or keys_of_packed. The rule holds at heads
+// of 64 and of 256 too (us, whole and in shares: a prompt of 1024 17.7 and 32.7, 39 and 44; of 4096,
+// 8 heads, 55 and 50, 132 and 119; 128 rows of 32 and of 16 heads over 4096 69 and 33, 167 and 52).
 inline bool worth_sharing(const Shape &shape, int rows, int batch, int kv_heads, int group,
                           int64_t most_keys) {
   if (shape.tile_rows == kFewRows) return most_keys > 2048;
   return most_keys * (512 - most_tiles(rows, batch, group, shape.tile_rows) * kv_heads) > 1 << 19;
+}
+
+// Keys of the longest sequence, as far as the host knows: what the caller says, or
+// of a cache what a row of its table has room for. Where that is far more than the sequences have,
+// a call in shares pays for parts that it does not have (us, said and not said, with a
+// table of 131072 keys: a prompt of 512 over 32 heads 18 and 41, 8 rows over up to 1000 keys 12 and
+// 23, one over 1000 13.7 and 17.4).
+inline int64_t keys_of_table(int said, int64_t room) { return said ? said : room; }
+// Of packed sequences twice their mean, as lengths spread evenly from none on have; their sum would
+// cut many short ones (us, whole and in shares: 8 prompts of 512 and 4 heads of 128 16.4 and 36.7,
+// 200 of 16 and 8 heads 22 and 32, 16 of 100 over one head of keys 12 and 44), their mean leave
+// spread ones whole (8 rows of 16 heads on 4 of 128 over 400, 800, .. 3200 keys 32 and 20). Where
+// one is longer still the caller has to say so (over 4000 and seven times 100 40 and 21).
+inline int64_t keys_of_packed(int said, int64_t all, int batch) {
+  const int64_t twice = 2 * ((all + batch - 1) / batch);
+  return said ? said : twice < all ? twice : all;
 }
 
 // Tiles of a short sequence run on one XCD, whose L2 then has their keys once. Workgroup b runs on

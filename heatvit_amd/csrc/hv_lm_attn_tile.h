@@ -960,7 +960,9 @@ static int attend(LmAttnArgs a, void *workspace, size_t bytes, hipStream_t s) {
     split.workgroups = shape.workgroups;
     split.tile_rows = shape.tile_rows;
     split.slot_floats = slot_floats_of(shape, a.width);
-    const int64_t most_keys = PAGED ? (int64_t)a.map.max_pages << a.map.shift : a.k_rows;
+    const int64_t most_keys =
+        PAGED ? keys_of_table(a.most_keys, (int64_t)a.map.max_pages << a.map.shift)
+              : keys_of_packed(a.most_keys, a.k_rows, a.batch);
     if (!worth_sharing(shape, a.rows, a.batch, a.kv_heads, a.group, most_keys)) shape.split = false;
   }
   a.run = run_of(shape, a.rows, a.batch, a.kv_heads, a.group);

@@ -549,7 +549,7 @@ def _aligned(name, t, *lds):
         raise ValueError(f"the heads of {name} must start at multiples of 16 bytes")
 
 
-def _attention_rows(q, kv_heads, starts, batch, scale, causal, window, lse, out):
+def _attention_rows(q, kv_heads, starts, batch, scale, causal, window, most_keys, lse, out):
     """The descriptor's fields of the rows, the result and the tensors to look at."""
     rows, heads, width, q_ld, q_head_ld = _heads("q", q, _HEAD_TYPES)
     if not 8 <= width <= _lib.HV_ATTENTION_MAX_WIDTH or width % 8:
@@ -563,6 +563,10 @@ def _attention_rows(q, kv_heads, starts, batch, scale, causal, window, lse, out)
         raise ValueError("scale must lie in (0, 1e30]")
     if window < 0 or (window and not causal):
         raise ValueError("window must not be negative, and goes with causal")
+    if most_keys is None:
+        most_keys = 0
+    elif most_keys < 0:
+        raise ValueError("most_keys must not be negative")
     _aligned("q", q, q_ld, q_head_ld)
     if out is None:
         out = Attended(torch.empty_like(q, memory_format=torch.contiguous_format),
@@ -577,12 +581,12 @@ def _attention_rows(q, kv_heads, starts, batch, scale, causal, window, lse, out)
             _given("out.lse", out[1], (rows, heads), torch.float32)
     values = (q.data_ptr(), out[0].data_ptr(), _ptr(out[1]), _ptr(starts), q_ld, q_head_ld, out_ld,
               out_head_ld, rows, batch, heads, kv_heads, width, _HEAD_TYPES[q.dtype], bool(causal),
-              window, scale, 0)
+              window, scale, most_keys)
     return values, Attended(*out), (out[0], out[1], starts)
 
 
-def attention(q, k, v, starts, *, k_starts=None, scale=None, causal=True, window=0, lse=False,
-              out=None, workspace=None):
+def attention(q, k, v, starts, *, k_starts=None, scale=None, causal=True, window=0, most_keys=None,
+              lse=False, out=None, workspace=None):
     """Attention of packed sequences: rows starts[b] .. starts[b+1] - 1 of q over
     rows k_starts[b] .. k_starts[b+1] - 1 of k and v (without k_starts, of starts).
 
@@ -594,7 +598,9 @@ def attention(q, k, v, starts, *, k_starts=None, scale=None, causal=True, window
     A row that sees nothing gets zeros (and -inf in lse); what a row does not
     see leaves no trace in it.  Sequences may be empty; offsets that leave the
     tensors are taken at their ends, and rows that several sequences claim hold
-    any values.  `out`: the Attended to write, its tensor q itself if wanted, and
+    any values.  most_keys: about as many keys as the longest sequence has, where
+    the program knows it (else twice the mean is taken): it says whether the work of
+    few long sequences is cut into shares, not what comes out.  `out`: the Attended to write, its tensor q itself if wanted, and
     apart from k and v.  Returns Attended(out, lse), lse [T][Hq] the logarithm of
     the sum of exponentials where asked for."""
     if not isinstance(k, torch.Tensor) or not isinstance(q, torch.Tensor):
@@ -608,8 +614,8 @@ def attention(q, k, v, starts, *, k_starts=None, scale=None, causal=True, window
     batch = _batch(starts, 0)
     if k_starts is not None:
         _ints("k_starts", k_starts, batch + 1)
-    values, out, tensors = _attention_rows(q, kv_heads, starts, batch, scale, causal, window, lse,
-                                           out)
+    values, out, tensors = _attention_rows(q, kv_heads, starts, batch, scale, causal, window,
+                                           most_keys, lse, out)
     if q.shape[2] != width or (k_starts is None and k_rows != q.shape[0]):
         raise ValueError(f"k of {list(k.shape)} does not go with q of {list(q.shape)}")
     _aligned("k", k, k_ld, k_head_ld)
@@ -624,12 +630,15 @@ def attention(q, k, v, starts, *, k_starts=None, scale=None, causal=True, window
 
 
 def paged_attention(q, cache, table, lengths, *, starts=None, scale=None, causal=True, window=0,
-                    lse=False, out=None, workspace=None):
+                    most_keys=None, lse=False, out=None, workspace=None):
     """Attention of new rows over a KvCache that holds their keys already
     (cache_write): rows starts[b] .. starts[b+1] - 1 of q (without `starts` row b)
     over the lengths[b] keys of sequence b, key j in page table[b][j / page].
 
-    q [T][Hq][D] of the cache's dtype; the rest as in attention.  A sequence
+    q [T][Hq][D] of the cache's dtype; the rest as in attention, but without
+    most_keys a sequence is taken to be as long as the table has room for: pass it
+    where the table is much wider than the sequences are long (in a captured
+    graph, for the lengths that it will be replayed with).  A sequence
     whose table has no room for its keys gets NaN, and so does a row that sees a
     page that the cache does not have (and perhaps others of its sequence);
     table entries of pages that no row sees, as those that a window has left
@@ -640,7 +649,7 @@ def paged_attention(q, cache, table, lengths, *, starts=None, scale=None, causal
         raise TypeError(f"q must be a tensor of {cache.dtype}")
     batch = _batch(starts, q.shape[0] if q.dim() else 0)
     values, out, tensors = _attention_rows(q, cache.kv_heads, starts, batch, scale, causal, window,
-                                           lse, out)
+                                           most_keys, lse, out)
     if q.shape[2] != cache.width:
         raise ValueError(f"q must be [rows][heads][{cache.width}]")
     more, held = cache._values(table, lengths, batch)

@@ -613,6 +613,10 @@ int hv_cache_write(const hv_cache_write_desc *d, hv_stream_t stream);
  * row's largest keeps all of its bits, and one under 2^-32 of it none.  Rows outside all sequences are
  * left as they were; those that several sequences claim hold any values.  out
  * may be q itself (same strides) and overlaps nothing else.
+ * most_keys: about as many keys as the longest sequence has, where the caller
+ * knows that, or 0: what a row of the table has room for, or twice the mean of
+ * packed sequences.  It says whether a call of few rows or tiles is cut into
+ * shares; the result holds with any.
  * Widths are multiples of 8 up to 256, strides multiples of 8, pointers 16-byte
  * aligned (lse 4); type HV_T_F16 or HV_T_BF16.  The workspace (16-byte aligned) holds
  * what the parts of a long axis leave, for the call alone; calls that overlap
@@ -625,7 +629,7 @@ typedef struct {
   int64_t q_ld, q_head_ld, out_ld, out_head_ld;
   int32_t rows, batch, heads, kv_heads, width, type, causal, window;
   float scale;
-  int32_t reserved;
+  int32_t most_keys;
 } hv_attention_rows;
 
 typedef struct {

@@ -59,6 +59,12 @@ int attention_run(int rows, int batch, int heads, int kv_heads, int width, int s
 int place_in_runs(int b, int run) { return place_of(b, run); }
 }
 
+// The longest sequence's keys, by what the host knows.
+extern "C" {
+long long table_keys(int said, long long room) { return keys_of_table(said, room); }
+long long packed_keys(int said, long long all, int batch) { return keys_of_packed(said, all, batch); }
+}
+
 // Lanes of a head of the rotary kernels.
 #include "hv_lm_rotary_plan.h"
 extern "C" int lanes_of_head(int pairs, int width) { return rotary_lanes(pairs, width); }

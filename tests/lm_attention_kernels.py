@@ -34,6 +34,8 @@ def library():
     L.attention_run.argtypes = [i] * 6
     L.place_in_runs.argtypes = [i] * 2
     L.share_numbers.argtypes = [i] * 5 + [p]
+    L.table_keys.argtypes, L.table_keys.restype = [i, n], n
+    L.packed_keys.argtypes, L.packed_keys.restype = [i, n, i], n
     return L
 
 

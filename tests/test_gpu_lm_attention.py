@@ -793,6 +793,30 @@ def test_attention_tiles_in_shares():
     _run_attention([4, 2], 4, 2, 64, "f16", True, 0, 5, [2500, 800])
 
 
+@pytest.mark.parametrize("new, lengths", (([1, 1], [300, 2500]), ([3, 2], [2300, 40]), ([90, 45], [700, 2500])))
+def test_what_is_said_of_the_longest_sequence(new, lengths):
+    """Any number of keys said of the longest sequence gives the result, over a
+    cache with a wide table and over packed keys, whole and in shares."""
+    from heatvit_amd import lm
+    book = _filled(lengths, 2, 64, 64, torch.bfloat16, False, 3)
+    q = torch.randn(sum(new), 4, 64, generator=_gen(1)).to(torch.bfloat16)
+    at, scale = _starts(new), 0.125
+    rows = [book.rows(b) for b in range(2)]
+    k, v = (torch.from_numpy(np.concatenate([r[i] for r in rows])).to(torch.bfloat16) for i in range(2))
+    table = torch.full((2, 2048), -1, dtype=torch.int32)
+    table[:, :book.table.shape[1]] = book.table
+    kernels = set()
+    for said in (None, 0, 1, max(lengths), 2 ** 31 - 1):
+        kernels.add(lm_attention_kernels.kernel_of(sum(new), 2, 4, 2, 64, said or 131072))
+        args = dict(most_keys=said, lse=True)
+        for got in (lm.paged_attention(q.cuda(), book.cache, table.cuda(), _i32(lengths).cuda(),
+                                       starts=_i32(at).cuda(), **args),
+                    lm.attention(q.cuda(), k.cuda(), v.cuda(), _i32(at).cuda(),
+                                 k_starts=_i32(_starts(lengths)).cuda(), **args)):
+            _check_attention(got, q, rows, at, scale, True, 0, torch.bfloat16, f"{new} said {said}")
+    assert len(kernels) == 2
+
+
 @pytest.mark.parametrize("new", ([2, 1], [90, 45]))
 def test_shares_leave_out_what_is_not_seen(new):
     """NaN and infinities that a row does not see leave no trace where the keys

@@ -100,6 +100,30 @@ def test_kernels():
             assert size == 0
 
 
+def test_kernels_by_the_longest_sequence():
+    """Many short sequences are no long one: neither their keys' sum nor a wide
+    table that the caller says more about cuts their work into shares."""
+    L, of = lm_attention_kernels.library(), lm_attention_kernels.kernel_of
+    for rows, batch, heads, kv, width in ((8 * 512, 8, 4, 4, 128), (16 * 100, 16, 8, 1, 64),
+                                          (32 * 128, 32, 8, 2, 128), (8 * 300, 8, 8, 2, 64),
+                                          (4 * 1024, 4, 8, 2, 128)):
+        assert of(rows, batch, heads, kv, width, rows) == "tiles in shares"
+        assert of(rows, batch, heads, kv, width, L.packed_keys(0, rows, batch)) == "tiles"
+    assert of(3200, 200, 8, 8, 128, 3200) == "few in shares"
+    assert of(3200, 200, 8, 8, 128, L.packed_keys(0, 3200, 200)) == "few"
+    assert of(4096, 1, 8, 8, 128, L.packed_keys(0, 4096, 1)) == "tiles in shares"
+    assert of(8, 8, 16, 4, 128, L.packed_keys(0, 4700, 8)) == "few"
+    assert of(8, 8, 16, 4, 128, L.packed_keys(4000, 4700, 8)) == "few in shares"
+    assert of(4, 4, 16, 4, 64, L.packed_keys(0, 16300, 4)) == "few in shares"
+    for rows, heads, kv, width, kind in ((512, 32, 8, 128, "tiles"), (1, 32, 8, 128, "few")):
+        assert of(rows, 1, heads, kv, width, L.table_keys(0, 131072)) == kind + " in shares"
+        assert of(rows, 1, heads, kv, width, L.table_keys(512, 131072)) == kind
+    assert L.table_keys(0, 96) == 96 and L.table_keys(7, 96) == 7
+    for said, total, batch, want in ((0, 0, 5, 0), (0, 1, 5, 1), (0, 10, 1, 10), (0, 10, 2, 10), (0, 10, 5, 4),
+                                     (3, 10, 5, 3), (0, 2 ** 24, 3, 2 * 5592406), (2 ** 31 - 1, 1, 1, 2 ** 31 - 1)):
+        assert L.packed_keys(said, total, batch) == want
+
+
 def test_runs():
     """Workgroups in runs take every place once, and an XCD's are side by side."""
     L = lm_attention_kernels.library()
@@ -296,7 +320,7 @@ def test_write_refusals():
     ))
 
 
-ROWS_BAD = (dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf),
+ROWS_BAD = (dict(most_keys=-1), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf),
             dict(window=-1), dict(window=3, causal=False),
             dict(q=torch.zeros(3, 5, 32, dtype=BF)), dict(q=torch.zeros(3, 4, 36, dtype=BF)),
             dict(q=torch.zeros(3, 4, 40, dtype=BF)), dict(q=torch.zeros(3, 0, 32, dtype=BF)),
@@ -440,7 +464,7 @@ ROWS_DIMENSION = (dict(rows=-1), dict(rows=1 << 24), dict(batch=-1), dict(heads=
                   dict(kv_heads=0), dict(heads=8192), dict(rows=1 << 20, heads=128), dict(width=0),
                   dict(width=20), dict(width=264), dict(window=-1), dict(window=2, causal=0),
                   dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf),
-                  dict(q_ld=100), dict(out_head_ld=4), dict(q_ld=-8))
+                  dict(q_ld=100), dict(out_head_ld=4), dict(q_ld=-8), dict(most_keys=-1))
 ROWS_ADDRESS = (dict(q=None), dict(out=None), dict(q=PTR + 8), dict(out=PTR + 2), dict(lse=PTR + 2),
                 dict(starts=PTR + 2))
 
