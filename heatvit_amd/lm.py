@@ -457,7 +457,8 @@ def rotary_qk(q, k, positions, freqs, *, q_weight=None, k_weight=None, eps=1e-6,
 class KvCache:
     """Pages of keys and values: k and v [pages][kv_heads][page][D] of float16
     or bfloat16, or of float8_e4m3fn with k_exps and v_exps [pages][kv_heads]
-    [page] int8 (value * 2^exps, rounded to `dtype` where it is read).  page is a
+    [page] int8 (value * 2^exps, rounded to `dtype` where it is read; -128 is
+    NaN).  page is a
     power of two from 16 to 4096, D a multiple of 8 (e4m3: 16) up to 256.
 
     The tensors are the caller's and are written in place; KvCache.empty
@@ -525,7 +526,8 @@ def cache_write(cache, k, v, table, lengths, *, starts=None):
 
     k, v [T][Hk][D] of the cache's dtype; table [B][pages] int32, lengths [B]
     and starts [B + 1] int32, all on the device.  In e4m3 each head of a row
-    gets the smallest exponent that holds it.  A row is not written where its
+    gets the smallest exponent that holds it (with an infinity, which is read back
+    as NaN, the largest).  A row is not written where its
     place lies before the first key, past the table or in a page that the
     cache does not have.  Sequences that share a page must not both write it."""
     if not isinstance(cache, KvCache):
@@ -597,8 +599,8 @@ def attention(q, k, v, starts, *, k_starts=None, scale=None, causal=True, window
     keys, each row before it one less; window > 0: the last `window` of those.
     A row that sees nothing gets zeros (and -inf in lse); what a row does not
     see leaves no trace in it.  Sequences may be empty; offsets that leave the
-    tensors are taken at their ends, and rows that several sequences claim hold
-    any values.  most_keys: about as many keys as the longest sequence has, where
+    tensors are taken at their ends, and where sequences overlap, rows of any of
+    the call's hold any values.  most_keys: about as many keys as the longest sequence has, where
     the program knows it (else twice the mean is taken): it says whether the work of
     few long sequences is cut into shares, not what comes out.  `out`: the Attended to write, its tensor q itself if wanted, and
     apart from k and v.  Returns Attended(out, lse), lse [T][Hq] the logarithm of

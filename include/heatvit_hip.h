@@ -553,7 +553,7 @@ int hv_rotary_qk(const hv_rotary_desc *d, hv_stream_t stream);
 /* A cache of keys and values in pages of 16 to 4096 keys (a power of two):
  * k and v are [pages][kv_heads][page][width] of the call's type
  * (HV_CACHE_SAME) or of e4m3 (HV_CACHE_E4M3: value * 2^exps, with
- * k_exps and v_exps [pages][kv_heads][page]), rounded to the call's type where
+ * k_exps and v_exps [pages][kv_heads][page] from -127 on; -128 is NaN), rounded to the call's type where
  * they are read.  Sequence b has lengths[b] keys, key j in page
  * table[b][j / page].  Widths are multiples of 8 (e4m3: 16) up to 256, k and v
  * 16-byte aligned. */
@@ -579,7 +579,8 @@ typedef struct {
  * each sequence).  Heads of e4m3 get the smallest exponent e >= -127 with
  * |x| <= 448 * 2^e and are rounded to nearest, ties to even; what would round
  * past the type's numbers (240 * 2^8 in float16, 240 * 2^120 in bfloat16) stays
- * at that, and an infinity or NaN is NaN.  A row whose place is before the
+ * at that, and an infinity or NaN is NaN.  A head with an infinity has the
+ * exponent 120, of which its finite elements under 2^110 leave zeros.  A row whose place is before the
  * sequence's first key, past the table or in a page outside the cache is not
  * written, nor are rows before starts[0] and from starts[batch] on.  Sequences
  * that share a page must not both write it. */
@@ -596,23 +597,25 @@ int hv_cache_write(const hv_cache_write_desc *d, hv_stream_t stream);
 /* Attention of packed sequences (hv_attention), or of new rows over a paged
  * cache (hv_paged_attention):
  *   out = sum over the keys j that a row sees of softmax(scale * q.k_j) v_j
- * for each head, query head h with key head h / (heads / kv_heads).  The rows
- * of sequence b are starts[b] .. starts[b+1] - 1 (NULL, paged alone: a row for
- * each sequence), its keys k_starts[b] .. k_starts[b+1] - 1 (NULL: starts) or
- * the cache's.  `causal`: row i of n sees the first keys - n + i + 1 keys, the
- * last `window` of those where that is not 0.  A row that sees nothing gets
- * zeros, and -infinity in lse, which (optional) is [rows][heads], the natural
- * logarithm of the sum of exponentials.  What a row does not see leaves no
- * trace in it, infinities and NaN among it; an infinity that it does see may
- * come out as NaN.  A sequence whose table has no room for its keys gets NaN,
- * and so does a row that sees a page outside the cache (other rows of its
- * sequence may); pages that no row of it sees may be anything, as those are
- * that a window has left behind.  Sums are held in 32 bits.  The softmax's terms are rounded to
- * the type for the product with v, as the sum of two of the type where a call
- * has at most 16 rows a sequence and key head; in f16 a term within 2^-21 of the
- * row's largest keeps all of its bits, and one under 2^-32 of it none.  Rows outside all sequences are
- * left as they were; those that several sequences claim hold any values.  out
- * may be q itself (same strides) and overlaps nothing else.
+ * for each head, query head h with key head h / (heads / kv_heads). The rows of
+ * sequence b are starts[b] .. starts[b+1] - 1 (NULL, paged alone: a row for each
+ * sequence), its keys k_starts[b] .. k_starts[b+1] - 1 (NULL: starts) or the
+ * cache's. `causal`: row i of n sees the first keys - n + i + 1 keys, the last
+ * `window` of those where that is not 0. A row that sees nothing gets zeros, and
+ * -infinity in lse, which (optional) is [rows][heads], the natural logarithm of
+ * the sum of exponentials. What a row does not see leaves no trace in it,
+ * infinities and NaN among it; an infinity that it does see may come out as NaN.
+ * A sequence whose table has no room for its keys gets NaN, and so does a row
+ * that sees a page outside the cache (other rows of its sequence may); pages that
+ * no row of it sees may be anything, as those are that a window has left behind.
+ * Sums are held in 32 bits. The softmax's terms are rounded to the type for the
+ * product with v, as the sum of two of the type where a call has at most 16 rows
+ * a sequence and key head; in f16 a term within 2^-21 of the row's largest keeps
+ * all of its bits, and one under 2^-32 of it none. Rows outside all sequences are
+ * left as they were; where sequences overlap, rows of any of the call's hold any
+ * values. A bfloat16 value times the number of a row's keys has to stay under
+ * 2^119, or the row may come out infinite or NaN. out may be q itself (same
+ * strides) and overlaps nothing else.
  * most_keys: about as many keys as the longest sequence has, where the caller
  * knows that, or 0: what a row of the table has room for, or twice the mean of
  * packed sequences.  It says whether a call of few rows or tiles is cut into

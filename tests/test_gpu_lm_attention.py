@@ -713,6 +713,32 @@ def test_paged_smallest_exponent():
     _check_attention(got, q, [book.rows(0)], [0, 1], 0.125, True, 0, torch.bfloat16, "exponents")
 
 
+@pytest.mark.parametrize("kind", HALVES)
+@pytest.mark.parametrize("new", ([1, 1], [70, 3]))
+def test_paged_exponent_that_is_none(kind, new):
+    """An exponent of -128 is NaN for the rows that see it, zeros among its
+    elements too, and leaves no trace in the others."""
+    from heatvit_amd import lm
+    book = _filled([200, 90], 2, 64, 16, TYPES[kind], True, 4)
+    q = torch.randn(sum(new), 4, 64, generator=_gen(1)).to(TYPES[kind]).cuda()
+    args = book.table.cuda(), _i32([200, 90]).cuda()
+    starts = _i32(_starts(new)).cuda()
+    clean = lm.paged_attention(q, book.cache, *args, starts=starts, lse=True)
+    at = 199 - new[0] // 2
+    page, i = book.place(0, at)
+    sees = (torch.arange(sum(new)) + 200 - new[0] >= at) & (torch.arange(sum(new)) < new[0])
+    assert sees.any() and not sees.all()
+    for values, exps in ((book.cache.k, book.cache.k_exps), (book.cache.v, book.cache.v_exps)):
+        old = values[page, 1, i].clone(), exps[page, 1, i].clone()
+        values.view(torch.uint8)[page, 1, i, ::2] = 0
+        exps[page, 1, i] = -128
+        got = lm.paged_attention(q, book.cache, *args, starts=starts, lse=True)
+        values[page, 1, i], exps[page, 1, i] = old
+        assert torch.equal(got.out[:, :2], clean.out[:, :2])  # of the other head of keys
+        assert torch.equal(got.out[~sees], clean.out[~sees]) and torch.equal(got.lse[~sees], clean.lse[~sees])
+        assert got.out[sees][:, 2:].isnan().all()
+
+
 @pytest.mark.parametrize("e4m3", (False, True))
 def test_paged_far_pages(e4m3):
     """Pages whose elements lie past 2^32, written and read."""
