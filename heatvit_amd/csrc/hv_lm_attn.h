@@ -1,5 +1,5 @@
 // hv_lm_attn.h -- what the attention kernels share: their arguments, where
-// their keys come from, and a row by a wavefront.
+// their rows and keys lie, and which tiles and shares of them a workgroup has.
 #pragma once
 
 #include <type_traits>
@@ -64,7 +64,8 @@ struct Pair8<f16> {
 };
 
 // 2^e of an exponent's byte. (The conversion takes its factor by the exponent alone, which 2^-127
-// still has; -128, which no write makes, has all of a NaN's exponent bits, and gives NaN.) A byte is taken as it was loaded: to extend its sign there would wait for it.
+// still has; -128, which no write makes, has all of a NaN's exponent bits, and gives NaN.) A byte is
+// taken as it was loaded: to extend its sign there would wait for it.
 __device__ __forceinline__ float factor_of(int byte) {
   return __builtin_bit_cast(float, ((byte ^ 0x80) - 1) << 23);
 }

@@ -35,9 +35,9 @@ inline Shape shape_of(int rows, int batch, int heads, int kv_heads, int width) {
 // workgroups have a tile, the better (64 rows of 32 heads over 1024 keys, 24 items: 30.3 and
 // 34.5, 2048 54 and 40; 1024 rows, 264 items, over 2048 64 and 68, 4096 116 and 102; a prompt
 // of 1536, 392 items, 38 and 59).
-// most_keys: of the longest sequence, by keys_of_table or keys_of_packed. The rule holds at heads
-// of 64 and of 256 too (us, whole and in shares: a prompt of 1024 17.7 and 32.7, 39 and 44; of 4096,
-// 8 heads, 55 and 50, 132 and 119; 128 rows of 32 and of 16 heads over 4096 69 and 33, 167 and 52).
+// The rule holds at heads of 64 and of 256 too (a prompt of 1024 17.7 and 32.7, 39 and 44; of
+// 4096, 8 heads, 55 and 50, 132 and 119; 128 rows of 32 and of 16 heads over 4096 69 and 33, 167
+// and 52). most_keys: of the longest sequence, by keys_of_table or keys_of_packed.
 inline bool worth_sharing(const Shape &shape, int rows, int batch, int kv_heads, int group,
                           int64_t most_keys) {
   if (shape.tile_rows == kFewRows) return most_keys > 2048;

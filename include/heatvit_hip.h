@@ -552,10 +552,10 @@ int hv_rotary_qk(const hv_rotary_desc *d, hv_stream_t stream);
 
 /* A cache of keys and values in pages of 16 to 4096 keys (a power of two):
  * k and v are [pages][kv_heads][page][width] of the call's type
- * (HV_CACHE_SAME) or of e4m3 (HV_CACHE_E4M3: value * 2^exps, with
- * k_exps and v_exps [pages][kv_heads][page] from -127 on; -128 is NaN), rounded to the call's type where
- * they are read.  Sequence b has lengths[b] keys, key j in page
- * table[b][j / page].  Widths are multiples of 8 (e4m3: 16) up to 256, k and v
+ * (HV_CACHE_SAME) or of e4m3 (HV_CACHE_E4M3: value * 2^exps, with k_exps and
+ * v_exps [pages][kv_heads][page] from -127 on; -128 is NaN), rounded to the
+ * call's type where they are read.  Sequence b has lengths[b] keys, key j in
+ * page table[b][j / page].  Widths are multiples of 8 (e4m3: 16) up to 256, k and v
  * 16-byte aligned. */
 #define HV_CACHE_SAME 0
 #define HV_CACHE_E4M3 1
@@ -580,9 +580,9 @@ typedef struct {
  * |x| <= 448 * 2^e and are rounded to nearest, ties to even; what would round
  * past the type's numbers (240 * 2^8 in float16, 240 * 2^120 in bfloat16) stays
  * at that, and an infinity or NaN is NaN.  A head with an infinity has the
- * exponent 120, of which its finite elements under 2^110 leave zeros.  A row whose place is before the
- * sequence's first key, past the table or in a page outside the cache is not
- * written, nor are rows before starts[0] and from starts[batch] on.  Sequences
+ * exponent 120, of which its finite elements under 2^110 leave zeros.  A row
+ * whose place is before the sequence's first key, past the table or in a page
+ * outside the cache is not written, nor are rows before starts[0] and from starts[batch] on.  Sequences
  * that share a page must not both write it. */
 typedef struct {
   hv_cache_desc cache;
