@@ -458,8 +458,8 @@ class KvCache:
     """Pages of keys and values: k and v [pages][kv_heads][page][D] of float16
     or bfloat16, or of float8_e4m3fn with k_exps and v_exps [pages][kv_heads]
     [page] int8 (value * 2^exps, rounded to `dtype` where it is read; -128 is
-    NaN).  page is a
-    power of two from 16 to 4096, D a multiple of 8 (e4m3: 16) up to 256.
+    NaN).  page is a power of two from 16 to 4096, D a multiple of 8 (e4m3: 16) up
+    to 256.
 
     The tensors are the caller's and are written in place; KvCache.empty
     makes them."""
@@ -592,19 +592,20 @@ def attention(q, k, v, starts, *, k_starts=None, scale=None, causal=True, window
     """Attention of packed sequences: rows starts[b] .. starts[b+1] - 1 of q over
     rows k_starts[b] .. k_starts[b+1] - 1 of k and v (without k_starts, of starts).
 
-    q [T][Hq][D], k and v [S][Hk][D] of float16 or bfloat16, Hq a multiple of
-    Hk (head h reads head h / (Hq / Hk)), D a multiple of 8 up to 256, heads at
-    multiples of 16 bytes; starts, k_starts [B + 1] int32 on the device.  scale:
-    1 / sqrt(D) if None.  causal: the last row of a sequence sees all of its
-    keys, each row before it one less; window > 0: the last `window` of those.
-    A row that sees nothing gets zeros (and -inf in lse); what a row does not
-    see leaves no trace in it.  Sequences may be empty; offsets that leave the
-    tensors are taken at their ends, and where sequences overlap, rows of any of
-    the call's hold any values.  most_keys: about as many keys as the longest sequence has, where
-    the program knows it (else twice the mean is taken): it says whether the work of
-    few long sequences is cut into shares, not what comes out.  `out`: the Attended to write, its tensor q itself if wanted, and
-    apart from k and v.  Returns Attended(out, lse), lse [T][Hq] the logarithm of
-    the sum of exponentials where asked for."""
+    q [T][Hq][D], k and v [S][Hk][D] of float16 or bfloat16, Hq a multiple of Hk
+    (head h reads head h / (Hq / Hk)), D a multiple of 8 up to 256, heads at
+    multiples of 16 bytes; starts, k_starts [B + 1] int32 on the device.  scale: 1 /
+    sqrt(D) if None.  causal: the last row of a sequence sees all of its keys, each
+    row before it one less; window > 0: the last `window` of those. A row that sees
+    nothing gets zeros (and -inf in lse); what a row does not see leaves no trace in
+    it.  Sequences may be empty; offsets that leave the tensors are taken at their
+    ends, and where sequences overlap, rows of any of the call's hold any values.
+    most_keys: about as many keys as the longest sequence has, where the program
+    knows it (else twice the mean is taken): it says whether the work of few long
+    sequences is cut into shares, and so no more than roundings.  `out`: the
+    Attended to write, its tensor q itself if wanted, and apart from k and v.
+    Returns Attended(out, lse), lse [T][Hq] the logarithm of the sum of exponentials
+    where asked for."""
     if not isinstance(k, torch.Tensor) or not isinstance(q, torch.Tensor):
         raise TypeError("q and k must be torch tensors")
     if q.dtype not in _HEAD_TYPES:
@@ -639,12 +640,11 @@ def paged_attention(q, cache, table, lengths, *, starts=None, scale=None, causal
 
     q [T][Hq][D] of the cache's dtype; the rest as in attention, but without
     most_keys a sequence is taken to be as long as the table has room for: pass it
-    where the table is much wider than the sequences are long (in a captured
-    graph, for the lengths that it will be replayed with).  A sequence
-    whose table has no room for its keys gets NaN, and so does a row that sees a
-    page that the cache does not have (and perhaps others of its sequence);
-    table entries of pages that no row sees, as those that a window has left
-    behind, may be anything."""
+    where the table is much wider than the sequences are long (in a captured graph,
+    for the lengths that it will be replayed with).  A sequence whose table has no
+    room for its keys gets NaN, and so does a row that sees a page that the cache
+    does not have (and perhaps others of its sequence); table entries of pages that
+    no row sees, as those that a window has left behind, may be anything."""
     if not isinstance(cache, KvCache):
         raise TypeError("cache must be a KvCache")
     if not isinstance(q, torch.Tensor) or q.dtype != cache.dtype:
