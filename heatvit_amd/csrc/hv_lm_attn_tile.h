@@ -137,7 +137,7 @@ struct TileLoader {
   static_assert(kUnits * NW * kRowsOf == kKeys && kRowsOf <= 16, "whole units");
   const LmAttnArgs &a;
   const Sequence &s;
-  int head, lane, wave, from, last;  // the first and the last key that the tile's rows see
+  int head, lane, wave, last;  // last: the last key that is there
   int page[PAGED ? kUnits : 1];
   int k_off[kUnits], v_off[kUnits];  // a lane's, from a unit's first row on
   bool bad;
@@ -147,9 +147,10 @@ struct TileLoader {
   __device__ __forceinline__ int row_of(int u) const {
     return (u * NW + wave) * kRowsOf + lane / kChunks;
   }
-  __device__ __forceinline__ TileLoader(const LmAttnArgs &args, const Work &w, int tid)
-      : a(args), s(w.s), head(w.head), lane(tid & 63), wave(uniform(tid >> 6)), from(w.from),
-        last(w.last), bad(false) {
+  __device__ __forceinline__ TileLoader(const LmAttnArgs &args, const Sequence &seq, int h,
+                                        int last_key, int tid)
+      : a(args), s(seq), head(h), lane(tid & 63), wave(uniform(tid >> 6)), last(last_key),
+        bad(false) {
     const int chunks = a.width * kBytes / 16, c = lane % kChunks, r = lane / kChunks;
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
@@ -210,19 +211,18 @@ struct TileLoader {
       to_lds(vs, v_size, v_off[u], row * v_stride(), v + (u * NW + wave) * 512);
     }
   }
-  // The row of a key, which starts a tile or a unit of `count` keys. A page that the cache does
-  // not have is bad where a row sees one of them: those before a window may be gone.
-  __device__ __forceinline__ int64_t place(int key, int count, int page_of_it) {
+  // The row of a key, which starts a tile or a unit.
+  __device__ __forceinline__ int64_t place(int key, int page_of_it) {
     if (!PAGED) return (int64_t)s.k_first + key;
     const int p = uniform(page_of_it);
     const bool none = (unsigned)p >= (unsigned)a.map.pages;
-    bad |= none && key + count > from;
+    bad |= none;
     return cache_row(a.map, a.kv_heads, none ? 0 : p, head, key);
   }
   // Tile t on its way into k and v (Q8: into registers).
   __device__ __forceinline__ void load(int t, T *k, T *v) {
     if (together()) {
-      const int64_t at = place(t * kKeys, kKeys, page[0]);
+      const int64_t at = place(t * kKeys, page[0]);
 #pragma unroll
       for (int u = 0; u < kUnits; ++u) load_unit(u, (u * NW + wave) * kRowsOf, at, t * kKeys, k, v);
       return;
@@ -231,7 +231,7 @@ struct TileLoader {
     for (int u = 0; u < kUnits; ++u) {
       const int first = t * kKeys + (u * NW + wave) * kRowsOf;
       // A unit behind the last key reads the last one's row again, all of whose scores are masked.
-      load_unit(u, 0, place(min(first, last), kRowsOf, page[u]), min(first, last), k, v);
+      load_unit(u, 0, place(min(first, last), page[u]), min(first, last), k, v);
     }
   }
   // Q8: what `load` brought, into k and v.
@@ -323,7 +323,7 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 3 : DP == 128 ? 2 : 1) void k_a
         q[i] = d < a.width ? *reinterpret_cast<const frag *>(from + d) : frag{};
       }
     }
-    TileLoader<T, DP, PAGED, Q8, NW> loader(a, w, tid);
+    TileLoader<T, DP, PAGED, Q8, NW> loader(a, s, head, w.last, tid);
     v16f o[kD];
     float m, l;
 
@@ -489,7 +489,12 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 3 : DP == 128 ? 2 : 1) void k_a
     const int out_token = at_row / a.group;
     const int out_head = head * a.group + at_row - out_token * a.group;
     l = sum_of_halves(l);
-    if (PAGED && __syncthreads_or(s.keys < 0 || loader.bad)) l = __builtin_nanf("");
+    if (PAGED && __syncthreads_or(s.keys < 0 || loader.bad)) {
+      const int from = seen_by(r0 / a.group, s.count, keys, a.causal, a.window).from;
+      const bool missing = missing_page(a, s.table, max(t0 * kKeys, from),
+                                        min(t1 * kKeys - 1, w.last), threadIdx.x, kThreads);
+      if (__syncthreads_or(s.keys < 0 || missing)) l = __builtin_nanf("");
+    }
     if (idle || w0 + col >= n_rows) continue;
     if (SPLIT && w.slot >= 0) {
       if (half == 0) *split.ml(w.slot, wave * 32 + col) = make_float2(m, l);
@@ -605,8 +610,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attention_few(LmAttn
     v4i kr[2][kLoads / 2], vr[kLoads];
     int ke[2], ve[Q8 ? kLoads : 1];
     int page[2];
-    // Sixteen keys from a multiple of sixteen on lie in one page, which may be gone if it is
-    // before what the rows see.
+    // Sixteen keys from a multiple of sixteen on lie in one page.
     auto group_of = [&](int key0, int i) { return min(key0 + 16 * i, last & ~15); };
     auto find = [&](int key0) __attribute__((always_inline)) {
       if (!PAGED) return;
@@ -621,7 +625,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attention_few(LmAttn
         if (PAGED) {
           const int p = uniform(page[i]);
           const bool none = (unsigned)p >= (unsigned)a.map.pages;
-          bad |= none && group_of(key0, i) + 16 > work.from;
+          bad |= none;
           base[i] = cache_row(a.map, a.kv_heads, none ? 0 : p, head, group_of(key0, i));
         } else {
           base[i] = (int64_t)s.k_first + group_of(key0, i);
@@ -785,6 +789,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void k_attention_few(LmAttn
 
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
+    if (PAGED && __builtin_amdgcn_ballot_w64(bad))
+      bad = missing_page(a, s.table, max(t0 * kKeys, top.from), end - 1, lane, 64);
     if (PAGED && __builtin_amdgcn_ballot_w64(s.keys < 0 || bad)) l = __builtin_nanf("");
     if (grp == 0) ml[wave][col] = make_float2(m, l);
     __syncthreads();
